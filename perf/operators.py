@@ -17,8 +17,6 @@ import math
 import torch
 
 own = False
-if own:
-    from kraken_b200 import capi
 
 
 def listed():
@@ -314,6 +312,7 @@ def _plain_logits(s):
 
 
 def _own(s):
+    from kraken_b200 import capi
     case, kind = s["case"], s["case"]["kind"]
     if kind == "rope":
         return capi.qk_norm_rope(s["q"], s["k"], s["pos"], s["inv_freq"], s["wq"], s["wk"], norm=case["norm"], eps=1e-6, interleaved=case["pairs"] == "adjacent")
