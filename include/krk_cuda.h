@@ -259,6 +259,84 @@ int krk_cuda_gemv_allgather(void *const host_y_peers[], void *const host_flag_pe
                             const void *x_f32, const void *w, int wt, int64_t n_out_local, int64_t n_in,
                             int64_t rows, void *stream);
 
+/* ---- between the projections and the output projection: query and key heads, the cache, attention ---- */
+
+/* Norm of each query and key head with the rotation of its position in the same pass, f32:
+ *   x' = R(pos) (w . x / sqrt(mean(x^2) + eps)),   R turns pairs (a, b) by pos * inv_freq[i]: (a cos - b sin, b cos + a sin).
+ * Pair i is (i, i + rot_dim / 2) of a head, or (2 i, 2 i + 1) with `interleaved`; values from rot_dim on are not turned. The angle
+ * keeps its fraction of a turn at any position (64 bits). The struct is read before the call returns; its pointers are
+ * device memory. The place of Backend::rope (include/krk/backend.hpp:1067) with a head norm before it. */
+struct krk_cuda_rope {
+    const void *pos;                  /* int32 [n_tok] */
+    const void *inv_freq;             /* f32 [rot_dim / 2]; NULL only with rot_dim 0 */
+    const void *q_weight, *k_weight;  /* f32 [head_dim] of the norm, NULL: all ones */
+    int64_t n_tok;
+    int64_t q_stride, k_stride;       /* floats from a token to the next, multiples of 4; heads follow each other */
+    int64_t q_out_stride, k_out_stride;
+    int n_heads, n_kv_heads;          /* n_kv_heads 0: no keys (k and k_out are not looked at) */
+    int head_dim, rot_dim;            /* multiples of 8, head_dim <= 256, rot_dim <= head_dim */
+    int norm, interleaved;            /* norm 0: the rotation alone */
+    float eps;
+};
+/* q_out / k_out may be q / k themselves (with the same stride), else they do not overlap them. 16-byte aligned. */
+int krk_cuda_qk_norm_rope(void *q_out_f32, void *k_out_f32, const void *q_f32, const void *k_f32, const struct krk_cuda_rope *host_rope,
+                          void *stream);
+
+/* A paged cache of keys and values. A page holds page_size positions of every key head:
+ * [n_pages][n_kv_heads][page_size][row], rows of head_dim values:
+ *   KV_F16  f16 (a finite value beyond its range saturates)
+ *   KV_Q8   one signed byte a value, d = f16(max|x| / 127), q = rint(x / d)
+ *   KV_Q4   m the value of largest magnitude (the positive one of equals), d = f16(m / -8), q = rint(x / d) + 8 in 0..15; byte j of a
+ *           block of 32 values has value j in its low and value j + 16 in its high half
+ * d of each block of 32 values is in [n_pages][n_kv_heads][page_size][head_dim / 32] f16 of its own (k_scale, v_scale; KV_F16: NULL).
+ * These are the values of Q8_0 and Q4_0 blocks, with rows that 16-byte copies can fetch. A block with an infinity or a NaN reads back as NaN. */
+#define KRK_CUDA_KV_F16 0
+#define KRK_CUDA_KV_Q8 1
+#define KRK_CUDA_KV_Q4 2
+struct krk_cuda_kv_cache {
+    void *k, *v, *k_scale, *v_scale;  /* device memory, 16-byte aligned */
+    int type, head_dim;               /* head_dim a multiple of 32, <= 256 */
+    int n_kv_heads, page_size;        /* page_size a multiple of 16 */
+    int64_t n_pages;
+};
+/* New keys and values [n_tok][n_kv_heads][head_dim] f32 (strides in floats from a token to the next, multiples of 4; 16-byte
+ * aligned) into positions slots[t] = page * page_size + place (int64). A token whose slot the cache does not have (-1, say) is
+ * left out; of tokens with the same slot the last one stays. The place of Backend::kv_append (include/krk/backend.hpp:1107). */
+int krk_cuda_kv_append(const struct krk_cuda_kv_cache *host_cache, const void *k_f32, const void *v_f32, int64_t k_stride, int64_t v_stride,
+                       const void *slots_i64, int64_t n_tok, void *stream);
+/* The rows of slots[i] as f32 [n][n_kv_heads][head_dim] (16-byte aligned); one that the cache does not have is a row of zeros. */
+int krk_cuda_kv_read(const struct krk_cuda_kv_cache *host_cache, void *k_f32, void *v_f32, const void *slots_i64, int64_t n, void *stream);
+
+/* Attention of the newest tokens of n_seq sequences over their cache, for a decode step (one token each) and for a tree of
+ * drafted tokens (up to KRK_CUDA_MAX_DRAFT each). Sequence s has rows q_start[s] .. q_start[s + 1] of q, at most max_q, and
+ * kv_len[s] positions, the last of which are those rows' own (already written). A row sees every position before them and, of
+ * them, the j-th where bit j of its mask is set (`tree` NULL: itself and those before it). Its own position is that of the first drafted
+ * token plus the bits of its mask, less one; with a window it sees, before the drafted tokens, the positions nearer than `window`.
+ *   out = sum_p w_p v_p / (sum_p w_p + exp(sink - max)),  w_p = exp(s_p - max),  s = scale * q . k  (softcap > 0: softcap tanh(s / softcap))
+ * A row that sees nothing, or only scores of -infinity, gives zeros. Query head h reads key head h / (n_heads / n_kv_heads). Position p of a sequence
+ * is place p % page_size of page page_table[s][p / page_size]; positions of a page that the cache does not have are not seen, and
+ * neither are those from max_kv_len on. Rows of out that no sequence has stay as they were. Infinities and NaN at positions
+ * that a row does not see do not reach it. The same call on the same device gives the same bits. The place of Backend::attention
+ * (include/krk/backend.hpp:1111). head_dim 64, 96, 128, 192 or 256. */
+#define KRK_CUDA_MAX_DRAFT 64
+struct krk_cuda_attention {
+    const void *q_start;              /* int32 [n_seq + 1] */
+    const void *kv_len;               /* int32 [n_seq] */
+    const void *page_table;           /* int32 [n_seq][table_width] */
+    const void *tree;                 /* uint64 [rows of q], or NULL */
+    const void *sinks;                /* f32 [n_heads], or NULL */
+    int64_t q_stride, out_stride;     /* floats from a token to the next, multiples of 4 */
+    int64_t max_kv_len;               /* of any sequence; 0: table_width * page_size */
+    int n_seq, n_heads, max_q, table_width;
+    int window;                       /* 0: none; else 64 or more */
+    float scale, softcap;
+};
+/* Bytes of workspace of such a call (0 for short contexts). They are scratch: nothing is kept there between calls, and calls
+ * that can overlap need one each. */
+size_t krk_cuda_attention_tree_workspace_bytes(const struct krk_cuda_kv_cache *host_cache, const struct krk_cuda_attention *host_attention);
+int krk_cuda_attention_tree(void *out_f32, const void *q_f32, const struct krk_cuda_kv_cache *host_cache,
+                            const struct krk_cuda_attention *host_attention, void *workspace, size_t ws_bytes, void *stream);
+
 /* ---- the steps either side of the output head ---- */
 
 /* Replaces Backend::embed (include/krk/backend.hpp:838; src/backend_cpu.cpp:746-778): out_f32[t] = decoded
@@ -276,6 +354,25 @@ size_t krk_cuda_logits_topk_workspace_bytes(int64_t n, int k);
 int krk_cuda_logits_topk(const void *logits_f32, int64_t n, int k, const void *pen_mask_u32, float rep_pen,
                          float softcap, float temp, void *ids_i32, void *vals_f32, void *mass_f32,
                          void *workspace, size_t ws_bytes, void *stream);
+
+/* Biases, penalties for repeated tokens and grammar masks on rows of f32 logits, before krk_cuda_logits_topk ranks them:
+ *   v = x + bias[id];  c > 0 times in the history:  v = v > 0 ? v / rep : v * rep (rep > 0),  v -= freq * c + pres;  not allowed: -infinity.
+ * hist: int32 [n_rows][hist_n], each row's first hist_len[row] ids (NULL: all); the same id may come many times. bias_ids / bias:
+ * [n_rows][bias_n], bias_len as hist_len; of an id that comes twice the last one holds. Ids outside the row (-1) are passed over. rep,
+ * freq, pres: f32 [n_rows], NULL: 1, 0, 0. mask: one bit a token, [n_masks][mask_stride] words, row r under mask mask_row[r] (NULL: r);
+ * a row whose number is none of them (-1) is not masked. Strides in elements. out may be logits. The struct is read before the
+ * call returns; its pointers are device memory, NULL where a part is not wanted. */
+struct krk_cuda_adjust {
+    int64_t n_rows, n_vocab, stride, out_stride;
+    const void *hist, *hist_len;
+    int64_t hist_n, hist_stride;
+    const void *rep, *freq, *pres;
+    const void *bias_ids, *bias, *bias_len;
+    int64_t bias_n, bias_stride;
+    const void *mask, *mask_row;
+    int64_t n_masks, mask_stride;
+};
+int krk_cuda_logits_adjust(void *out_f32, const void *logits_f32, const struct krk_cuda_adjust *host_adjust, void *stream);
 
 /* Expert-sharded FFN, exchange step: all-gather of partial sums over NVLink peer stores fused with the
  * rank-ordered sum that follows (no counterpart in the reference, which is single-device). part_f32

@@ -20,7 +20,8 @@ Q4_0, Q8_0, Q4_K, Q6_K = 2, 8, 12, 14
 Q5_0, Q5_1, Q5_K = 6, 7, 13
 Q2_K, Q3_K, IQ4_NL = 10, 11, 20
 X_F32, X_F16 = 0, 1
-MAX_GROUP, MAX_ROWS = 16, 8
+KV_F16, KV_Q8, KV_Q4 = 0, 1, 2
+MAX_GROUP, MAX_ROWS, MAX_DRAFT = 16, 8, 64
 
 
 class KrkCudaError(RuntimeError):
@@ -50,6 +51,33 @@ class ExpertBank(C.Structure):
     """struct krk_cuda_expert_bank"""
     _fields_ = [("gate", _vp), ("up", _vp), ("down", _vp), ("wt_gate_up", _int), ("wt_down", _int),
                 ("n_local", _int), ("expert_base", _int), ("n_embd", _i64), ("n_ff", _i64)]
+
+
+class KvCacheStruct(C.Structure):
+    """struct krk_cuda_kv_cache"""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("type", _int), ("head_dim", _int), ("n_kv_heads", _int),
+                ("page_size", _int), ("n_pages", _i64)]
+
+
+class Rope(C.Structure):
+    """struct krk_cuda_rope"""
+    _fields_ = [("pos", _vp), ("inv_freq", _vp), ("q_weight", _vp), ("k_weight", _vp), ("n_tok", _i64), ("q_stride", _i64), ("k_stride", _i64),
+                ("q_out_stride", _i64), ("k_out_stride", _i64), ("n_heads", _int), ("n_kv_heads", _int), ("head_dim", _int), ("rot_dim", _int),
+                ("norm", _int), ("interleaved", _int), ("eps", C.c_float)]
+
+
+class Attention(C.Structure):
+    """struct krk_cuda_attention"""
+    _fields_ = [("q_start", _vp), ("kv_len", _vp), ("page_table", _vp), ("tree", _vp), ("sinks", _vp), ("q_stride", _i64), ("out_stride", _i64),
+                ("max_kv_len", _i64), ("n_seq", _int), ("n_heads", _int), ("max_q", _int), ("table_width", _int), ("window", _int),
+                ("scale", C.c_float), ("softcap", C.c_float)]
+
+
+class Adjust(C.Structure):
+    """struct krk_cuda_adjust"""
+    _fields_ = [("n_rows", _i64), ("n_vocab", _i64), ("stride", _i64), ("out_stride", _i64), ("hist", _vp), ("hist_len", _vp), ("hist_n", _i64),
+                ("hist_stride", _i64), ("rep", _vp), ("freq", _vp), ("pres", _vp), ("bias_ids", _vp), ("bias", _vp), ("bias_len", _vp),
+                ("bias_n", _i64), ("bias_stride", _i64), ("mask", _vp), ("mask_row", _vp), ("n_masks", _i64), ("mask_stride", _i64)]
 
 
 # name -> (restype, argtypes); the list tests/ checks against the header.
@@ -91,6 +119,12 @@ SIGNATURES = {
     "krk_cuda_embed": (_int, [_vp, _vp, _int, _i64, _i64, _vp, _i64, _vp]),
     "krk_cuda_logits_topk_workspace_bytes": (_sz, [_i64, _int]),
     "krk_cuda_logits_topk": (_int, [_vp, _i64, _int, _vp, C.c_float, C.c_float, C.c_float, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "krk_cuda_qk_norm_rope": (_int, [_vp, _vp, _vp, _vp, C.POINTER(Rope), _vp]),
+    "krk_cuda_kv_append": (_int, [C.POINTER(KvCacheStruct), _vp, _vp, _i64, _i64, _vp, _i64, _vp]),
+    "krk_cuda_kv_read": (_int, [C.POINTER(KvCacheStruct), _vp, _vp, _vp, _i64, _vp]),
+    "krk_cuda_attention_tree_workspace_bytes": (_sz, [C.POINTER(KvCacheStruct), C.POINTER(Attention)]),
+    "krk_cuda_attention_tree": (_int, [_vp, _vp, C.POINTER(KvCacheStruct), C.POINTER(Attention), _vp, _sz, _vp]),
+    "krk_cuda_logits_adjust": (_int, [_vp, _vp, C.POINTER(Adjust), _vp]),
     "krk_cuda_allgather_sum": (_int, [C.POINTER(_vp), C.POINTER(_vp), _int, _int, _i64, _vp, _vp, _i64, _vp]),
     "krk_cuda_peer_alloc": (_int, [C.POINTER(_vp), C.c_size_t, C.c_char_p]),
     "krk_cuda_peer_open": (_int, [C.POINTER(_vp), C.c_char_p]),
@@ -351,6 +385,72 @@ def logits_topk(logits, k: int, pen_mask=None, rep_pen: float = 1.0, softcap: fl
                 want_mass: bool = True, workspace=None, stream=None):
     """Device top-k of one f32 logits row: (ids int32 [k], vals f32 [k], mass f32 [1] or None)."""
     return _fc.logits_topk(logits, k, pen_mask, rep_pen, softcap, temp, want_mass, workspace, stream)
+
+
+def logits_adjust(logits, hist=None, hist_len=None, rep=None, freq=None, pres=None, bias_ids=None, bias=None, mask=None, mask_row=None,
+                  bias_len=None, out=None, stream=None):
+    """Biases, penalties for repeated tokens and grammar masks on f32 logits [rows, vocab] (or one row), before logits_topk: hist int32
+    [rows, n] with hist_len int32 [rows]; rep / freq / pres f32 [rows]; bias_ids int32 and bias f32 [rows, n]; mask [masks, words] of
+    32 tokens (int32 or uint32), row r under mask mask_row[r] (-1: none). out may be logits."""
+    return _fc.logits_adjust(logits, hist, hist_len, rep, freq, pres, bias_ids, bias, mask, mask_row, bias_len, out, stream)
+
+
+def qk_norm_rope(q, k, pos, inv_freq, q_weight=None, k_weight=None, norm: bool = True, eps: float = 1e-6, interleaved: bool = False, q_out=None,
+                 k_out=None, stream=None):
+    """Norm of each head of q [tokens, heads, d] and k [tokens, kv heads, d] (or None), and the rotation of the first 2 * len(inv_freq)
+    values by pos (int32) * inv_freq, in one pass: (q', k'). norm=False: the rotation alone; inv_freq None: the norm alone."""
+    return _fc.qk_norm_rope(q, k, pos, inv_freq, q_weight, k_weight, norm, eps, interleaved, q_out, k_out, stream)
+
+
+class KvCache:
+    """A paged cache over tensors of its pages: k and v [pages, kv heads, page size, row], with rows of d f16 values (KV_F16), d int8
+    quants (KV_Q8) or d / 2 bytes (uint8) of 4-bit ones (KV_Q4), and scales f16 [pages, kv heads, page size, d / 32] for the last two."""
+
+    def __init__(self, kind: int, k, v, k_scale=None, v_scale=None):
+        dtype = {KV_F16: torch.float16, KV_Q8: torch.int8, KV_Q4: torch.uint8}[kind]
+        pages, heads, page_size, row = k.shape
+        d = 2 * row if kind == KV_Q4 else row
+        given = [(k, k.shape, dtype), (v, k.shape, dtype)]
+        if kind != KV_F16:
+            given += [(s, (pages, heads, page_size, d // 32), torch.float16) for s in (k_scale, v_scale)]
+        for t, shape, want in given:
+            if t is None or tuple(t.shape) != tuple(shape) or t.dtype != want or not t.is_contiguous() or t.device != k.device:
+                raise ValueError("a cache's tensors are contiguous, on one device, of the shapes and types of their kind")
+        self.kind, self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = kind, pages, heads, page_size, d
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.struct = KvCacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if kind != KV_F16 else 0, v_scale.data_ptr() if kind != KV_F16 else 0,
+                                    kind, d, heads, page_size, pages)
+        self.addr = C.addressof(self.struct)
+
+    @classmethod
+    def empty(cls, kind: int, n_pages: int, n_kv_heads: int, page_size: int, head_dim: int, device="cuda") -> "KvCache":
+        shape = (n_pages, n_kv_heads, page_size)
+
+        def one(width, dtype):
+            return torch.zeros((*shape, width), dtype=dtype, device=device)
+        if kind == KV_F16:
+            return cls(kind, one(head_dim, torch.float16), one(head_dim, torch.float16))
+        width, dtype = (head_dim, torch.int8) if kind == KV_Q8 else (head_dim // 2, torch.uint8)
+        return cls(kind, one(width, dtype), one(width, dtype), one(head_dim // 32, torch.float16), one(head_dim // 32, torch.float16))
+
+
+def kv_append(cache: KvCache, k, v, slots, stream=None) -> None:
+    """Writes k and v [tokens, kv heads, d] into positions slots (int64, page * page size + place; -1: left out) of the cache."""
+    _fc.kv_append(cache.addr, k, v, slots, stream)
+
+
+def kv_read(cache: KvCache, slots, k_out=None, v_out=None, stream=None):
+    """The rows of slots (int64) as f32: (k, v) [slots, kv heads, d]; a slot that the cache does not have gives zeros."""
+    return _fc.kv_read(cache.addr, slots, k_out, v_out, stream)
+
+
+def attention_tree(q, cache: KvCache, q_start, kv_len, page_table, max_q: int, tree=None, scale=None, softcap: float = 0.0, window: int = 0,
+                   sinks=None, max_kv_len: int = 0, out=None, workspace=None, stream=None):
+    """Attention of the newest tokens of each sequence over its cache. q f32 [rows, heads, d]: sequence s has rows q_start[s] ..
+    q_start[s + 1] (int32), at most max_q <= 64, which are the last of its kv_len[s] (int32) positions; position p is place p % page
+    size of page page_table[s][p // page size] (int32). tree (int64 / uint64 [rows]): bit j set where the row sees its sequence's j-th
+    row; None: itself and those before it. Returns out, f32 like q; rows that no sequence has are left as they were."""
+    return _fc.attention_tree(q, cache.addr, q_start, kv_len, page_table, max_q, tree, scale, softcap, window, sinks, max_kv_len, out, workspace, stream)
 
 
 def allgather_sum(gather_peer_ptrs, flag_peer_ptrs, my_rank: int, slot_stride: int, part, out, stream=None):

@@ -1,0 +1,11 @@
+// Attention over a cache of type F16: the kernel's instantiations.
+#include "krk_attn_kernel.cuh"
+
+namespace krk_cuda {
+
+int launch_attn_f16(const attn::Params &p, int head_dim, int tiles_of_rows, cudaStream_t st) {
+    return attn::launch_type<KRK_CUDA_KV_F16>(p, head_dim, tiles_of_rows, st);
+}
+int attn_ctas_f16(int head_dim, int tiles_of_rows) { return attn::ctas_of<KRK_CUDA_KV_F16>(head_dim, tiles_of_rows); }
+
+} // namespace krk_cuda

@@ -319,6 +319,14 @@ int launch_embed(float *out, const uint8_t *table, int wt, int64_t n_vocab, int6
 size_t logits_topk_workspace_bytes(int64_t n, int k);
 int launch_logits_topk(const float *logits, int64_t n, int k, const uint32_t *pen_mask, float rep_pen, float softcap,
                        float temp, int32_t *ids, float *vals, float *mass_out, void *workspace, cudaStream_t st);
+int launch_logits_adjust(float *out, const float *logits, const krk_cuda_adjust &a, cudaStream_t st);
+// Query and key heads, the paged cache (krk_kv.cu), attention over it (krk_attn_tree.cu).
+int launch_qk_norm_rope(float *q_out, float *k_out, const float *q, const float *k, const krk_cuda_rope &r, cudaStream_t st);
+int launch_kv_append(const krk_cuda_kv_cache &cache, const float *k, const float *v, int64_t k_stride, int64_t v_stride, const int64_t *slots,
+                     int64_t n, cudaStream_t st);
+int launch_kv_read(const krk_cuda_kv_cache &cache, float *k, float *v, const int64_t *slots, int64_t n, cudaStream_t st);
+size_t attention_tree_workspace_bytes(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a);
+int launch_attention_tree(float *out, const float *q, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, void *workspace, cudaStream_t st);
 int launch_route(int32_t *ids, float *wts, const float *logits, int64_t n_tok, int n_expert, int k,
                  cudaStream_t st);
 int launch_router_softmax(float *probs, const float *logits, int64_t n_rows, int n_expert, cudaStream_t st);

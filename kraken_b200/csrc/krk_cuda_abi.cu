@@ -409,6 +409,127 @@ int krk_cuda_logits_topk(const void *logits_f32, int64_t n, int k, const void *p
                               static_cast<float *>(mass_f32), workspace, static_cast<cudaStream_t>(stream));
 }
 
+static int check_cache(const krk_cuda_kv_cache *c) {
+    if (!c) return KRK_CUDA_ENULL;
+    if (c->type != KRK_CUDA_KV_F16 && c->type != KRK_CUDA_KV_Q8 && c->type != KRK_CUDA_KV_Q4) return KRK_CUDA_EDTYPE;
+    if (c->head_dim < 32 || c->head_dim > 256 || c->head_dim % 32 != 0 || c->n_kv_heads < 1 || c->n_kv_heads > 65536 || c->page_size < 16 ||
+        c->page_size % 16 != 0 || c->n_pages < 0 || c->n_pages > INT32_MAX)
+        return KRK_CUDA_ESHAPE;
+    if (c->n_pages > 0) {
+        if (!c->k || !c->v || (c->type != KRK_CUDA_KV_F16 && (!c->k_scale || !c->v_scale))) return KRK_CUDA_ENULL;
+        if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 16) || !aligned(c->v_scale, 16)) return KRK_CUDA_EALIGN;
+    }
+    return KRK_CUDA_OK;
+}
+
+int krk_cuda_qk_norm_rope(void *q_out_f32, void *k_out_f32, const void *q_f32, const void *k_f32, const krk_cuda_rope *r, void *stream) {
+    if (!r) return KRK_CUDA_ENULL;
+    if (r->n_tok < 0 || r->n_heads < 0 || r->n_kv_heads < 0 || (int64_t)r->n_heads + r->n_kv_heads > 65536 || r->head_dim < 8 || r->head_dim > 256 ||
+        r->head_dim % 8 != 0 || r->rot_dim < 0 || r->rot_dim > r->head_dim || r->rot_dim % 8 != 0)
+        return KRK_CUDA_ESHAPE;
+    if (r->n_tok == 0 || r->n_heads + r->n_kv_heads == 0) return KRK_CUDA_OK;
+    if (r->norm && !(r->eps >= 0.0f)) return KRK_CUDA_EARG;
+    if ((r->n_heads > 0 && (!q_f32 || !q_out_f32)) || (r->n_kv_heads > 0 && (!k_f32 || !k_out_f32)) || (r->rot_dim > 0 && (!r->pos || !r->inv_freq)))
+        return KRK_CUDA_ENULL;
+    const bool q = r->n_heads > 0, k = r->n_kv_heads > 0;
+    if (r->n_tok > 1 && ((q && (r->q_stride % 4 != 0 || r->q_out_stride % 4 != 0)) || (k && (r->k_stride % 4 != 0 || r->k_out_stride % 4 != 0)))) return KRK_CUDA_EALIGN;
+    if (r->n_tok > 1 && ((q && (r->q_stride < (int64_t)r->n_heads * r->head_dim || r->q_out_stride < (int64_t)r->n_heads * r->head_dim)) ||
+                         (k && (r->k_stride < (int64_t)r->n_kv_heads * r->head_dim || r->k_out_stride < (int64_t)r->n_kv_heads * r->head_dim))))
+        return KRK_CUDA_ESHAPE;
+    if ((q && (!aligned(q_f32, 16) || !aligned(q_out_f32, 16))) || (k && (!aligned(k_f32, 16) || !aligned(k_out_f32, 16))) ||
+        (r->norm && (!aligned(r->q_weight, 16) || !aligned(r->k_weight, 16))) || !aligned(r->pos, 4) || !aligned(r->inv_freq, 4))
+        return KRK_CUDA_EALIGN;
+    if (!device_state()) return KRK_CUDA_EDEVICE;
+    return launch_qk_norm_rope(static_cast<float *>(q_out_f32), static_cast<float *>(k_out_f32), static_cast<const float *>(q_f32),
+                               static_cast<const float *>(k_f32), *r, static_cast<cudaStream_t>(stream));
+}
+
+int krk_cuda_kv_append(const krk_cuda_kv_cache *cache, const void *k_f32, const void *v_f32, int64_t k_stride, int64_t v_stride,
+                       const void *slots_i64, int64_t n_tok, void *stream) {
+    const int rc = check_cache(cache);
+    if (rc != KRK_CUDA_OK) return rc;
+    if (n_tok < 0) return KRK_CUDA_ESHAPE;
+    if (n_tok == 0 || cache->n_pages == 0) return KRK_CUDA_OK;
+    if (!k_f32 || !v_f32 || !slots_i64) return KRK_CUDA_ENULL;
+    const int64_t row = (int64_t)cache->n_kv_heads * cache->head_dim;
+    if (n_tok > 1 && (k_stride < row || v_stride < row)) return KRK_CUDA_ESHAPE;
+    if (!aligned(k_f32, 16) || !aligned(v_f32, 16) || !aligned(slots_i64, 8) || (n_tok > 1 && (k_stride % 4 != 0 || v_stride % 4 != 0))) return KRK_CUDA_EALIGN;
+    if (!device_state()) return KRK_CUDA_EDEVICE;
+    return launch_kv_append(*cache, static_cast<const float *>(k_f32), static_cast<const float *>(v_f32), k_stride, v_stride,
+                            static_cast<const int64_t *>(slots_i64), n_tok, static_cast<cudaStream_t>(stream));
+}
+
+int krk_cuda_kv_read(const krk_cuda_kv_cache *cache, void *k_f32, void *v_f32, const void *slots_i64, int64_t n, void *stream) {
+    const int rc = check_cache(cache);
+    if (rc != KRK_CUDA_OK) return rc;
+    if (n < 0) return KRK_CUDA_ESHAPE;
+    if (n == 0) return KRK_CUDA_OK;
+    if (!k_f32 || !v_f32 || !slots_i64) return KRK_CUDA_ENULL;
+    if (!aligned(k_f32, 16) || !aligned(v_f32, 16) || !aligned(slots_i64, 8)) return KRK_CUDA_EALIGN;
+    if (!device_state()) return KRK_CUDA_EDEVICE;
+    return launch_kv_read(*cache, static_cast<float *>(k_f32), static_cast<float *>(v_f32), static_cast<const int64_t *>(slots_i64), n,
+                          static_cast<cudaStream_t>(stream));
+}
+
+// `a` with max_kv_len filled in.
+static int check_attention(const krk_cuda_kv_cache *cache, const krk_cuda_attention *from, krk_cuda_attention &a) {
+    const int rc = check_cache(cache);
+    if (rc != KRK_CUDA_OK) return rc;
+    if (!from) return KRK_CUDA_ENULL;
+    a = *from;
+    const int d = cache->head_dim;
+    if (d != 64 && d != 96 && d != 128 && d != 192 && d != 256) return KRK_CUDA_ESHAPE;
+    if (a.n_seq < 0 || a.n_heads < 1 || a.n_heads > 65536 || a.n_heads % cache->n_kv_heads != 0 || a.max_q < 0 || a.max_q > KRK_CUDA_MAX_DRAFT || a.table_width < 1 ||
+        a.max_kv_len < 0)
+        return KRK_CUDA_ESHAPE;
+    const int64_t room = (int64_t)a.table_width * cache->page_size;
+    if (a.max_kv_len == 0) a.max_kv_len = room;
+    if (a.max_kv_len > room || a.max_kv_len > (1ll << 30)) return KRK_CUDA_ESHAPE;
+    if (a.window < 0 || (a.window > 0 && a.window < KRK_CUDA_MAX_DRAFT) || !(a.softcap >= 0.0f)) return KRK_CUDA_EARG;
+    return KRK_CUDA_OK;
+}
+
+size_t krk_cuda_attention_tree_workspace_bytes(const krk_cuda_kv_cache *cache, const krk_cuda_attention *attention) {
+    krk_cuda_attention a;
+    if (check_attention(cache, attention, a) != KRK_CUDA_OK || a.n_seq == 0 || a.max_q == 0) return 0;
+    return attention_tree_workspace_bytes(*cache, a);
+}
+
+int krk_cuda_attention_tree(void *out_f32, const void *q_f32, const krk_cuda_kv_cache *cache, const krk_cuda_attention *attention,
+                            void *workspace, size_t ws_bytes, void *stream) {
+    krk_cuda_attention a;
+    const int rc = check_attention(cache, attention, a);
+    if (rc != KRK_CUDA_OK) return rc;
+    if (a.n_seq == 0 || a.max_q == 0) return KRK_CUDA_OK;
+    if (!out_f32 || !q_f32 || !a.q_start || !a.kv_len || !a.page_table) return KRK_CUDA_ENULL;
+    const int64_t row = (int64_t)a.n_heads * cache->head_dim;
+    if (a.q_stride < row || a.out_stride < row) return KRK_CUDA_ESHAPE;
+    if (!aligned(out_f32, 16) || !aligned(q_f32, 16) || a.q_stride % 4 != 0 || a.out_stride % 4 != 0 || !aligned(a.q_start, 4) || !aligned(a.kv_len, 4) ||
+        !aligned(a.page_table, 4) || !aligned(a.tree, 8) || !aligned(a.sinks, 4))
+        return KRK_CUDA_EALIGN;
+    if (!device_state()) return KRK_CUDA_EDEVICE;
+    const size_t need = attention_tree_workspace_bytes(*cache, a);
+    if (need > 0 && (!workspace || ws_bytes < need || !aligned(workspace, 16))) return KRK_CUDA_EWORKSPACE;
+    return launch_attention_tree(static_cast<float *>(out_f32), static_cast<const float *>(q_f32), *cache, a, workspace, static_cast<cudaStream_t>(stream));
+}
+
+int krk_cuda_logits_adjust(void *out_f32, const void *logits_f32, const krk_cuda_adjust *a, void *stream) {
+    if (!a) return KRK_CUDA_ENULL;
+    if (a->n_rows < 0 || a->n_vocab < 0 || a->n_vocab > INT32_MAX || a->hist_n < 0 || a->hist_n > INT32_MAX || a->bias_n < 0 || a->bias_n > INT32_MAX - 1 ||
+        a->n_masks < 0 || a->n_masks > INT32_MAX)
+        return KRK_CUDA_ESHAPE;
+    if (a->n_rows == 0 || a->n_vocab == 0) return KRK_CUDA_OK;
+    if (!out_f32 || !logits_f32 || (a->bias && !a->bias_ids)) return KRK_CUDA_ENULL;
+    if (a->n_rows > 1 && (a->stride < a->n_vocab || a->out_stride < a->n_vocab || (a->hist && a->hist_stride < a->hist_n) || (a->bias && a->bias_stride < a->bias_n)))
+        return KRK_CUDA_ESHAPE;
+    if (a->mask && a->mask_stride < (a->n_vocab + 31) / 32) return KRK_CUDA_ESHAPE;
+    const void *const lists[] = {out_f32, logits_f32, a->hist, a->hist_len, a->rep, a->freq, a->pres, a->bias_ids, a->bias, a->bias_len, a->mask, a->mask_row};
+    for (const void *p : lists)
+        if (!aligned(p, 4)) return KRK_CUDA_EALIGN;
+    if (!device_state()) return KRK_CUDA_EDEVICE;
+    return launch_logits_adjust(static_cast<float *>(out_f32), static_cast<const float *>(logits_f32), *a, static_cast<cudaStream_t>(stream));
+}
+
 int krk_cuda_allgather_sum(void *const host_gather_peers[], void *const host_flag_peers[], int n_peers, int my_rank,
                            int64_t slot_stride, const void *part_f32, void *out_f32, int64_t n, void *stream) {
     if (n_peers < 1 || n_peers > KRK_CUDA_MAX_PEERS || my_rank < 0 || my_rank >= n_peers) return KRK_CUDA_EARG;

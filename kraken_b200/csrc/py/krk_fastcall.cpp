@@ -8,10 +8,13 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <array>
+#include <cmath>
+#include <optional>
 
 #include "krk_cuda.h"
 
@@ -531,6 +534,244 @@ PyObject *backend_gemm_group(PyObject *, PyObject *const *a, Py_ssize_t n) {
     KRK_CATCH
 }
 
+// ---- query and key heads, the cache, attention, logits --------------------------------------------------------------
+// These look at what they are given: types, shapes and strides become sizes of the C call, so a wrong one is an error here.
+
+bool refuse(const char *what) {
+    PyErr_SetString(PyExc_ValueError, what);
+    return false;
+}
+// The device of the tensors, and the stream of the call, for as long as this lives; what is allocated meanwhile belongs to that stream.
+struct Where {
+    c10::cuda::CUDAGuard device;
+    std::optional<c10::cuda::CUDAStreamGuard> other;
+    void *stream;
+    Where(const at::Tensor &t, bool given, void *st) : device(t.device()) {
+        if (given) {
+            other.emplace(c10::cuda::getStreamFromExternal((cudaStream_t)st, t.device().index()));
+            stream = st;
+        } else {
+            stream = c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
+        }
+    }
+};
+bool on_device(const at::Tensor *t, const at::Tensor *first, const char *name) {
+    if (t->is_cuda() && t->device() == first->device()) return true;
+    PyErr_Format(PyExc_ValueError, "%s: not on the device of the first tensor, or not on a GPU", name);
+    return false;
+}
+bool typed(const at::Tensor *t, const at::Tensor *first, at::ScalarType type, const char *name) {
+    if (!on_device(t, first, name)) return false;
+    if (t->scalar_type() == type) return true;
+    PyErr_Format(PyExc_ValueError, "%s: expected %s", name, c10::toString(type));
+    return false;
+}
+// A list of n elements one behind the other (n < 0: of any number).
+bool listed(const at::Tensor *t, const at::Tensor *first, at::ScalarType type, int64_t n, const char *name) {
+    if (!t) return true;
+    if (!typed(t, first, type, name)) return false;
+    if (t->dim() == 1 && (n < 0 || t->numel() == n) && t->is_contiguous()) return true;
+    PyErr_Format(PyExc_ValueError, "%s: expected a contiguous list%s", name, n < 0 ? "" : " of as many elements as there are rows");
+    return false;
+}
+// f32 [rows][heads][d], heads behind each other; the stride of the rows is free.
+bool headed(const at::Tensor *t, const at::Tensor *first, int64_t rows, int64_t heads, int64_t d, const char *name) {
+    if (!typed(t, first, at::kFloat, name)) return false;
+    if (t->dim() == 3 && (rows < 0 || t->size(0) == rows) && (heads < 0 || t->size(1) == heads) && t->size(2) == d && (d <= 1 || t->stride(2) == 1) &&
+        (t->size(1) <= 1 || t->stride(1) == d))
+        return true;
+    PyErr_Format(PyExc_ValueError, "%s: expected [rows][heads][values] with the heads of a row behind each other", name);
+    return false;
+}
+// [rows][n], the elements of a row behind each other.
+bool tabled(const at::Tensor *t, const at::Tensor *first, at::ScalarType type, int64_t rows, const char *name) {
+    if (!t) return true;
+    if (!typed(t, first, type, name)) return false;
+    if (t->dim() == 2 && (rows < 0 || t->size(0) == rows) && (t->size(1) <= 1 || t->stride(1) == 1)) return true;
+    PyErr_Format(PyExc_ValueError, "%s: expected [rows][elements]", name);
+    return false;
+}
+PyObject *given_or_made(PyObject *given, const at::Tensor &made) {
+    if (given == Py_None) return THPVariable_Wrap(made);
+    Py_INCREF(given);
+    return given;
+}
+int64_t row_stride(const at::Tensor *t) { return t->size(0) > 1 ? t->stride(0) : t->dim() == 3 ? t->size(1) * t->size(2) : t->size(1); }
+
+// q, k, pos, inv_freq, q_weight, k_weight, norm, eps, interleaved, q_out, k_out, stream -> (q_out, k_out)
+PyObject *qk_norm_rope(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    KRK_NARGS(12, "qk_norm_rope")
+    KRK_TRY
+    Args g{a};
+    const at::Tensor *q = g.t(0), *k = g.t_or_none(1), *pos = g.t_or_none(2), *freq = g.t_or_none(3), *wq = g.t_or_none(4), *wk = g.t_or_none(5), *qo = g.t_or_none(9),
+                     *ko = g.t_or_none(10);
+    krk_cuda_rope r = {};
+    r.norm = g.b(6), r.eps = g.f(7), r.interleaved = g.b(8);
+    void *st = a[11] == Py_None ? nullptr : g.stream(11);
+    if (!g.ok) return nullptr;
+    if (q->dim() != 3) return refuse("q: expected [rows][heads][values]"), nullptr;
+    const int64_t rows = q->size(0), d = q->size(2);
+    if (!headed(q, q, rows, -1, d, "q") || (k && !headed(k, q, rows, -1, d, "k")) || !listed(freq, q, at::kFloat, -1, "inv_freq") ||
+        !listed(pos, q, at::kInt, rows, "pos") || !listed(wq, q, at::kFloat, d, "q_weight") || !listed(wk, q, at::kFloat, d, "k_weight"))
+        return nullptr;
+    Where where(*q, a[11] != Py_None, st);
+    at::Tensor made_q, made_k;
+    if (!qo) qo = &(made_q = empty_like_device(*q, {rows, q->size(1), d}, at::kFloat));
+    else if (!headed(qo, q, rows, q->size(1), d, "q_out")) return nullptr;
+    if (k && !ko) ko = &(made_k = empty_like_device(*q, {rows, k->size(1), d}, at::kFloat));
+    else if (k && !headed(ko, q, rows, k->size(1), d, "k_out")) return nullptr;
+    r.pos = pos ? Args::ptr(pos) : nullptr, r.inv_freq = freq ? Args::ptr(freq) : nullptr;
+    r.q_weight = Args::ptr(wq), r.k_weight = Args::ptr(wk);
+    r.n_tok = rows, r.n_heads = (int)q->size(1), r.n_kv_heads = k ? (int)k->size(1) : 0, r.head_dim = (int)d, r.rot_dim = freq ? (int)(2 * freq->numel()) : 0;
+    r.q_stride = row_stride(q), r.q_out_stride = row_stride(qo);
+    if (k) r.k_stride = row_stride(k), r.k_out_stride = row_stride(ko);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS rc = krk_cuda_qk_norm_rope(Args::ptr(qo), k ? Args::ptr(ko) : nullptr, Args::ptr(q), k ? Args::ptr(k) : nullptr, &r, where.stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return fail(rc, "qk_norm_rope");
+    PyObject *y = given_or_made(a[9], made_q), *z = k ? given_or_made(a[10], made_k) : Py_NewRef(Py_None);
+    PyObject *both = y && z ? PyTuple_Pack(2, y, z) : nullptr;
+    Py_XDECREF(y);
+    Py_XDECREF(z);
+    return both;
+    KRK_CATCH
+}
+
+PyObject *kv_append(PyObject *, PyObject *const *a, Py_ssize_t n) {   // cache, k, v, slots, stream
+    KRK_NARGS(5, "kv_append")
+    KRK_TRY
+    Args g{a};
+    const auto *c = (const krk_cuda_kv_cache *)g.addr(0);
+    const at::Tensor *k = g.t(1), *v = g.t(2), *slots = g.t(3);
+    void *st = a[4] == Py_None ? nullptr : g.stream(4);
+    if (!g.ok) return nullptr;
+    if (k->dim() != 3) return refuse("k: expected [rows][heads][values]"), nullptr;
+    const int64_t rows = k->size(0);
+    if (!headed(k, k, rows, c->n_kv_heads, c->head_dim, "k") || !headed(v, k, rows, c->n_kv_heads, c->head_dim, "v") || !listed(slots, k, at::kLong, rows, "slots")) return nullptr;
+    Where where(*k, a[4] != Py_None, st);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS rc = krk_cuda_kv_append(c, Args::ptr(k), Args::ptr(v), row_stride(k), row_stride(v), Args::ptr(slots), rows, where.stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return fail(rc, "kv_append");
+    Py_RETURN_NONE;
+    KRK_CATCH
+}
+
+PyObject *kv_read(PyObject *, PyObject *const *a, Py_ssize_t n) {   // cache, slots, k_out, v_out, stream -> (k, v)
+    KRK_NARGS(5, "kv_read")
+    KRK_TRY
+    Args g{a};
+    const auto *c = (const krk_cuda_kv_cache *)g.addr(0);
+    const at::Tensor *slots = g.t(1), *k = g.t_or_none(2), *v = g.t_or_none(3);
+    void *st = a[4] == Py_None ? nullptr : g.stream(4);
+    if (!g.ok || !listed(slots, slots, at::kLong, -1, "slots")) return nullptr;
+    const int64_t rows = slots->numel(), h = c->n_kv_heads, d = c->head_dim;
+    Where where(*slots, a[4] != Py_None, st);
+    at::Tensor made_k, made_v;
+    if (!k) k = &(made_k = empty_like_device(*slots, {rows, h, d}, at::kFloat));
+    if (!v) v = &(made_v = empty_like_device(*slots, {rows, h, d}, at::kFloat));
+    if (!headed(k, slots, rows, h, d, "k") || !headed(v, slots, rows, h, d, "v")) return nullptr;
+    if (!k->is_contiguous() || !v->is_contiguous()) return refuse("kv_read writes contiguous tensors"), nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS rc = krk_cuda_kv_read(c, Args::ptr(k), Args::ptr(v), Args::ptr(slots), rows, where.stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return fail(rc, "kv_read");
+    PyObject *y = given_or_made(a[2], made_k), *z = given_or_made(a[3], made_v);
+    PyObject *both = y && z ? PyTuple_Pack(2, y, z) : nullptr;
+    Py_XDECREF(y);
+    Py_XDECREF(z);
+    return both;
+    KRK_CATCH
+}
+
+// q, cache, q_start, kv_len, page_table, max_q, tree, scale, softcap, window, sinks, max_kv_len, out, workspace, stream -> out
+PyObject *attention_tree(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    KRK_NARGS(15, "attention_tree")
+    KRK_TRY
+    Args g{a};
+    const at::Tensor *q = g.t(0), *start = g.t(2), *len = g.t(3), *table = g.t(4), *tree = g.t_or_none(6), *sinks = g.t_or_none(10), *out = g.t_or_none(12), *ws = g.t_or_none(13);
+    const auto *c = (const krk_cuda_kv_cache *)g.addr(1);
+    krk_cuda_attention t = {};
+    const int64_t max_q = g.i(5), window = g.i(9);
+    t.max_kv_len = g.i(11), t.softcap = g.f(8);
+    if (a[7] != Py_None) t.scale = g.f(7);
+    void *st = a[14] == Py_None ? nullptr : g.stream(14);
+    if (!g.ok) return nullptr;
+    if (a[7] == Py_None) t.scale = 1.0f / std::sqrt((float)c->head_dim);
+    if (!headed(q, q, -1, -1, c->head_dim, "q") || !tabled(table, q, at::kInt, -1, "page_table")) return nullptr;
+    const int64_t rows = q->size(0), heads = q->size(1), n_seq = table->size(0);
+    if (!listed(start, q, at::kInt, n_seq + 1, "q_start") || !listed(len, q, at::kInt, n_seq, "kv_len") || !listed(sinks, q, at::kFloat, heads, "sinks")) return nullptr;
+    if (tree && !listed(tree, q, tree->scalar_type() == at::kUInt64 ? at::kUInt64 : at::kLong, rows, "tree")) return nullptr;
+    if (!table->is_contiguous()) return refuse("page_table: expected a contiguous table"), nullptr;
+    if (max_q < 0 || max_q > KRK_CUDA_MAX_DRAFT || window < 0 || window > INT32_MAX || heads > 65536 || table->size(1) > INT32_MAX)
+        return refuse("attention_tree: max_q, window, heads or pages out of range"), nullptr;
+    Where where(*q, a[14] != Py_None, st);
+    at::Tensor made, made_ws;
+    if (!out) out = &(made = empty_like_device(*q, {rows, heads, (int64_t)c->head_dim}, at::kFloat));
+    else if (!headed(out, q, rows, heads, c->head_dim, "out")) return nullptr;
+    t.q_start = Args::ptr(start), t.kv_len = Args::ptr(len), t.page_table = Args::ptr(table), t.tree = Args::ptr(tree), t.sinks = Args::ptr(sinks);
+    t.q_stride = row_stride(q), t.out_stride = row_stride(out);
+    t.n_seq = (int)n_seq, t.n_heads = (int)heads, t.max_q = (int)max_q, t.table_width = (int)table->size(1), t.window = (int)window;
+    if (ws) {
+        if (!typed(ws, q, at::kByte, "workspace")) return nullptr;
+        if (!ws->is_contiguous()) return refuse("workspace: expected contiguous bytes"), nullptr;
+    } else if (const size_t need = krk_cuda_attention_tree_workspace_bytes(c, &t)) {
+        ws = &(made_ws = empty_like_device(*q, {(int64_t)need}, at::kByte));
+    }
+    int rc;
+    Py_BEGIN_ALLOW_THREADS rc = krk_cuda_attention_tree(Args::ptr(out), Args::ptr(q), c, &t, Args::ptr(ws), ws ? (size_t)ws->numel() : 0, where.stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return fail(rc, "attention_tree");
+    return given_or_made(a[12], made);
+    KRK_CATCH
+}
+
+// logits, hist, hist_len, rep, freq, pres, bias_ids, bias, mask, mask_row, bias_len, out, stream -> out
+PyObject *logits_adjust(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    KRK_NARGS(13, "logits_adjust")
+    KRK_TRY
+    Args g{a};
+    const at::Tensor *x = g.t(0), *hist = g.t_or_none(1), *hist_len = g.t_or_none(2), *rep = g.t_or_none(3), *freq = g.t_or_none(4), *pres = g.t_or_none(5), *ids = g.t_or_none(6),
+                     *bias = g.t_or_none(7), *mask = g.t_or_none(8), *mask_row = g.t_or_none(9), *bias_len = g.t_or_none(10), *out = g.t_or_none(11);
+    void *st = a[12] == Py_None ? nullptr : g.stream(12);
+    if (!g.ok || !typed(x, x, at::kFloat, "logits")) return nullptr;
+    at::Tensor one;
+    const bool flat = x->dim() == 1;
+    if (flat) x = &(one = x->unsqueeze(0));
+    if (!tabled(x, x, at::kFloat, -1, "logits")) return nullptr;
+    const int64_t rows = x->size(0), vocab = x->size(1);
+    const at::ScalarType words = mask && mask->scalar_type() == at::kUInt32 ? at::kUInt32 : at::kInt;
+    if (!tabled(hist, x, at::kInt, rows, "hist") || !listed(hist_len, x, at::kInt, rows, "hist_len") || !listed(rep, x, at::kFloat, rows, "rep") ||
+        !listed(freq, x, at::kFloat, rows, "freq") || !listed(pres, x, at::kFloat, rows, "pres") || !tabled(ids, x, at::kInt, rows, "bias_ids") ||
+        !tabled(bias, x, at::kFloat, rows, "bias") || !listed(bias_len, x, at::kInt, rows, "bias_len") || !tabled(mask, x, words, -1, "mask") ||
+        !listed(mask_row, x, at::kInt, rows, "mask_row"))
+        return nullptr;
+    if ((bias == nullptr) != (ids == nullptr) || (bias && (bias->size(1) != ids->size(1) || (rows > 1 && bias->stride(0) != ids->stride(0)))))
+        return refuse("bias and bias_ids: expected two tables of one shape and layout"), nullptr;
+    Where where(*x, a[12] != Py_None, st);
+    at::Tensor made, out_one;
+    if (!out) {
+        made = flat ? empty_like_device(*x, {vocab}, at::kFloat) : empty_like_device(*x, {rows, vocab}, at::kFloat);
+        out = &made;
+    }
+    if (out->dim() == 1) out = &(out_one = out->unsqueeze(0));
+    if (!tabled(out, x, at::kFloat, rows, "out")) return nullptr;
+    if (out->size(1) != vocab) return refuse("out: expected the shape of logits"), nullptr;
+    krk_cuda_adjust j = {};
+    j.n_rows = rows, j.n_vocab = vocab, j.stride = row_stride(x), j.out_stride = row_stride(out);
+    j.hist = Args::ptr(hist), j.hist_len = Args::ptr(hist_len), j.rep = Args::ptr(rep), j.freq = Args::ptr(freq), j.pres = Args::ptr(pres);
+    j.bias_ids = Args::ptr(ids), j.bias = Args::ptr(bias), j.bias_len = Args::ptr(bias_len), j.mask = Args::ptr(mask), j.mask_row = Args::ptr(mask_row);
+    if (hist) j.hist_n = hist->size(1), j.hist_stride = row_stride(hist);
+    if (bias) j.bias_n = bias->size(1), j.bias_stride = row_stride(bias);
+    if (mask) j.n_masks = mask->size(0), j.mask_stride = row_stride(mask);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS rc = krk_cuda_logits_adjust(Args::ptr(out), Args::ptr(x), &j, where.stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return fail(rc, "logits_adjust");
+    return given_or_made(a[11], made);
+    KRK_CATCH
+}
+
 #define KRK_FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"set_raise", set_raise, METH_O, nullptr},
                          {"set_address", set_address, METH_O, nullptr},
@@ -540,6 +781,11 @@ PyMethodDef methods[] = {{"set_raise", set_raise, METH_O, nullptr},
                          KRK_FAST(silu_mul),
                          KRK_FAST(embed),
                          KRK_FAST(logits_topk),
+                         KRK_FAST(qk_norm_rope),
+                         KRK_FAST(kv_append),
+                         KRK_FAST(kv_read),
+                         KRK_FAST(attention_tree),
+                         KRK_FAST(logits_adjust),
                          KRK_FAST(moe_ffn),
                          KRK_FAST(moe_ffn_routed),
                          KRK_FAST(backend_upload),
