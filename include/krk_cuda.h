@@ -296,7 +296,7 @@ int krk_cuda_qk_norm_rope(void *q_out_f32, void *k_out_f32, const void *q_f32, c
 struct krk_cuda_kv_cache {
     void *k, *v, *k_scale, *v_scale;  /* device memory, 16-byte aligned */
     int type, head_dim;               /* head_dim a multiple of 32, <= 256 */
-    int n_kv_heads, page_size;        /* page_size a multiple of 16 */
+    int n_kv_heads, page_size;        /* up to 1024 heads; page_size a multiple of 16 */
     int64_t n_pages;
 };
 /* New keys and values [n_tok][n_kv_heads][head_dim] f32 (strides in floats from a token to the next, multiples of 4; 16-byte

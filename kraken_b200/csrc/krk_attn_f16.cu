@@ -3,9 +3,9 @@
 
 namespace krk_cuda {
 
-int launch_attn_f16(const attn::Params &p, int head_dim, int tiles_of_rows, cudaStream_t st) {
-    return attn::launch_type<KRK_CUDA_KV_F16>(p, head_dim, tiles_of_rows, st);
+int launch_attn_f16(const attn::Params &p, int head_dim, int rows, cudaStream_t st) {
+    return attn::launch_type<KRK_CUDA_KV_F16>(p, head_dim, rows, st);
 }
-int attn_ctas_f16(int head_dim, int tiles_of_rows) { return attn::ctas_of<KRK_CUDA_KV_F16>(head_dim, tiles_of_rows); }
+int attn_ctas_f16(int head_dim, int rows) { return attn::ctas_per_sm(KRK_CUDA_KV_F16, head_dim, rows); }
 
 } // namespace krk_cuda

@@ -5,66 +5,54 @@ namespace krk_cuda {
 namespace attn {
 namespace {
 
-// CTA (b, y): the item that CTA b - 1 of the first kernel began and CTA b went on with, if there is one; rows y, y + gridDim.y, ...
-// of it. Four warps take the parts in turn, in the order of the CTAs; their sums are added in the order of the warps.
-template <int D, int BM>
+// CTA (b, y): the item that CTA b of the first kernel went on with as the second one to have a part of it, if there is one; rows y,
+// y + gridDim.y, ... of it. Four warps take the parts in turn, in the order of the CTAs; their sums are added in the order of the warps.
+template <int D>
 __global__ void __launch_bounds__(kThreads)
-merge_kernel(const __grid_constant__ Params p) {
+merge_kernel(const __grid_constant__ Params p, int r_block) {
     constexpr int NB = D / 32;
     __shared__ float s_sum[kWarps][D];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int b = blockIdx.x + 1;
-    const Place place = find_place<BM>(p, b);
-    if (place.at >= place.total) return;
-    const Seq sq = sequence<BM>(p, place.seq);
-    const int64_t in_seq = place.at - place.before;
-    const int per_item = item_units(p, sq), item = (int)(in_seq / per_item);
-    // the item's tiles, as units
-    const int64_t first = place.at - (in_seq - (int64_t)item * per_item) + kSetup, item_end = first + sq.tiles;
-    const int64_t prev = first_unit(place.total, p.grid, b - 1);
-    if (place.at <= first || prev == place.at || prev > first) return;
-    // CTAs b .. last - 1 went on with the item: those that begin before its end
-    const int last = (int)min((int64_t)p.grid, (item_end * p.grid + place.total - 1) / place.total);
-    const int parts = last - b + 1;
-    const bool all_there = place.total >= p.grid;
-    const int kvh = item / sq.blocks, block = item - kvh * sq.blocks;
-    const int n_rows = min(BM, sq.n_q * p.group - block * BM);
-    for (int r = blockIdx.y; r < n_rows; r += gridDim.y) {
-        // part i: CTA b - 1 + i; a CTA without units has none
-        auto part = [&](int i) -> const float * { return part_row<D, BM>(p, b - 1 + i, i == 0 ? 1 : 0, r); };
-        auto there = [&](int i) { return all_there || first_unit(place.total, p.grid, b - 1 + i) < first_unit(place.total, p.grid, b + i); };
-        float top = -INFINITY, all = 0.0f;
-        for (int i = lane; i < parts; i += 32)
-            if (there(i)) top = fmaxf(top, part(i)[D]);
+    const Shared it = p.shared[b];
+    if (it.parts == 0) return;
+    const size_t pitch = (size_t)2 * r_block * (D + 2);   // from a CTA's parts to the next one's
+    for (int r = blockIdx.y; r < it.n_rows; r += gridDim.y) {
+        // part 0: CTA b - 1, place 1; part i: CTA b - 1 + i, place 0
+        const float *first = p.part + (size_t)(b - 1) * pitch + (size_t)(r_block + r) * (D + 2), *others = p.part + (size_t)(b - 1) * pitch + (size_t)r * (D + 2);
+        auto part = [&](int i) { return i == 0 ? first : others + i * pitch; };
+        float2 ml = lane < it.parts ? *reinterpret_cast<const float2 *>(part(lane) + D) : make_float2(-INFINITY, 0.0f);
+        for (int i = lane + 32; i < it.parts; i += 32) {
+            const float2 more = *reinterpret_cast<const float2 *>(part(i) + D);
+            const float top = fmaxf(ml.x, more.x);
+            ml.y = (ml.x == -INFINITY ? 0.0f : ml.y * exp2f(ml.x - top)) + (more.x == -INFINITY ? 0.0f : more.y * exp2f(more.x - top));
+            ml.x = top;
+        }
+        float top = ml.x;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        for (int i = lane; i < parts; i += 32)
-            if (there(i)) {
-                const float2 ml = *reinterpret_cast<const float2 *>(part(i) + D);
-                if (ml.x != -INFINITY) all += ml.y * exp2f(ml.x - top);
-            }
+        float all = ml.x == -INFINITY ? 0.0f : ml.y * exp2f(ml.x - top);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xFFFFFFFFu, all, o);
         float x[NB];
 #pragma unroll
         for (int j = 0; j < NB; j++) x[j] = 0.0f;
 #pragma unroll 4
-        for (int i = warp; i < parts; i += kWarps) {
-            if (!there(i)) continue;
-            const float *from_part = part(i);
-            const float m = from_part[D], f = m == -INFINITY ? 0.0f : exp2f(m - top);
+        for (int i = warp; i < it.parts; i += kWarps) {
+            const float *from = part(i);
+            const float m = from[D], f = m == -INFINITY ? 0.0f : exp2f(m - top);
 #pragma unroll
-            for (int j = 0; j < NB; j++) x[j] += f * from_part[32 * j + lane];
+            for (int j = 0; j < NB; j++) x[j] += f * from[32 * j + lane];
         }
 #pragma unroll
         for (int j = 0; j < NB; j++) s_sum[warp][32 * j + lane] = x[j];
         __syncthreads();
-        const int rr = block * BM + r, head = kvh * p.group + rr % p.group;
+        const int rr = it.row0 + r, head = it.kvh * p.group + rr % p.group;
         float keep;
         const float f = norm_of(p, head, top, all, keep);
-        float *to = p.out + (int64_t)(sq.q0 + rr / p.group) * p.out_stride + head * D;
+        float *to = p.out + (int64_t)(it.q0 + rr / p.group) * p.out_stride + head * D;
         for (int c = tid; c < D; c += kThreads) {
             float sum = s_sum[0][c];
 #pragma unroll
@@ -75,37 +63,26 @@ merge_kernel(const __grid_constant__ Params p) {
     }
 }
 
-template <int D, int BM>
-int merge_one(const Params &p, int rows, cudaStream_t st) {
-    return launched(launch_overlapped(merge_kernel<D, BM>, dim3((unsigned)(p.grid - 1), (unsigned)(rows < 8 ? rows : 8)), dim3(kThreads), st, p));
-}
-
-int launch_merge(const Params &p, int d, int mt, int rows, cudaStream_t st) {
-    switch (d) {
-    case 64: return mt == 2 ? merge_one<64, 32>(p, rows, st) : merge_one<64, 16>(p, rows, st);
-    case 96: return mt == 2 ? merge_one<96, 32>(p, rows, st) : merge_one<96, 16>(p, rows, st);
-    case 128: return mt == 2 ? merge_one<128, 32>(p, rows, st) : merge_one<128, 16>(p, rows, st);
-    case 192: return merge_one<192, 16>(p, rows, st);
-    default: return merge_one<256, 16>(p, rows, st);
-    }
+int launch_merge(const Params &p, int d, int r_block, int rows, cudaStream_t st) {
+    auto kernel = d == 64 ? merge_kernel<64> : d == 96 ? merge_kernel<96> : d == 128 ? merge_kernel<128> : d == 192 ? merge_kernel<192> : merge_kernel<256>;
+    return launched(launch_overlapped(kernel, dim3((unsigned)(p.grid - 1), (unsigned)(rows < 8 ? rows : 8)), dim3(kThreads), st, p, r_block));
 }
 
 struct Form {
-    int mt, grid, rows, whole;   // row tiles of a block, CTAs, rows of an item at most, items not divided
+    int block, grid, rows, whole;   // rows of a block, CTAs, rows of an item at most, items not divided
 };
 Form form_of(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a) {
     Form f;
     const int type = cache.type, d = cache.head_dim;
     const int64_t rows = (int64_t)a.max_q * (a.n_heads / cache.n_kv_heads);
-    f.mt = rows > 16 && d <= 128 ? 2 : 1;
-    const int bm = 16 * f.mt;
-    f.rows = (int)(rows < bm ? rows : bm);
+    f.block = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 || d > 128 ? 16 : 32;
+    f.rows = (int)(rows < f.block ? rows : f.block);
     const int64_t tiles = (a.max_kv_len + kTile - 1) / kTile;
     // Short contexts: a CTA walks a whole item, which costs less than the second kernel.
     f.whole = tiles <= kWholeTiles;
-    const int64_t items = (int64_t)a.n_seq * cache.n_kv_heads * ((rows + bm - 1) / bm);
+    const int64_t items = (int64_t)a.n_seq * cache.n_kv_heads * ((rows + f.block - 1) / f.block);
     const int64_t units = f.whole ? items : items * (tiles + kSetup);
-    const int ctas = type == KRK_CUDA_KV_F16 ? attn_ctas_f16(d, f.mt) : type == KRK_CUDA_KV_Q8 ? attn_ctas_q8(d, f.mt) : attn_ctas_q4(d, f.mt);
+    const int ctas = type == KRK_CUDA_KV_F16 ? attn_ctas_f16(d, f.block) : type == KRK_CUDA_KV_Q8 ? attn_ctas_q8(d, f.block) : attn_ctas_q4(d, f.block);
     const int64_t fill = (int64_t)ctas * sm_count();
     f.grid = (int)(units < fill ? units : fill);
     return f;
@@ -116,7 +93,7 @@ Form form_of(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a) {
 
 size_t attention_tree_workspace_bytes(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a) {
     const attn::Form f = attn::form_of(cache, a);
-    return f.whole ? 0 : (size_t)f.grid * 2 * 16 * f.mt * (cache.head_dim + 2) * sizeof(float);
+    return f.whole ? 0 : attn::shared_bytes(f.grid) + (size_t)f.grid * 2 * f.block * (cache.head_dim + 2) * sizeof(float);
 }
 
 int launch_attention_tree(float *out, const float *q, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, void *workspace, cudaStream_t st) {
@@ -135,7 +112,8 @@ int launch_attention_tree(float *out, const float *q, const krk_cuda_kv_cache &c
     p.kv_len = static_cast<const int32_t *>(a.kv_len);
     p.tree = static_cast<const uint64_t *>(a.tree);
     p.sinks = static_cast<const float *>(a.sinks);
-    p.part = static_cast<float *>(workspace);
+    p.shared = static_cast<attn::Shared *>(workspace);
+    p.part = f.whole ? nullptr : reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + attn::shared_bytes(f.grid));
     p.n_pages = cache.n_pages;
     p.table_width = a.table_width;
     p.page_size = cache.page_size;
@@ -150,9 +128,9 @@ int launch_attention_tree(float *out, const float *q, const krk_cuda_kv_cache &c
     p.grid = f.grid;
     p.scale = a.scale;
     p.softcap = a.softcap;
-    int rc = cache.type == KRK_CUDA_KV_F16 ? launch_attn_f16(p, cache.head_dim, f.mt, st)
-             : cache.type == KRK_CUDA_KV_Q8 ? launch_attn_q8(p, cache.head_dim, f.mt, st) : launch_attn_q4(p, cache.head_dim, f.mt, st);
-    if (rc == KRK_CUDA_OK && !f.whole && f.grid > 1) rc = attn::launch_merge(p, cache.head_dim, f.mt, f.rows, st);
+    int rc = cache.type == KRK_CUDA_KV_F16 ? launch_attn_f16(p, cache.head_dim, f.block, st)
+             : cache.type == KRK_CUDA_KV_Q8 ? launch_attn_q8(p, cache.head_dim, f.block, st) : launch_attn_q4(p, cache.head_dim, f.block, st);
+    if (rc == KRK_CUDA_OK && !f.whole && f.grid > 1) rc = attn::launch_merge(p, cache.head_dim, f.block, f.rows, st);
     return rc;
 }
 

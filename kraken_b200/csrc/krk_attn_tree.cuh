@@ -20,6 +20,13 @@ constexpr int kTile = kChunk * kWarps;    // positions the warps of a CTA take t
 constexpr int kSetup = 3;                 // what an item costs beside its tiles, in tiles (queries, joining the warps' sums, latencies)
 constexpr int kWholeTiles = 8;            // up to so many tiles an item is not divided, see launch
 
+// An item that several CTAs have parts of, noted by the second one of them: parts 0 elsewhere.
+struct Shared {
+    int parts, n_rows, kvh, row0;   // row0: of the item's first row among its key head's
+    int q0, pad[3];
+};
+inline size_t shared_bytes(int grid) { return (size_t)grid * sizeof(Shared); }
+
 struct Params {
     const float *q;
     float *out;
@@ -30,29 +37,30 @@ struct Params {
     const int32_t *q_start, *kv_len;
     const uint64_t *tree;
     const float *sinks;
-    float *part;                          // [grid][2][BM][D + 2]: see part_row
+    Shared *shared;                       // [grid]
+    float *part;                          // [grid][2][R][D + 2]: see part_row
     int64_t n_pages;
     int table_width, page_size, max_len, n_seq, n_heads, n_kv, group, max_q, window, whole, grid;
     float scale, softcap;
 };
 
-// The work, in the order of its units: sequences, their key heads, blocks of BM rows, tiles of positions. A unit is a tile, and each
+// The work, in the order of its units: sequences, their key heads, blocks of R rows, tiles of positions. A unit is a tile, and each
 // item, all tiles of a block of rows, has kSetup more at its beginning (without them a CTA whose share was 40 items of one tile
 // took four times as long as the others); or, where items are not divided (Params::whole), a unit is an item. The CTAs take equal shares of
 // the units, whatever the lengths are, so at most a CTA's first and last items are shared with others; those leave partial
-// sums, which a second kernel adds up in the order of the CTAs (the same bits every time).
+// sums, which a second kernel adds up in the order of the CTAs (the same bits every time; finding the items anew in that kernel took it 14 to 24 us).
 struct Seq {
     int q0, n_q, len, before;   // first row of q, drafted tokens, positions, positions before the drafted ones (may be negative)
     int blocks, tile0, tiles;   // blocks of rows; first tile that any row sees, tiles from there on (at least one where there are rows)
 };
-template <int BM>
+template <int R>
 __device__ __forceinline__ Seq sequence(const Params &p, int s) {
     Seq q;
     q.q0 = p.q_start[s];
     q.n_q = min(max(p.q_start[s + 1] - q.q0, 0), p.max_q);
     q.len = min(max(p.kv_len[s], 0), p.max_len);
     q.before = q.len - q.n_q;
-    q.blocks = (q.n_q * p.group + BM - 1) / BM;
+    q.blocks = (q.n_q * p.group + R - 1) / R;
     const int first = p.window > 0 ? max(0, q.before - p.window) : 0;   // (the shallowest row is at `before`, or a position less where its mask is empty)
     q.tile0 = min(first, max(q.len - 1, 0)) / kTile;
     q.tiles = max(1, (q.len + kTile - 1) / kTile - q.tile0);
@@ -62,15 +70,15 @@ __device__ __forceinline__ int item_units(const Params &p, const Seq &q) { retur
 __device__ __forceinline__ int64_t units_of(const Params &p, const Seq &q) { return (int64_t)p.n_kv * q.blocks * item_units(p, q); }
 
 // Units [first(b), first(b + 1)) are CTA b's.
-__device__ __forceinline__ int64_t first_unit(int64_t total, int grid, int b) { return total * b / grid; }
+__device__ __forceinline__ int64_t first_unit(int64_t total, int grid, int b) { return total * min(b, grid) / grid; }
 
-// By a whole CTA of 128 threads: the number of all units, and the sequence that unit first_unit(total, grid, b) lies in (n_seq where it
-// lies behind the last one) with the units before that sequence.
+// By a whole CTA of 128 threads: the number of all units, the CTAs that share them (no more than there are units, so that each has some),
+// and the sequence that CTA b's first one lies in (n_seq where it has none) with the units before that sequence.
 struct Place {
     int64_t total, at, before;
-    int seq;
+    int grid, seq;
 };
-template <int BM>
+template <int R>
 __device__ __forceinline__ Place find_place(const Params &p, int b) {
     __shared__ int64_t s_sum[kWarps];
     __shared__ int64_t s_before;
@@ -81,7 +89,7 @@ __device__ __forceinline__ Place find_place(const Params &p, int b) {
     int64_t lo = 0, mine = 0;   // of this thread's sequence of the last 128
     auto scan = [&](int s0, int64_t base) {
         const int s = s0 + tid;
-        mine = s < p.n_seq ? units_of(p, sequence<BM>(p, s)) : 0;
+        mine = s < p.n_seq ? units_of(p, sequence<R>(p, s)) : 0;
         int64_t upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -101,7 +109,8 @@ __device__ __forceinline__ Place find_place(const Params &p, int b) {
         return all;
     };
     for (int s0 = 0; s0 < p.n_seq; s0 += kThreads) r.total += scan(s0, r.total);
-    r.at = first_unit(r.total, p.grid, b);
+    r.grid = (int)max(min((int64_t)p.grid, r.total), (int64_t)1);
+    r.at = first_unit(r.total, r.grid, b);
     if (tid == 0) {
         s_found = p.n_seq;
         s_before = r.total;
@@ -123,9 +132,9 @@ __device__ __forceinline__ Place find_place(const Params &p, int b) {
 
 // Rows of partial sums of CTA b: place 0 its first item's, where that began before the CTA; place 1 its last item's, where that
 // goes on behind it and place 0 is not it. A row: D sums, the maximum (log2 domain), the sum of weights.
-template <int D, int BM>
+template <int D, int R>
 __device__ __forceinline__ float *part_row(const Params &p, int b, int place, int row) {
-    return p.part + (((size_t)b * 2 + place) * BM + row) * (D + 2);
+    return p.part + (((size_t)b * 2 + place) * R + row) * (D + 2);
 }
 
 // out = sums / weights, with the sink's weight among the latter. Nothing seen: zero.
@@ -142,12 +151,12 @@ __device__ __forceinline__ float norm_of(const Params &p, int head, float m, flo
 
 }   // namespace attn
 
-int launch_attn_f16(const attn::Params &p, int head_dim, int tiles_of_rows, cudaStream_t st);
-int launch_attn_q8(const attn::Params &p, int head_dim, int tiles_of_rows, cudaStream_t st);
-int launch_attn_q4(const attn::Params &p, int head_dim, int tiles_of_rows, cudaStream_t st);
+int launch_attn_f16(const attn::Params &p, int head_dim, int rows, cudaStream_t st);
+int launch_attn_q8(const attn::Params &p, int head_dim, int rows, cudaStream_t st);
+int launch_attn_q4(const attn::Params &p, int head_dim, int rows, cudaStream_t st);
 // CTAs that an SM holds at once
-int attn_ctas_f16(int head_dim, int tiles_of_rows);
-int attn_ctas_q8(int head_dim, int tiles_of_rows);
-int attn_ctas_q4(int head_dim, int tiles_of_rows);
+int attn_ctas_f16(int head_dim, int rows);
+int attn_ctas_q8(int head_dim, int rows);
+int attn_ctas_q4(int head_dim, int rows);
 
 }   // namespace krk_cuda

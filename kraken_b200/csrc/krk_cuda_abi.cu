@@ -412,7 +412,7 @@ int krk_cuda_logits_topk(const void *logits_f32, int64_t n, int k, const void *p
 static int check_cache(const krk_cuda_kv_cache *c) {
     if (!c) return KRK_CUDA_ENULL;
     if (c->type != KRK_CUDA_KV_F16 && c->type != KRK_CUDA_KV_Q8 && c->type != KRK_CUDA_KV_Q4) return KRK_CUDA_EDTYPE;
-    if (c->head_dim < 32 || c->head_dim > 256 || c->head_dim % 32 != 0 || c->n_kv_heads < 1 || c->n_kv_heads > 65536 || c->page_size < 16 ||
+    if (c->head_dim < 32 || c->head_dim > 256 || c->head_dim % 32 != 0 || c->n_kv_heads < 1 || c->n_kv_heads > 1024 || c->page_size < 16 ||
         c->page_size % 16 != 0 || c->n_pages < 0 || c->n_pages > INT32_MAX)
         return KRK_CUDA_ESHAPE;
     if (c->n_pages > 0) {
@@ -515,7 +515,7 @@ int krk_cuda_attention_tree(void *out_f32, const void *q_f32, const krk_cuda_kv_
 
 int krk_cuda_logits_adjust(void *out_f32, const void *logits_f32, const krk_cuda_adjust *a, void *stream) {
     if (!a) return KRK_CUDA_ENULL;
-    if (a->n_rows < 0 || a->n_vocab < 0 || a->n_vocab > INT32_MAX || a->hist_n < 0 || a->hist_n > INT32_MAX || a->bias_n < 0 || a->bias_n > INT32_MAX - 1 ||
+    if (a->n_rows < 0 || a->n_vocab < 0 || a->n_vocab > (1ll << 30) || a->hist_n < 0 || a->hist_n > INT32_MAX || a->bias_n < 0 || a->bias_n > INT32_MAX - 1 ||
         a->n_masks < 0 || a->n_masks > INT32_MAX)
         return KRK_CUDA_ESHAPE;
     if (a->n_rows == 0 || a->n_vocab == 0) return KRK_CUDA_OK;

@@ -2,6 +2,8 @@
 // are written into in f16, 8 or 4 bits a value, and read back out of.
 #include "krk_common.cuh"
 
+#include <algorithm>
+
 namespace krk_cuda {
 
 namespace {
@@ -22,15 +24,17 @@ struct RopeParams {
     const int32_t *pos;
     const float *inv_freq;
     int64_t n_tok;
-    int heads[2], d, rot, interleaved, norm, chunks;
+    int heads[2], d, rot, norm, chunks;
     float eps;
 };
 
 __device__ __forceinline__ float4 ld4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
 __device__ __forceinline__ void st4(float *p, const float v[4]) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
 
-template <int L>
-__global__ void __launch_bounds__(256)
+constexpr int kRopeHeads = 2;
+
+template <int L, bool INTERLEAVED>
+__global__ void __launch_bounds__(256, 4)
 qk_norm_rope_kernel(const __grid_constant__ RopeParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int j = threadIdx.x % L, pairs = p.rot / 8, half = p.rot / 2;
@@ -39,9 +43,27 @@ qk_norm_rope_kernel(const __grid_constant__ RopeParams p) {
     const int chunk = (int)(group - tok * p.chunks), all = p.heads[0] + p.heads[1];
     const bool mine = tok < p.n_tok && 8 * j < p.d, turns = j < pairs;
     // first values of the lane's two runs of four
-    const int a0 = !turns ? p.rot + 8 * (j - pairs) : p.interleaved ? 8 * j : 4 * j, b0 = turns && !p.interleaved ? half + 4 * j : a0 + 4;
-    float cs[4], sn[4];
+    const int a0 = !turns ? p.rot + 8 * (j - pairs) : INTERLEAVED ? 8 * j : 4 * j, b0 = turns && !INTERLEAVED ? half + 4 * j : a0 + 4;
+    // heads in equal runs, kRopeHeads at a time: the next ones' values are on their way while some are worked on
+    const int h0 = (int)((int64_t)all * chunk / p.chunks), h1 = (int)((int64_t)all * (chunk + 1) / p.chunks);
+    auto load = [&](int hb, float (&v)[kRopeHeads][8]) {
+#pragma unroll
+        for (int u = 0; u < kRopeHeads; u++) {
+            const int h = hb + u, which = h >= p.heads[0], head = h - (which ? p.heads[0] : 0);
+            const float *x = p.x[which] + tok * p.x_stride[which] + head * p.d;
+            if (mine && h < h1) {
+                const float4 a = ld4(x + a0), b = ld4(x + b0);
+                v[u][0] = a.x, v[u][1] = a.y, v[u][2] = a.z, v[u][3] = a.w, v[u][4] = b.x, v[u][5] = b.y, v[u][6] = b.z, v[u][7] = b.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[u][i] = 0.0f;
+            }
+        }
+    };
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    float v[kRopeHeads][8], next[kRopeHeads][8];
+    load(h0, next);
+    float cs[4], sn[4];
     if (mine && turns) {
         const double at = (double)p.pos[tok] * 0.15915494309189535;   // turns per unit of frequency
 #pragma unroll
@@ -50,44 +72,53 @@ qk_norm_rope_kernel(const __grid_constant__ RopeParams p) {
             sincospif((float)(2.0 * (turn - rint(turn))), &sn[i], &cs[i]);
         }
     }
-    // heads in equal runs
-    const int h0 = (int)((int64_t)all * chunk / p.chunks), h1 = (int)((int64_t)all * (chunk + 1) / p.chunks);
-#pragma unroll 2
-    for (int h = h0; h < h1; h++) {
-        const int which = h >= p.heads[0], head = h - (which ? p.heads[0] : 0);
-        const float *x = p.x[which] + tok * p.x_stride[which] + (int64_t)head * p.d;
-        float v[8] = {};
-        if (mine) {
-            const float4 a = ld4(x + a0), b = ld4(x + b0);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        }
+    for (int hb = h0; hb < h1; hb += kRopeHeads) {
+#pragma unroll
+        for (int u = 0; u < kRopeHeads; u++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[u][i] = next[u][i];
+        load(hb + kRopeHeads, next);
         if (p.norm) {
-            float sum = 0.0f;
+            float sum[kRopeHeads];
 #pragma unroll
-            for (int i = 0; i < 8; i++) sum += v[i] * v[i];
+            for (int u = 0; u < kRopeHeads; u++) {
+                sum[u] = 0.0f;
 #pragma unroll
-            for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-            const float r = 1.0f / sqrtf(sum / (float)p.d + p.eps);
+                for (int i = 0; i < 8; i++) sum[u] += v[u][i] * v[u][i];
+            }
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] *= r;
-            if (mine && p.w[which]) {
-                const float4 a = ld4(p.w[which] + a0), b = ld4(p.w[which] + b0);
-                v[0] *= a.x, v[1] *= a.y, v[2] *= a.z, v[3] *= a.w, v[4] *= b.x, v[5] *= b.y, v[6] *= b.z, v[7] *= b.w;
+            for (int o = L / 2; o > 0; o >>= 1)
+#pragma unroll
+                for (int u = 0; u < kRopeHeads; u++) sum[u] += __shfl_xor_sync(0xFFFFFFFFu, sum[u], o);
+#pragma unroll
+            for (int u = 0; u < kRopeHeads; u++) {
+                const int which = hb + u >= p.heads[0];
+                const float r = 1.0f / sqrtf(sum[u] / (float)p.d + p.eps);
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[u][i] *= r;
+                if (mine && p.w[which]) {
+                    const float4 a = ld4(p.w[which] + a0), b = ld4(p.w[which] + b0);
+                    v[u][0] *= a.x, v[u][1] *= a.y, v[u][2] *= a.z, v[u][3] *= a.w, v[u][4] *= b.x, v[u][5] *= b.y, v[u][6] *= b.z, v[u][7] *= b.w;
+                }
             }
         }
-        if (!mine) continue;
-        if (turns) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float &a = v[p.interleaved ? 2 * i : i], &b = v[p.interleaved ? 2 * i + 1 : i + 4];
-                const float u = a * cs[i] - b * sn[i];
-                b = b * cs[i] + a * sn[i];
-                a = u;
+        for (int u = 0; u < kRopeHeads; u++) {
+            const int h = hb + u, which = h >= p.heads[0], head = h - (which ? p.heads[0] : 0);
+            if (!mine || h >= h1) continue;
+            if (turns) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float &a = INTERLEAVED ? v[u][2 * i] : v[u][i], &b = INTERLEAVED ? v[u][2 * i + 1] : v[u][i + 4];
+                    const float z = a * cs[i] - b * sn[i];
+                    b = b * cs[i] + a * sn[i];
+                    a = z;
+                }
             }
+            float *y = p.y[which] + tok * p.y_stride[which] + head * p.d;
+            st4(y + a0, v[u]);
+            st4(y + b0, v[u] + 4);
         }
-        float *y = p.y[which] + tok * p.y_stride[which] + (int64_t)head * p.d;
-        st4(y + a0, v);
-        st4(y + b0, v + 4);
     }
 }
 
@@ -102,138 +133,197 @@ struct CacheParams {
     const int64_t *slots;
     int64_t n, n_slots;
     int heads, d, page_size, per_block;
+    uint32_t of_row_inv, of_tok_inv;   // see part
 };
+constexpr int kMostTokens = 32;   // of a block of threads
 
-// Where a row of the pools lies: (page, head, slot of the page).
-__device__ __forceinline__ int64_t pool_row(const CacheParams &p, int64_t slot, int head) {
-    const int64_t page = slot / p.page_size;
-    return (page * p.heads + head) * p.page_size + (slot - page * p.page_size);
+// u / by for u * by < 2^32, inv = ceil(2^32 / by): u inv / 2^32 is too large by less than u / 2^32, and a quotient's distance to the next whole
+// number is at least 1 / by.
+__device__ __forceinline__ int part(int u, uint32_t inv) { return (int)__umulhi((uint32_t)u, inv); }
+
+// Where the rows of a block's tokens lie: row of the pools of head 0 (heads are page_size rows apart), or -1. Dividing by the page size takes
+// longer than what is done with eight values, so a token's slot is looked at once.
+__device__ __forceinline__ void find_rows(const CacheParams &p, int64_t t0, int n_tok, int64_t *rows) {
+    if ((int)threadIdx.x < n_tok) {
+        const int64_t slot = p.slots[t0 + threadIdx.x];
+        const int64_t page = slot / p.page_size;
+        rows[threadIdx.x] = slot < 0 || slot >= p.n_slots ? -1 : page * p.heads * p.page_size + (slot - page * p.page_size);
+    }
 }
 
 // Append: reads x once, writes the rows. A lane has eight values, four lanes a block of 32, whose largest value is two
 // shuffles. Of tokens with the same slot the last one stays: a block of threads looks through the slots behind its tokens while its
-// first values are on their way (from 1184 tokens on, a block has more than one token, which share the look).
+// first values are on their way (a block's tokens share the look).
 template <int CT>
 __global__ void __launch_bounds__(256)
 kv_append_kernel(const __grid_constant__ CacheParams p) {
-    constexpr int kMost = 32;
-    __shared__ int64_t s_slot[kMost];
-    __shared__ int s_drop[kMost];
+    __shared__ int64_t s_slot[kMostTokens], s_row[kMostTokens];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, of_row = p.d / 8, of_tok = 2 * p.heads * of_row;
     const int64_t t0 = (int64_t)blockIdx.x * p.per_block;
     const int n_tok = (int)min((int64_t)p.per_block, p.n - t0), total = n_tok * of_tok;
+    struct Unit {
+        int tok, kv, head, c;
+    };
+    auto unit = [&](int u) {
+        Unit w;
+        w.tok = part(u, p.of_tok_inv);
+        const int in_tok = u - w.tok * of_tok;
+        w.kv = in_tok >= of_tok / 2;
+        const int at = in_tok - (w.kv ? of_tok / 2 : 0);
+        w.head = part(at, p.of_row_inv);
+        w.c = at - w.head * of_row;
+        return w;
+    };
     auto load = [&](int u, float x[8]) {
         if (u >= total) return;
-        const int tok = u / of_tok, in_tok = u - tok * of_tok, kv = in_tok >= of_tok / 2, at = in_tok - (kv ? of_tok / 2 : 0);
-        const float *from = p.x[kv] + (t0 + tok) * p.x_stride[kv] + 8 * at;
+        const Unit w = unit(u);
+        const float *from = p.x[w.kv] + (t0 + w.tok) * p.x_stride[w.kv] + w.head * p.d + 8 * w.c;
         const float4 a = ld4(from), b = ld4(from + 4);
         x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
     };
     float x[8] = {};
     load(tid, x);
-    if (tid < n_tok) {
-        const int64_t slot = p.slots[t0 + tid];
-        s_slot[tid] = slot;
-        s_drop[tid] = slot < 0 || slot >= p.n_slots;
-    }
+    if (tid < n_tok) s_slot[tid] = p.slots[t0 + tid];
+    find_rows(p, t0, n_tok, s_row);
     __syncthreads();
     for (int64_t j = t0 + 1 + tid; j < p.n; j += 256) {
         const int64_t slot = p.slots[j];
         for (int i = 0; i < n_tok; i++)
-            if (slot == s_slot[i] && t0 + i < j) s_drop[i] = 1;
+            if (slot == s_slot[i] && t0 + i < j) s_row[i] = -1;
     }
     __syncthreads();
     for (int base = 0; base < total; base += 256) {
+        float next[8] = {};
+        load(base + 256 + tid, next);
         const int u = base + tid;
-        if (base) load(u, x);
-        const int uu = min(u, total - 1), tok = uu / of_tok, in_tok = uu - tok * of_tok, kv = in_tok >= of_tok / 2, at = in_tok - (kv ? of_tok / 2 : 0);
-        const int head = at / of_row, c = at - head * of_row;
-        const bool keep = u < total && !s_drop[tok];
-        const int64_t row = keep ? pool_row(p, s_slot[tok], head) : 0;
+        const Unit w = unit(min(u, total - 1));
+        const int c = w.c, kv = w.kv;
+        const bool keep = u < total && s_row[w.tok] >= 0;
+        const int64_t row = keep ? s_row[w.tok] + w.head * p.page_size : 0;
         if constexpr (CT == KRK_CUDA_KV_F16) {
             __half2 h[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) h[i] = __halves2half2(half_sat(x[2 * i]), half_sat(x[2 * i + 1]));
             if (keep) *reinterpret_cast<uint4 *>(p.pool[kv] + (row * p.d + 8 * c) * 2) = *reinterpret_cast<uint4 *>(h);
         } else {
-            float hi = x[0], lo = x[0];
-            bool odd = false;
+            float hi = x[0], lo = x[0], all = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 hi = fmaxf(hi, x[i]);
                 lo = fminf(lo, x[i]);
-                odd |= !(fabsf(x[i]) <= 3.4028234e38f);
+                all = fmaf(x[i], 0.0f, all);   // (NaN where an infinity or a NaN is)
             }
 #pragma unroll
             for (int o = 1; o < 4; o <<= 1) {
                 hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
                 lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
-                odd |= __shfl_xor_sync(0xFFFFFFFFu, odd, o);
+                all += __shfl_xor_sync(0xFFFFFFFFu, all, o);
             }
             // a block that holds an infinity or a NaN reads back as NaN
             constexpr bool k8 = CT == KRK_CUDA_KV_Q8;
+            const bool odd = all != all;
             const __half dh = odd ? __ushort_as_half(0x7FFF) : half_sat(__fdiv_rn(k8 ? fmaxf(hi, -lo) : hi >= -lo ? hi : lo, k8 ? 127.0f : -8.0f));
-            const float d = __half2float(dh);
-            uint32_t w[2] = {};
+            const float d = __half2float(dh), inv = 1.0f / d;
+            const bool none = d == 0.0f || odd;
+            // rint(x / d) as x / d rounds to f32: the product with the reciprocal is off by less than 2^-21 of up to 128, so only quotients that
+            // near to a half are divided (and those of a scale that ran out of bits)
+            float r[8];
+            bool near = false;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float r = d == 0.0f || odd ? 0.0f : rintf(__fdiv_rn(x[i], d));
-                if constexpr (k8)
-                    w[i >> 2] |= ((uint32_t)(int)fminf(fmaxf(r, -127.0f), 127.0f) & 255u) << (8 * (i & 3));
-                else
-                    w[i >> 2] |= (uint32_t)(int)(fminf(fmaxf(r, -8.0f), 7.0f) + 8.0f) << (8 * (i & 3));
+                const float q = x[i] * inv;
+                r[i] = rintf(q);
+                near |= !(fabsf(q - r[i]) < 0.499f) || !(fabsf(q) < 256.0f);
+            }
+            if (near) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) r[i] = none ? 0.0f : rintf(__fdiv_rn(x[i], d));
+            }
+            uint32_t b[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                uint32_t u[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {   // a whole number in the low bits of 1.5 * 2^23 more
+                    const float f = k8 ? fminf(fmaxf(r[4 * i + j], -127.0f), 127.0f) : fminf(fmaxf(r[4 * i + j], -8.0f), 7.0f);
+                    u[j] = __float_as_uint(f + (k8 ? 12582912.0f : 12582920.0f));
+                }
+                b[i] = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
             }
             if constexpr (k8) {
-                if (keep) *reinterpret_cast<uint2 *>(p.pool[kv] + row * p.d + 8 * c) = make_uint2(w[0], w[1]);
+                if (keep) *reinterpret_cast<uint2 *>(p.pool[kv] + row * p.d + 8 * c) = make_uint2(b[0], b[1]);
             } else {
                 // values 16 .. 31 of a block (lanes 2, 3 of its four) are the high halves of the bytes of values 0 .. 15
-                const uint32_t h0 = __shfl_down_sync(0xFFFFFFFFu, w[0], 2), h1 = __shfl_down_sync(0xFFFFFFFFu, w[1], 2);
-                if (keep && (c & 3) < 2) *reinterpret_cast<uint2 *>(p.pool[kv] + row * (p.d / 2) + 16 * (c >> 2) + 8 * (c & 3)) = make_uint2(w[0] | h0 << 4, w[1] | h1 << 4);
+                const uint32_t h0 = __shfl_down_sync(0xFFFFFFFFu, b[0], 2), h1 = __shfl_down_sync(0xFFFFFFFFu, b[1], 2);
+                if (keep && (c & 3) < 2) *reinterpret_cast<uint2 *>(p.pool[kv] + row * (p.d / 2) + 16 * (c >> 2) + 8 * (c & 3)) = make_uint2(b[0] | h0 << 4, b[1] | h1 << 4);
             }
             if (keep && (c & 3) == 0) p.scale[kv][row * (p.d / 32) + (c >> 2)] = dh;
         }
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = next[i];
     }
 }
 
-// Read: the rows of the slots as f32; a slot that the cache does not have is a row of zeros. A lane has eight values.
+// Read: the rows of the slots as f32; a slot that the cache does not have is a row of zeros. A lane has four values of a row of keys and
+// of the row of values (eight, written 32 bytes apart, wrote each sector of level 2 twice), of several rows at a time.
 template <int CT>
 __global__ void __launch_bounds__(256)
 kv_read_kernel(const __grid_constant__ CacheParams p) {
+    __shared__ int64_t s_row[kMostTokens];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int of_row = p.d / 8, of_tok = p.heads * of_row;
-    const int64_t total = 2 * p.n * of_tok;
-    for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += (int64_t)gridDim.x * 256) {
-        const int64_t tk = u / of_tok, tok = tk >> 1;
-        const int kv = (int)(tk & 1), at = (int)(u - tk * of_tok), head = at / of_row, c = at - head * of_row;
-        const int64_t slot = p.slots[tok];
-        float x[8] = {};
-        if (slot >= 0 && slot < p.n_slots) {
-            const int64_t row = pool_row(p, slot, head);
-            if constexpr (CT == KRK_CUDA_KV_F16) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(p.pool[kv] + (row * p.d + 8 * c) * 2);
-                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    const int tid = threadIdx.x, of_row = p.d / 4, of_tok = p.heads * of_row;
+    const int64_t t0 = (int64_t)blockIdx.x * p.per_block;
+    const int n_tok = (int)min((int64_t)p.per_block, p.n - t0), total = n_tok * of_tok;
+    find_rows(p, t0, n_tok, s_row);
+    __syncthreads();
+    constexpr int kAt = 2;
+    for (int base = 0; base < total; base += kAt * 256) {
+        uint2 w[kAt][2];
+        float d[kAt][2];
+        int where[kAt];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&ws[i]));
-                    x[2 * i] = f.x, x[2 * i + 1] = f.y;
-                }
-            } else {
-                const float d = __half2float(p.scale[kv][row * (p.d / 32) + (c >> 2)]);
-                const uint2 w = CT == KRK_CUDA_KV_Q8 ? *reinterpret_cast<const uint2 *>(p.pool[kv] + row * p.d + 8 * c)
-                                                     : *reinterpret_cast<const uint2 *>(p.pool[kv] + row * (p.d / 2) + 16 * (c >> 2) + 8 * (c & 1));
+        for (int k = 0; k < kAt; k++) {
+            const int u = min(base + k * 256 + tid, total - 1), tok = part(u, p.of_tok_inv), at = u - tok * of_tok, head = part(at, p.of_row_inv), c = at - head * of_row;
+            const int64_t first = s_row[tok], row = first + head * p.page_size;
+            where[k] = first < 0 ? -1 : c;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const uint32_t byte = (i < 4 ? w.x : w.y) >> (8 * (i & 3)) & 255u;
-                    x[i] = __fmul_rn(d, CT == KRK_CUDA_KV_Q8 ? (float)(int8_t)byte : (float)((int)((c & 2) ? byte >> 4 : byte & 15u) - 8));
+            for (int kv = 0; kv < 2; kv++) {
+                w[k][kv] = make_uint2(0u, 0u);
+                d[k][kv] = 0.0f;
+                if (first < 0) continue;
+                if constexpr (CT == KRK_CUDA_KV_F16) {
+                    w[k][kv] = *reinterpret_cast<const uint2 *>(p.pool[kv] + (row * p.d + 4 * c) * 2);
+                } else {
+                    w[k][kv].x = *reinterpret_cast<const uint32_t *>(CT == KRK_CUDA_KV_Q8 ? p.pool[kv] + row * p.d + 4 * c : p.pool[kv] + row * (p.d / 2) + 16 * (c >> 3) + 4 * (c & 3));
+                    d[k][kv] = __half2float(p.scale[kv][row * (p.d / 32) + (c >> 3)]);
                 }
             }
         }
-        float *to = p.y[kv] + tok * (int64_t)of_tok * 8 + 8 * at;
-        st4(to, x);
-        st4(to + 4, x + 4);
+#pragma unroll
+        for (int k = 0; k < kAt; k++) {
+            const int u = base + k * 256 + tid;
+            if (u >= total) continue;
+#pragma unroll
+            for (int kv = 0; kv < 2; kv++) {
+                float x[4] = {};
+                if (where[k] >= 0) {
+                    if constexpr (CT == KRK_CUDA_KV_F16) {
+                        const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&w[k][kv].x)), f1 = __half22float2(*reinterpret_cast<const __half2 *>(&w[k][kv].y));
+                        x[0] = f0.x, x[1] = f0.y, x[2] = f1.x, x[3] = f1.y;
+                    } else {
+                        // a byte under the exponent of 2^23 is 2^23 more than its value
+                        const uint32_t q = CT == KRK_CUDA_KV_Q8 ? w[k][kv].x ^ 0x80808080u : ((where[k] & 4) ? w[k][kv].x >> 4 : w[k][kv].x) & 0x0F0F0F0Fu;
+                        const float off = CT == KRK_CUDA_KV_Q8 ? 8388608.0f + 128.0f : 8388608.0f + 8.0f;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) x[i] = __fmul_rn(d[k][kv], __fsub_rn(__uint_as_float(__byte_perm(q, 0x4B000000u, 0x7650u | i)), off));
+                    }
+                }
+                st4(p.y[kv] + (t0 * of_tok + u) * 4, x);   // (a token's rows follow each other)
+            }
+        }
     }
 }
 
@@ -251,6 +341,13 @@ CacheParams cache_params(const krk_cuda_kv_cache &cache, const int64_t *slots, i
     p.page_size = cache.page_size;
     return p;
 }
+// Tokens of a block: a block for each up to `blocks` blocks an SM, then equal shares, as far as part() divides.
+void set_per_block(CacheParams &p, int blocks, int of_head, int values) {
+    const int64_t of_row = p.d / values, of_tok = of_head * p.heads * of_row, per = p.n / (blocks * (int64_t)sm_count()), most = 0xFFFFFFFFll / (of_tok * of_tok);
+    p.per_block = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(per, most), kMostTokens));
+    p.of_row_inv = (uint32_t)((0x100000000ll + of_row - 1) / of_row);
+    p.of_tok_inv = (uint32_t)((0x100000000ll + of_tok - 1) / of_tok);
+}
 
 #define KRK_DISPATCH_KV(type, kernel) \
     ((type) == KRK_CUDA_KV_F16 ? kernel<KRK_CUDA_KV_F16> : (type) == KRK_CUDA_KV_Q8 ? kernel<KRK_CUDA_KV_Q8> : kernel<KRK_CUDA_KV_Q4>)
@@ -266,15 +363,16 @@ int launch_qk_norm_rope(float *q_out, float *k_out, const float *q, const float 
     p.inv_freq = static_cast<const float *>(r.inv_freq);
     p.n_tok = r.n_tok;
     p.heads[0] = r.n_heads, p.heads[1] = r.n_kv_heads;
-    p.d = r.head_dim, p.rot = r.rot_dim, p.interleaved = r.interleaved, p.norm = r.norm;
+    p.d = r.head_dim, p.rot = r.rot_dim, p.norm = r.norm;
     p.eps = r.eps;
     const int lanes = r.head_dim <= 64 ? 8 : r.head_dim <= 128 ? 16 : 32, all = r.n_heads + r.n_kv_heads;
-    // Groups for about 1024 threads an SM, each with as many heads of a token as that leaves; a head each for few tokens.
-    const int64_t groups = (int64_t)sm_count() * 1024 / lanes, want = (groups + r.n_tok - 1) / r.n_tok;
-    p.chunks = (int)(want < all ? want : all);
+    // At most as many groups as run at once, 1024 threads an SM, each with as many heads of a token as that leaves; a head each for few tokens.
+    const int64_t groups = (int64_t)sm_count() * 1024 / lanes, want = groups / r.n_tok;
+    p.chunks = (int)(want < 1 ? 1 : want < all ? want : all);
     const int64_t blocks = (r.n_tok * p.chunks + 256 / lanes - 1) / (256 / lanes);
     if (blocks > INT32_MAX) return KRK_CUDA_ESHAPE;
-    auto kernel = lanes == 8 ? qk_norm_rope_kernel<8> : lanes == 16 ? qk_norm_rope_kernel<16> : qk_norm_rope_kernel<32>;
+    auto kernel = r.interleaved ? (lanes == 8 ? qk_norm_rope_kernel<8, true> : lanes == 16 ? qk_norm_rope_kernel<16, true> : qk_norm_rope_kernel<32, true>)
+                                : (lanes == 8 ? qk_norm_rope_kernel<8, false> : lanes == 16 ? qk_norm_rope_kernel<16, false> : qk_norm_rope_kernel<32, false>);
     return launched(launch_overlapped(kernel, dim3((unsigned)blocks), dim3(256), st, p));
 }
 
@@ -282,8 +380,7 @@ int launch_kv_append(const krk_cuda_kv_cache &cache, const float *k, const float
     CacheParams p = cache_params(cache, slots, n);
     p.x[0] = k, p.x[1] = v;
     p.x_stride[0] = k_stride, p.x_stride[1] = v_stride;
-    const int64_t per = n / (8 * (int64_t)sm_count());
-    p.per_block = (int)(per < 1 ? 1 : per > 32 ? 32 : per);
+    set_per_block(p, 4, 2, 8);
     const int64_t blocks = (n + p.per_block - 1) / p.per_block;
     if (blocks > INT32_MAX) return KRK_CUDA_ESHAPE;
     return launched(launch_overlapped(KRK_DISPATCH_KV(cache.type, kv_append_kernel), dim3((unsigned)blocks), dim3(256), st, p));
@@ -292,8 +389,10 @@ int launch_kv_append(const krk_cuda_kv_cache &cache, const float *k, const float
 int launch_kv_read(const krk_cuda_kv_cache &cache, float *k, float *v, const int64_t *slots, int64_t n, cudaStream_t st) {
     CacheParams p = cache_params(cache, slots, n);
     p.y[0] = k, p.y[1] = v;
-    const int64_t want = (2 * n * cache.n_kv_heads * (cache.head_dim / 8) + 255) / 256, fill = (int64_t)sm_count() * 16;
-    return launched(launch_overlapped(KRK_DISPATCH_KV(cache.type, kv_read_kernel), dim3((unsigned)(want < fill ? want : fill)), dim3(256), st, p));
+    set_per_block(p, 16, 1, 4);
+    const int64_t blocks = (n + p.per_block - 1) / p.per_block;
+    if (blocks > INT32_MAX) return KRK_CUDA_ESHAPE;
+    return launched(launch_overlapped(KRK_DISPATCH_KV(cache.type, kv_read_kernel), dim3((unsigned)blocks), dim3(256), st, p));
 }
 
 } // namespace krk_cuda
