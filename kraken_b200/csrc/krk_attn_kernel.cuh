@@ -115,6 +115,8 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// The soft limit of a score, in the log2 domain.
+static __device__ __noinline__ float capped(float x, float cap) { return cap * 1.44269504f * tanhf(x / cap); }
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 half2_of(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
 // Two f32 as the sum of two f16 each.
@@ -198,48 +200,18 @@ attn_kernel(const __grid_constant__ Params p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    const Place place = find_place<R>(p, blockIdx.x);
-    int64_t at = place.at;
-    const int64_t end = first_unit(place.total, place.grid, blockIdx.x + 1);
+    Walk<R> walk;
+    walk.start(p);
     if (!p.whole && tid == 0) p.shared[blockIdx.x].parts = 0;
-    if (at >= end) return;
-    int s = place.seq;
-    int64_t in_seq = at - place.before;
-    Seq sq = sequence<R>(p, s);
     const uint32_t ring = smem_addr(smem) + warp * S::kRing * S::kStage;
     uint8_t *ring_mem = smem + warp * S::kRing * S::kStage;
     int64_t *stage_rows = reinterpret_cast<int64_t *>(warp_ml + kWarps * R) + warp * S::kRing;   // the pool's row that a stage begins with
 
-    while (at < end) {
-        while (in_seq >= units_of(p, sq)) {   // (sequences without drafted tokens have no units)
-            in_seq -= units_of(p, sq);
-            sq = sequence<R>(p, ++s);
-        }
-        const int per_item = item_units(p, sq);
-        const int item = (int)(in_seq / per_item), from_unit = (int)(in_seq - (int64_t)item * per_item);
-        const int units = (int)min((int64_t)(per_item - from_unit), end - at);
-        // units to tiles: the first kSetup units of an item stand for what it costs beside its tiles
-        const int from = p.whole ? 0 : max(from_unit - kSetup, 0), upto = p.whole ? sq.tiles : from_unit + units - kSetup;
-        const int64_t item_at = at - from_unit;   // (the item's first unit)
-        at += units;
-        in_seq += units;
-        if (upto <= from) continue;
-        const bool begins = from == 0, ends = upto == sq.tiles;
-        const int kvh = item / sq.blocks, block = item - kvh * sq.blocks;
-        const int tile0 = sq.tile0 + from, tile1 = sq.tile0 + upto;
-        const int n_rows = min(R, sq.n_q * p.group - block * R), n_tiles = (n_rows + 7) / 8;
-
-        if (from > 0 && tid == 0 && first_unit(place.total, place.grid, blockIdx.x - 1) <= item_at + kSetup) {
-            // the second part of the item: the CTAs from the one before this to the last one that begins before the item's end have the parts
-            Shared it;
-            it.parts = (int)min((int64_t)place.grid, ((item_at + per_item) * place.grid + place.total - 1) / place.total) - blockIdx.x + 1;
-            it.n_rows = n_rows;
-            it.kvh = kvh;
-            it.row0 = block * R;
-            it.q0 = sq.q0;
-            it.pad[0] = it.pad[1] = it.pad[2] = 0;
-            p.shared[blockIdx.x] = it;
-        }
+    while (walk.next(p)) {
+        const Seq &sq = walk.sq;
+        const int s = walk.s, kvh = walk.kvh, block = walk.block, n_rows = walk.n_rows, n_tiles = (n_rows + 7) / 8, tile0 = walk.tile0, tile1 = tile0 + walk.tiles;
+        const bool begins = walk.begins, ends = walk.ends;
+        if (walk.parts > 0 && tid == 0) walk.note(p);
 
         // ---- pages of this warp's chunks: lane l holds that of the l-th from the last refill on, as a row of the pool
         const int chunk0 = tile0 * kWarps + warp, n_chunks = tile1 - tile0;
@@ -508,52 +480,78 @@ attn_kernel(const __grid_constant__ Params p) {
                     }
                 }
 
-                // ---- weights
-    #pragma unroll
-                for (int n = 0; n < NA; n++) {
-                    float base[NC], corr[NC];
-                    bool higher = e_corr != 1.0f;
-    #pragma unroll
-                    for (int c = 0; c < NC; c++) {
-    #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            sc[n][h][c] *= row_scale[n][c];
-                            if (p.softcap > 0.0f) sc[n][h][c] = p.softcap * 1.44269504f * tanhf(sc[n][h][c] / p.softcap);
-                            if (masked && !sees(row_of(n, c), pos0 + g + 8 * h)) sc[n][h][c] = -INFINITY;
-                        }
-                        base[c] = fmaxf(sc[n][0][c], sc[n][1][c]);
-                    }
-    #pragma unroll
-                    for (int o2 = 4; o2 < 32; o2 <<= 1)
-    #pragma unroll
-                        for (int c = 0; c < NC; c++) base[c] = fmaxf(base[c], __shfl_xor_sync(0xFFFFFFFFu, base[c], o2));
-    #pragma unroll
-                    for (int c = 0; c < NC; c++) {
-                        const float top = fmaxf(base[c], m[n][c]);
-                        higher |= top > m[n][c];
-                        base[c] = top == -INFINITY ? 0.0f : top;
-                        corr[c] = ex2(m[n][c] - base[c]);
-                        m[n][c] = top;
-                    }
-                    if (__any_sync(0xFFFFFFFFu, higher)) {
-    #pragma unroll
+                // ---- weights. (What is rarely done has loops of its own: in one with the rest, each value's code was jumped over, and fetching
+                // the instructions behind it took half of the time.)
+#pragma unroll
+                for (int n = 0; n < NA; n++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int c = 0; c < NC; c++) sc[n][h][c] *= row_scale[n][c];
+                if (p.softcap > 0.0f) {
+#pragma unroll
+                    for (int n = 0; n < NA; n++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+#pragma unroll
+                            for (int c = 0; c < NC; c++) sc[n][h][c] = capped(sc[n][h][c], p.softcap);
+                }
+                if (masked) {
+#pragma unroll
+                    for (int n = 0; n < NA; n++)
+#pragma unroll
                         for (int c = 0; c < NC; c++) {
+                            const Rows &r = row_of(n, c);
+#pragma unroll
+                            for (int h = 0; h < 2; h++)
+                                if (!sees(r, pos0 + g + 8 * h)) sc[n][h][c] = -INFINITY;
+                        }
+                }
+                float base[NA][NC];
+                bool higher = e_corr != 1.0f;
+#pragma unroll
+                for (int n = 0; n < NA; n++)
+#pragma unroll
+                    for (int c = 0; c < NC; c++) base[n][c] = fmaxf(sc[n][0][c], sc[n][1][c]);
+#pragma unroll
+                for (int o2 = 4; o2 < 32; o2 <<= 1)
+#pragma unroll
+                    for (int n = 0; n < NA; n++)
+#pragma unroll
+                        for (int c = 0; c < NC; c++) base[n][c] = fmaxf(base[n][c], __shfl_xor_sync(0xFFFFFFFFu, base[n][c], o2));
+#pragma unroll
+                for (int n = 0; n < NA; n++)
+#pragma unroll
+                    for (int c = 0; c < NC; c++) higher |= base[n][c] > m[n][c];
+                if (__any_sync(0xFFFFFFFFu, higher)) {
+#pragma unroll
+                    for (int n = 0; n < NA; n++) {
+                        float corr[NC];
+#pragma unroll
+                        for (int c = 0; c < NC; c++) {
+                            const float top = fmaxf(base[n][c], m[n][c]);
+                            corr[c] = top == -INFINITY ? 1.0f : ex2(m[n][c] - top);
+                            m[n][c] = top;
                             l[n][c] *= corr[c];
                             corr[c] *= e_corr;
                         }
-    #pragma unroll
+#pragma unroll
                         for (int j = 0; j < NM; j++)
-    #pragma unroll
+#pragma unroll
                             for (int c = 0; c < 4; c++) o[j][n][c] *= corr[kPair ? 0 : c & 1];
                     }
-    #pragma unroll
-                    for (int c = 0; c < NC; c++)
-    #pragma unroll
+                }
+#pragma unroll
+                for (int n = 0; n < NA; n++)
+#pragma unroll
+                    for (int c = 0; c < NC; c++) {
+                        const float from = m[n][c] == -INFINITY ? 0.0f : m[n][c];
+#pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            sc[n][h][c] = ex2(sc[n][h][c] - base[c]);
+                            sc[n][h][c] = ex2(sc[n][h][c] - from);
                             l[n][c] += sc[n][h][c];
                         }
-                }
+                    }
                 // weights w[h][c] as an operand: [first terms of positions 0 - 7, of 8 - 15, second terms]; with kPair both in [0], [1]
                 auto operand = [&](const float (&w)[2][NC], uint32_t (&f)[kQF]) {
     #pragma unroll

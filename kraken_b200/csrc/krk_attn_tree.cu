@@ -75,14 +75,14 @@ Form form_of(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a) {
     Form f;
     const int type = cache.type, d = cache.head_dim;
     const int64_t rows = (int64_t)a.max_q * (a.n_heads / cache.n_kv_heads);
-    f.block = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 || d > 128 ? 16 : 32;
+    f.block = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 || d > 128 ? 16 : type == KRK_CUDA_KV_F16 ? kWideRows : 32;
     f.rows = (int)(rows < f.block ? rows : f.block);
-    const int64_t tiles = (a.max_kv_len + kTile - 1) / kTile;
+    const int64_t tiles = (a.max_kv_len + tile_of(f.block) - 1) / tile_of(f.block);
     // Short contexts: a CTA walks a whole item, which costs less than the second kernel.
-    f.whole = tiles <= kWholeTiles;
+    f.whole = a.max_kv_len <= kWholeTiles * kTile;
     const int64_t items = (int64_t)a.n_seq * cache.n_kv_heads * ((rows + f.block - 1) / f.block);
-    const int64_t units = f.whole ? items : items * (tiles + kSetup);
-    const int ctas = type == KRK_CUDA_KV_F16 ? attn_ctas_f16(d, f.block) : type == KRK_CUDA_KV_Q8 ? attn_ctas_q8(d, f.block) : attn_ctas_q4(d, f.block);
+    const int64_t units = f.whole ? items : items * tiles;   // (a tile or more to a CTA)
+    const int ctas = f.block == kWideRows ? 1 : type == KRK_CUDA_KV_F16 ? attn_ctas_f16(d, f.block) : type == KRK_CUDA_KV_Q8 ? attn_ctas_q8(d, f.block) : attn_ctas_q4(d, f.block);
     const int64_t fill = (int64_t)ctas * sm_count();
     f.grid = (int)(units < fill ? units : fill);
     return f;
@@ -128,7 +128,9 @@ int launch_attention_tree(float *out, const float *q, const krk_cuda_kv_cache &c
     p.grid = f.grid;
     p.scale = a.scale;
     p.softcap = a.softcap;
-    int rc = cache.type == KRK_CUDA_KV_F16 ? launch_attn_f16(p, cache.head_dim, f.block, st)
+    p.status = device_status_word();
+    if (!p.status) return KRK_CUDA_EDEVICE;
+    int rc = f.block == attn::kWideRows ? launch_attn_wide_f16(p, cache.head_dim, st) : cache.type == KRK_CUDA_KV_F16 ? launch_attn_f16(p, cache.head_dim, f.block, st)
              : cache.type == KRK_CUDA_KV_Q8 ? launch_attn_q8(p, cache.head_dim, f.block, st) : launch_attn_q4(p, cache.head_dim, f.block, st);
     if (rc == KRK_CUDA_OK && !f.whole && f.grid > 1) rc = attn::launch_merge(p, cache.head_dim, f.block, f.rows, st);
     return rc;
