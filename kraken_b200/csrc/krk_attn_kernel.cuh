@@ -25,7 +25,7 @@ namespace attn {
 __host__ __device__ constexpr int row_bytes_of(int type, int d) { return type == KRK_CUDA_KV_F16 ? 2 * d : type == KRK_CUDA_KV_Q8 ? d : d / 2; }
 __host__ __device__ constexpr int scale_bytes_of(int type, int d) { return type == KRK_CUDA_KV_F16 ? 0 : d / 16; }   // of a row
 
-// R: rows of a block, 4 (both terms of a query in one product), 8, 16 or 32.
+// R: rows of a block, 4 (both terms of a query in one product), 8 or 16.
 // Shared memory of a CTA: the ring, the query block, row data. As many CTAs an SM as registers and a ring of three stages (of two, for the
 // second CTA) leave room for.
 __host__ __device__ constexpr int stage_bytes(int ct, int d) { return 2 * kChunk * (row_bytes_of(ct, d) + scale_bytes_of(ct, d)); }   // keys and values of a chunk, then their scales
@@ -676,8 +676,7 @@ attn_kernel(const __grid_constant__ Params p) {
             }
         };
         if (NT == 1 || n_tiles == 1) chunks(std::integral_constant<int, 1>{});
-        else if (NT == 2 || n_tiles == 2) chunks(std::integral_constant<int, NT < 2 ? 1 : 2>{});
-        else chunks(std::integral_constant<int, NT < 4 ? 1 : 4>{});
+        else chunks(std::integral_constant<int, NT>{});
         copies_wait<0>();
 
         // ---- the warps' sums together. The outputs lie where the ring was.
@@ -774,14 +773,13 @@ int launch_one(const Params &p, cudaStream_t st) {
     return launched(cudaLaunchKernelEx(&cfg, attn_kernel<D, CT, R>, p));
 }
 
-// Blocks of 32 rows up to heads of 128 values: their outputs take 128 registers of a lane.
-#define KRK_ATTN_FORMS(d, r, call)                                                                                      \
-    switch (d) {                                                                                                        \
-    case 64: return r == 4 ? call(64, 4) : r == 8 ? call(64, 8) : r == 16 ? call(64, 16) : call(64, 32);                \
-    case 96: return r == 4 ? call(96, 4) : r == 8 ? call(96, 8) : r == 16 ? call(96, 16) : call(96, 32);                \
-    case 128: return r == 4 ? call(128, 4) : r == 8 ? call(128, 8) : r == 16 ? call(128, 16) : call(128, 32);           \
-    case 192: return r == 4 ? call(192, 4) : r == 8 ? call(192, 8) : call(192, 16);                                     \
-    default: return r == 4 ? call(256, 4) : r == 8 ? call(256, 8) : call(256, 16);                                      \
+#define KRK_ATTN_FORMS(d, r, call)                                                    \
+    switch (d) {                                                                      \
+    case 64: return r == 4 ? call(64, 4) : r == 8 ? call(64, 8) : call(64, 16);       \
+    case 96: return r == 4 ? call(96, 4) : r == 8 ? call(96, 8) : call(96, 16);       \
+    case 128: return r == 4 ? call(128, 4) : r == 8 ? call(128, 8) : call(128, 16);   \
+    case 192: return r == 4 ? call(192, 4) : r == 8 ? call(192, 8) : call(192, 16);   \
+    default: return r == 4 ? call(256, 4) : r == 8 ? call(256, 8) : call(256, 16);    \
     }
 template <int CT>
 int launch_type(const Params &p, int d, int r, cudaStream_t st) {

@@ -75,11 +75,16 @@ Form form_of(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a) {
     Form f;
     const int type = cache.type, d = cache.head_dim;
     const int64_t rows = (int64_t)a.max_q * (a.n_heads / cache.n_kv_heads);
-    f.block = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 || d > 128 ? 16 : type == KRK_CUDA_KV_F16 ? kWideRows : 32;
-    f.rows = (int)(rows < f.block ? rows : f.block);
-    const int64_t tiles = (a.max_kv_len + tile_of(f.block) - 1) / tile_of(f.block);
     // Short contexts: a CTA walks a whole item, which costs less than the second kernel.
     f.whole = a.max_kv_len <= kWholeTiles * kTile;
+    // Blocks as small as the rows, 16 of them at most: 32 with their outputs in 128 registers of a lane took longer than two blocks of 16 (48
+    // ragged sequences of 4 to 32 rows, 8 bits: 214 us against 157; blocks of 8: 207). Over f16 caches more than 32 rows go to the
+    // tensor memory's form, heads of 96 and 128 values over contexts that are divided (4 sequences of 16,000, 64 rows: 99 us against 145, 128
+    // rows 166 against 296; 32 rows 80 against 94 there, but 27 against 23 at 2000; heads of 64: 91 against 87, 152 against 157).
+    const bool wide = type == KRK_CUDA_KV_F16 && rows > 32 && (d == 96 || d == 128) && !f.whole;
+    f.block = wide ? kWideRows : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+    f.rows = (int)(rows < f.block ? rows : f.block);
+    const int64_t tiles = (a.max_kv_len + tile_of(f.block) - 1) / tile_of(f.block);
     const int64_t items = (int64_t)a.n_seq * cache.n_kv_heads * ((rows + f.block - 1) / f.block);
     const int64_t units = f.whole ? items : items * tiles;   // (a tile or more to a CTA)
     const int ctas = f.block == kWideRows ? 1 : type == KRK_CUDA_KV_F16 ? attn_ctas_f16(d, f.block) : type == KRK_CUDA_KV_Q8 ? attn_ctas_q8(d, f.block) : attn_ctas_q4(d, f.block);

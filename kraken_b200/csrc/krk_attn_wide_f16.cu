@@ -4,7 +4,7 @@
 namespace krk_cuda {
 
 int launch_attn_wide_f16(const attn::Params &p, int head_dim, cudaStream_t st) {
-    return head_dim == 64 ? attn::launch_wide<64>(p, st) : head_dim == 96 ? attn::launch_wide<96>(p, st) : attn::launch_wide<128>(p, st);
+    return head_dim == 96 ? attn::launch_wide<96>(p, st) : attn::launch_wide<128>(p, st);
 }
 
 } // namespace krk_cuda
