@@ -468,6 +468,14 @@ void krk_cuda_backend_embed(void *be, void *out, const void *tok_embd, int tt, i
 void krk_cuda_backend_logits_topk(void *be, const void *logits, int64_t n, int32_t k, const void *pen_mask, float rep_pen,
                                   float softcap, float temp, int32_t *ids, float *vals, float *mass_out, void *scratch,
                                   int32_t cand_cap, int64_t *count_out);
+/* the operators between the projections and the logits, on the backend's stream and workspace */
+void krk_cuda_backend_qk_norm_rope(void *be, void *q_out, void *k_out, const void *q, const void *k, const struct krk_cuda_rope *host_rope);
+void krk_cuda_backend_kv_append(void *be, const struct krk_cuda_kv_cache *host_cache, const void *k, const void *v, int64_t k_stride,
+                                int64_t v_stride, const int64_t *slots, int64_t n_tok);
+void krk_cuda_backend_kv_read(void *be, const struct krk_cuda_kv_cache *host_cache, void *k, void *v, const int64_t *slots, int64_t n);
+void krk_cuda_backend_attention_tree(void *be, void *out, const void *q, const struct krk_cuda_kv_cache *host_cache,
+                                     const struct krk_cuda_attention *host_attention);
+void krk_cuda_backend_logits_adjust(void *be, void *out, const void *logits, const struct krk_cuda_adjust *host_adjust);
 void krk_cuda_backend_silu_mul(void *be, void *out, const void *gate, const void *up, int64_t n, int64_t row_len,
                                float *host_row_scale);
 void krk_cuda_backend_gather_rows(void *be, void *dst, const void *src, const int32_t *rows, int64_t n_rows, int64_t n);

@@ -15,6 +15,11 @@
 #include <cstdint>
 #include <string>
 
+struct krk_cuda_rope;        // krk_cuda.h
+struct krk_cuda_kv_cache;
+struct krk_cuda_attention;
+struct krk_cuda_adjust;
+
 namespace krk_cuda {
 
 using i32 = int32_t;
@@ -88,6 +93,15 @@ public:
     // candidate buffer is the backend's own workspace, and the set is never truncated: *count_out = min(n, k)).
     void logits_topk(const void *logits, i64 n, i32 k, const void *pen_mask, f32 rep_pen, f32 softcap, f32 temp,
                      i32 *ids, f32 *vals, f32 *mass_out, void *scratch, i32 cand_cap, i64 *count_out);
+
+    // Between the projections and the output projection, and before the ranking: the entries of krk_cuda.h of these names, whose structs
+    // carry the sizes and device pointers. Like the members above they log and abort on what the kernels cannot address; the workspace of
+    // the attention is the backend's own.
+    void qk_norm_rope(void *q_out, void *k_out, const void *q, const void *k, const krk_cuda_rope &rope);
+    void kv_append(const krk_cuda_kv_cache &cache, const void *k, const void *v, i64 k_stride, i64 v_stride, const i64 *slots, i64 n_tok);
+    void kv_read(const krk_cuda_kv_cache &cache, void *k, void *v, const i64 *slots, i64 n);
+    void attention_tree(void *out, const void *q, const krk_cuda_kv_cache &cache, const krk_cuda_attention &attention);
+    void logits_adjust(void *out, const void *logits, const krk_cuda_adjust &adjust);
 
     // The router on the device, in the interface's three steps (backend.hpp:934-986); all pointers device memory.
     bool router_softmax_supported() const { return true; }

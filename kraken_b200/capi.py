@@ -146,6 +146,11 @@ SIGNATURES = {
     "krk_cuda_backend_embed": (None, [_vp, _vp, _vp, _int, _i64, _i64, _vp, _i64]),
     "krk_cuda_backend_logits_topk": (None, [_vp, _vp, _i64, C.c_int32, _vp, C.c_float, C.c_float, C.c_float, _vp, _vp, _vp, _vp,
                                             C.c_int32, _vp]),
+    "krk_cuda_backend_qk_norm_rope": (None, [_vp, _vp, _vp, _vp, _vp, C.POINTER(Rope)]),
+    "krk_cuda_backend_kv_append": (None, [_vp, C.POINTER(KvCacheStruct), _vp, _vp, _i64, _i64, _vp, _i64]),
+    "krk_cuda_backend_kv_read": (None, [_vp, C.POINTER(KvCacheStruct), _vp, _vp, _vp, _i64]),
+    "krk_cuda_backend_attention_tree": (None, [_vp, _vp, _vp, C.POINTER(KvCacheStruct), C.POINTER(Attention)]),
+    "krk_cuda_backend_logits_adjust": (None, [_vp, _vp, _vp, C.POINTER(Adjust)]),
     "krk_cuda_backend_silu_mul": (None, [_vp, _vp, _vp, _vp, _i64, _i64, _vp]),
     "krk_cuda_backend_gather_rows": (None, [_vp, _vp, _vp, _vp, _i64, _i64]),
     "krk_cuda_backend_scatter_axpy_rows": (None, [_vp, _vp, _vp, _vp, _vp, _i64, _i64]),
@@ -579,6 +584,21 @@ class Backend:
 
     def moe_plan_build(self, ids: int, n_rows: int, k: int, n_expert: int, off: int, rows: int, wt: int, wts: int) -> None:
         lib.krk_cuda_backend_moe_plan_build(self.h, ids, n_rows, k, n_expert, off, rows, wt, wts)
+
+    def qk_norm_rope(self, q_out: int, k_out: int, q: int, k: int, rope: Rope) -> None:
+        lib.krk_cuda_backend_qk_norm_rope(self.h, q_out, k_out, q, k, C.byref(rope))
+
+    def kv_append(self, cache: KvCacheStruct, k: int, v: int, k_stride: int, v_stride: int, slots: int, n_tok: int) -> None:
+        lib.krk_cuda_backend_kv_append(self.h, C.byref(cache), k, v, k_stride, v_stride, slots, n_tok)
+
+    def kv_read(self, cache: KvCacheStruct, k: int, v: int, slots: int, n: int) -> None:
+        lib.krk_cuda_backend_kv_read(self.h, C.byref(cache), k, v, slots, n)
+
+    def attention_tree(self, out: int, q: int, cache: KvCacheStruct, attention: Attention) -> None:
+        lib.krk_cuda_backend_attention_tree(self.h, out, q, C.byref(cache), C.byref(attention))
+
+    def logits_adjust(self, out: int, logits: int, adjust: Adjust) -> None:
+        lib.krk_cuda_backend_logits_adjust(self.h, out, logits, C.byref(adjust))
 
     def fill0(self, p: int, nbytes: int) -> None:
         lib.krk_cuda_backend_fill0(self.h, p, nbytes)

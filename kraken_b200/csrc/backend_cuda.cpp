@@ -271,6 +271,37 @@ void CudaBackend::logits_topk(const void *logits, i64 n, i32 k, const void *pen_
     }
 }
 
+void CudaBackend::qk_norm_rope(void *q_out, void *k_out, const void *q, const void *k, const krk_cuda_rope &rope) {
+    use();
+    const int rc = krk_cuda_qk_norm_rope(q_out, k_out, q, k, &rope, stream_);
+    if (rc != KRK_CUDA_OK) die("qk_norm_rope", rc, rope.n_tok, rope.n_heads, rope.head_dim, rope.rot_dim);
+}
+
+void CudaBackend::kv_append(const krk_cuda_kv_cache &cache, const void *k, const void *v, i64 k_stride, i64 v_stride, const i64 *slots, i64 n_tok) {
+    use();
+    const int rc = krk_cuda_kv_append(&cache, k, v, k_stride, v_stride, slots, n_tok, stream_);
+    if (rc != KRK_CUDA_OK) die("kv_append", rc, n_tok, cache.n_kv_heads, cache.head_dim, cache.type);
+}
+
+void CudaBackend::kv_read(const krk_cuda_kv_cache &cache, void *k, void *v, const i64 *slots, i64 n) {
+    use();
+    const int rc = krk_cuda_kv_read(&cache, k, v, slots, n, stream_);
+    if (rc != KRK_CUDA_OK) die("kv_read", rc, n, cache.n_kv_heads, cache.head_dim, cache.type);
+}
+
+void CudaBackend::attention_tree(void *out, const void *q, const krk_cuda_kv_cache &cache, const krk_cuda_attention &attention) {
+    use();
+    const size_t need = krk_cuda_attention_tree_workspace_bytes(&cache, &attention);
+    const int rc = krk_cuda_attention_tree(out, q, &cache, &attention, need ? workspace(need) : nullptr, need, stream_);
+    if (rc != KRK_CUDA_OK) die("attention_tree", rc, attention.n_seq, attention.n_heads, cache.head_dim, cache.type);
+}
+
+void CudaBackend::logits_adjust(void *out, const void *logits, const krk_cuda_adjust &adjust) {
+    use();
+    const int rc = krk_cuda_logits_adjust(out, logits, &adjust, stream_);
+    if (rc != KRK_CUDA_OK) die("logits_adjust", rc, adjust.n_rows, adjust.n_vocab, adjust.hist_n, 0);
+}
+
 } // namespace krk_cuda
 
 // ---- C shim over the class (declared in krk_cuda.h) -------------------------------------------
@@ -313,6 +344,23 @@ void krk_cuda_backend_logits_topk(void *be, const void *logits, int64_t n, int32
                                   int32_t cand_cap, int64_t *count_out) {
     static_cast<CudaBackend *>(be)->logits_topk(logits, n, k, pen_mask, rep_pen, softcap, temp, ids, vals, mass_out, scratch,
                                                 cand_cap, count_out);
+}
+void krk_cuda_backend_qk_norm_rope(void *be, void *q_out, void *k_out, const void *q, const void *k, const krk_cuda_rope *host_rope) {
+    static_cast<CudaBackend *>(be)->qk_norm_rope(q_out, k_out, q, k, *host_rope);
+}
+void krk_cuda_backend_kv_append(void *be, const krk_cuda_kv_cache *host_cache, const void *k, const void *v, int64_t k_stride, int64_t v_stride,
+                                const int64_t *slots, int64_t n_tok) {
+    static_cast<CudaBackend *>(be)->kv_append(*host_cache, k, v, k_stride, v_stride, slots, n_tok);
+}
+void krk_cuda_backend_kv_read(void *be, const krk_cuda_kv_cache *host_cache, void *k, void *v, const int64_t *slots, int64_t n) {
+    static_cast<CudaBackend *>(be)->kv_read(*host_cache, k, v, slots, n);
+}
+void krk_cuda_backend_attention_tree(void *be, void *out, const void *q, const krk_cuda_kv_cache *host_cache,
+                                     const krk_cuda_attention *host_attention) {
+    static_cast<CudaBackend *>(be)->attention_tree(out, q, *host_cache, *host_attention);
+}
+void krk_cuda_backend_logits_adjust(void *be, void *out, const void *logits, const krk_cuda_adjust *host_adjust) {
+    static_cast<CudaBackend *>(be)->logits_adjust(out, logits, *host_adjust);
 }
 void krk_cuda_backend_silu_mul(void *be, void *out, const void *gate, const void *up, int64_t n, int64_t row_len,
                                float *host_row_scale) {

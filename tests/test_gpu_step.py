@@ -103,3 +103,40 @@ def test_bindings_check_shapes(cuda):
         with pytest.raises((ValueError, cuda.KrkCudaError)):
             cuda.logits_adjust(f(2, 100), **a)
     assert cuda.launch_count() == before
+
+
+def test_through_the_backend_object(cuda):
+    """The members of the backend, on its own stream and workspace, give what the functions give."""
+    import torch
+    rng = np.random.default_rng(4)
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    heads, kv, d, page, n_q, total = 8, 2, 64, 16, 4, 2000
+    q, k, v = (dev(rng.standard_normal((n, h, d)).astype(np.float32)) for n, h in ((n_q, heads), (total, kv), (total, kv)))
+    pos, freq = dev(np.arange(n_q, dtype=np.int32) + total - n_q), dev(rng.random(d // 2).astype(np.float32))
+    slots = torch.randperm(total // page * page, device="cuda")
+    table = torch.arange(total // page, dtype=torch.int32, device="cuda").view(1, -1)
+    start, length = dev(np.array([0, n_q], np.int32)), dev(np.array([total], np.int32))
+    hist, rep = dev(rng.integers(0, 500, (n_q, 20)).astype(np.int32)), dev(np.full(n_q, 1.2, np.float32))
+    logits = dev(rng.standard_normal((n_q, 500)).astype(np.float32))
+    want_cache, cache = (cuda.KvCache.empty(cuda.KV_Q8, total // page, kv, page, d) for _ in range(2))
+    q_want, _ = cuda.qk_norm_rope(q, None, pos, freq)
+    cuda.kv_append(want_cache, k, v, slots)
+    want = cuda.attention_tree(q_want, want_cache, start, length, table, n_q)
+    k_want, v_want = cuda.kv_read(want_cache, slots[:50])
+    l_want = cuda.logits_adjust(logits, hist, rep=rep)
+
+    be = cuda.Backend(0)
+    torch.cuda.synchronize()
+    q_got, got, k_got, v_got, l_got = (torch.zeros_like(t) for t in (q_want, want, k_want, v_want, l_want))
+    p = lambda t: t.data_ptr()  # noqa: E731
+    rope = cuda.Rope(pos=p(pos), inv_freq=p(freq), n_tok=n_q, q_stride=heads * d, q_out_stride=heads * d, n_heads=heads, head_dim=d, rot_dim=d, norm=1, eps=1e-6)
+    be.qk_norm_rope(p(q_got), None, p(q), None, rope)
+    be.kv_append(cache.struct, p(k), p(v), kv * d, kv * d, p(slots), total)
+    be.attention_tree(p(got), p(q_got), cache.struct, cuda.Attention(q_start=p(start), kv_len=p(length), page_table=p(table), q_stride=heads * d, out_stride=heads * d,
+                                                                     n_seq=1, n_heads=heads, max_q=n_q, table_width=total // page, scale=d ** -0.5))
+    be.kv_read(cache.struct, p(k_got), p(v_got), p(slots), 50)
+    be.logits_adjust(p(l_got), p(logits), cuda.Adjust(n_rows=n_q, n_vocab=500, stride=500, out_stride=500, hist=p(hist), hist_n=20, hist_stride=20, rep=p(rep)))
+    be.sync()
+    for a, b in ((q_got, q_want), (got, want), (k_got, k_want), (v_got, v_want), (l_got, l_want)):
+        assert (a == b).all()
+    be.close()
