@@ -297,7 +297,7 @@ struct krk_cuda_kv_cache {
     void *k, *v, *k_scale, *v_scale;  /* device memory, 16-byte aligned */
     int type, head_dim;               /* head_dim a multiple of 32, <= 256 */
     int n_kv_heads, page_size;        /* up to 1024 heads; page_size a multiple of 16 */
-    int64_t n_pages;
+    int64_t n_pages;                  /* n_pages * n_kv_heads * page_size below 2^31 */
 };
 /* New keys and values [n_tok][n_kv_heads][head_dim] f32 (strides in floats from a token to the next, multiples of 4; 16-byte
  * aligned) into positions slots[t] = page * page_size + place (int64). A token whose slot the cache does not have (-1, say) is

@@ -213,6 +213,17 @@ attn_kernel(const __grid_constant__ Params p) {
         const bool begins = walk.begins, ends = walk.ends;
         if (walk.parts > 0 && tid == 0) walk.note(p);
 
+        // ---- the block's queries: a warp takes rows in turn; all its rows' loads go out before the pages are waited for
+        constexpr int kPer = R / kWarps;
+        float x[kPer][NB];
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            const int r = warp + kWarps * j, rr = block * R + r, i = rr / p.group;
+            const float *from = p.q + (int64_t)(sq.q0 + i) * p.q_stride + (kvh * p.group + rr - i * p.group) * D + lane;
+#pragma unroll
+            for (int c = 0; c < NB; c++) x[j][c] = r < n_rows ? from[32 * c] : 0.0f;
+        }
+
         // ---- pages of this warp's chunks: lane l holds that of the l-th from the last refill on, as a row of the pool
         const int chunk0 = tile0 * kWarps + warp, n_chunks = tile1 - tile0;
         const int32_t *table = p.table + (size_t)s * p.table_width;
@@ -256,16 +267,7 @@ attn_kernel(const __grid_constant__ Params p) {
 #pragma unroll
         for (int i = 0; i < S::kRing - 1; i++) load(i);
 
-        // ---- the block's rows: data, and queries in two f16 terms. A warp takes rows in turn; all its rows' loads go out first.
-        constexpr int kPer = R / kWarps;
-        float x[kPer][NB];
-#pragma unroll
-        for (int j = 0; j < kPer; j++) {
-            const int r = warp + kWarps * j, rr = block * R + r, i = rr / p.group;
-            const float *from = p.q + (int64_t)(sq.q0 + i) * p.q_stride + (kvh * p.group + rr - i * p.group) * D + lane;
-#pragma unroll
-            for (int c = 0; c < NB; c++) x[j][c] = r < n_rows ? from[32 * c] : 0.0f;
-        }
+        // ---- the rows' data, and the queries in two f16 terms
         float most[kPer];
 #pragma unroll
         for (int j = 0; j < kPer; j++) {

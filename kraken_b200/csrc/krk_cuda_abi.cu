@@ -413,7 +413,7 @@ static int check_cache(const krk_cuda_kv_cache *c) {
     if (!c) return KRK_CUDA_ENULL;
     if (c->type != KRK_CUDA_KV_F16 && c->type != KRK_CUDA_KV_Q8 && c->type != KRK_CUDA_KV_Q4) return KRK_CUDA_EDTYPE;
     if (c->head_dim < 32 || c->head_dim > 256 || c->head_dim % 32 != 0 || c->n_kv_heads < 1 || c->n_kv_heads > 1024 || c->page_size < 16 ||
-        c->page_size % 16 != 0 || c->n_pages < 0 || c->n_pages > INT32_MAX)
+        c->page_size % 16 != 0 || c->n_pages < 0 || c->n_pages > INT32_MAX || c->n_pages * c->n_kv_heads > INT32_MAX / c->page_size)
         return KRK_CUDA_ESHAPE;
     if (c->n_pages > 0) {
         if (!c->k || !c->v || (c->type != KRK_CUDA_KV_F16 && (!c->k_scale || !c->v_scale))) return KRK_CUDA_ENULL;

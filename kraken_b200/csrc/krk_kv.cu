@@ -143,11 +143,11 @@ __device__ __forceinline__ int part(int u, uint32_t inv) { return (int)__umulhi(
 
 // Where the rows of a block's tokens lie: row of the pools of head 0 (heads are page_size rows apart), or -1. Dividing by the page size takes
 // longer than what is done with eight values, so a token's slot is looked at once.
-__device__ __forceinline__ void find_rows(const CacheParams &p, int64_t t0, int n_tok, int64_t *rows) {
+__device__ __forceinline__ void find_rows(const CacheParams &p, int64_t t0, int n_tok, int *rows) {
     if ((int)threadIdx.x < n_tok) {
         const int64_t slot = p.slots[t0 + threadIdx.x];
         const int64_t page = slot / p.page_size;
-        rows[threadIdx.x] = slot < 0 || slot >= p.n_slots ? -1 : page * p.heads * p.page_size + (slot - page * p.page_size);
+        rows[threadIdx.x] = slot < 0 || slot >= p.n_slots ? -1 : (int)(page * p.heads * p.page_size + (slot - page * p.page_size));
     }
 }
 
@@ -157,7 +157,8 @@ __device__ __forceinline__ void find_rows(const CacheParams &p, int64_t t0, int 
 template <int CT>
 __global__ void __launch_bounds__(256)
 kv_append_kernel(const __grid_constant__ CacheParams p) {
-    __shared__ int64_t s_slot[kMostTokens], s_row[kMostTokens];
+    __shared__ int64_t s_slot[kMostTokens];
+    __shared__ int s_row[kMostTokens];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, of_row = p.d / 8, of_tok = 2 * p.heads * of_row;
@@ -201,12 +202,12 @@ kv_append_kernel(const __grid_constant__ CacheParams p) {
         const Unit w = unit(min(u, total - 1));
         const int c = w.c, kv = w.kv;
         const bool keep = u < total && s_row[w.tok] >= 0;
-        const int64_t row = keep ? s_row[w.tok] + w.head * p.page_size : 0;
+        const int row = keep ? s_row[w.tok] + w.head * p.page_size : 0;
         if constexpr (CT == KRK_CUDA_KV_F16) {
             __half2 h[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) h[i] = __halves2half2(half_sat(x[2 * i]), half_sat(x[2 * i + 1]));
-            if (keep) *reinterpret_cast<uint4 *>(p.pool[kv] + (row * p.d + 8 * c) * 2) = *reinterpret_cast<uint4 *>(h);
+            if (keep) *reinterpret_cast<uint4 *>(p.pool[kv] + ((int64_t)row * p.d + 8 * c) * 2) = *reinterpret_cast<uint4 *>(h);
         } else {
             float hi = x[0], lo = x[0], all = 0.0f;
 #pragma unroll
@@ -227,39 +228,35 @@ kv_append_kernel(const __grid_constant__ CacheParams p) {
             const __half dh = odd ? __ushort_as_half(0x7FFF) : half_sat(__fdiv_rn(k8 ? fmaxf(hi, -lo) : hi >= -lo ? hi : lo, k8 ? 127.0f : -8.0f));
             const float d = __half2float(dh), inv = 1.0f / d;
             const bool none = d == 0.0f || odd;
-            // rint(x / d) as x / d rounds to f32: the product with the reciprocal is off by less than 2^-21 of up to 128, so only quotients that
-            // near to a half are divided (and those of a scale that ran out of bits)
-            float r[8];
-            bool near = false;
+            // rint(x / d) as x / d rounds to f32: the product with the reciprocal is off by less than 2^-16 of up to 128, so only quotients that
+            // near to a half are divided (and those of a scale that ran out of bits). A whole number is in the low bits of 1.5 * 2^23 more.
+            constexpr float kMagic = 12582912.0f, kLeast = k8 ? -127.0f : -8.0f, kMost = k8 ? 127.0f : 7.0f;
+            uint32_t u[8];
+            bool near = none;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float q = x[i] * inv;
-                r[i] = rintf(q);
-                near |= !(fabsf(q - r[i]) < 0.499f) || !(fabsf(q) < 256.0f);
+                const float q = x[i] * inv, f = fminf(fmaxf(q, kLeast), kMost) + kMagic;
+                near |= !(fabsf(q - (f - kMagic)) < 0.49998f);   // (beyond the limits, too)
+                u[i] = __float_as_uint(f);
             }
             if (near) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) r[i] = none ? 0.0f : rintf(__fdiv_rn(x[i], d));
+                for (int i = 0; i < 8; i++) u[i] = __float_as_uint((none ? 0.0f : fminf(fmaxf(rintf(__fdiv_rn(x[i], d)), kLeast), kMost)) + kMagic);
             }
             uint32_t b[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                uint32_t u[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {   // a whole number in the low bits of 1.5 * 2^23 more
-                    const float f = k8 ? fminf(fmaxf(r[4 * i + j], -127.0f), 127.0f) : fminf(fmaxf(r[4 * i + j], -8.0f), 7.0f);
-                    u[j] = __float_as_uint(f + (k8 ? 12582912.0f : 12582920.0f));
-                }
-                b[i] = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+                b[i] = __byte_perm(__byte_perm(u[4 * i], u[4 * i + 1], 0x0040), __byte_perm(u[4 * i + 2], u[4 * i + 3], 0x0040), 0x5410);
+                if constexpr (!k8) b[i] = (b[i] ^ 0x08080808u) & 0x0F0F0F0Fu;   // (-8 .. 7 in four bits to 0 .. 15)
             }
             if constexpr (k8) {
-                if (keep) *reinterpret_cast<uint2 *>(p.pool[kv] + row * p.d + 8 * c) = make_uint2(b[0], b[1]);
+                if (keep) *reinterpret_cast<uint2 *>(p.pool[kv] + (int64_t)row * p.d + 8 * c) = make_uint2(b[0], b[1]);
             } else {
                 // values 16 .. 31 of a block (lanes 2, 3 of its four) are the high halves of the bytes of values 0 .. 15
                 const uint32_t h0 = __shfl_down_sync(0xFFFFFFFFu, b[0], 2), h1 = __shfl_down_sync(0xFFFFFFFFu, b[1], 2);
-                if (keep && (c & 3) < 2) *reinterpret_cast<uint2 *>(p.pool[kv] + row * (p.d / 2) + 16 * (c >> 2) + 8 * (c & 3)) = make_uint2(b[0] | h0 << 4, b[1] | h1 << 4);
+                if (keep && (c & 3) < 2) *reinterpret_cast<uint2 *>(p.pool[kv] + (int64_t)row * (p.d / 2) + 16 * (c >> 2) + 8 * (c & 3)) = make_uint2(b[0] | h0 << 4, b[1] | h1 << 4);
             }
-            if (keep && (c & 3) == 0) p.scale[kv][row * (p.d / 32) + (c >> 2)] = dh;
+            if (keep && (c & 3) == 0) p.scale[kv][(int64_t)row * (p.d / 32) + (c >> 2)] = dh;
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = next[i];
@@ -271,7 +268,7 @@ kv_append_kernel(const __grid_constant__ CacheParams p) {
 template <int CT>
 __global__ void __launch_bounds__(256)
 kv_read_kernel(const __grid_constant__ CacheParams p) {
-    __shared__ int64_t s_row[kMostTokens];
+    __shared__ int s_row[kMostTokens];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, of_row = p.d / 4, of_tok = p.heads * of_row;
@@ -287,7 +284,7 @@ kv_read_kernel(const __grid_constant__ CacheParams p) {
 #pragma unroll
         for (int k = 0; k < kAt; k++) {
             const int u = min(base + k * 256 + tid, total - 1), tok = part(u, p.of_tok_inv), at = u - tok * of_tok, head = part(at, p.of_row_inv), c = at - head * of_row;
-            const int64_t first = s_row[tok], row = first + head * p.page_size;
+            const int first = s_row[tok], row = first + head * p.page_size;
             where[k] = first < 0 ? -1 : c;
 #pragma unroll
             for (int kv = 0; kv < 2; kv++) {
@@ -295,10 +292,10 @@ kv_read_kernel(const __grid_constant__ CacheParams p) {
                 d[k][kv] = 0.0f;
                 if (first < 0) continue;
                 if constexpr (CT == KRK_CUDA_KV_F16) {
-                    w[k][kv] = *reinterpret_cast<const uint2 *>(p.pool[kv] + (row * p.d + 4 * c) * 2);
+                    w[k][kv] = *reinterpret_cast<const uint2 *>(p.pool[kv] + ((int64_t)row * p.d + 4 * c) * 2);
                 } else {
-                    w[k][kv].x = *reinterpret_cast<const uint32_t *>(CT == KRK_CUDA_KV_Q8 ? p.pool[kv] + row * p.d + 4 * c : p.pool[kv] + row * (p.d / 2) + 16 * (c >> 3) + 4 * (c & 3));
-                    d[k][kv] = __half2float(p.scale[kv][row * (p.d / 32) + (c >> 3)]);
+                    w[k][kv].x = *reinterpret_cast<const uint32_t *>(CT == KRK_CUDA_KV_Q8 ? p.pool[kv] + (int64_t)row * p.d + 4 * c : p.pool[kv] + (int64_t)row * (p.d / 2) + 16 * (c >> 3) + 4 * (c & 3));
+                    d[k][kv] = __half2float(p.scale[kv][(int64_t)row * (p.d / 32) + (c >> 3)]);
                 }
             }
         }

@@ -23,13 +23,15 @@ struct AdjustParams {
     int hist_n, bias_n, n_masks, slices;
 };
 
-// PER: values of a thread. VEC: rows begin on 16-byte boundaries, four values at a time.
-template <int kThreads, int PER, bool VEC>
-__global__ void __launch_bounds__(kThreads, 2048 / kThreads)
+// PER: values of a thread. VEC: rows begin on 16-byte boundaries, four values at a time. PACKED: lists of less than 2^16 ids, whose
+// counts and places share a word.
+template <int kThreads, int PER, bool VEC, bool PACKED>
+__global__ void __launch_bounds__(kThreads, 1536 / kThreads)
 logits_adjust_kernel(const __grid_constant__ AdjustParams p) {
-    constexpr int kSlice = PER * kThreads, kEarly = 2;
-    __shared__ __align__(16) int count[kSlice];
-    __shared__ __align__(16) int last[kSlice];   // place in the list of biases, plus one
+    constexpr int kSlice = PER * kThreads, kEarly = 1;
+    __shared__ __align__(16) int table[PACKED ? kSlice : 2 * kSlice];
+    int *const count = table, *const last = table + (PACKED ? 0 : kSlice);   // last: place in the list of biases plus one, in the upper half of a word if packed
+    constexpr int kPlace = PACKED ? 16 : 0, kTimes = PACKED ? 0xFFFF : -1;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x;
@@ -54,6 +56,8 @@ logits_adjust_kernel(const __grid_constant__ AdjustParams p) {
     int4 early[kEarly];
 #pragma unroll
     for (int i = 0; i < kEarly; i++) early[i] = 4 * (tid + i * kThreads) < wide ? reinterpret_cast<const int4 *>(hist)[tid + i * kThreads] : make_int4(-1, -1, -1, -1);
+    const int32_t *bias_ids = p.bias_ids + row * p.bias_stride;
+    const int early_bias = p.bias && tid < p.bias_n ? bias_ids[tid] : -1;
     const int n_hist = !p.hist ? 0 : p.hist_len ? min(max(p.hist_len[row], 0), p.hist_n) : p.hist_n;
     const int n_bias = !p.bias ? 0 : p.bias_len ? min(max(p.bias_len[row], 0), p.bias_n) : p.bias_n;
     const int32_t m_row = !p.mask ? -1 : p.mask_row ? p.mask_row[row] : (int32_t)row;
@@ -64,11 +68,16 @@ logits_adjust_kernel(const __grid_constant__ AdjustParams p) {
         const int j = at(VEC ? 4 * i : i);
         ok[i] = mask && j < n ? mask[(lo + j) >> 5] >> ((lo + j) & 31) : 0xFFFFFFFFu;
     }
-    if (n_hist > 0)
-        for (int i = 4 * tid; i < kSlice; i += 4 * kThreads) *reinterpret_cast<int4 *>(count + i) = make_int4(0, 0, 0, 0);
-    if (n_bias > 0)
-        for (int i = 4 * tid; i < kSlice; i += 4 * kThreads) *reinterpret_cast<int4 *>(last + i) = make_int4(0, 0, 0, 0);
+    if (n_hist > 0 || n_bias > 0)
+        for (int i = 4 * tid; i < (PACKED ? kSlice : 2 * kSlice); i += 4 * kThreads) *reinterpret_cast<int4 *>(table + i) = make_int4(0, 0, 0, 0);
     __syncthreads();
+    if (n_bias > 0) {
+        for (int i = tid; i < n_bias; i += kThreads) {
+            const uint32_t j = (uint32_t)(i == tid ? early_bias : bias_ids[i]) - (uint32_t)lo;
+            if (j < (uint32_t)n) atomicMax(reinterpret_cast<unsigned *>(&last[j]), (unsigned)(i + 1) << kPlace);
+        }
+        if (PACKED) __syncthreads();   // (the counts go on top)
+    }
     // (an id outside the row is outside every slice: those below lo, and -1, wrap around)
     auto meet = [&](int32_t id) {
         const uint32_t j = (uint32_t)id - (uint32_t)lo;
@@ -85,11 +94,6 @@ logits_adjust_kernel(const __grid_constant__ AdjustParams p) {
         if (4 * (tid + i * kThreads) < n_hist) meet4(early[i], 4 * (tid + i * kThreads));
     for (int i = 4 * (tid + kEarly * kThreads); i < wide && i < n_hist; i += 4 * kThreads) meet4(*reinterpret_cast<const int4 *>(hist + i), i);
     for (int i = wide + tid; i < n_hist; i += kThreads) meet(hist[i]);
-    const int32_t *ids = p.bias_ids + row * p.bias_stride;
-    for (int i = tid; i < n_bias; i += kThreads) {
-        const uint32_t j = (uint32_t)ids[i] - (uint32_t)lo;
-        if (j < (uint32_t)n) atomicMax(&last[j], i + 1);
-    }
     __syncthreads();
     const float rep = p.rep ? p.rep[row] : 1.0f, freq = p.freq ? p.freq[row] : 0.0f, pres = p.pres ? p.pres[row] : 0.0f;
     const bool repeats = rep > 0.0f && rep != 1.0f;
@@ -97,25 +101,29 @@ logits_adjust_kernel(const __grid_constant__ AdjustParams p) {
     float *y = p.y + row * p.y_stride + lo;
 #pragma unroll
     for (int i = 0; i < PER; i += 4) {
-        int of[4], times[4];
+        int word[4], place[4];
+        const bool listed = n_hist > 0 || n_bias > 0;
         if constexpr (VEC) {
-            *reinterpret_cast<int4 *>(of) = n_bias > 0 ? *reinterpret_cast<const int4 *>(last + at(i)) : make_int4(0, 0, 0, 0);
-            *reinterpret_cast<int4 *>(times) = n_hist > 0 ? *reinterpret_cast<const int4 *>(count + at(i)) : make_int4(0, 0, 0, 0);
+            *reinterpret_cast<int4 *>(word) = listed ? *reinterpret_cast<const int4 *>(count + at(i)) : make_int4(0, 0, 0, 0);
+            if constexpr (!PACKED) *reinterpret_cast<int4 *>(place) = listed ? *reinterpret_cast<const int4 *>(last + at(i)) : make_int4(0, 0, 0, 0);
         } else {
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                of[c] = n_bias > 0 ? last[at(i + c)] : 0;
-                times[c] = n_hist > 0 ? count[at(i + c)] : 0;
+                word[c] = listed ? count[at(i + c)] : 0;
+                if constexpr (!PACKED) place[c] = listed ? last[at(i + c)] : 0;
             }
         }
-        if (of[0] | of[1] | of[2] | of[3] | times[0] | times[1] | times[2] | times[3]) {   // (few ids are in a list)
+        int any = word[0] | word[1] | word[2] | word[3];
+        if constexpr (!PACKED) any |= place[0] | place[1] | place[2] | place[3];
+        if (any) {   // (few ids are in a list)
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 float &z = v[i + c];
-                if (of[c]) z += bias[of[c] - 1];
-                if (times[c]) {
+                const int of = PACKED ? (int)((unsigned)word[c] >> kPlace) : place[c], times = word[c] & kTimes;
+                if (of) z += bias[of - 1];
+                if (times) {
                     if (repeats) z = z > 0.0f ? __fdiv_rn(z, rep) : __fmul_rn(z, rep);
-                    z = __fsub_rn(z, __fadd_rn(__fmul_rn(freq, (float)times[c]), pres));
+                    z = __fsub_rn(z, __fadd_rn(__fmul_rn(freq, (float)times), pres));
                 }
             }
         }
@@ -150,13 +158,15 @@ int launch_logits_adjust(float *out, const float *logits, const krk_cuda_adjust 
     const bool vec = ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) & 15) == 0 &&
                      (a.n_rows == 1 || (a.stride % 4 == 0 && a.out_stride % 4 == 0));
     // A block looks through the whole lists for its slice: 4096 values a block, but 1024 where the longer slices would leave SMs without one
-    // (64 rows of 128,256 with up to 4096 ids each: 38.6 us with 1024, 22.5 with 4096).
-    const bool wide = (a.n_vocab + 4095) / 4096 * a.n_rows >= 2 * sm_count();
+    // (64 rows of 128,256 with up to 4096 ids each: 38.6 us with 1024, 23 with 4096, 26 with 8192).
+    const bool packed = a.hist_n < 65536 && a.bias_n < 65535, wide = packed && (a.n_vocab + 4095) / 4096 * a.n_rows >= 2 * sm_count();
     const int threads = wide ? 512 : 256, slice = wide ? 4096 : 1024;
     const int64_t slices = (a.n_vocab + slice - 1) / slice;
     if (slices * a.n_rows > INT32_MAX) return KRK_CUDA_ESHAPE;
     p.slices = (int)slices;
-    auto kernel = wide ? (vec ? logits_adjust_kernel<512, 8, true> : logits_adjust_kernel<512, 8, false>) : vec ? logits_adjust_kernel<256, 4, true> : logits_adjust_kernel<256, 4, false>;
+    auto kernel = wide ? (vec ? logits_adjust_kernel<512, 8, true, true> : logits_adjust_kernel<512, 8, false, true>)
+                  : packed ? (vec ? logits_adjust_kernel<256, 4, true, true> : logits_adjust_kernel<256, 4, false, true>)
+                           : (vec ? logits_adjust_kernel<256, 4, true, false> : logits_adjust_kernel<256, 4, false, false>);
     return launched(launch_overlapped(kernel, dim3((unsigned)(slices * a.n_rows)), dim3(threads), st, p));
 }
 

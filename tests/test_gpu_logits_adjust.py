@@ -58,7 +58,7 @@ def lists(rng, rows, n, hist, biases, masks):
     return k
 
 
-@pytest.mark.parametrize("rows,n,hist,biases,masks", [(1, 1, 3, 1, 1), (1, 128256, 700, 20, 1), (3, 32000, 64, 0, 0), (5, 1023, 4000, 9, 2), (4, 4097, 1, 5, 4), (2, 50257, 5000, 300, 1), (33, 8192, 30, 40, 7)])
+@pytest.mark.parametrize("rows,n,hist,biases,masks", [(1, 1, 3, 1, 1), (1, 128256, 700, 20, 1), (3, 32000, 64, 0, 0), (5, 1023, 4000, 9, 2), (4, 4097, 1, 5, 4), (2, 50257, 5000, 300, 1), (33, 8192, 30, 40, 7), (2, 3000, 70000, 3, 1), (300, 9001, 65535, 1000, 5), (2, 5000, 10, 65600, 0)])
 def test_against_the_definition(cuda, rows, n, hist, biases, masks):
     rng = np.random.default_rng(n)
     run(cuda, 4 * rng.standard_normal((rows, n)).astype(np.float32), **lists(rng, rows, n, hist, biases, masks))
@@ -76,6 +76,14 @@ def test_each_part_alone(cuda):
     run(cuda, x, mask=k["mask"])
     run(cuda, x, mask=k["mask"][:2])   # the third row has none
     assert np.isneginf(run(cuda, x, mask=np.zeros((3, 157), np.int32))).all()
+
+
+def test_counts_of_long_histories(cuda):
+    """One id 65,535 times, and beside its bias; 70,000 times."""
+    x = np.array([[1.5, -2.0, 0.25, 3.0]], np.float32)
+    for times in (65535, 70000):
+        hist = np.full((1, times), 2, np.int32)
+        run(cuda, x, hist=hist, freq=np.array([0.5], np.float32), bias_ids=np.array([[2, 3, 2]], np.int32), bias=np.array([[9, 8, 7]], np.float32))
 
 
 def test_infinities_nan_and_zeros(cuda):
