@@ -133,7 +133,7 @@ struct CacheParams {
     const int64_t *slots;
     int64_t n, n_slots;
     int heads, d, page_size, per_block;
-    uint32_t of_row_inv, of_tok_inv;   // see part
+    uint32_t of_row_inv;    // see part
 };
 constexpr int kMostTokens = 32;   // of a block of threads
 
@@ -151,58 +151,72 @@ __device__ __forceinline__ void find_rows(const CacheParams &p, int64_t t0, int 
     }
 }
 
-// Append: reads x once, writes the rows. A lane has eight values, four lanes a block of 32, whose largest value is two
-// shuffles. Of tokens with the same slot the last one stays: a block of threads looks through the slots behind its tokens while its
-// first values are on their way (a block's tokens share the look).
+// Append: reads x once, writes the rows. A lane has eight values, four lanes a block of 32, whose largest value is two shuffles; its place
+// in a token stays, and the block's tokens follow each other there, the next one's values on their way. Of tokens with the same slot the last
+// one stays: a block of threads looks through the slots behind its tokens while its first values are on their way.
 template <int CT>
 __global__ void __launch_bounds__(256)
 kv_append_kernel(const __grid_constant__ CacheParams p) {
     __shared__ int64_t s_slot[kMostTokens];
     __shared__ int s_row[kMostTokens];
+    __shared__ uint32_t s_met[64];   // bit slot % 2048 of the block's slots
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, of_row = p.d / 8, of_tok = 2 * p.heads * of_row;
     const int64_t t0 = (int64_t)blockIdx.x * p.per_block;
-    const int n_tok = (int)min((int64_t)p.per_block, p.n - t0), total = n_tok * of_tok;
-    struct Unit {
-        int tok, kv, head, c;
+    const int n_tok = (int)min((int64_t)p.per_block, p.n - t0);
+    struct Place {
+        bool there;
+        int kv, head, c;
+        const float *from;
     };
-    auto unit = [&](int u) {
-        Unit w;
-        w.tok = part(u, p.of_tok_inv);
-        const int in_tok = u - w.tok * of_tok;
-        w.kv = in_tok >= of_tok / 2;
-        const int at = in_tok - (w.kv ? of_tok / 2 : 0);
+    auto place = [&](int at) {
+        Place w;
+        w.there = at < of_tok;
+        at = min(at, of_tok - 1);
+        w.kv = at >= of_tok / 2;
+        if (w.kv) at -= of_tok / 2;
         w.head = part(at, p.of_row_inv);
         w.c = at - w.head * of_row;
+        w.from = p.x[w.kv] + t0 * p.x_stride[w.kv] + w.head * p.d + 8 * w.c;
         return w;
     };
-    auto load = [&](int u, float x[8]) {
-        if (u >= total) return;
-        const Unit w = unit(u);
-        const float *from = p.x[w.kv] + (t0 + w.tok) * p.x_stride[w.kv] + w.head * p.d + 8 * w.c;
+    auto load = [&](const Place &w, int tok, float x[8]) {
+        if (!w.there || tok >= n_tok) return;
+        const float *from = w.from + tok * p.x_stride[w.kv];
         const float4 a = ld4(from), b = ld4(from + 4);
         x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
     };
-    float x[8] = {};
-    load(tid, x);
+    Place w = place(tid);
+    float next[8] = {};
+    load(w, 0, next);
     if (tid < n_tok) s_slot[tid] = p.slots[t0 + tid];
+    if (tid < 64) s_met[tid] = 0u;
     find_rows(p, t0, n_tok, s_row);
     __syncthreads();
+    if (tid < n_tok) atomicOr(&s_met[(s_slot[tid] >> 5) & 63], 1u << (s_slot[tid] & 31));
+    __syncthreads();
+#pragma unroll 4
     for (int64_t j = t0 + 1 + tid; j < p.n; j += 256) {
         const int64_t slot = p.slots[j];
-        for (int i = 0; i < n_tok; i++)
-            if (slot == s_slot[i] && t0 + i < j) s_row[i] = -1;
+        if ((s_met[(slot >> 5) & 63] >> (slot & 31)) & 1)   // (8191 tokens: 31 us; each against every later one 55)
+            for (int i = 0; i < n_tok; i++)
+                if (slot == s_slot[i] && t0 + i < j) s_row[i] = -1;
     }
     __syncthreads();
-    for (int base = 0; base < total; base += 256) {
-        float next[8] = {};
-        load(base + 256 + tid, next);
-        const int u = base + tid;
-        const Unit w = unit(min(u, total - 1));
-        const int c = w.c, kv = w.kv;
-        const bool keep = u < total && s_row[w.tok] >= 0;
-        const int row = keep ? s_row[w.tok] + w.head * p.page_size : 0;
+    for (int base = 0, tok = 0; base < of_tok;) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = next[i];
+        const int kv = w.kv, head = w.head, c = w.c;
+        const int first = s_row[tok], row = first + head * p.page_size;
+        const bool keep = w.there && first >= 0;
+        if (++tok == n_tok) {   // the next place
+            tok = 0;
+            base += 256;
+            w = place(base + tid);
+        }
+        load(w, tok, next);
         if constexpr (CT == KRK_CUDA_KV_F16) {
             __half2 h[4];
 #pragma unroll
@@ -229,14 +243,14 @@ kv_append_kernel(const __grid_constant__ CacheParams p) {
             const float d = __half2float(dh), inv = 1.0f / d;
             const bool none = d == 0.0f || odd;
             // rint(x / d) as x / d rounds to f32: the product with the reciprocal is off by less than 2^-16 of up to 128, so only quotients that
-            // near to a half are divided (and those of a scale that ran out of bits). A whole number is in the low bits of 1.5 * 2^23 more.
+            // near to a half are divided. A whole number is in the low bits of 1.5 * 2^23 more.
             constexpr float kMagic = 12582912.0f, kLeast = k8 ? -127.0f : -8.0f, kMost = k8 ? 127.0f : 7.0f;
             uint32_t u[8];
             bool near = none;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float q = x[i] * inv, f = fminf(fmaxf(q, kLeast), kMost) + kMagic;
-                near |= !(fabsf(q - (f - kMagic)) < 0.49998f);   // (beyond the limits, too)
+                const float q = fminf(fmaxf(x[i] * inv, kLeast), kMost), f = q + kMagic;   // (beyond the limits nothing is near)
+                near |= !(fabsf(q - (f - kMagic)) < 0.49998f);
                 u[i] = __float_as_uint(f);
             }
             if (near) {
@@ -258,13 +272,12 @@ kv_append_kernel(const __grid_constant__ CacheParams p) {
             }
             if (keep && (c & 3) == 0) p.scale[kv][(int64_t)row * (p.d / 32) + (c >> 2)] = dh;
         }
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = next[i];
     }
 }
 
 // Read: the rows of the slots as f32; a slot that the cache does not have is a row of zeros. A lane has four values of a row of keys and
-// of the row of values (eight, written 32 bytes apart, wrote each sector of level 2 twice), of several rows at a time.
+// of the row of values (eight, written 32 bytes apart, wrote each sector of level 2 twice); its place in a token stays, and
+// the block's tokens follow each other there, two at a time.
 template <int CT>
 __global__ void __launch_bounds__(256)
 kv_read_kernel(const __grid_constant__ CacheParams p) {
@@ -273,52 +286,37 @@ kv_read_kernel(const __grid_constant__ CacheParams p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, of_row = p.d / 4, of_tok = p.heads * of_row;
     const int64_t t0 = (int64_t)blockIdx.x * p.per_block;
-    const int n_tok = (int)min((int64_t)p.per_block, p.n - t0), total = n_tok * of_tok;
+    const int n_tok = (int)min((int64_t)p.per_block, p.n - t0);
     find_rows(p, t0, n_tok, s_row);
     __syncthreads();
-    constexpr int kAt = 2;
-    for (int base = 0; base < total; base += kAt * 256) {
-        uint2 w[kAt][2];
-        float d[kAt][2];
-        int where[kAt];
-#pragma unroll
-        for (int k = 0; k < kAt; k++) {
-            const int u = min(base + k * 256 + tid, total - 1), tok = part(u, p.of_tok_inv), at = u - tok * of_tok, head = part(at, p.of_row_inv), c = at - head * of_row;
-            const int first = s_row[tok], row = first + head * p.page_size;
-            where[k] = first < 0 ? -1 : c;
-#pragma unroll
-            for (int kv = 0; kv < 2; kv++) {
-                w[k][kv] = make_uint2(0u, 0u);
-                d[k][kv] = 0.0f;
-                if (first < 0) continue;
-                if constexpr (CT == KRK_CUDA_KV_F16) {
-                    w[k][kv] = *reinterpret_cast<const uint2 *>(p.pool[kv] + ((int64_t)row * p.d + 4 * c) * 2);
-                } else {
-                    w[k][kv].x = *reinterpret_cast<const uint32_t *>(CT == KRK_CUDA_KV_Q8 ? p.pool[kv] + (int64_t)row * p.d + 4 * c : p.pool[kv] + (int64_t)row * (p.d / 2) + 16 * (c >> 3) + 4 * (c & 3));
-                    d[k][kv] = __half2float(p.scale[kv][(int64_t)row * (p.d / 32) + (c >> 3)]);
-                }
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < kAt; k++) {
-            const int u = base + k * 256 + tid;
-            if (u >= total) continue;
+    for (int at = tid; at < of_tok; at += 256) {
+        const int head = part(at, p.of_row_inv), c = at - head * of_row;
+        const int in_head = head * p.page_size;
+        const int of_pool = CT == KRK_CUDA_KV_F16 ? 2 * p.d : CT == KRK_CUDA_KV_Q8 ? p.d : p.d / 2;   // bytes of a row
+        const int in_row = CT == KRK_CUDA_KV_F16 ? 8 * c : CT == KRK_CUDA_KV_Q8 ? 4 * c : 16 * (c >> 3) + 4 * (c & 3);
+#pragma unroll 2
+        for (int tok = 0; tok < n_tok; tok++) {
+            const int first = s_row[tok], row = first + in_head;
 #pragma unroll
             for (int kv = 0; kv < 2; kv++) {
                 float x[4] = {};
-                if (where[k] >= 0) {
+                if (first >= 0) {
+                    const uint8_t *from = p.pool[kv] + (int64_t)row * of_pool + in_row;
                     if constexpr (CT == KRK_CUDA_KV_F16) {
-                        const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&w[k][kv].x)), f1 = __half22float2(*reinterpret_cast<const __half2 *>(&w[k][kv].y));
+                        const uint2 w = *reinterpret_cast<const uint2 *>(from);
+                        const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&w.x)), f1 = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
                         x[0] = f0.x, x[1] = f0.y, x[2] = f1.x, x[3] = f1.y;
                     } else {
+                        const uint32_t w = *reinterpret_cast<const uint32_t *>(from);
+                        const float d = __half2float(p.scale[kv][(int64_t)row * (p.d / 32) + (c >> 3)]);
                         // a byte under the exponent of 2^23 is 2^23 more than its value
-                        const uint32_t q = CT == KRK_CUDA_KV_Q8 ? w[k][kv].x ^ 0x80808080u : ((where[k] & 4) ? w[k][kv].x >> 4 : w[k][kv].x) & 0x0F0F0F0Fu;
+                        const uint32_t q = CT == KRK_CUDA_KV_Q8 ? w ^ 0x80808080u : ((c & 4) ? w >> 4 : w) & 0x0F0F0F0Fu;
                         const float off = CT == KRK_CUDA_KV_Q8 ? 8388608.0f + 128.0f : 8388608.0f + 8.0f;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) x[i] = __fmul_rn(d[k][kv], __fsub_rn(__uint_as_float(__byte_perm(q, 0x4B000000u, 0x7650u | i)), off));
+                        for (int i = 0; i < 4; i++) x[i] = __fmul_rn(d, __fsub_rn(__uint_as_float(__byte_perm(q, 0x4B000000u, 0x7650u | i)), off));
                     }
                 }
-                st4(p.y[kv] + (t0 * of_tok + u) * 4, x);   // (a token's rows follow each other)
+                st4(p.y[kv] + ((t0 + tok) * of_tok + at) * 4, x);
             }
         }
     }
@@ -338,12 +336,11 @@ CacheParams cache_params(const krk_cuda_kv_cache &cache, const int64_t *slots, i
     p.page_size = cache.page_size;
     return p;
 }
-// Tokens of a block: a block for each up to `blocks` blocks an SM, then equal shares, as far as part() divides.
-void set_per_block(CacheParams &p, int blocks, int of_head, int values) {
-    const int64_t of_row = p.d / values, of_tok = of_head * p.heads * of_row, per = p.n / (blocks * (int64_t)sm_count()), most = 0xFFFFFFFFll / (of_tok * of_tok);
-    p.per_block = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(per, most), kMostTokens));
+// Tokens of a block: a block for each up to `blocks` blocks an SM, then equal shares.
+void set_per_block(CacheParams &p, int blocks, int values) {
+    const int64_t of_row = p.d / values, per = p.n / (blocks * (int64_t)sm_count());
+    p.per_block = (int)std::max<int64_t>(1, std::min<int64_t>(per, kMostTokens));
     p.of_row_inv = (uint32_t)((0x100000000ll + of_row - 1) / of_row);
-    p.of_tok_inv = (uint32_t)((0x100000000ll + of_tok - 1) / of_tok);
 }
 
 #define KRK_DISPATCH_KV(type, kernel) \
@@ -377,7 +374,7 @@ int launch_kv_append(const krk_cuda_kv_cache &cache, const float *k, const float
     CacheParams p = cache_params(cache, slots, n);
     p.x[0] = k, p.x[1] = v;
     p.x_stride[0] = k_stride, p.x_stride[1] = v_stride;
-    set_per_block(p, 4, 2, 8);
+    set_per_block(p, 4, 8);
     const int64_t blocks = (n + p.per_block - 1) / p.per_block;
     if (blocks > INT32_MAX) return KRK_CUDA_ESHAPE;
     return launched(launch_overlapped(KRK_DISPATCH_KV(cache.type, kv_append_kernel), dim3((unsigned)blocks), dim3(256), st, p));
@@ -386,7 +383,7 @@ int launch_kv_append(const krk_cuda_kv_cache &cache, const float *k, const float
 int launch_kv_read(const krk_cuda_kv_cache &cache, float *k, float *v, const int64_t *slots, int64_t n, cudaStream_t st) {
     CacheParams p = cache_params(cache, slots, n);
     p.y[0] = k, p.y[1] = v;
-    set_per_block(p, 16, 1, 4);
+    set_per_block(p, 16, 4);
     const int64_t blocks = (n + p.per_block - 1) / p.per_block;
     if (blocks > INT32_MAX) return KRK_CUDA_ESHAPE;
     return launched(launch_overlapped(KRK_DISPATCH_KV(cache.type, kv_read_kernel), dim3((unsigned)blocks), dim3(256), st, p));
