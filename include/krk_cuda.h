@@ -315,8 +315,9 @@ int krk_cuda_kv_read(const struct krk_cuda_kv_cache *host_cache, void *k_f32, vo
  *   out = sum_p w_p v_p / (sum_p w_p + exp(sink - max)),  w_p = exp(s_p - max),  s = scale * q . k  (softcap > 0: softcap tanh(s / softcap))
  * A row that sees nothing, or only scores of -infinity, gives zeros. Query head h reads key head h / (n_heads / n_kv_heads). Position p of a sequence
  * is place p % page_size of page page_table[s][p / page_size]; positions of a page that the cache does not have are not seen, and
- * neither are those from max_kv_len on. Rows of out that no sequence has stay as they were. Infinities and NaN at positions
- * that a row does not see do not reach it. The same call on the same device gives the same bits. The place of Backend::attention
+ * neither are those from max_kv_len on. Rows of out that no sequence has stay as they were; out does not overlap q. Infinities and NaN
+ * at positions that a row does not see do not reach it; infinite keys and values that it sees may come out as NaN where the formula has an
+ * infinity or a weight of zero. The same call on the same device gives the same bits. The place of Backend::attention
  * (include/krk/backend.hpp:1111). head_dim 64, 96, 128, 192 or 256. */
 #define KRK_CUDA_MAX_DRAFT 64
 struct krk_cuda_attention {

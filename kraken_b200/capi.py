@@ -425,7 +425,13 @@ class KvCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.struct = KvCacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if kind != KV_F16 else 0, v_scale.data_ptr() if kind != KV_F16 else 0,
                                     kind, d, heads, page_size, pages)
-        self.addr = C.addressof(self.struct)
+        self.addr, self.device = C.addressof(self.struct), k.device
+
+    def on(self, t) -> int:
+        """The struct's address, for a call with tensors of the cache's device."""
+        if t.device != self.device:
+            raise ValueError(f"the cache is on {self.device}, the tensors of the call on {t.device}")
+        return self.addr
 
     @classmethod
     def empty(cls, kind: int, n_pages: int, n_kv_heads: int, page_size: int, head_dim: int, device="cuda") -> "KvCache":
@@ -441,12 +447,12 @@ class KvCache:
 
 def kv_append(cache: KvCache, k, v, slots, stream=None) -> None:
     """Writes k and v [tokens, kv heads, d] into positions slots (int64, page * page size + place; -1: left out) of the cache."""
-    _fc.kv_append(cache.addr, k, v, slots, stream)
+    _fc.kv_append(cache.on(k), k, v, slots, stream)
 
 
 def kv_read(cache: KvCache, slots, k_out=None, v_out=None, stream=None):
     """The rows of slots (int64) as f32: (k, v) [slots, kv heads, d]; a slot that the cache does not have gives zeros."""
-    return _fc.kv_read(cache.addr, slots, k_out, v_out, stream)
+    return _fc.kv_read(cache.on(slots), slots, k_out, v_out, stream)
 
 
 def attention_tree(q, cache: KvCache, q_start, kv_len, page_table, max_q: int, tree=None, scale=None, softcap: float = 0.0, window: int = 0,
@@ -455,7 +461,7 @@ def attention_tree(q, cache: KvCache, q_start, kv_len, page_table, max_q: int, t
     q_start[s + 1] (int32), at most max_q <= 64, which are the last of its kv_len[s] (int32) positions; position p is place p % page
     size of page page_table[s][p // page size] (int32). tree (int64 / uint64 [rows]): bit j set where the row sees its sequence's j-th
     row; None: itself and those before it. Returns out, f32 like q; rows that no sequence has are left as they were."""
-    return _fc.attention_tree(q, cache.addr, q_start, kv_len, page_table, max_q, tree, scale, softcap, window, sinks, max_kv_len, out, workspace, stream)
+    return _fc.attention_tree(q, cache.on(q), q_start, kv_len, page_table, max_q, tree, scale, softcap, window, sinks, max_kv_len, out, workspace, stream)
 
 
 def allgather_sum(gather_peer_ptrs, flag_peer_ptrs, my_rank: int, slot_stride: int, part, out, stream=None):

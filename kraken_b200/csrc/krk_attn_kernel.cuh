@@ -357,7 +357,7 @@ attn_kernel(const __grid_constant__ Params p) {
         const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_piece = lane >> 4;
         const int v_row = kQuant ? k_row : (lane & 7) + (lane >> 4) * 8, v_piece = kQuant ? lane >> 4 : (lane >> 3) & 1;
         auto sees = [&](const Rows &r, int pos) {
-            return pos < sq.before ? pos >= r.first : pos < sq.len && ((r.mask >> (pos - sq.before)) & 1) != 0;
+            return pos < sq.len && (pos < sq.before ? pos >= r.first : ((r.mask >> (pos - sq.before)) & 1) != 0);
         };
 
         // (compiled for each number of tiles of columns that has rows: branches around single products cost twice the time)
@@ -373,7 +373,7 @@ attn_kernel(const __grid_constant__ Params p) {
                 if (row0 < 0) continue;
                 const uint32_t k_at = ring + stage * S::kStage, v_at = k_at + kChunk * RB;
                 const uint8_t *k_mem = ring_mem + stage * S::kStage;
-                const bool masked = pos0 + kChunk > sq.before || pos0 < all_from;
+                const bool masked = pos0 + kChunk > min(sq.before, sq.len) || pos0 < all_from;
 
                 // ---- scores: [n][h][c], h: position g or g + 8
                 float sc[NA][2][NC];

@@ -57,7 +57,7 @@ struct Params {
 // sums, which a second kernel adds up in the order of the CTAs (the same bits every time; finding the items anew in that kernel took it 14 to 24 us).
 // (With equal units for all tiles, and none for items, a CTA whose share was 40 items of one tile took four times as long as the others.)
 struct Seq {
-    int q0, n_q, len, before;   // first row of q, drafted tokens, positions, positions before the drafted ones (may be negative)
+    int q0, n_q, len, before;   // first row of q, drafted tokens, positions that are looked at, positions before the drafted ones (may be negative, or beyond len)
     int blocks, tile0, tiles;   // blocks of rows; first tile that any row sees, tiles from there on (at least one where there are rows)
 };
 template <int R>
@@ -65,8 +65,9 @@ __device__ __forceinline__ Seq sequence(const Params &p, int s) {
     Seq q;
     q.q0 = p.q_start[s];
     q.n_q = min(max(p.q_start[s + 1] - q.q0, 0), p.max_q);
-    q.len = min(max(p.kv_len[s], 0), p.max_len);
-    q.before = q.len - q.n_q;
+    const int len = min(max(p.kv_len[s], 0), 1 << 30);
+    q.len = min(len, p.max_len);
+    q.before = len - q.n_q;
     q.blocks = (q.n_q * p.group + R - 1) / R;
     const int first = p.window > 0 ? max(0, q.before - p.window) : 0;   // (the shallowest row is at `before`, or a position less where its mask is empty)
     q.tile0 = min(first, max(q.len - 1, 0)) / tile_of(R);
@@ -230,7 +231,7 @@ __device__ __forceinline__ float norm_of(const Params &p, int head, float m, flo
         const float sink = p.sinks[head] * 1.44269504f;
         const float top = fmaxf(m, sink);
         keep = m == -INFINITY ? 0.0f : exp2f(m - top);
-        l = l * keep + (sink == -INFINITY ? 0.0f : exp2f(sink - top));
+        l = l * keep + (sink == -INFINITY ? 0.0f : sink == top ? 1.0f : exp2f(sink - top));
     }
     return l == 0.0f ? 0.0f : keep / l;
 }

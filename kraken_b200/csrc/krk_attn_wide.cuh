@@ -55,7 +55,7 @@ static __device__ __noinline__ uint32_t seen_of(const Rows *rows, int c0, int po
         const uint32_t w = *reinterpret_cast<const uint32_t *>(from + j * sizeof(Rows));
         seen |= (earlier ? (uint32_t)(pos >= (int)w) : (w >> (bit & 31)) & 1u) << j;
     }
-    return earlier || pos < len ? seen : 0u;
+    return pos < len ? seen : 0u;
 }
 
 struct WideMeta {
@@ -323,7 +323,7 @@ attn_wide_kernel(const __grid_constant__ Params p) {
                 const int hv = n_half + 2 * i + 1;
                 bar_wait(bar(meta.kv_full[hv % kSlots]), (hv / kSlots) & 1, gave_up, p.status);
                 const unsigned long long there = *reinterpret_cast<volatile unsigned long long *>(&meta.ok[hv % kSlots]);
-                const bool masked = pos0 + kWideTile > before || pos0 < all_from || there != 0x0101010101010101ull, mine = (there >> (8 * (place_in / kChunk))) & 1;
+                const bool masked = pos0 + kWideTile > min(before, sq.len) || pos0 < all_from || there != 0x0101010101010101ull, mine = (there >> (8 * (place_in / kChunk))) & 1;
                 bar_wait(bar(meta.s_full[n_tile & 1]), (n_tile >> 1) & 1, gave_up, p.status);
                 tc_after();
                 uint32_t v[16];

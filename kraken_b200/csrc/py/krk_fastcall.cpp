@@ -577,8 +577,8 @@ bool listed(const at::Tensor *t, const at::Tensor *first, at::ScalarType type, i
 // f32 [rows][heads][d], heads behind each other; the stride of the rows is free.
 bool headed(const at::Tensor *t, const at::Tensor *first, int64_t rows, int64_t heads, int64_t d, const char *name) {
     if (!typed(t, first, at::kFloat, name)) return false;
-    if (t->dim() == 3 && (rows < 0 || t->size(0) == rows) && (heads < 0 || t->size(1) == heads) && t->size(2) == d && (d <= 1 || t->stride(2) == 1) &&
-        (t->size(1) <= 1 || t->stride(1) == d))
+    if (t->dim() == 3 && (rows < 0 || t->size(0) == rows) && (heads < 0 || t->size(1) == heads) && t->size(2) == d &&
+        (t->numel() == 0 || ((d <= 1 || t->stride(2) == 1) && (t->size(1) <= 1 || t->stride(1) == d))))
         return true;
     PyErr_Format(PyExc_ValueError, "%s: expected [rows][heads][values] with the heads of a row behind each other", name);
     return false;
@@ -587,7 +587,7 @@ bool headed(const at::Tensor *t, const at::Tensor *first, int64_t rows, int64_t 
 bool tabled(const at::Tensor *t, const at::Tensor *first, at::ScalarType type, int64_t rows, const char *name) {
     if (!t) return true;
     if (!typed(t, first, type, name)) return false;
-    if (t->dim() == 2 && (rows < 0 || t->size(0) == rows) && (t->size(1) <= 1 || t->stride(1) == 1)) return true;
+    if (t->dim() == 2 && (rows < 0 || t->size(0) == rows) && (t->numel() == 0 || t->size(1) <= 1 || t->stride(1) == 1)) return true;
     PyErr_Format(PyExc_ValueError, "%s: expected [rows][elements]", name);
     return false;
 }
@@ -712,6 +712,7 @@ PyObject *attention_tree(PyObject *, PyObject *const *a, Py_ssize_t n) {
     t.q_start = Args::ptr(start), t.kv_len = Args::ptr(len), t.page_table = Args::ptr(table), t.tree = Args::ptr(tree), t.sinks = Args::ptr(sinks);
     t.q_stride = row_stride(q), t.out_stride = row_stride(out);
     t.n_seq = (int)n_seq, t.n_heads = (int)heads, t.max_q = (int)max_q, t.table_width = (int)table->size(1), t.window = (int)window;
+    if (rows == 0) return given_or_made(a[12], made);   // (no sequence has a row)
     if (ws) {
         if (!typed(ws, q, at::kByte, "workspace")) return nullptr;
         if (!ws->is_contiguous()) return refuse("workspace: expected contiguous bytes"), nullptr;

@@ -40,11 +40,12 @@ def attention(q, k, v, seen, scale, softcap=0.0, sinks=None):
 
     The tolerance counts, for each output, against sum(w |v|) / sum(w) =: a, with s the scores:
       queries in two f16 terms 2^-22, products summed in f32 in steps of 16 (a rounding of 2^-23 each, truncations included): a score is off by
-      at most (2^-22 + (d / 16 + 4) 2^-23) scale sum|q||k|; the score times log2(e), its difference from the maximum and the exponential
-      round by 2^-24 (|s| + |max|) + 2^-22, tanh by 2^-21 of the softcap; a weight is off by the sum of these, in numerator and denominator;
+      at most (2^-22 + (d / 16 + 4) 2^-23) scale sum|q||k|; the score times log2(e), its difference from the maximum (a second time where that rises) and the exponential
+      round by 2 2^-24 (|s| + |max|) + 2^-22, tanh by 2^-21 of the softcap; a weight is off by the sum of these, in numerator and denominator;
       weights in two f16 terms 2^-22 each, times 2^14 under a power of two up to twice the values' greatest scale; f16 ends in steps of 2^-24, so a weight
-      is off by 2^-25 / 2^14 of twice the greatest value besides, whatever its own size: 2^-38 max|v| for each position that is seen (what is left of a
-      sum where the heavy positions' values are zeros: scale of a weight of one, divided by the sum of weights as the output is); sums over the positions: a step of 16 of each of four warps and the joining of up to 300 parts, 2^-23 each.
+      is off by 2^-25 / 2^14 of twice the greatest value besides, whatever its own size (what is left of a
+      sum where the heavy positions' values are zeros); with many rows weights are times 2^11 under a reference that the greatest weight is up to 2^4
+      above: 2^-25 / 2^11 of the greatest value, 2^-35 max|v| for each position that is seen covers both; sums over the positions: a step of 16 of each of four warps and the joining of up to 300 parts, 2^-23 each.
     """
     rows, heads, d = q.shape
     group = heads // k.shape[1]
@@ -68,7 +69,7 @@ def attention(q, k, v, seen, scale, softcap=0.0, sinks=None):
                 out[r, h] = w @ vv[at] / total
                 a = w @ np.abs(vv[at]) / total
                 off = (2.0 ** -22 + (d / 16 + 4) * 2.0 ** -23) * size.max() + 2.0 ** -24 * 2 * (np.abs(s).max() + abs(top)) + 2.0 ** -22 + softcap * 2.0 ** -21
-                floor = len(at) * 2.0 ** -38 * np.nan_to_num(np.abs(v.astype(np.float64)), nan=0.0, posinf=0.0).max() * np.exp(s.max() - top) / total
+                floor = len(at) * 2.0 ** -35 * np.nan_to_num(np.abs(v.astype(np.float64)), nan=0.0, posinf=0.0).max() * np.exp(s.max() - top) / total
                 tol[r, h] = a * (2 * off + 2.0 ** -21 + (n / 16 + 300) * 2.0 ** -23) + floor
     return out, tol
 

@@ -280,3 +280,121 @@ def test_strides_streams_and_graphs(cuda):
     graphs[1].replay()
     torch.cuda.synchronize()
     assert (outs[1].cpu().numpy() == b.check()).all()
+
+
+# ---- more than 32 rows to a key head over an f16 cache, heads of 96 and 128 values, contexts that are divided: the form on tcgen05
+
+
+@pytest.mark.parametrize("d,group,n_q,page", [(128, 4, 9, 16), (128, 1, 33, 48), (96, 8, 8, 16), (96, 5, 13, 64), (128, 7, 64, 32), (128, 16, 4, 16), (96, 2, 64, 16), (128, 3, 17, 272)])
+def test_many_rows(cuda, d, group, n_q, page):
+    rng = np.random.default_rng(d + n_q)
+    counts = [n_q, 1, n_q - 1, 0, n_q, 3]
+    lens = [n_q + 2100, 900, n_q - 1, 40, n_q + 131, 129]
+    Batch(cuda, rng, 0, d, 2, group, page, counts, lens, [tree_masks(rng, c) for c in counts]).check()
+
+
+@pytest.mark.parametrize("n", [1, 40, 127, 128, 129, 255, 257, 1000, 5000])
+def test_many_rows_over_lengths(cuda, n):
+    rng = np.random.default_rng(n)
+    Batch(cuda, rng, 0, 128, 1, 4, 16, [min(n, 40), 12], [n, 600], None).check()
+
+
+def test_many_rows_windows_sinks_and_limits(cuda):
+    rng = np.random.default_rng(21)
+    b = Batch(cuda, rng, 0, 128, 2, 4, 16, [12, 30, 1], [1500, 130, 700], [tree_masks(rng, 12), tree_masks(rng, 30), [1]], q_size=6.0)
+    sinks = (5 * rng.standard_normal(8)).astype(np.float32)
+    sinks[0], sinks[3] = -np.inf, 60.0
+    for window in (0, 64, 100, 513, 1400):
+        b.check(window=window)
+        b.check(window=window, sinks=sinks, softcap=25.0)
+    b.check(scale=-0.1)
+    b.masks[1][4] = b.masks[1][9] = 0
+    b.lens[1] = 30
+    got = b.check()
+    assert (got[12 + 4] == 0).all() and (got[12 + 9] == 0).all()
+
+
+def test_many_rows_values_of_unlike_size(cuda):
+    """The greatest scores late, and far above the first ones: references that have to follow."""
+    rng = np.random.default_rng(22)
+    b = Batch(cuda, rng, 0, 128, 1, 4, 16, [10], [3000], None, q_size=3.0)
+    for t in range(0, 2900, 97):
+        page = b.table[0, t // 16]
+        b.raw[0][0][page, 0, t % 16] *= np.float16(1 + t / 300)
+    got = b.check()
+    assert (got == b.check()).all()
+    for q_size in (1e-20, 1e4):
+        b.q = (q_size * rng.standard_normal(b.q.shape)).astype(np.float32)
+        b.check(scale=1.0 / q_size / 11)
+
+
+def test_many_rows_what_is_not_seen(cuda):
+    rng = np.random.default_rng(23)
+    counts, lens = [12, 1], [905, 1003]
+    masks = [[1, 3, 5, 9, 24 | 1, 1 << 5, 3 << 5, 1 << 7, 1 << 8, 1 << 9, 1 << 10, 1 << 11], [1]]
+    b = Batch(cuda, rng, 0, 128, 1, 4, 16, counts, lens, masks)
+    clean = b.check(window=200)
+    vals = np.array([np.nan, np.inf, -np.inf, 65504], np.float16)
+    for a, _ in b.raw:
+        keep = np.zeros((len(a), 16), bool)
+        for s, (c, n) in enumerate(zip(counts, lens)):
+            for p in range(max(0, n - c - 200), n):
+                keep[b.table[s, p // 16], p % 16] = True
+        a[...] = np.where(keep[:, None, :, None], a, vals[rng.integers(0, 4, a.shape)])
+    assert (b.check(window=200) == clean).all()
+    p = lens[0] - 12 + np.array([1, 6])   # seen by row 1, by row 6
+    for a, _ in b.raw:
+        a[b.table[0, p // 16], 0, p % 16, 5] = np.nan
+    got = b.check(window=200)
+    assert np.isnan(got[1]).any() and np.isnan(got[6]).any() and np.isfinite(np.delete(got, [1, 6], 0)).all()
+    b.raw[0][0][b.table[0, p // 16], 0, p % 16, 5] = 0     # the values alone
+    got = b.check(window=200)
+    assert np.isnan(got[[1, 6], :, 5]).all() and np.isnan(got).sum() == 8
+
+
+def test_many_rows_bad_pages_graphs_and_limits(cuda):
+    import torch
+    rng = np.random.default_rng(24)
+    b = Batch(cuda, rng, 0, 128, 2, 4, 16, [10, 16], [1700, 100], [tree_masks(rng, 10), tree_masks(rng, 16)])
+    b.table[0, 3], b.table[0, 20], b.table[0, 106], b.table[1, 2] = -1, 1 << 30, len(b.raw[0][0]), -5
+    want = b.check()
+    cache, args, q = b.cache(), b.args(), b.dev(b.q)
+    out = torch.zeros_like(q)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        cuda.attention_tree(q, cache, out=out, **args)
+    for _ in range(2):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert (out.cpu().numpy()[:26] == want).all()
+    assert cuda.device_status() == 0
+
+
+@pytest.mark.parametrize("kind,n_q", [("f16", 3), ("q8", 3), ("f16", 40)])
+def test_positions_behind_max_kv_len(cuda, kind, n_q):
+    """The drafted tokens stay the last of kv_len; what lies behind the limit is not seen."""
+    rng = np.random.default_rng(25)
+    b = Batch(cuda, rng, KINDS[kind], 128, 1, 2, 16, [n_q, 1], [1200, 300], [tree_masks(rng, n_q), [1]])
+    for limit in (1190, 900, 299, 3):
+        out = b.dev(np.zeros_like(b.q))
+        cuda.attention_tree(b.dev(b.q), b.cache(), scale=0.1, max_kv_len=limit, out=out, **b.args())
+        got, row = out.cpu().numpy(), 0
+        for s, (c, n) in enumerate(zip(b.counts, b.lens)):
+            p = np.arange(n)
+            at = b.table[s, p // 16], slice(None), p % 16
+            k, v = (decode(np.asarray(a)[at], None if x is None else np.asarray(x)[at], b.kind) for a, x in b.raw)
+            want, tol = attention(b.q[row:row + c], k, v, visible(b.masks[s], c, n) & (p < limit), 0.1)
+            assert (np.abs(got[row:row + c] - want) <= tol + 1e-30).all()
+            row += c
+
+
+def test_no_rows_and_infinite_sinks(cuda):
+    import torch
+    rng = np.random.default_rng(26)
+    b = Batch(cuda, rng, 0, 64, 1, 2, 16, [0, 0], [50, 0], None, extra_rows=0)
+    assert cuda.attention_tree(b.dev(b.q), b.cache(), **b.args()).shape == (0, 2, 64)
+    b = Batch(cuda, rng, 0, 64, 1, 2, 16, [2], [50], None, extra_rows=0)
+    sinks = torch.tensor([float("inf"), 0.0], device="cuda")
+    got = cuda.attention_tree(b.dev(b.q), b.cache(), sinks=sinks, **b.args())
+    assert (got[:, 0] == 0).all() and (got[:, 1] != 0).all()

@@ -129,6 +129,8 @@ def test_python_checks_what_it_is_given():
     k = torch.zeros((3, 2, 64))
     with pytest.raises(ValueError, match="GPU"):
         capi.kv_append(c, k, k, torch.zeros(3, dtype=torch.long))
+    with pytest.raises(ValueError, match="on cpu"):
+        capi.kv_append(c, k.to("meta"), k, torch.zeros(3, dtype=torch.long))
     with pytest.raises(ValueError):
         capi.qk_norm_rope(k, None, None, None)
     with pytest.raises(ValueError):
