@@ -28,7 +28,7 @@ constexpr int kSoftThreads = 32 * kSoftWarps;
 constexpr int kSlots = 4;                       // half tiles (keys, values in turn) in shared memory
 constexpr uint32_t kTmemCols = 512, kTmemO = 256;   // scores at 0 and 128, outputs at 256
 constexpr float kHeadroom = 4.0f;               // log2: scores stay below m + this
-constexpr float kWeightUp = 11.0f;              // log2
+constexpr float kWeightUp = 2048.0f;            // 2^11: weights in two f16 terms
 constexpr long long kWaitLimit = 4000000000ll;  // clocks
 
 template <int D>
@@ -61,7 +61,7 @@ static __device__ __noinline__ uint32_t seen_of(const Rows *rows, int c0, int po
 struct WideMeta {
     unsigned long long kv_full[kSlots], kv_empty[kSlots], s_full[2], s_empty[2], q_full, p_full, pv_done;
     alignas(16) Rows rows[kWideRows];
-    // of columns, read four at a time: a score's log2 is product * scale; base: the weights' 2^11 less the reference m
+    // of columns, read four at a time: a score's log2 is product * scale; base: less the reference m (the weights' 2^11 in it took three bits of the greatest ones)
     alignas(16) float scale[kWideRows];
     alignas(16) float one[kWideRows];
     alignas(16) float base[kWideRows];
@@ -302,7 +302,7 @@ attn_wide_kernel(const __grid_constant__ Params p) {
                 meta.rows[r] = row;
                 meta.one[r] = 1.0f;
                 meta.m[r] = -INFINITY;
-                meta.base[r] = kWeightUp;
+                meta.base[r] = 0.0f;
                 meta.to[r] = walk.begins && walk.ends ? p.out + (int64_t)row.q_row * p.out_stride + row.head * D : part_row<D, kWideRows>(p, blockIdx.x, walk.begins ? 1 : 0, r);
             }
             async_fence();
@@ -352,7 +352,7 @@ attn_wide_kernel(const __grid_constant__ Params p) {
                     }
                     scale = meta.one;
                 }
-                // x = score - m + 11, which is the weight's log2, and whether one is too far above the reference
+                // x = score - m, the weight's log2, and whether one is too far above the reference
                 float x[16], most = -INFINITY;
                 if (has) {
 #pragma unroll
@@ -365,7 +365,7 @@ attn_wide_kernel(const __grid_constant__ Params p) {
                         most = fmaxf(fmaxf(fmaxf(most, x[j]), fmaxf(x[j + 1], x[j + 2])), x[j + 3]);
                     }
                 }
-                if (has && group_any(group, pending || most > kWeightUp + kHeadroom)) {
+                if (has && group_any(group, pending || most > kHeadroom)) {
                     // ---- new references: the columns' maxima over the 128 lanes
                     const int c = c0 + (lane & 15);
                     {
@@ -382,7 +382,7 @@ attn_wide_kernel(const __grid_constant__ Params p) {
                         const float top = fmaxf(fmaxf(meta.red[0][c], meta.red[1][c]), fmaxf(meta.red[2][c], meta.red[3][c]));
                         const float now = fmaxf(old, top - from);
                         meta.m[c] = now;
-                        meta.base[c] = now == -INFINITY ? kWeightUp : kWeightUp - now;
+                        meta.base[c] = now == -INFINITY ? 0.0f : -now;
                         meta.more[c] = meta.base[c] - from;
                         meta.corr[c] = now == -INFINITY ? 1.0f : ex2(old - now);
                         none = now == -INFINITY;
@@ -442,7 +442,7 @@ attn_wide_kernel(const __grid_constant__ Params p) {
                         uint32_t hi[4], lo[4];
 #pragma unroll
                         for (int c = 0; c < 8; c += 2) {
-                            const float w0 = ex2(x[j + c]), w1 = ex2(x[j + c + 1]);
+                            const float w0 = kWeightUp * ex2(x[j + c]), w1 = kWeightUp * ex2(x[j + c + 1]);
                             l[j + c] += w0;
                             l[j + c + 1] += w1;
                             split(w0, w1, hi[c / 2], lo[c / 2]);
@@ -493,7 +493,7 @@ attn_wide_kernel(const __grid_constant__ Params p) {
                 const float sum = across(l, [](float a, float b) { return a + b; });
                 if (lane < 16) meta.red[lanes][c] = sum;
                 group_sync(group);
-                constexpr float kDown = 1.0f / 2048.0f;   // 2^-kWeightUp
+                constexpr float kDown = 1.0f / kWeightUp;
                 if (lanes == 0 && lane < 16) {
                     const float all = kDown * ((meta.red[0][c] + meta.red[1][c]) + (meta.red[2][c] + meta.red[3][c]));
                     float keep;
