@@ -154,12 +154,12 @@ int launch_logits_adjust(float *out, const float *logits, const krk_cuda_adjust 
     p.bias_ids = static_cast<const int32_t *>(a.bias_ids), p.bias = static_cast<const float *>(a.bias), p.bias_len = static_cast<const int32_t *>(a.bias_len);
     p.rep = static_cast<const float *>(a.rep), p.freq = static_cast<const float *>(a.freq), p.pres = static_cast<const float *>(a.pres);
     p.mask = static_cast<const uint32_t *>(a.mask), p.mask_row = static_cast<const int32_t *>(a.mask_row);
-    p.hist_n = (int)a.hist_n, p.bias_n = (int)a.bias_n, p.n_masks = a.mask ? a.n_masks : 0;
+    p.hist_n = a.hist ? (int)a.hist_n : 0, p.bias_n = a.bias ? (int)a.bias_n : 0, p.n_masks = a.mask ? a.n_masks : 0;
     const bool vec = ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) & 15) == 0 &&
                      (a.n_rows == 1 || (a.stride % 4 == 0 && a.out_stride % 4 == 0));
     // A block looks through the whole lists for its slice: 4096 values a block, but 1024 where the longer slices would leave SMs without one
     // (64 rows of 128,256 with up to 4096 ids each: 38.6 us with 1024, 23 with 4096, 26 with 8192).
-    const bool packed = a.hist_n < 65536 && a.bias_n < 65535, wide = packed && (a.n_vocab + 4095) / 4096 * a.n_rows >= 2 * sm_count();
+    const bool packed = p.hist_n < 65536 && p.bias_n < 65535, wide = packed && (a.n_vocab + 4095) / 4096 * a.n_rows >= 2 * sm_count();
     const int threads = wide ? 512 : 256, slice = wide ? 4096 : 1024;
     const int64_t slices = (a.n_vocab + slice - 1) / slice;
     if (slices * a.n_rows > INT32_MAX) return KRK_CUDA_ESHAPE;

@@ -131,3 +131,19 @@ def test_before_the_top_k(cuda):
     assert int(ids[0]) == best and all(int(i) % 100 == 0 for i in ids) and torch.isfinite(mass).all()
     y = cuda.logits_adjust(x, hist=torch.tensor([[best, best]], dtype=torch.int32, device="cuda"), pres=torch.full((1,), 100.0, device="cuda"), mask=mask)
     assert best not in cuda.logits_topk(y, 5)[0].tolist()
+
+
+@pytest.mark.parametrize("rows,n", [(1, 1000), (70, 40000)])
+def test_lists_that_are_not_there(cuda, rows, n):
+    """Sizes, strides and other parts of a list whose pointer is NULL are not looked at."""
+    import ctypes as C
+
+    import torch
+    x = torch.from_numpy(np.random.default_rng(n).standard_normal((rows, n)).astype(np.float32)).cuda()
+    ones = torch.ones(rows, device="cuda")
+    ids = torch.zeros((rows, 8), dtype=torch.int32, device="cuda")
+    a = cuda.Adjust(n_rows=rows, n_vocab=n, stride=n, out_stride=n, hist_n=4096, hist_stride=4096, rep=ones.data_ptr(), freq=ones.data_ptr(), pres=ones.data_ptr(),
+                    bias_ids=ids.data_ptr(), bias_n=8, bias_stride=8, mask_row=ids.data_ptr(), n_masks=3, mask_stride=0)
+    out = torch.empty_like(x)
+    assert cuda.lib.krk_cuda_logits_adjust(out.data_ptr(), x.data_ptr(), C.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out, x)
