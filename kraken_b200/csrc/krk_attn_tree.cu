@@ -81,7 +81,8 @@ Form form_of(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a) {
     // ragged sequences of 4 to 32 rows, 8 bits: 214 us against 157; blocks of 8: 207). Over f16 caches more than 32 rows go to the
     // tensor memory's form, heads of 96 and 128 values over contexts that are divided (4 sequences of 16,000, 64 rows: 99 us against 145, 128
     // rows 166 against 296; 32 rows 80 against 94 there, but 27 against 23 at 2000; heads of 64: 91 against 87, 152 against 157).
-    const bool wide = type == KRK_CUDA_KV_F16 && rows > 32 && (d == 96 || d == 128) && !f.whole;
+    // A cache without pages has no memory: that form's copies of rows that are not there have a row's address all the same.
+    const bool wide = type == KRK_CUDA_KV_F16 && rows > 32 && (d == 96 || d == 128) && !f.whole && cache.n_pages > 0;
     f.block = wide ? kWideRows : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
     f.rows = (int)(rows < f.block ? rows : f.block);
     const int64_t tiles = (a.max_kv_len + tile_of(f.block) - 1) / tile_of(f.block);

@@ -398,3 +398,22 @@ def test_no_rows_and_infinite_sinks(cuda):
     sinks = torch.tensor([float("inf"), 0.0], device="cuda")
     got = cuda.attention_tree(b.dev(b.q), b.cache(), sinks=sinks, **b.args())
     assert (got[:, 0] == 0).all() and (got[:, 1] != 0).all()
+
+
+@pytest.mark.parametrize("kind,n_q,width", [(0, 3, 4), (0, 40, 100), (1, 3, 100), (2, 40, 4)])
+def test_a_cache_without_pages(cuda, kind, n_q, width):
+    """No memory behind it: nothing is seen."""
+    import ctypes as C
+
+    import torch
+    q = torch.ones((n_q, 2, 128), device="cuda")
+    out = torch.full_like(q, 7.0)
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    start, length, table = i32(0, n_q), i32(1500), torch.zeros((1, width), dtype=torch.int32, device="cuda")
+    cache = cuda.KvCacheStruct(type=kind, head_dim=128, n_kv_heads=1, page_size=16, n_pages=0)
+    a = cuda.Attention(q_start=start.data_ptr(), kv_len=length.data_ptr(), page_table=table.data_ptr(), q_stride=256, out_stride=256, n_seq=1, n_heads=2,
+                       max_q=n_q, table_width=width, scale=0.1)
+    size = cuda.lib.krk_cuda_attention_tree_workspace_bytes(C.byref(cache), C.byref(a))
+    ws = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
+    assert cuda.lib.krk_cuda_attention_tree(out.data_ptr(), q.data_ptr(), C.byref(cache), C.byref(a), ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream) == 0
+    assert (out == 0).all()
