@@ -312,7 +312,7 @@ int krk_cuda_kv_read(const struct krk_cuda_kv_cache *host_cache, void *k_f32, vo
  * kv_len[s] positions, the last of which are those rows' own (already written). A row sees every position before them and, of
  * them, the j-th where bit j of its mask is set (`tree` NULL: itself and those before it). Its own position is that of the first drafted
  * token plus the bits of its mask, less one; with a window it sees, before the drafted tokens, the positions nearer than `window`.
- *   out = sum_p w_p v_p / (sum_p w_p + exp(sink - max)),  w_p = exp(s_p - max),  s = scale * q . k  (softcap > 0: softcap tanh(s / softcap))
+ *   out = sum_p w_p v_p / (sum_p w_p + exp(sink - max)),  w_p = exp(s_p - max),  s = scale * q . k  (softcap > 0, finite: softcap tanh(s / softcap))
  * A row that sees nothing, or only scores of -infinity, gives zeros. Query head h reads key head h / (n_heads / n_kv_heads). Position p of a sequence
  * is place p % page_size of page page_table[s][p / page_size]; positions of a page that the cache does not have are not seen, and
  * neither are those from max_kv_len on. Rows of out that no sequence has stay as they were; out does not overlap q. Infinities and NaN

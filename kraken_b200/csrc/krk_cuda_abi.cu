@@ -1,5 +1,6 @@
 // The extern "C" surface declared in include/krk_cuda.h: argument checks, then a launch.
 // Nothing here computes on the host.
+#include <cfloat>
 #include <atomic>
 #include <cstring>
 #include <mutex>
@@ -485,7 +486,7 @@ static int check_attention(const krk_cuda_kv_cache *cache, const krk_cuda_attent
     const int64_t room = (int64_t)a.table_width * cache->page_size;
     if (a.max_kv_len == 0) a.max_kv_len = room;
     if (a.max_kv_len > room || a.max_kv_len > (1ll << 30)) return KRK_CUDA_ESHAPE;
-    if (a.window < 0 || (a.window > 0 && a.window < KRK_CUDA_MAX_DRAFT) || !(a.softcap >= 0.0f)) return KRK_CUDA_EARG;
+    if (a.window < 0 || (a.window > 0 && a.window < KRK_CUDA_MAX_DRAFT) || !(a.softcap >= 0.0f && a.softcap <= FLT_MAX)) return KRK_CUDA_EARG;
     return KRK_CUDA_OK;
 }
 

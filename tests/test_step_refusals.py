@@ -143,3 +143,9 @@ def test_python_checks_what_it_is_given():
         capi.KvCache(capi.KV_Q8, c.k, c.v, c.k_scale, c.v_scale.transpose(0, 1))
     with pytest.raises(KeyError):
         capi.KvCache(7, c.k, c.v)
+
+
+def test_a_softcap_without_end():
+    a = attention(softcap=float("inf"))   # (infinity times tanh(0) is no score)
+    assert L.krk_cuda_attention_tree(P, P, C.byref(cache()), C.byref(a), P, 1 << 40, None) == EARG
+    assert L.krk_cuda_attention_tree_workspace_bytes(C.byref(cache()), C.byref(a)) == 0
