@@ -12,6 +12,9 @@
 // neighbouring columns of one product, else products in a row. Cache values enter exactly: f16 as they are; 8- and 4-bit quants as whole
 // numbers, whose block scales multiply the f32 sums of a block's products (keys) and the weights before they are split (values; there
 // under the power of two of the greatest scale met so far, which the sums are rescaled to like to a new maximum).
+//
+// Measured, 16 sequences of 8192 positions, 8 key heads of 128 values, four rows each (bytes of the cache a second): f16 6.0 TB/s, 8 bits 4.1,
+// 4 bits 2.1. In 8 and 4 bits the latency of the dependent steps from quants to operands bounds it: 15 % fewer instructions changed nothing.
 #pragma once
 
 #include <atomic>

@@ -13,8 +13,9 @@
 // at most 2^4, times 2^11 it is below the f16 range), which a vote finds; only then are columns reduced and sums rescaled.
 //
 // Warps 0 - 15: softmax, four groups that have 16 columns each; 16 - 18: copies of keys and values into a ring of half tiles (16 bytes
-// a lane, asynchronous); 19: issue of the products. (Two groups with 32 columns each took half as long again: a group's phases wait for each
-// other, and there was less to do meanwhile.) Waits are bounded as in krk_gemm_tc.cu: one that gives up raises the status word, and
+// a lane, asynchronous); 19: issue of the products. (Two groups with 32 columns each: an item cost 17 us beside its tiles instead of 11, for
+// its phases wait for each other.) Four sequences of up to 16,384 positions and 64 drafted
+// tokens, 32 heads of 128 values on 8: 119 us (both forms side by side: form_of in krk_attn_tree.cu). Waits are bounded as in krk_gemm_tc.cu: one that gives up raises the status word, and
 // the CTA runs to its end without waiting again and frees its tensor memory.
 #pragma once
 
@@ -618,7 +619,7 @@ attn_wide_kernel(const __grid_constant__ Params p) {
                 tc_after();
 #pragma unroll
                 for (int k = 0; k < kWideTile / 16; k++) {
-                    const uint32_t a = desc_lo(base + slot * W::kHalf + 2048 * k, W::kCols > 1 ? kWideTile * 128 : 0);
+                    const uint32_t a = desc_lo(base + slot * W::kHalf + 2048 * k, kWideTile * 128);
                     const uint32_t b = desc_lo(base + W::kP + 2048 * k, kWideTile * 128);
                     product(tmem + kTmemO, a, kDescHi, b, kDescHi, pv, i > 0 || k > 0, elected);
                 }
