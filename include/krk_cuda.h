@@ -308,7 +308,7 @@ int krk_cuda_kv_append(const struct krk_cuda_kv_cache *host_cache, const void *k
 int krk_cuda_kv_read(const struct krk_cuda_kv_cache *host_cache, void *k_f32, void *v_f32, const void *slots_i64, int64_t n, void *stream);
 
 /* Attention of the newest tokens of n_seq sequences over their cache, for a decode step (one token each) and for a tree of
- * drafted tokens (up to KRK_CUDA_MAX_DRAFT each). Sequence s has rows q_start[s] .. q_start[s + 1] of q, at most max_q, and
+ * drafted tokens (up to KRK_CUDA_MAX_DRAFT each). Sequence s has rows q_start[s] .. q_start[s + 1] of q (they have to be there), at most max_q, and
  * kv_len[s] positions, the last of which are those rows' own (already written). A row sees every position before them and, of
  * them, the j-th where bit j of its mask is set (`tree` NULL: itself and those before it). Its own position is that of the first drafted
  * token plus the bits of its mask, less one; with a window it sees, before the drafted tokens, the positions nearer than `window`.

@@ -749,6 +749,7 @@ PyObject *logits_adjust(PyObject *, PyObject *const *a, Py_ssize_t n) {
         return nullptr;
     if ((bias == nullptr) != (ids == nullptr) || (bias && (bias->size(1) != ids->size(1) || (rows > 1 && bias->stride(0) != ids->stride(0)))))
         return refuse("bias and bias_ids: expected two tables of one shape and layout"), nullptr;
+    if (mask && mask->size(1) < (vocab + 31) / 32) return refuse("mask: expected a bit for each logit of a row"), nullptr;
     Where where(*x, a[12] != Py_None, st);
     at::Tensor made, out_one;
     if (!out) {

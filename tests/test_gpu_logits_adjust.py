@@ -147,3 +147,13 @@ def test_lists_that_are_not_there(cuda, rows, n):
     out = torch.empty_like(x)
     assert cuda.lib.krk_cuda_logits_adjust(out.data_ptr(), x.data_ptr(), C.byref(a), torch.cuda.current_stream().cuda_stream) == 0
     assert torch.equal(out, x)
+
+
+def test_masks_narrower_than_a_row(cuda):
+    import torch
+    x = torch.zeros((2, 1000), device="cuda")
+    table = torch.full((2, 64), -1, dtype=torch.int32, device="cuda")
+    for mask in (table[:, 40:], table[:, :31], table[1:, 33:64]):   # 24, 31 and 31 words where 32 are read; rows 64 apart
+        with pytest.raises(ValueError):
+            cuda.logits_adjust(x, mask=mask)
+    assert torch.equal(cuda.logits_adjust(x, mask=table[:, 32:]), x)
