@@ -24,7 +24,7 @@ struct RopeParams {
     const int32_t *pos;
     const float *inv_freq;
     int64_t n_tok;
-    int heads[2], d, rot, norm, chunks;
+    int heads[2], d, rot, norm, chunks, trips;   // chunks: runs of a token's heads; trips: of the loop over the longest of them
     float eps;
 };
 
@@ -72,7 +72,9 @@ qk_norm_rope_kernel(const __grid_constant__ RopeParams p) {
             sincospif((float)(2.0 * (turn - rint(turn))), &sn[i], &cs[i]);
         }
     }
-    for (int hb = h0; hb < h1; hb += kRopeHeads) {
+    // (The runs of a warp's groups may differ by a head, and the sums below name all lanes of the warp: every group makes as many trips as
+    // the longest run takes; heads behind its own are zeros that are not written. 2048 tokens: 16.5 us, 16.4 with a trip count for each group.)
+    for (int trip = p.trips, hb = h0; trip > 0; trip--, hb += kRopeHeads) {
 #pragma unroll
         for (int u = 0; u < kRopeHeads; u++)
 #pragma unroll
@@ -363,6 +365,7 @@ int launch_qk_norm_rope(float *q_out, float *k_out, const float *q, const float 
     // At most as many groups as run at once, 1024 threads an SM, each with as many heads of a token as that leaves; a head each for few tokens.
     const int64_t groups = (int64_t)sm_count() * 1024 / lanes, want = groups / r.n_tok;
     p.chunks = (int)(want < 1 ? 1 : want < all ? want : all);
+    p.trips = ((all + p.chunks - 1) / p.chunks + kRopeHeads - 1) / kRopeHeads;
     const int64_t blocks = (r.n_tok * p.chunks + 256 / lanes - 1) / (256 / lanes);
     if (blocks > INT32_MAX) return KRK_CUDA_ESHAPE;
     auto kernel = r.interleaved ? (lanes == 8 ? qk_norm_rope_kernel<8, true> : lanes == 16 ? qk_norm_rope_kernel<16, true> : qk_norm_rope_kernel<32, true>)

@@ -59,6 +59,24 @@ def test_norm_and_rotation(cuda, interleaved, tokens, heads, kv, d, rot, norm, f
         assert (np.abs(kd.cpu().numpy() - want) <= tol + 1e-30).all()
 
 
+@pytest.mark.parametrize("tokens,heads,kv,d", [(475, 32, 8, 128), (592, 32, 8, 128), (600, 28, 4, 128), (1024, 32, 8, 128), (1500, 32, 8, 128), (1500, 28, 4, 64), (300, 28, 4, 256), (700, 27, 0, 96)])
+def test_norm_over_runs_of_unlike_length(cuda, tokens, heads, kv, d):
+    """Token counts at which the groups of lanes of one warp walk runs of heads that differ by one (148 SMs: 2 and 3 heads at 475 and 592 tokens of 40
+    heads, 4 and 5 at 1024), so that one of them is through a trip of the loop earlier."""
+    import torch
+    rng = np.random.default_rng(tokens)
+    q, k = (rng.standard_normal((tokens, h, d)).astype(np.float32) for h in (heads, kv))
+    pos = np.arange(tokens, dtype=np.int32)
+    freq = (10000.0 ** (-np.arange(0, d, 2) / d)).astype(np.float32)
+    wq, wk = (rng.uniform(0.5, 1.5, d).astype(np.float32) for _ in range(2))
+    dev = lambda a: torch.from_numpy(a).cuda()  # noqa: E731
+    got = cuda.qk_norm_rope(dev(q), dev(k) if kv else None, dev(pos), dev(freq), dev(wq), dev(wk))
+    for y, x, w in ((got[0], q, wq), (got[1], k, wk)):
+        if y is not None:
+            want, tol = rope_plain(x, pos, freq, w, True, 1e-6, False)
+            assert (np.abs(y.cpu().numpy() - want) <= tol + 1e-30).all()
+
+
 def test_norm_of_zeros_and_negative_positions(cuda):
     import torch
     q = torch.zeros((2, 1, 64), device="cuda")
