@@ -273,7 +273,7 @@ struct krk_cuda_rope {
     int64_t n_tok;
     int64_t q_stride, k_stride;       /* floats from a token to the next, multiples of 4; heads follow each other */
     int64_t q_out_stride, k_out_stride;
-    int n_heads, n_kv_heads;          /* n_kv_heads 0: no keys (k and k_out are not looked at) */
+    int n_heads, n_kv_heads;          /* n_kv_heads 0: no keys (k, k_out and k_weight are not looked at) */
     int head_dim, rot_dim;            /* multiples of 8, head_dim <= 256, rot_dim <= head_dim */
     int norm, interleaved;            /* norm 0: the rotation alone */
     float eps;

@@ -353,7 +353,7 @@ void set_per_block(CacheParams &p, int blocks, int values) {
 int launch_qk_norm_rope(float *q_out, float *k_out, const float *q, const float *k, const krk_cuda_rope &r, cudaStream_t st) {
     RopeParams p;
     p.x[0] = q, p.x[1] = k, p.y[0] = q_out, p.y[1] = k_out;
-    p.w[0] = static_cast<const float *>(r.q_weight), p.w[1] = static_cast<const float *>(r.k_weight);
+    p.w[0] = static_cast<const float *>(r.q_weight), p.w[1] = r.n_kv_heads > 0 ? static_cast<const float *>(r.k_weight) : nullptr;   // (an odd last head's partner is the first key head, there or not)
     p.x_stride[0] = r.q_stride, p.x_stride[1] = r.k_stride, p.y_stride[0] = r.q_out_stride, p.y_stride[1] = r.k_out_stride;
     p.pos = static_cast<const int32_t *>(r.pos);
     p.inv_freq = static_cast<const float *>(r.inv_freq);

@@ -88,6 +88,16 @@ def test_norm_of_zeros_and_negative_positions(cuda):
     assert (np.abs(cuda.qk_norm_rope(q, None, pos, freq)[0].cpu().numpy() - want) <= tol).all()
 
 
+@pytest.mark.parametrize("heads", [1, 5])
+def test_weights_of_keys_that_are_not_there(cuda, heads):
+    """Heads are worked on in pairs: of an odd number of query heads the last one's partner would be the first key head."""
+    import torch
+    q = torch.randn((3, heads, 64), device="cuda")
+    pos, freq = torch.arange(3, dtype=torch.int32, device="cuda"), torch.rand(32, device="cuda")
+    want = cuda.qk_norm_rope(q, None, pos, freq)[0]
+    assert torch.equal(cuda.qk_norm_rope(q, None, pos, freq, None, torch.full((64,), float("nan"), device="cuda"))[0], want)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("tokens,kv,d,page", [(1, 8, 128, 16), (5, 3, 32, 48), (37, 2, 96, 16), (130, 1, 256, 64), (2500, 2, 64, 32)])
 def test_append_and_read(cuda, kind, tokens, kv, d, page):
