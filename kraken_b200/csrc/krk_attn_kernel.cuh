@@ -118,8 +118,8 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// The soft limit of a score, in the log2 domain.
-static __device__ __noinline__ float capped(float x, float cap) { return cap * 1.44269504f * tanhf(x / cap); }
+// The soft limit of a score, in the log2 domain (log2(e) goes to the tangent: times a limit beyond 2.3e38 it would be infinite).
+static __device__ __noinline__ float capped(float x, float cap) { return cap * (1.44269504f * tanhf(x / cap)); }
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 half2_of(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
 // Two f32 as the sum of two f16 each.

@@ -417,3 +417,16 @@ def test_a_cache_without_pages(cuda, kind, n_q, width):
     ws = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
     assert cuda.lib.krk_cuda_attention_tree(out.data_ptr(), q.data_ptr(), C.byref(cache), C.byref(a), ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream) == 0
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("kind,n_q", [("f16", 3), ("q8", 3), ("q4", 3), ("f16", 20)])
+@pytest.mark.parametrize("softcap", [1e30, 3e38])
+def test_soft_limits_far_above_the_scores(cuda, kind, n_q, softcap):
+    """The formula is the one without a limit there. A score over such a limit lies below the normal numbers: half a step of the quotient and
+    two of the tangent, 2.5 2^-149, come back times the limit (3e38 is below 2^128) as 1.25 2^-20 at most, two products as 2^-23 of the score each;
+    attention()'s tolerance counts 2^-22 and 2^-23 of the score beside others, so that six of it hold both."""
+    rng = np.random.default_rng(27)
+    b = Batch(cuda, rng, KINDS[kind], 128, 1, 4, 16, [n_q, 1], [900, 30], [tree_masks(rng, n_q), [1]])
+    want, tol, rows = b.want(0.1)
+    got = cuda.attention_tree(b.dev(b.q), b.cache(), scale=0.1, softcap=softcap, **b.args()).cpu().numpy()
+    assert (np.abs(got[:rows] - want[:rows]) <= 6 * tol[:rows] + 1e-30).all()
