@@ -317,8 +317,9 @@ int krk_cuda_kv_read(const struct krk_cuda_kv_cache *host_cache, void *k_f32, vo
  * is place p % page_size of page page_table[s][p / page_size]; positions of a page that the cache does not have are not seen, and
  * neither are those from max_kv_len on. Rows of out that no sequence has stay as they were; out does not overlap q. Infinities and NaN
  * at positions that a row does not see do not reach it; infinite keys and values that it sees may come out as NaN where the formula has an
- * infinity or a weight of zero. The same call on the same device gives the same bits. The place of Backend::attention
- * (include/krk/backend.hpp:1111). head_dim 64, 96, 128, 192 or 256. */
+ * infinity or a weight of zero. Queries and weights enter the products with 22 bits each, and what a weight adds ends at 2^-35 of the greatest
+ * value that the row sees (KV_Q8, KV_Q4: that any row of its block of up to 16 rows of a key head sees); sums are f32. The same call on the same
+ * device gives the same bits. The place of Backend::attention (include/krk/backend.hpp:1111). head_dim 64, 96, 128, 192 or 256. */
 #define KRK_CUDA_MAX_DRAFT 64
 struct krk_cuda_attention {
     const void *q_start;              /* int32 [n_seq + 1] */

@@ -11,7 +11,7 @@
 // and so do the weights of a step (times 2^14: terms far below the maximum keep their bits). Up to four rows the two terms are
 // neighbouring columns of one product, else products in a row. Cache values enter exactly: f16 as they are; 8- and 4-bit quants as whole
 // numbers, whose block scales multiply the f32 sums of a block's products (keys) and the weights before they are split (values; there
-// under the power of two of the greatest scale met so far, which the sums are rescaled to like to a new maximum).
+// under the power of two of the greatest scale that any row of the block has seen so far, which the sums are rescaled to like to a new maximum).
 //
 // Measured, 16 sequences of 8192 positions, 8 key heads of 128 values, four rows each (bytes of the cache a second): f16 6.0 TB/s, 8 bits 4.1,
 // 4 bits 2.1. In 8 and 4 bits the latency of the dependent steps from quants to operands bounds it: 15 % fewer instructions changed nothing.
@@ -181,7 +181,7 @@ struct Rows {   // of a block of rows, in shared memory
     int first;         // first position before the drafted tokens that it sees
     uint64_t mask;     // drafted tokens that it sees
     int q_row, head;   // its place in q and out; -1: no row
-    int pad[2];
+    uint64_t any;      // of the first row: drafted tokens that some row of the block sees
 };
 static_assert(sizeof(Rows) == 32, "Shape::kRows");
 
@@ -308,10 +308,16 @@ attn_kernel(const __grid_constant__ Params p) {
             row.mask = mask;
             row.q_row = ok ? sq.q0 + i : -1;
             row.head = kvh * p.group + rr - i * p.group;
-            row.pad[0] = row.pad[1] = 0;
+            row.any = 0;
             rows[r] = row;
         }
         __syncthreads();
+        if constexpr (kQuant) {   // (each warp for itself: they all write the same)
+            const uint64_t mask = rows[lane % R].mask;
+            const uint32_t lo = __reduce_or_sync(0xFFFFFFFFu, (uint32_t)mask), hi = __reduce_or_sync(0xFFFFFFFFu, (uint32_t)(mask >> 32));
+            if (lane == 0) rows[0].any = (uint64_t)hi << 32 | lo;
+            __syncwarp();
+        }
         // every row sees [all_from, before), none what is before any_from
         const int all_from = p.window > 0 ? sq.before + KRK_CUDA_MAX_DRAFT - p.window : 0, any_from = p.window > 0 ? sq.before - p.window : 0;
 
@@ -466,16 +472,25 @@ attn_kernel(const __grid_constant__ Params p) {
                 // ---- the scales of the values, and the power of two above them
                 float vd[2][NB], e_corr = 1.0f;
                 if constexpr (kQuant) {
-                    float most = 0.0f;
+                    float own[2] = {0.0f, 0.0f};   // the greatest of a position (a NaN is none)
     #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         scales<NB>(vd[h], k_mem + 2 * kChunk * RB + kChunk * SB + (g + 8 * h) * SB);
-                        const int pos = pos0 + g + 8 * h;
-                        if (!masked || (pos >= any_from && pos < sq.len)) {
     #pragma unroll
-                            for (int b = 0; b < NB; b++) most = fmaxf(most, fabsf(vd[h][b]));   // (a NaN is no maximum)
+                        for (int b = 0; b < NB; b++) own[h] = fmaxf(own[h], fabsf(vd[h][b]));
+                    }
+                    // What no row of the block sees does not count, nor does an infinite one that not all of them see (the values of those that do are
+                    // no numbers): f16 has sixteen bits below the two terms of a weight, and a scale far above the others takes them.
+                    if (masked) {
+                        const uint64_t any = rows[0].any;
+    #pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int pos = pos0 + g + 8 * h, bit = pos - sq.before;
+                            const bool counts = bit < 0 ? pos >= any_from : ((any >> (bit & 63)) & 1) != 0;
+                            own[h] = counts && pos < sq.len && own[h] <= 65504.0f ? own[h] : 0.0f;
                         }
                     }
+                    float most = fmaxf(own[0], own[1]);
     #pragma unroll
                     for (int o2 = 4; o2 < 32; o2 <<= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o2));
                     const int e = min(16, (int)(__float_as_uint(most) >> 23) - 126);

@@ -299,7 +299,7 @@ attn_wide_kernel(const __grid_constant__ Params p) {
                 row.mask = mask;
                 row.q_row = ok ? sq.q0 + i : -1;
                 row.head = walk.kvh * p.group + rr - i * p.group;
-                row.pad[0] = row.pad[1] = 0;
+                row.any = 0;
                 meta.rows[r] = row;
                 meta.one[r] = 1.0f;
                 meta.m[r] = -INFINITY;

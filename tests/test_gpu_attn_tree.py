@@ -430,3 +430,31 @@ def test_soft_limits_far_above_the_scores(cuda, kind, n_q, softcap):
     want, tol, rows = b.want(0.1)
     got = cuda.attention_tree(b.dev(b.q), b.cache(), scale=0.1, softcap=softcap, **b.args()).cpu().numpy()
     assert (np.abs(got[:rows] - want[:rows]) <= 6 * tol[:rows] + 1e-30).all()
+
+
+@pytest.mark.parametrize("kind", ["q8", "q4"])
+@pytest.mark.parametrize("group,n_q,bad", [(1, 4, np.inf), (2, 4, np.inf), (4, 4, np.inf), (1, 40, np.inf), (1, 40, 65504.0), (1, 40, 100.0), (4, 13, 65504.0)])
+def test_scales_that_a_row_does_not_see(cuda, kind, group, n_q, bad):
+    """Small values, and at a drafted token of another branch a scale many powers of two above theirs (an infinite one, or one that no row of the same
+    block of 16 sees): the rows that do not see it are as near to the formula as without it."""
+    rng = np.random.default_rng(28)
+    # the last token is the first one's sibling, all others are below the first one
+    masks = [[1] + [1 | 1 << i for i in range(1, n_q - 1)] + [1 << n_q - 1], [1]]
+    b = Batch(cuda, rng, KINDS[kind], 64, 1, group, 16, [n_q, 1], [n_q + 21, 700], masks)
+    x = rng.standard_normal(b.raw[1][0].shape[:3] + (64,)).astype(np.float32) * 2.0 ** -8
+    b.raw[1] = [np.array(a) for a in encode(x, KINDS[kind])]
+    b.check()
+    want, tol, rows = b.want(64 ** -0.5)
+    p = 21 + n_q - 1
+    block = [i for i in range(n_q - 1) if np.isinf(bad) or i * group // 16 < (n_q - 1) * group // 16]
+    for which in (slice(0, 1), slice(0, 2)):
+        keep = b.raw[1][1].copy()
+        b.raw[1][1][b.table[0, p // 16], 0, p % 16, which] = bad
+        got = cuda.attention_tree(b.dev(b.q), b.cache(), **b.args()).cpu().numpy()[:rows]
+        with np.errstate(invalid="ignore"):
+            ok = np.abs(got - want[:rows]) <= tol[:rows]
+        assert ok[block].all() and ok[n_q].all()
+        assert np.isfinite(got[n_q - 1]).all() == np.isfinite(bad)
+        if np.isinf(bad) and which == slice(0, 1):   # an infinite scale of one block leaves the other one's values
+            assert ok[:n_q, :, 32:].all()
+        b.raw[1][1] = keep
