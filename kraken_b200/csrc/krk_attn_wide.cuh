@@ -16,7 +16,9 @@
 // a lane, asynchronous); 19: issue of the products. (Two groups with 32 columns each: an item cost 17 us beside its tiles instead of 11, for
 // its phases wait for each other.) Four sequences of up to 16,384 positions and 64 drafted
 // tokens, 32 heads of 128 values on 8: 119 us (both forms side by side: form_of in krk_attn_tree.cu). Waits are bounded as in krk_gemm_tc.cu: one that gives up raises the status word, and
-// the CTA runs to its end without waiting again and frees its tensor memory.
+// the CTA runs to its end without waiting again, lets the products that it issued finish (bounded too) and frees its tensor memory. What is
+// in shared memory may be anything by then: the softmax's barriers, which have no bound, are met on the sequences' lengths alone, by all of
+// its threads, and what is found in a tile decides on no address that is not checked.
 #pragma once
 
 #include "krk_attn_kernel.cuh"
@@ -60,7 +62,7 @@ static __device__ __noinline__ uint32_t seen_of(const Rows *rows, int c0, int po
 }
 
 struct WideMeta {
-    unsigned long long kv_full[kSlots], kv_empty[kSlots], s_full[2], s_empty[2], q_full, p_full, pv_done;
+    unsigned long long kv_full[kSlots], kv_empty[kSlots], s_full[2], s_empty[2], q_full, p_full, pv_done, drained;
     alignas(16) Rows rows[kWideRows];
     // of columns, read four at a time: a score's log2 is product * scale; base: less the reference m (the weights' 2^11 in it took three bits of the greatest ones)
     alignas(16) float scale[kWideRows];
@@ -111,6 +113,11 @@ __device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, volatile
     if (bar_try(bar, parity)) return;
     if (*gave_up) return;
     bar_wait_long(bar, parity, gave_up, status);
+}
+// The products in flight of a CTA that has given up.
+static __device__ __noinline__ void bar_wait_drained(uint32_t bar) {
+    const long long t0 = clock64();
+    while (!bar_try(bar, 0) && clock64() - t0 <= kWaitLimit) __nanosleep(32);
 }
 // The 128 threads of a group of softmax warps: meet, and learn whether any of them says so. All groups: meet.
 __device__ __forceinline__ bool group_any(int group, bool mine) {
@@ -208,6 +215,7 @@ attn_wide_kernel(const __grid_constant__ Params p) {
             bar_init(bar(meta.q_full), kSoftWarps);
             bar_init(bar(meta.p_full), kSoftWarps);
             bar_init(bar(meta.pv_done), 1);
+            bar_init(bar(meta.drained), 1);
             meta.gave_up = 0;
         }
         __syncwarp();
@@ -324,7 +332,8 @@ attn_wide_kernel(const __grid_constant__ Params p) {
                 const int hv = n_half + 2 * i + 1;
                 bar_wait(bar(meta.kv_full[hv % kSlots]), (hv / kSlots) & 1, gave_up, p.status);
                 const unsigned long long there = *reinterpret_cast<volatile unsigned long long *>(&meta.ok[hv % kSlots]);
-                const bool masked = pos0 + kWideTile > min(before, sq.len) || pos0 < all_from || there != 0x0101010101010101ull, mine = (there >> (8 * (place_in / kChunk))) & 1;
+                // masked: not all rows see all positions, by the lengths; holes: pages that are not there (zeros, which no row sees)
+                const bool masked = pos0 + kWideTile > min(before, sq.len) || pos0 < all_from, holes = there != 0x0101010101010101ull, mine = (there >> (8 * (place_in / kChunk))) & 1;
                 bar_wait(bar(meta.s_full[n_tile & 1]), (n_tile >> 1) & 1, gave_up, p.status);
                 tc_after();
                 uint32_t v[16];
@@ -343,8 +352,8 @@ attn_wide_kernel(const __grid_constant__ Params p) {
                 // What is rarely done has code of its own, in loops where it can be: code that is jumped over, or met for the first time, is
                 // fetched at the pace of thousands of clocks. It leaves log2 scores in place of the products.
                 const float *scale = meta.scale;
-                if (has && (masked || p.softcap > 0.0f)) {
-                    const uint32_t seen = !masked ? 0xFFFFu : !mine ? 0u : seen_of(meta.rows, c0, pos0 + place_in, before, sq.len);
+                if (has && (masked || holes || p.softcap > 0.0f)) {
+                    const uint32_t seen = !mine ? 0u : !masked ? 0xFFFFu : seen_of(meta.rows, c0, pos0 + place_in, before, sq.len);
 #pragma unroll
                     for (int j = 0; j < 16; j++) {
                         float x = __uint_as_float(v[j]) * meta.scale[c0 + j];
@@ -466,7 +475,9 @@ attn_wide_kernel(const __grid_constant__ Params p) {
                         tmem_loaded();
                         for (int j = 0; j < kWideTile; j++) {
                             if (!((meta.odd[j >> 5] >> (j & 31)) & 1)) continue;
-                            const int page = p.table[(size_t)walk.s * p.table_width + (pos0 + j) / p.page_size];   // (a page that is there: its values were)
+                            if (pos0 + j >= sq.len) continue;   // (its values were there, unless a wait gave up: the page likewise)
+                            const int page = p.table[(size_t)walk.s * p.table_width + (pos0 + j) / p.page_size];
+                            if (page < 0 || page >= p.n_pages) continue;
                             const int64_t row = ((int64_t)page * p.n_kv + walk.kvh) * p.page_size + (pos0 + j) % p.page_size;
                             const float y = dim < D ? __half2float(reinterpret_cast<const __half *>(p.v)[row * D + dim]) : 0.0f;
                             if (fabsf(y) <= 65504.0f) continue;
@@ -628,6 +639,10 @@ attn_wide_kernel(const __grid_constant__ Params p) {
             }
             n_tile += walk.tiles;
             n_half += 2 * walk.tiles;
+        }
+        if (*gave_up) {
+            products_commit(bar(meta.drained), elected);
+            bar_wait_drained(bar(meta.drained));
         }
     }
     tc_before();

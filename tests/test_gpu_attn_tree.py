@@ -458,3 +458,17 @@ def test_scales_that_a_row_does_not_see(cuda, kind, group, n_q, bad):
         if np.isinf(bad) and which == slice(0, 1):   # an infinite scale of one block leaves the other one's values
             assert ok[:n_q, :, 32:].all()
         b.raw[1][1] = keep
+
+
+def test_many_rows_holes_beside_infinite_values(cuda):
+    """Pages that are not there inside tiles that all rows see (of 128 positions), and an infinite value in such a tile: its place is no number, all
+    others are as they should be; a tile without a page."""
+    rng = np.random.default_rng(30)
+    b = Batch(cuda, rng, 0, 128, 2, 4, 16, [10, 16], [1700, 1100], [tree_masks(rng, 10), tree_masks(rng, 16)])
+    b.table[0, 20], b.table[0, 22], b.table[1, 16:24], b.table[1, 40] = -1, len(b.raw[0][0]), -1, 1 << 30
+    b.check()
+    p = 300   # (page 18, in the tile of pages 16 to 23)
+    b.raw[1][0][b.table[0, p // 16], :, p % 16, 77] = np.inf
+    got = b.check()
+    assert not np.isfinite(got[:10, :, 77]).any() and np.isfinite(np.delete(got, 77, 2)).all() and np.isfinite(got[10:]).all()
+    assert cuda.device_status() == 0
