@@ -301,7 +301,8 @@ struct krk_cuda_kv_cache {
 };
 /* New keys and values [n_tok][n_kv_heads][head_dim] f32 (strides in floats from a token to the next, multiples of 4; 16-byte
  * aligned) into positions slots[t] = page * page_size + place (int64). A token whose slot the cache does not have (-1, say) is
- * left out; of tokens with the same slot the last one stays. The place of Backend::kv_append (include/krk/backend.hpp:1107). */
+ * left out; of tokens with the same slot the last one stays. One launch up to 8191 tokens, beyond that one for about 4096 of them. The place of
+ * Backend::kv_append (include/krk/backend.hpp:1107). */
 int krk_cuda_kv_append(const struct krk_cuda_kv_cache *host_cache, const void *k_f32, const void *v_f32, int64_t k_stride, int64_t v_stride,
                        const void *slots_i64, int64_t n_tok, void *stream);
 /* The rows of slots[i] as f32 [n][n_kv_heads][head_dim] (16-byte aligned); one that the cache does not have is a row of zeros. */

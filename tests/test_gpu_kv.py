@@ -156,6 +156,28 @@ def test_slots_that_are_none_or_come_twice(cuda, kind):
     assert (gk == 0).all() and (gv == 0).all()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("tokens", [8191, 8192, 13001, 40000])
+def test_long_appends_go_in_pieces(cuda, kind, tokens):
+    """Whose number grows with the tokens (each piece is looked through for its own slots); of tokens of different pieces with one slot the last stays."""
+    import torch
+    gen = torch.Generator("cuda").manual_seed(tokens)
+    cache = cuda.KvCache.empty(KINDS[kind], 700, 1, 16, 32)
+    k = torch.randn((tokens, 1, 32), device="cuda", generator=gen)
+    slots = torch.randint(-300, 11500, (tokens,), device="cuda", generator=gen)
+    slots[0], slots[tokens // 2], slots[-1] = 77, 77, 77
+    before = cuda.launch_count()
+    cuda.kv_append(cache, k, -k, slots)
+    assert cuda.launch_count() - before == {8191: 1, 8192: 2, 13001: 3, 40000: 10}[tokens]
+    last = {s: i for i, s in enumerate(slots.tolist()) if 0 <= s < 11200}
+    gk, gv = (x.cpu().numpy() for x in cuda.kv_read(cache, torch.arange(11200, device="cuda")))
+    at = np.array(sorted(last))
+    x = k.cpu().numpy()[[last[s] for s in at.tolist()]]
+    for got, want in ((gk, x), (gv, -x)):
+        assert (got[at] == decode(*encode(want, KINDS[kind]), KINDS[kind]).astype(np.float32)).all()
+        assert (np.delete(got, at, 0) == 0).all()
+
+
 @pytest.mark.parametrize("kind", ["q8", "q4"])
 def test_infinities_and_nan_stay_in_their_block(cuda, kind):
     import torch
