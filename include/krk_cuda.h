@@ -278,7 +278,7 @@ struct krk_cuda_rope {
     int norm, interleaved;            /* norm 0: the rotation alone */
     float eps;
 };
-/* q_out / k_out may be q / k themselves (with the same stride), else they do not overlap them. 16-byte aligned. */
+/* q_out / k_out may be q / k themselves (with the same stride: KRK_CUDA_EARG otherwise), else they do not overlap them. 16-byte aligned. */
 int krk_cuda_qk_norm_rope(void *q_out_f32, void *k_out_f32, const void *q_f32, const void *k_f32, const struct krk_cuda_rope *host_rope,
                           void *stream);
 
@@ -363,8 +363,8 @@ int krk_cuda_logits_topk(const void *logits_f32, int64_t n, int k, const void *p
  * hist: int32 [n_rows][hist_n], each row's first hist_len[row] ids (NULL: all); the same id may come many times. bias_ids / bias:
  * [n_rows][bias_n], bias_len as hist_len; of an id that comes twice the last one holds. Ids outside the row (-1) are passed over. rep,
  * freq, pres: f32 [n_rows], NULL: 1, 0, 0. mask: one bit a token, [n_masks][mask_stride] words, row r under mask mask_row[r] (NULL: r);
- * a row whose number is none of them (-1) is not masked. Strides in elements. out may be logits. The struct is read before the
- * call returns; its pointers are device memory, NULL where a part is not wanted. */
+ * a row whose number is none of them (-1) is not masked. Strides in elements. out may be logits (with the same stride). The struct is
+ * read before the call returns; its pointers are device memory, NULL where a part is not wanted. */
 struct krk_cuda_adjust {
     int64_t n_rows, n_vocab, stride, out_stride;
     const void *hist, *hist_len;

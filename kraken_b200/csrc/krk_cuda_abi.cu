@@ -437,6 +437,7 @@ int krk_cuda_qk_norm_rope(void *q_out_f32, void *k_out_f32, const void *q_f32, c
     if (r->n_tok > 1 && ((q && (r->q_stride < (int64_t)r->n_heads * r->head_dim || r->q_out_stride < (int64_t)r->n_heads * r->head_dim)) ||
                          (k && (r->k_stride < (int64_t)r->n_kv_heads * r->head_dim || r->k_out_stride < (int64_t)r->n_kv_heads * r->head_dim))))
         return KRK_CUDA_ESHAPE;
+    if (r->n_tok > 1 && ((q && q_out_f32 == q_f32 && r->q_out_stride != r->q_stride) || (k && k_out_f32 == k_f32 && r->k_out_stride != r->k_stride))) return KRK_CUDA_EARG;
     if ((q && (!aligned(q_f32, 16) || !aligned(q_out_f32, 16))) || (k && (!aligned(k_f32, 16) || !aligned(k_out_f32, 16))) ||
         (r->norm && (!aligned(r->q_weight, 16) || !aligned(r->k_weight, 16))) || !aligned(r->pos, 4) || !aligned(r->inv_freq, 4))
         return KRK_CUDA_EALIGN;
@@ -523,6 +524,7 @@ int krk_cuda_logits_adjust(void *out_f32, const void *logits_f32, const krk_cuda
     if (!out_f32 || !logits_f32 || (a->bias && !a->bias_ids)) return KRK_CUDA_ENULL;
     if (a->n_rows > 1 && (a->stride < a->n_vocab || a->out_stride < a->n_vocab || (a->hist && a->hist_stride < a->hist_n) || (a->bias && a->bias_stride < a->bias_n)))
         return KRK_CUDA_ESHAPE;
+    if (a->n_rows > 1 && out_f32 == logits_f32 && a->out_stride != a->stride) return KRK_CUDA_EARG;   // (a row's place would be another one's)
     if (a->mask && a->mask_stride < (a->n_vocab + 31) / 32) return KRK_CUDA_ESHAPE;
     const void *const lists[] = {out_f32, logits_f32, a->hist, a->hist_len, a->rep, a->freq, a->pres, a->bias_ids, a->bias, a->bias_len, a->mask, a->mask_row};
     for (const void *p : lists)

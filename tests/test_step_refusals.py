@@ -149,3 +149,12 @@ def test_a_softcap_without_end():
     a = attention(softcap=float("inf"))   # (infinity times tanh(0) is no score)
     assert L.krk_cuda_attention_tree(P, P, C.byref(cache()), C.byref(a), P, 1 << 40, None) == EARG
     assert L.krk_cuda_attention_tree_workspace_bytes(C.byref(cache()), C.byref(a)) == 0
+
+
+def test_rows_in_place_keep_their_strides():
+    """A row written over another one's place before that one is read."""
+    Q, K = 1 << 40, 1 << 41
+    for r in (rope(q_out_stride=4100), rope(k_out_stride=1028)):
+        assert L.krk_cuda_qk_norm_rope(Q, K, Q, K, C.byref(r), None) == EARG
+    for a in (adjust(out_stride=104), adjust(stride=104)):
+        assert L.krk_cuda_logits_adjust(Q, Q, C.byref(a), None) == EARG
