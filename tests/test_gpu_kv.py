@@ -88,6 +88,23 @@ def test_norm_of_zeros_and_negative_positions(cuda):
     assert (np.abs(cuda.qk_norm_rope(q, None, pos, freq)[0].cpu().numpy() - want) <= tol).all()
 
 
+@pytest.mark.parametrize("far", [2000, 1 << 30])
+def test_sines_and_cosines(cuda, far):
+    """Of pairs (1, 0) nothing else is left: the f32 sine and cosine of a half turn's fraction are off by a unit in the last place at most, 2^-24 below 1;
+    the angle's rest is put right with one rounding, 2^-25."""
+    import torch
+    rng = np.random.default_rng(far)
+    pos = rng.integers(-far, far, 4096).astype(np.int32)
+    freq = rng.uniform(0.0, 1.0, 64).astype(np.float32)
+    q = torch.zeros((4096, 1, 128), device="cuda")
+    q[..., :64] = 1
+    got = cuda.qk_norm_rope(q, None, torch.from_numpy(pos).cuda(), torch.from_numpy(freq).cuda(), norm=False)[0].cpu().numpy()[:, 0]
+    # (64 bits: the product of 31 and 24 bits rounds 2^-53 of it, the division by a turn, on either side, twice that)
+    angle = pos.astype(np.float64)[:, None] * freq.astype(np.float64)
+    tol = 1.5 * 2.0 ** -24 + np.abs(angle).max() * 2.0 ** -52
+    assert np.abs(got[:, :64] - np.cos(angle)).max() <= tol and np.abs(got[:, 64:] - np.sin(angle)).max() <= tol
+
+
 @pytest.mark.parametrize("heads", [1, 5])
 def test_weights_of_keys_that_are_not_there(cuda, heads):
     """Heads are worked on in pairs: of an odd number of query heads the last one's partner would be the first key head."""
