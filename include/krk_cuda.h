@@ -329,7 +329,7 @@ struct krk_cuda_attention {
     const void *tree;                 /* uint64 [rows of q], or NULL */
     const void *sinks;                /* f32 [n_heads], or NULL */
     int64_t q_stride, out_stride;     /* floats from a token to the next, multiples of 4 */
-    int64_t max_kv_len;               /* of any sequence; 0: table_width * page_size */
+    int64_t max_kv_len;               /* of any sequence; 0: table_width * page_size. Under a wide table a closer limit spares short contexts a launch */
     int n_seq, n_heads, max_q, table_width;
     int window;                       /* 0: none; else 64 or more */
     float scale, softcap;

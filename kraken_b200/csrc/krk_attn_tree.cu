@@ -78,7 +78,9 @@ Form form_of(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a) {
     // Short contexts: a CTA walks a whole item, which costs less than the second kernel.
     f.whole = a.max_kv_len <= kWholeTiles * kTile;
     // Blocks as small as the rows, 16 of them at most: 32 with their outputs in 128 registers of a lane took longer than two blocks of 16 (48
-    // ragged sequences of 4 to 32 rows, 8 bits: 214 us against 157; blocks of 8: 207). Over f16 caches more than 32 rows go to the
+    // ragged sequences of 4 to 32 rows, heads of 128 in 8 bits: 214 us against 157; blocks of 8: 207; windows over heads of 64 in 4 bits: 29 against 24.6, blocks of 8 25.1).
+    // The longest sequence is not known here: by max_kv_len, or the table's width, short contexts under a wide table are divided (one token, 300
+    // positions, f16, a table for 131,072: 9.1 us, 8.0 with the limit given; 8 bits 8.6 and 8.4). Over f16 caches more than 32 rows go to the
     // tensor memory's form, heads of 96 and 128 values over contexts that are divided (4 sequences of 16,000, 64 rows: 99 us against 145, 128
     // rows 166 against 296; 32 rows 80 against 94 there, but 27 against 23 at 2000; heads of 64: 91 against 87, 152 against 157).
     // A cache without pages has no memory: that form's copies of rows that are not there have a row's address all the same.

@@ -21,7 +21,8 @@ constexpr int kWideRows = 64;             // the form on tcgen05 (krk_attn_wide.
 constexpr int kWideTile = 128;
 __host__ __device__ constexpr int tile_of(int r) { return r == kWideRows ? kWideTile : kTile; }
 // Units of work: of a tile of a block of R rows of which `rows` are there, and of an item beside its tiles (its queries, the joining of sums, the
-// fetching of code and data that nothing overlaps). About 0.6 us, measured with one item of one tile and one of 32 to a CTA.
+// fetching of code and data that nothing overlaps). About 0.6 us, measured with one item of one tile and one of 32 to a CTA, heads of 128 values in 8 bits
+// (the form on tcgen05: in f16). For other head sizes and types the shares are only about as equal; no result depends on them.
 __host__ __device__ constexpr int tile_units(int r, int rows) { return r == kWideRows ? (rows > 32 ? 4 : 3) : rows <= 8 ? 2 : 3; }
 __host__ __device__ constexpr int setup_units(int r) { return r == kWideRows ? 26 : 14; }
 constexpr int kWholeTiles = 8;            // up to so many tiles an item is not divided, see launch
