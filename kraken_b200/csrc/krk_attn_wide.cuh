@@ -641,14 +641,14 @@ attn_wide_kernel(const __grid_constant__ Params p) {
             n_tile += walk.tiles;
             n_half += 2 * walk.tiles;
         }
-        if (*gave_up) {
-            products_commit(bar(meta.drained), elected);
-            bar_wait_drained(bar(meta.drained));
-        }
     }
     tc_before();
     __syncthreads();
     tc_after();
+    if (warp == kSoftWarps + kCopyWarps && *gave_up) {   // (nobody waits any more, so this is the last word on it)
+        products_commit(bar(meta.drained), elected_lane());
+        bar_wait_drained(bar(meta.drained));
+    }
     if (warp == kSoftWarps + kCopyWarps) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
