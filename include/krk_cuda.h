@@ -340,6 +340,47 @@ size_t krk_cuda_attention_tree_workspace_bytes(const struct krk_cuda_kv_cache *h
 int krk_cuda_attention_tree(void *out_f32, const void *q_f32, const struct krk_cuda_kv_cache *host_cache,
                             const struct krk_cuda_attention *host_attention, void *workspace, size_t ws_bytes, void *stream);
 
+/* The same over chunks of prompts, for max_q of any size: a row sees itself and the positions before it (host_attention->tree is NULL), with a window,
+ * of one or more, only the nearest `window` of those. out and q are f32, or out f16 and q f32 or f16 (KRK_CUDA_X_F32, KRK_CUDA_X_F16; strides in
+ * elements, multiples of 4 of f32 and 8 of f16). f32: queries and weights enter the products as above. f16: queries and weights enter with 11 bits, and 8- and
+ * 4-bit keys and values rounded to f16 (infinite beyond its range); maxima and sums are f32. Meant for sequences with tens of new tokens and more; single tokens among them
+ * are taken too. A window that leaves a row nothing, and pages, lengths, infinities and rows of no sequence, are as above. */
+size_t krk_cuda_attention_chunk_workspace_bytes(const struct krk_cuda_kv_cache *host_cache, const struct krk_cuda_attention *host_attention, int out_dtype);
+int krk_cuda_attention_chunk(void *out, int out_dtype, const void *q, int q_dtype, const struct krk_cuda_kv_cache *host_cache,
+                             const struct krk_cuda_attention *host_attention, void *workspace, size_t ws_bytes, void *stream);
+
+/* The plan of a step from its requests' lengths. Sequence s has kv_before[s] positions and gets n_new[s] more (negative: 0), in the order of the
+ * sequences. Positions that begin a page take one from the stack of free pages, the last of its first n_free[0] entries first, and page_table[s] gets its number;
+ * where the stack is empty it gets -1. Positions beyond the table have no page. Written, all int32 but the slots:
+ *   q_start [n_seq + 1], kv_len [n_seq], last [n_seq]   as attention wants them (the new positions among kv_len); the row of a sequence's last token, -1: no new ones
+ *   positions [max_tok], slots int64 [max_tok]          of the tokens, as qk_norm_rope and kv_append want them; -1 slots where there is no page, and
+ *                                                       0 and -1 behind the last token
+ *   counts [4]                                          free pages left, pages that were missing, tokens, tokens beyond max_tok (they get nothing: the sequences end before them)
+ * n_free itself stays as it is (counts has its successor), so that a call that is repeated gives the same. The struct is read before the call returns. */
+struct krk_cuda_step {
+    const void *kv_before, *n_new;    /* int32 [n_seq] */
+    void *page_table;                 /* int32 [n_seq][table_width]: read and written */
+    const void *free_pages, *n_free;  /* int32 [free_cap], int32 [1] */
+    void *q_start, *kv_len, *last, *positions, *slots, *counts;
+    int64_t max_tok, free_cap;
+    int n_seq, table_width, page_size;
+};
+int krk_cuda_step_plan(const struct krk_cuda_step *host_step, void *stream);
+
+/* Between two blocks, for rows of n values:
+ *   h = residual + alpha * gate * P(x),  P(x) = x / sqrt(mean(x^2) + eps) * (offset + post_weight)  (post_norm 0: x),   y = h / sqrt(mean(h^2) + eps) * (offset + weight)
+ * h is f32, y f32 or, as the f16 X of krk_cuda_gemm, f16 (y_dtype). gate: a row for all (gate_stride 0) or one each. NULL: residual 0, gate and weights (with their offset) 1.
+ * h_out may be x or the residual (with the same stride), else nothing overlaps; h_out NULL: h is not wanted. Strides in elements. The place of
+ * Backend::rmsnorm with add_inplace before it (include/krk/backend.hpp:855, 1340). */
+struct krk_cuda_norm {
+    const void *residual, *gate, *post_weight, *weight;   /* f32 */
+    int64_t rows, n;                  /* n up to 65,536 */
+    int64_t x_stride, residual_stride, gate_stride, h_stride, y_stride;
+    int post_norm, y_dtype;
+    float alpha, eps, offset;
+};
+int krk_cuda_block_norm(void *y, void *h_out_f32, const void *x_f32, const struct krk_cuda_norm *host_norm, void *stream);
+
 /* ---- the steps either side of the output head ---- */
 
 /* Replaces Backend::embed (include/krk/backend.hpp:838; src/backend_cpu.cpp:746-778): out_f32[t] = decoded
@@ -376,6 +417,29 @@ struct krk_cuda_adjust {
     int64_t n_masks, mask_stride;
 };
 int krk_cuda_logits_adjust(void *out_f32, const void *logits_f32, const struct krk_cuda_adjust *host_adjust, void *stream);
+
+/* Drafted tokens against the target's probabilities. Sequence s has rows row_start[s] .. row_start[s + 1] of the target's f32 logits, one more than it has drafted
+ * tokens; row r judges draft[r], the last row of a sequence judges none. With p = softmax(row / temp[s]) and q the same of the drafter's row:
+ *   token t = draft[r] is accepted where accept_u[r] * q(t) < p(t); the first one that is not ends the sequence
+ *   in its place one is drawn from max(p - q, 0) (from p, where that leaves nothing), or, where all were accepted, from the last row's p:
+ *   the lowest i with  sum_{k <= i} w_k > sample_u[s] * sum w
+ * draft_logits NULL: the drafts are certain, q(t) = 1. temp[s] <= 0: greedy, a token is accepted where it is the lowest of the greatest logits, and that one stands in the place of
+ * the first one that is not. temp NULL: 1; draft_temp NULL: temp (one of 0 or less counts as 1). Written: tokens int32 [rows], the accepted tokens, the drawn one, -1 behind it; n_accepted int32 [n_seq];
+ * logprob f32 [rows] (may be NULL), the logarithm of p of what came out (greedy: under a temperature of 1), 0 beside a -1. Of a row with a NaN, an infinity or nothing
+ * but -infinity nothing is accepted or drawn (-1); a greedy one passes over NaN. Weights and sums of a drawn row have 64 bits. Rows of no sequence stay as they were. The
+ * workspace is scratch; calls that can overlap need one each. */
+struct krk_cuda_verify {
+    const void *row_start;            /* int32 [n_seq + 1] */
+    const void *draft;                /* int32 [n_rows] */
+    const void *accept_u, *sample_u;  /* f32 [n_rows], [n_seq], in [0, 1) */
+    const void *temp, *draft_temp;    /* f32 [n_seq] */
+    const void *draft_logits;         /* f32 [n_rows][n_vocab] */
+    int64_t n_rows, n_vocab, stride, draft_stride;
+    int n_seq;
+};
+size_t krk_cuda_verify_draft_workspace_bytes(const struct krk_cuda_verify *host_verify);
+int krk_cuda_verify_draft(void *tokens_i32, void *n_accepted_i32, void *logprob_f32, const void *logits_f32, const struct krk_cuda_verify *host_verify,
+                          void *workspace, size_t ws_bytes, void *stream);
 
 /* Expert-sharded FFN, exchange step: all-gather of partial sums over NVLink peer stores fused with the
  * rank-ordered sum that follows (no counterpart in the reference, which is single-device). part_f32
@@ -479,6 +543,11 @@ void krk_cuda_backend_kv_read(void *be, const struct krk_cuda_kv_cache *host_cac
 void krk_cuda_backend_attention_tree(void *be, void *out, const void *q, const struct krk_cuda_kv_cache *host_cache,
                                      const struct krk_cuda_attention *host_attention);
 void krk_cuda_backend_logits_adjust(void *be, void *out, const void *logits, const struct krk_cuda_adjust *host_adjust);
+void krk_cuda_backend_attention_chunk(void *be, void *out, int out_dtype, const void *q, int q_dtype, const struct krk_cuda_kv_cache *host_cache,
+                                      const struct krk_cuda_attention *host_attention);
+void krk_cuda_backend_step_plan(void *be, const struct krk_cuda_step *host_step);
+void krk_cuda_backend_block_norm(void *be, void *y, void *h_out, const void *x, const struct krk_cuda_norm *host_norm);
+void krk_cuda_backend_verify_draft(void *be, void *tokens, void *n_accepted, void *logprob, const void *logits, const struct krk_cuda_verify *host_verify);
 void krk_cuda_backend_silu_mul(void *be, void *out, const void *gate, const void *up, int64_t n, int64_t row_len,
                                float *host_row_scale);
 void krk_cuda_backend_gather_rows(void *be, void *dst, const void *src, const int32_t *rows, int64_t n_rows, int64_t n);

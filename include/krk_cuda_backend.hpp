@@ -19,6 +19,9 @@ struct krk_cuda_rope;        // krk_cuda.h
 struct krk_cuda_kv_cache;
 struct krk_cuda_attention;
 struct krk_cuda_adjust;
+struct krk_cuda_step;
+struct krk_cuda_norm;
+struct krk_cuda_verify;
 
 namespace krk_cuda {
 
@@ -102,6 +105,11 @@ public:
     void kv_read(const krk_cuda_kv_cache &cache, void *k, void *v, const i64 *slots, i64 n);
     void attention_tree(void *out, const void *q, const krk_cuda_kv_cache &cache, const krk_cuda_attention &attention);
     void logits_adjust(void *out, const void *logits, const krk_cuda_adjust &adjust);
+    // A step of prompts and drafted tokens around them: its plan, attention of chunks, norms between blocks, verification of the drafts.
+    void attention_chunk(void *out, int out_dtype, const void *q, int q_dtype, const krk_cuda_kv_cache &cache, const krk_cuda_attention &attention);
+    void step_plan(const krk_cuda_step &step);
+    void block_norm(void *y, void *h_out, const void *x, const krk_cuda_norm &norm);
+    void verify_draft(void *tokens, void *n_accepted, void *logprob, const void *logits, const krk_cuda_verify &verify);
 
     // The router on the device, in the interface's three steps (backend.hpp:934-986); all pointers device memory.
     bool router_softmax_supported() const { return true; }

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from typing import NamedTuple
 
 import torch   # before the extension, which links its libraries
 
@@ -80,6 +81,26 @@ class Adjust(C.Structure):
                 ("bias_n", _i64), ("bias_stride", _i64), ("mask", _vp), ("mask_row", _vp), ("n_masks", _i64), ("mask_stride", _i64)]
 
 
+
+class Step(C.Structure):
+    """struct krk_cuda_step"""
+    _fields_ = [("kv_before", _vp), ("n_new", _vp), ("page_table", _vp), ("free_pages", _vp), ("n_free", _vp), ("q_start", _vp), ("kv_len", _vp), ("last", _vp),
+                ("positions", _vp), ("slots", _vp), ("counts", _vp), ("max_tok", _i64), ("free_cap", _i64), ("n_seq", _int), ("table_width", _int), ("page_size", _int)]
+
+
+class Norm(C.Structure):
+    """struct krk_cuda_norm"""
+    _fields_ = [("residual", _vp), ("gate", _vp), ("post_weight", _vp), ("weight", _vp), ("rows", _i64), ("n", _i64), ("x_stride", _i64), ("residual_stride", _i64),
+                ("gate_stride", _i64), ("h_stride", _i64), ("y_stride", _i64), ("post_norm", _int), ("y_dtype", _int), ("alpha", C.c_float), ("eps", C.c_float),
+                ("offset", C.c_float)]
+
+
+class Verify(C.Structure):
+    """struct krk_cuda_verify"""
+    _fields_ = [("row_start", _vp), ("draft", _vp), ("accept_u", _vp), ("sample_u", _vp), ("temp", _vp), ("draft_temp", _vp), ("draft_logits", _vp), ("n_rows", _i64),
+                ("n_vocab", _i64), ("stride", _i64), ("draft_stride", _i64), ("n_seq", _int)]
+
+
 # name -> (restype, argtypes); the list tests/ checks against the header.
 SIGNATURES = {
     "krk_cuda_strerror": (C.c_char_p, [_int]),
@@ -124,6 +145,12 @@ SIGNATURES = {
     "krk_cuda_kv_read": (_int, [C.POINTER(KvCacheStruct), _vp, _vp, _vp, _i64, _vp]),
     "krk_cuda_attention_tree_workspace_bytes": (_sz, [C.POINTER(KvCacheStruct), C.POINTER(Attention)]),
     "krk_cuda_attention_tree": (_int, [_vp, _vp, C.POINTER(KvCacheStruct), C.POINTER(Attention), _vp, _sz, _vp]),
+    "krk_cuda_attention_chunk_workspace_bytes": (_sz, [C.POINTER(KvCacheStruct), C.POINTER(Attention), _int]),
+    "krk_cuda_attention_chunk": (_int, [_vp, _int, _vp, _int, C.POINTER(KvCacheStruct), C.POINTER(Attention), _vp, _sz, _vp]),
+    "krk_cuda_step_plan": (_int, [C.POINTER(Step), _vp]),
+    "krk_cuda_block_norm": (_int, [_vp, _vp, _vp, C.POINTER(Norm), _vp]),
+    "krk_cuda_verify_draft_workspace_bytes": (_sz, [C.POINTER(Verify)]),
+    "krk_cuda_verify_draft": (_int, [_vp, _vp, _vp, _vp, C.POINTER(Verify), _vp, _sz, _vp]),
     "krk_cuda_logits_adjust": (_int, [_vp, _vp, C.POINTER(Adjust), _vp]),
     "krk_cuda_allgather_sum": (_int, [C.POINTER(_vp), C.POINTER(_vp), _int, _int, _i64, _vp, _vp, _i64, _vp]),
     "krk_cuda_peer_alloc": (_int, [C.POINTER(_vp), C.c_size_t, C.c_char_p]),
@@ -150,6 +177,10 @@ SIGNATURES = {
     "krk_cuda_backend_kv_append": (None, [_vp, C.POINTER(KvCacheStruct), _vp, _vp, _i64, _i64, _vp, _i64]),
     "krk_cuda_backend_kv_read": (None, [_vp, C.POINTER(KvCacheStruct), _vp, _vp, _vp, _i64]),
     "krk_cuda_backend_attention_tree": (None, [_vp, _vp, _vp, C.POINTER(KvCacheStruct), C.POINTER(Attention)]),
+    "krk_cuda_backend_attention_chunk": (None, [_vp, _vp, _int, _vp, _int, C.POINTER(KvCacheStruct), C.POINTER(Attention)]),
+    "krk_cuda_backend_step_plan": (None, [_vp, C.POINTER(Step)]),
+    "krk_cuda_backend_block_norm": (None, [_vp, _vp, _vp, _vp, C.POINTER(Norm)]),
+    "krk_cuda_backend_verify_draft": (None, [_vp, _vp, _vp, _vp, _vp, C.POINTER(Verify)]),
     "krk_cuda_backend_logits_adjust": (None, [_vp, _vp, _vp, C.POINTER(Adjust)]),
     "krk_cuda_backend_silu_mul": (None, [_vp, _vp, _vp, _vp, _i64, _i64, _vp]),
     "krk_cuda_backend_gather_rows": (None, [_vp, _vp, _vp, _vp, _i64, _i64]),
@@ -464,6 +495,49 @@ def attention_tree(q, cache: KvCache, q_start, kv_len, page_table, max_q: int, t
     return _fc.attention_tree(q, cache.on(q), q_start, kv_len, page_table, max_q, tree, scale, softcap, window, sinks, max_kv_len, out, workspace, stream)
 
 
+def attention_chunk(q, cache: KvCache, q_start, kv_len, page_table, max_q: int, scale=None, softcap: float = 0.0, window: int = 0, sinks=None, max_kv_len: int = 0,
+                    out=None, workspace=None, stream=None):
+    """attention_tree for chunks of prompts, max_q of any size: a row sees itself and the positions before it (with a window, of one or more, the nearest of
+    them). q f32 or f16; out f32 or f16 (None: like q), not f32 from f16. f16 results come from f16 products. Rows that no sequence has are left as they were."""
+    return _fc.attention_chunk(q, cache.on(q), q_start, kv_len, page_table, max_q, scale, softcap, window, sinks, max_kv_len, out, workspace, stream)
+
+
+class StepPlan(NamedTuple):
+    """What a step's other calls take: q_start, kv_len for attention, positions for qk_norm_rope, slots (int64) for kv_append, the row of each
+    sequence's last token (-1: none), counts (free pages left, pages missing, tokens, tokens beyond the buffer), and the page table."""
+    q_start: torch.Tensor
+    kv_len: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+    last: torch.Tensor
+    counts: torch.Tensor
+    page_table: torch.Tensor
+
+
+def step_plan(kv_before, n_new, page_table, free_pages, n_free, page_size: int, max_tok: int, out=None, stream=None) -> StepPlan:
+    """Pages, slots and positions of a step's new tokens from the requests' lengths (int32 [n_seq] each): sequence s has kv_before[s] positions and gets
+    n_new[s] more; pages come off the stack free_pages[:n_free[0]] (int32; n_free int32 [1]) into page_table (int32 [n_seq, width], written in place), -1
+    where there are none. max_tok: places of positions and slots, whose rest is 0 and -1. out: a StepPlan to write into again."""
+    return StepPlan(*_fc.step_plan(kv_before, n_new, page_table, free_pages, n_free, page_size, max_tok, tuple(out) if out is not None else None, stream))
+
+
+def block_norm(x, weight=None, residual=None, post_weight=None, post_norm=None, gate=None, alpha: float = 1.0, eps: float = 1e-6, offset: float = 0.0, dtype=None,
+               h_out=None, out=None, stream=None):
+    """Between two blocks: h = residual + alpha * gate * P(x), y = norm(h) * (offset + weight); P(x) the norm of x times (offset + post_weight), or x where there
+    is neither post_weight nor post_norm. x, residual f32 [rows, n]; gate f32 [n] or [rows, n]. Returns (y, h), y f32 or (dtype=torch.float16) f16."""
+    return _fc.block_norm(x, weight, residual, post_weight, post_weight is not None if post_norm is None else post_norm, gate, alpha, eps, offset, dtype is torch.float16, h_out,
+                          out, stream)
+
+
+def verify_draft(logits, row_start, draft, accept_u, sample_u, draft_logits=None, temp=None, draft_temp=None, tokens=None, n_accepted=None, logprob=None, workspace=None,
+                 stream=None):
+    """Drafted tokens against the target's probabilities: logits f32 [rows, vocab], sequence s has rows row_start[s] .. row_start[s + 1] (int32), one more than
+    drafted tokens; draft int32 [rows] (a sequence's last one is not looked at); accept_u f32 [rows] and sample_u f32 [n_seq] in [0, 1); draft_logits
+    f32 [rows, vocab] of the drafter, None where its tokens are certain; temp, draft_temp f32 [n_seq] (0: greedy). Returns (tokens int32 [rows]: the
+    accepted ones, the drawn one, -1; n_accepted int32 [n_seq]; logprob f32 [rows]); rows of no sequence are left as they were."""
+    return _fc.verify_draft(logits, row_start, draft, accept_u, sample_u, draft_logits, temp, draft_temp, tokens, n_accepted, logprob, workspace, stream)
+
+
 def allgather_sum(gather_peer_ptrs, flag_peer_ptrs, my_rank: int, slot_stride: int, part, out, stream=None):
     """Exchange step of an expert-sharded FFN: all-gather of `part` over peer stores + rank-ordered sum."""
     n = len(gather_peer_ptrs)
@@ -605,6 +679,18 @@ class Backend:
 
     def logits_adjust(self, out: int, logits: int, adjust: Adjust) -> None:
         lib.krk_cuda_backend_logits_adjust(self.h, out, logits, C.byref(adjust))
+
+    def attention_chunk(self, out: int, out_dtype: int, q: int, q_dtype: int, cache: KvCacheStruct, attention: Attention) -> None:
+        lib.krk_cuda_backend_attention_chunk(self.h, out, out_dtype, q, q_dtype, C.byref(cache), C.byref(attention))
+
+    def step_plan(self, step: Step) -> None:
+        lib.krk_cuda_backend_step_plan(self.h, C.byref(step))
+
+    def block_norm(self, y: int, h_out: int, x: int, norm: Norm) -> None:
+        lib.krk_cuda_backend_block_norm(self.h, y, h_out, x, C.byref(norm))
+
+    def verify_draft(self, tokens: int, n_accepted: int, logprob: int, logits: int, verify: Verify) -> None:
+        lib.krk_cuda_backend_verify_draft(self.h, tokens, n_accepted, logprob, logits, C.byref(verify))
 
     def fill0(self, p: int, nbytes: int) -> None:
         lib.krk_cuda_backend_fill0(self.h, p, nbytes)

@@ -302,6 +302,32 @@ void CudaBackend::logits_adjust(void *out, const void *logits, const krk_cuda_ad
     if (rc != KRK_CUDA_OK) die("logits_adjust", rc, adjust.n_rows, adjust.n_vocab, adjust.hist_n, 0);
 }
 
+void CudaBackend::attention_chunk(void *out, int out_dtype, const void *q, int q_dtype, const krk_cuda_kv_cache &cache, const krk_cuda_attention &attention) {
+    use();
+    const size_t need = krk_cuda_attention_chunk_workspace_bytes(&cache, &attention, out_dtype);
+    const int rc = krk_cuda_attention_chunk(out, out_dtype, q, q_dtype, &cache, &attention, need ? workspace(need) : nullptr, need, stream_);
+    if (rc != KRK_CUDA_OK) die("attention_chunk", rc, attention.n_seq, attention.n_heads, cache.head_dim, cache.type);
+}
+
+void CudaBackend::step_plan(const krk_cuda_step &step) {
+    use();
+    const int rc = krk_cuda_step_plan(&step, stream_);
+    if (rc != KRK_CUDA_OK) die("step_plan", rc, step.n_seq, step.max_tok, step.table_width, step.page_size);
+}
+
+void CudaBackend::block_norm(void *y, void *h_out, const void *x, const krk_cuda_norm &norm) {
+    use();
+    const int rc = krk_cuda_block_norm(y, h_out, x, &norm, stream_);
+    if (rc != KRK_CUDA_OK) die("block_norm", rc, norm.rows, norm.n, norm.y_dtype, norm.post_norm);
+}
+
+void CudaBackend::verify_draft(void *tokens, void *n_accepted, void *logprob, const void *logits, const krk_cuda_verify &verify) {
+    use();
+    const size_t need = krk_cuda_verify_draft_workspace_bytes(&verify);
+    const int rc = krk_cuda_verify_draft(tokens, n_accepted, logprob, logits, &verify, need ? workspace(need) : nullptr, need, stream_);
+    if (rc != KRK_CUDA_OK) die("verify_draft", rc, verify.n_seq, verify.n_rows, verify.n_vocab, 0);
+}
+
 } // namespace krk_cuda
 
 // ---- C shim over the class (declared in krk_cuda.h) -------------------------------------------
@@ -361,6 +387,17 @@ void krk_cuda_backend_attention_tree(void *be, void *out, const void *q, const k
 }
 void krk_cuda_backend_logits_adjust(void *be, void *out, const void *logits, const krk_cuda_adjust *host_adjust) {
     static_cast<CudaBackend *>(be)->logits_adjust(out, logits, *host_adjust);
+}
+void krk_cuda_backend_attention_chunk(void *be, void *out, int out_dtype, const void *q, int q_dtype, const krk_cuda_kv_cache *host_cache,
+                                      const krk_cuda_attention *host_attention) {
+    static_cast<CudaBackend *>(be)->attention_chunk(out, out_dtype, q, q_dtype, *host_cache, *host_attention);
+}
+void krk_cuda_backend_step_plan(void *be, const krk_cuda_step *host_step) { static_cast<CudaBackend *>(be)->step_plan(*host_step); }
+void krk_cuda_backend_block_norm(void *be, void *y, void *h_out, const void *x, const krk_cuda_norm *host_norm) {
+    static_cast<CudaBackend *>(be)->block_norm(y, h_out, x, *host_norm);
+}
+void krk_cuda_backend_verify_draft(void *be, void *tokens, void *n_accepted, void *logprob, const void *logits, const krk_cuda_verify *host_verify) {
+    static_cast<CudaBackend *>(be)->verify_draft(tokens, n_accepted, logprob, logits, *host_verify);
 }
 void krk_cuda_backend_silu_mul(void *be, void *out, const void *gate, const void *up, int64_t n, int64_t row_len,
                                float *host_row_scale) {

@@ -327,6 +327,13 @@ int launch_kv_append(const krk_cuda_kv_cache &cache, const float *k, const float
 int launch_kv_read(const krk_cuda_kv_cache &cache, float *k, float *v, const int64_t *slots, int64_t n, cudaStream_t st);
 size_t attention_tree_workspace_bytes(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a);
 int launch_attention_tree(float *out, const float *q, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, void *workspace, cudaStream_t st);
+size_t attention_chunk_workspace_bytes(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, int out_dtype);
+int launch_attention_chunk(void *out, int out_dtype, const void *q, int q_dtype, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, void *workspace, cudaStream_t st);
+// Plan of a step (krk_step.cu), norms between blocks (krk_norm.cu), verification of drafted tokens (krk_verify.cu).
+int launch_step_plan(const krk_cuda_step &s, cudaStream_t st);
+int launch_block_norm(void *y, float *h_out, const float *x, const krk_cuda_norm &n, cudaStream_t st);
+size_t verify_draft_workspace_bytes(const krk_cuda_verify &v);
+int launch_verify_draft(int32_t *tokens, int32_t *n_accepted, float *logprob, const float *logits, const krk_cuda_verify &v, void *workspace, cudaStream_t st);
 int launch_route(int32_t *ids, float *wts, const float *logits, int64_t n_tok, int n_expert, int k,
                  cudaStream_t st);
 int launch_router_softmax(float *probs, const float *logits, int64_t n_rows, int n_expert, cudaStream_t st);

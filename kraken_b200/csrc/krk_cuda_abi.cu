@@ -473,21 +473,22 @@ int krk_cuda_kv_read(const krk_cuda_kv_cache *cache, void *k_f32, void *v_f32, c
                           static_cast<cudaStream_t>(stream));
 }
 
-// `a` with max_kv_len filled in.
-static int check_attention(const krk_cuda_kv_cache *cache, const krk_cuda_attention *from, krk_cuda_attention &a) {
+// `a` with max_kv_len filled in. most_q: rows of a sequence at most; least_window: of a window that there is.
+static int check_attention(const krk_cuda_kv_cache *cache, const krk_cuda_attention *from, krk_cuda_attention &a, int64_t most_q = KRK_CUDA_MAX_DRAFT,
+                           int least_window = KRK_CUDA_MAX_DRAFT) {
     const int rc = check_cache(cache);
     if (rc != KRK_CUDA_OK) return rc;
     if (!from) return KRK_CUDA_ENULL;
     a = *from;
     const int d = cache->head_dim;
     if (d != 64 && d != 96 && d != 128 && d != 192 && d != 256) return KRK_CUDA_ESHAPE;
-    if (a.n_seq < 0 || a.n_heads < 1 || a.n_heads > 65536 || a.n_heads % cache->n_kv_heads != 0 || a.max_q < 0 || a.max_q > KRK_CUDA_MAX_DRAFT || a.table_width < 1 ||
+    if (a.n_seq < 0 || a.n_heads < 1 || a.n_heads > 65536 || a.n_heads % cache->n_kv_heads != 0 || a.max_q < 0 || a.max_q > most_q || a.table_width < 1 ||
         a.max_kv_len < 0)
         return KRK_CUDA_ESHAPE;
     const int64_t room = (int64_t)a.table_width * cache->page_size;
     if (a.max_kv_len == 0) a.max_kv_len = room;
     if (a.max_kv_len > room || a.max_kv_len > (1ll << 30)) return KRK_CUDA_ESHAPE;
-    if (a.window < 0 || (a.window > 0 && a.window < KRK_CUDA_MAX_DRAFT) || !(a.softcap >= 0.0f && a.softcap <= FLT_MAX)) return KRK_CUDA_EARG;
+    if (a.window < 0 || (a.window > 0 && a.window < least_window) || !(a.softcap >= 0.0f && a.softcap <= FLT_MAX)) return KRK_CUDA_EARG;
     return KRK_CUDA_OK;
 }
 
@@ -513,6 +514,101 @@ int krk_cuda_attention_tree(void *out_f32, const void *q_f32, const krk_cuda_kv_
     const size_t need = attention_tree_workspace_bytes(*cache, a);
     if (need > 0 && (!workspace || ws_bytes < need || !aligned(workspace, 16))) return KRK_CUDA_EWORKSPACE;
     return launch_attention_tree(static_cast<float *>(out_f32), static_cast<const float *>(q_f32), *cache, a, workspace, static_cast<cudaStream_t>(stream));
+}
+
+// Rows of chunks in all stay within 31 bits for a key head: a block of rows is found with them.
+static int check_chunk(const krk_cuda_kv_cache *cache, const krk_cuda_attention *from, krk_cuda_attention &a, int out_dtype, int q_dtype) {
+    if ((out_dtype != KRK_CUDA_X_F32 && out_dtype != KRK_CUDA_X_F16) || (q_dtype != KRK_CUDA_X_F32 && q_dtype != KRK_CUDA_X_F16) ||
+        (out_dtype == KRK_CUDA_X_F32 && q_dtype == KRK_CUDA_X_F16))
+        return KRK_CUDA_EARG;
+    const int rc = check_attention(cache, from, a, 1 << 24, 1);
+    if (rc != KRK_CUDA_OK) return rc;
+    if (a.tree) return KRK_CUDA_EARG;
+    if ((int64_t)a.max_q * (a.n_heads / cache->n_kv_heads) > (1 << 30)) return KRK_CUDA_ESHAPE;
+    return KRK_CUDA_OK;
+}
+
+size_t krk_cuda_attention_chunk_workspace_bytes(const krk_cuda_kv_cache *cache, const krk_cuda_attention *attention, int out_dtype) {
+    krk_cuda_attention a;
+    if (check_chunk(cache, attention, a, out_dtype, KRK_CUDA_X_F32) != KRK_CUDA_OK || a.n_seq == 0 || a.max_q == 0) return 0;
+    return attention_chunk_workspace_bytes(*cache, a, out_dtype);
+}
+
+int krk_cuda_attention_chunk(void *out, int out_dtype, const void *q, int q_dtype, const krk_cuda_kv_cache *cache, const krk_cuda_attention *attention,
+                             void *workspace, size_t ws_bytes, void *stream) {
+    krk_cuda_attention a;
+    const int rc = check_chunk(cache, attention, a, out_dtype, q_dtype);
+    if (rc != KRK_CUDA_OK) return rc;
+    if (a.n_seq == 0 || a.max_q == 0) return KRK_CUDA_OK;
+    if (!out || !q || !a.q_start || !a.kv_len || !a.page_table) return KRK_CUDA_ENULL;
+    const int64_t row = (int64_t)a.n_heads * cache->head_dim;
+    if (a.q_stride < row || a.out_stride < row) return KRK_CUDA_ESHAPE;
+    if (!aligned(out, 16) || !aligned(q, 16) || a.q_stride % (q_dtype == KRK_CUDA_X_F16 ? 8 : 4) != 0 || a.out_stride % (out_dtype == KRK_CUDA_X_F16 ? 8 : 4) != 0 ||
+        !aligned(a.q_start, 4) || !aligned(a.kv_len, 4) || !aligned(a.page_table, 4) || !aligned(a.sinks, 4))
+        return KRK_CUDA_EALIGN;
+    if (!device_state()) return KRK_CUDA_EDEVICE;
+    const size_t need = attention_chunk_workspace_bytes(*cache, a, out_dtype);
+    if (need > 0 && (!workspace || ws_bytes < need || !aligned(workspace, 16))) return KRK_CUDA_EWORKSPACE;
+    return launch_attention_chunk(out, out_dtype, q, q_dtype, *cache, a, workspace, static_cast<cudaStream_t>(stream));
+}
+
+int krk_cuda_step_plan(const krk_cuda_step *s, void *stream) {
+    if (!s) return KRK_CUDA_ENULL;
+    if (s->n_seq < 0 || s->table_width < 0 || s->page_size < 1 || s->max_tok < 0 || s->max_tok > INT32_MAX || s->free_cap < 0 || s->free_cap > INT32_MAX) return KRK_CUDA_ESHAPE;
+    if (!s->q_start || !s->counts || !s->n_free || (s->free_cap > 0 && !s->free_pages)) return KRK_CUDA_ENULL;
+    if (s->n_seq > 0 && (!s->kv_before || !s->n_new || !s->kv_len || !s->last || (s->table_width > 0 && !s->page_table))) return KRK_CUDA_ENULL;
+    if (s->max_tok > 0 && (!s->positions || !s->slots)) return KRK_CUDA_ENULL;
+    const void *const lists[] = {s->kv_before, s->n_new, s->page_table, s->free_pages, s->n_free, s->q_start, s->kv_len, s->last, s->positions, s->counts};
+    for (const void *p : lists)
+        if (!aligned(p, 4)) return KRK_CUDA_EALIGN;
+    if (!aligned(s->slots, 8)) return KRK_CUDA_EALIGN;
+    if (!device_state()) return KRK_CUDA_EDEVICE;
+    return launch_step_plan(*s, static_cast<cudaStream_t>(stream));
+}
+
+int krk_cuda_block_norm(void *y, void *h_out_f32, const void *x_f32, const krk_cuda_norm *m, void *stream) {
+    if (!m) return KRK_CUDA_ENULL;
+    if (m->y_dtype != KRK_CUDA_X_F32 && m->y_dtype != KRK_CUDA_X_F16) return KRK_CUDA_EARG;
+    if (m->rows < 0 || m->rows > INT32_MAX || m->n < 0 || m->n > 65536 || m->gate_stride < 0) return KRK_CUDA_ESHAPE;
+    if (m->rows == 0 || m->n == 0) return KRK_CUDA_OK;
+    if (!(m->eps >= 0.0f)) return KRK_CUDA_EARG;
+    if (!y || !x_f32) return KRK_CUDA_ENULL;
+    if (m->rows > 1 && (m->x_stride < m->n || m->y_stride < m->n || (h_out_f32 && m->h_stride < m->n) || (m->residual && m->residual_stride < m->n) ||
+                        (m->gate && m->gate_stride > 0 && m->gate_stride < m->n)))
+        return KRK_CUDA_ESHAPE;
+    if (m->rows > 1 && h_out_f32 && ((h_out_f32 == x_f32 && m->h_stride != m->x_stride) || (h_out_f32 == m->residual && m->h_stride != m->residual_stride))) return KRK_CUDA_EARG;
+    const void *const floats[] = {h_out_f32, x_f32, m->residual, m->gate, m->post_weight, m->weight};
+    for (const void *p : floats)
+        if (!aligned(p, 4)) return KRK_CUDA_EALIGN;
+    if (!aligned(y, m->y_dtype == KRK_CUDA_X_F16 ? 2 : 4)) return KRK_CUDA_EALIGN;
+    if (!device_state()) return KRK_CUDA_EDEVICE;
+    return launch_block_norm(y, static_cast<float *>(h_out_f32), static_cast<const float *>(x_f32), *m, static_cast<cudaStream_t>(stream));
+}
+
+static int check_verify(const krk_cuda_verify *v) {
+    if (!v) return KRK_CUDA_ENULL;
+    if (v->n_seq < 0 || v->n_rows < 0 || v->n_rows > (1 << 24) || v->n_vocab < 0 || v->n_vocab > (1 << 30)) return KRK_CUDA_ESHAPE;
+    if (v->n_rows > 1 && (v->stride < v->n_vocab || (v->draft_logits && v->draft_stride < v->n_vocab))) return KRK_CUDA_ESHAPE;
+    return KRK_CUDA_OK;
+}
+size_t krk_cuda_verify_draft_workspace_bytes(const krk_cuda_verify *v) {
+    return check_verify(v) != KRK_CUDA_OK || v->n_seq == 0 || v->n_rows == 0 ? 0 : verify_draft_workspace_bytes(*v);
+}
+int krk_cuda_verify_draft(void *tokens_i32, void *n_accepted_i32, void *logprob_f32, const void *logits_f32, const krk_cuda_verify *v, void *workspace, size_t ws_bytes,
+                          void *stream) {
+    const int rc = check_verify(v);
+    if (rc != KRK_CUDA_OK) return rc;
+    if (v->n_seq == 0) return KRK_CUDA_OK;
+    if (!n_accepted_i32 || !v->row_start || !v->sample_u) return KRK_CUDA_ENULL;
+    if (v->n_rows > 0 && (!tokens_i32 || !v->draft || !v->accept_u || (v->n_vocab > 0 && !logits_f32))) return KRK_CUDA_ENULL;
+    const void *const lists[] = {tokens_i32, n_accepted_i32, logprob_f32, logits_f32, v->row_start, v->draft, v->accept_u, v->sample_u, v->temp, v->draft_temp, v->draft_logits};
+    for (const void *p : lists)
+        if (!aligned(p, 4)) return KRK_CUDA_EALIGN;
+    if (!device_state()) return KRK_CUDA_EDEVICE;
+    const size_t need = v->n_rows == 0 ? 0 : verify_draft_workspace_bytes(*v);
+    if (need > 0 && (!workspace || ws_bytes < need || !aligned(workspace, 16))) return KRK_CUDA_EWORKSPACE;
+    return launch_verify_draft(static_cast<int32_t *>(tokens_i32), static_cast<int32_t *>(n_accepted_i32), static_cast<float *>(logprob_f32), static_cast<const float *>(logits_f32),
+                               *v, workspace, static_cast<cudaStream_t>(stream));
 }
 
 int krk_cuda_logits_adjust(void *out_f32, const void *logits_f32, const krk_cuda_adjust *a, void *stream) {

@@ -774,6 +774,214 @@ PyObject *logits_adjust(PyObject *, PyObject *const *a, Py_ssize_t n) {
     KRK_CATCH
 }
 
+bool headed16(const at::Tensor *t, const at::Tensor *first, int64_t rows, int64_t heads, int64_t d, const char *name) {   // as headed, f32 or f16
+    if (!on_device(t, first, name)) return false;
+    if (t->scalar_type() == at::kFloat) return headed(t, first, rows, heads, d, name);
+    if (!typed(t, first, at::kHalf, name)) return false;
+    if (t->dim() == 3 && (rows < 0 || t->size(0) == rows) && (heads < 0 || t->size(1) == heads) && t->size(2) == d &&
+        (t->numel() == 0 || ((d <= 1 || t->stride(2) == 1) && (t->size(1) <= 1 || t->stride(1) == d))))
+        return true;
+    PyErr_Format(PyExc_ValueError, "%s: expected [rows][heads][values] with the heads of a row behind each other", name);
+    return false;
+}
+int x_dtype(const at::Tensor *t) { return t->scalar_type() == at::kHalf ? KRK_CUDA_X_F16 : KRK_CUDA_X_F32; }
+
+// q, cache, q_start, kv_len, page_table, max_q, scale, softcap, window, sinks, max_kv_len, out, workspace, stream -> out
+PyObject *attention_chunk(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    KRK_NARGS(14, "attention_chunk")
+    KRK_TRY
+    Args g{a};
+    const at::Tensor *q = g.t(0), *start = g.t(2), *len = g.t(3), *table = g.t(4), *sinks = g.t_or_none(9), *out = g.t_or_none(11), *ws = g.t_or_none(12);
+    const auto *c = (const krk_cuda_kv_cache *)g.addr(1);
+    krk_cuda_attention t = {};
+    const int64_t max_q = g.i(5), window = g.i(8);
+    t.max_kv_len = g.i(10), t.softcap = g.f(7);
+    if (a[6] != Py_None) t.scale = g.f(6);
+    void *st = a[13] == Py_None ? nullptr : g.stream(13);
+    if (!g.ok) return nullptr;
+    if (a[6] == Py_None) t.scale = 1.0f / std::sqrt((float)c->head_dim);
+    if (!headed16(q, q, -1, -1, c->head_dim, "q") || !tabled(table, q, at::kInt, -1, "page_table")) return nullptr;
+    const int64_t rows = q->size(0), heads = q->size(1), n_seq = table->size(0);
+    if (!listed(start, q, at::kInt, n_seq + 1, "q_start") || !listed(len, q, at::kInt, n_seq, "kv_len") || !listed(sinks, q, at::kFloat, heads, "sinks")) return nullptr;
+    if (!table->is_contiguous()) return refuse("page_table: expected a contiguous table"), nullptr;
+    if (max_q < 0 || max_q > INT32_MAX || window < 0 || window > INT32_MAX || heads > 65536 || table->size(1) > INT32_MAX || n_seq > INT32_MAX)
+        return refuse("attention_chunk: max_q, window, heads or pages out of range"), nullptr;
+    Where where(*q, a[13] != Py_None, st);
+    at::Tensor made, made_ws;
+    if (!out) out = &(made = empty_like_device(*q, {rows, heads, (int64_t)c->head_dim}, q->scalar_type()));
+    else if (!headed16(out, q, rows, heads, c->head_dim, "out")) return nullptr;
+    t.q_start = Args::ptr(start), t.kv_len = Args::ptr(len), t.page_table = Args::ptr(table), t.sinks = Args::ptr(sinks);
+    t.q_stride = row_stride(q), t.out_stride = row_stride(out);
+    t.n_seq = (int)n_seq, t.n_heads = (int)heads, t.max_q = (int)(max_q < rows ? max_q : rows), t.table_width = (int)table->size(1), t.window = (int)window;
+    if (rows == 0) return given_or_made(a[11], made);   // (no sequence has a row)
+    if (ws) {
+        if (!typed(ws, q, at::kByte, "workspace")) return nullptr;
+        if (!ws->is_contiguous()) return refuse("workspace: expected contiguous bytes"), nullptr;
+    } else if (const size_t need = krk_cuda_attention_chunk_workspace_bytes(c, &t, x_dtype(out))) {
+        ws = &(made_ws = empty_like_device(*q, {(int64_t)need}, at::kByte));
+    }
+    int rc;
+    Py_BEGIN_ALLOW_THREADS rc =
+        krk_cuda_attention_chunk(Args::ptr(out), x_dtype(out), Args::ptr(q), x_dtype(q), c, &t, Args::ptr(ws), ws ? (size_t)ws->numel() : 0, where.stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return fail(rc, "attention_chunk");
+    return given_or_made(a[11], made);
+    KRK_CATCH
+}
+
+// kv_before, n_new, page_table, free_pages, n_free, page_size, max_tok, out (seven tensors) or None, stream -> q_start, kv_len, positions, slots, last, counts, page_table
+PyObject *step_plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    KRK_NARGS(9, "step_plan")
+    KRK_TRY
+    Args g{a};
+    const at::Tensor *before = g.t(0), *fresh = g.t(1), *table = g.t(2), *free = g.t(3), *n_free = g.t(4);
+    const int64_t page = g.i(5), max_tok = g.i(6);
+    void *st = a[8] == Py_None ? nullptr : g.stream(8);
+    if (!g.ok) return nullptr;
+    if (!listed(before, before, at::kInt, -1, "kv_before")) return nullptr;
+    const int64_t n_seq = before->numel();
+    if (!listed(fresh, before, at::kInt, n_seq, "n_new") || !tabled(table, before, at::kInt, n_seq, "page_table") || !listed(free, before, at::kInt, -1, "free_pages") ||
+        !listed(n_free, before, at::kInt, 1, "n_free"))
+        return nullptr;
+    if (!table->is_contiguous()) return refuse("page_table: expected a contiguous table"), nullptr;
+    if (page < 1 || page > INT32_MAX || max_tok < 0 || max_tok > INT32_MAX || n_seq >= INT32_MAX || table->size(1) > INT32_MAX)
+        return refuse("step_plan: page_size, max_tok, sequences or pages out of range"), nullptr;
+    Where where(*before, a[8] != Py_None, st);
+    static const char *const names[6] = {"q_start", "kv_len", "positions", "slots", "last", "counts"};
+    const int64_t sizes[6] = {n_seq + 1, n_seq, max_tok, max_tok, n_seq, 4};
+    std::array<at::Tensor, 6> made;
+    std::array<PyObject *, 6> objects{};
+    std::array<const at::Tensor *, 6> to{};
+    if (a[7] != Py_None) {
+        if (!PyTuple_Check(a[7]) || PyTuple_GET_SIZE(a[7]) != 7) return refuse("out: expected a StepPlan"), nullptr;
+        Args o{&PyTuple_GET_ITEM(a[7], 0)};
+        for (int i = 0; i < 6; i++) {
+            to[i] = o.t(i);
+            if (!o.ok || !listed(to[i], before, i == 3 ? at::kLong : at::kInt, sizes[i], names[i])) return nullptr;
+            objects[i] = PyTuple_GET_ITEM(a[7], i);
+        }
+    } else {
+        for (int i = 0; i < 6; i++) to[i] = &(made[i] = empty_like_device(*before, {sizes[i]}, i == 3 ? at::kLong : at::kInt));
+    }
+    krk_cuda_step s = {};
+    s.kv_before = Args::ptr(before), s.n_new = Args::ptr(fresh), s.page_table = Args::ptr(table), s.free_pages = Args::ptr(free), s.n_free = Args::ptr(n_free);
+    s.q_start = Args::ptr(to[0]), s.kv_len = Args::ptr(to[1]), s.positions = Args::ptr(to[2]), s.slots = Args::ptr(to[3]), s.last = Args::ptr(to[4]), s.counts = Args::ptr(to[5]);
+    s.max_tok = max_tok, s.free_cap = free->numel(), s.n_seq = (int)n_seq, s.table_width = (int)table->size(1), s.page_size = (int)page;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS rc = krk_cuda_step_plan(&s, where.stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return fail(rc, "step_plan");
+    PyObject *all = PyTuple_New(7);
+    if (!all) return nullptr;
+    for (int i = 0; i < 6; i++) {
+        PyObject *x = objects[i] ? Py_NewRef(objects[i]) : THPVariable_Wrap(made[i]);
+        if (!x) {
+            Py_DECREF(all);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(all, i, x);
+    }
+    PyTuple_SET_ITEM(all, 6, Py_NewRef(a[2]));
+    return all;
+    KRK_CATCH
+}
+
+// x, weight, residual, post_weight, post_norm, gate, alpha, eps, offset, half, h_out, out, stream -> (y, h)
+PyObject *block_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    KRK_NARGS(13, "block_norm")
+    KRK_TRY
+    Args g{a};
+    const at::Tensor *x = g.t(0), *w = g.t_or_none(1), *res = g.t_or_none(2), *post = g.t_or_none(3), *gate = g.t_or_none(5), *h = g.t_or_none(10), *y = g.t_or_none(11);
+    krk_cuda_norm m = {};
+    m.post_norm = g.b(4), m.alpha = g.f(6), m.eps = g.f(7), m.offset = g.f(8);
+    const bool half = g.b(9);
+    void *st = a[12] == Py_None ? nullptr : g.stream(12);
+    if (!g.ok || !tabled(x, x, at::kFloat, -1, "x")) return nullptr;
+    const int64_t rows = x->size(0), width = x->size(1);
+    if (!listed(w, x, at::kFloat, width, "weight") || !tabled(res, x, at::kFloat, rows, "residual") || !listed(post, x, at::kFloat, width, "post_weight")) return nullptr;
+    if (res && res->size(1) != width) return refuse("residual: expected the shape of x"), nullptr;
+    if (post && !m.post_norm) return refuse("post_weight without post_norm"), nullptr;
+    if (gate && gate->dim() == 1) {
+        if (!listed(gate, x, at::kFloat, width, "gate")) return nullptr;
+    } else if (gate) {
+        if (!tabled(gate, x, at::kFloat, rows, "gate")) return nullptr;
+        if (gate->size(1) != width) return refuse("gate: expected a row of x, or one for each"), nullptr;
+        m.gate_stride = rows > 1 ? gate->stride(0) : width;
+    }
+    Where where(*x, a[12] != Py_None, st);
+    at::Tensor made_y, made_h;
+    if (!h) h = &(made_h = empty_like_device(*x, {rows, width}, at::kFloat));
+    else if (!tabled(h, x, at::kFloat, rows, "h_out")) return nullptr;
+    if (!y) y = &(made_y = empty_like_device(*x, {rows, width}, half ? at::kHalf : at::kFloat));
+    else if (!on_device(y, x, "out") || !tabled(y, x, y->scalar_type() == at::kHalf ? at::kHalf : at::kFloat, rows, "out")) return nullptr;
+    if (h->size(1) != width || y->size(1) != width) return refuse("out, h_out: expected the shape of x"), nullptr;
+    if (rows == 0 || width == 0) {
+        PyObject *both = PyTuple_Pack(2, given_or_made(a[11], made_y), given_or_made(a[10], made_h));
+        return both;
+    }
+    m.residual = Args::ptr(res), m.gate = Args::ptr(gate), m.post_weight = Args::ptr(post), m.weight = Args::ptr(w);
+    m.rows = rows, m.n = width, m.x_stride = row_stride(x), m.h_stride = row_stride(h), m.y_stride = row_stride(y);
+    if (res) m.residual_stride = row_stride(res);
+    m.y_dtype = x_dtype(y);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS rc = krk_cuda_block_norm(Args::ptr(y), Args::ptr(h), Args::ptr(x), &m, where.stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return fail(rc, "block_norm");
+    PyObject *oy = given_or_made(a[11], made_y), *oh = given_or_made(a[10], made_h);
+    PyObject *both = oy && oh ? PyTuple_Pack(2, oy, oh) : nullptr;
+    Py_XDECREF(oy);
+    Py_XDECREF(oh);
+    return both;
+    KRK_CATCH
+}
+
+// logits, row_start, draft, accept_u, sample_u, draft_logits, temp, draft_temp, tokens, n_accepted, logprob, workspace, stream -> (tokens, n_accepted, logprob)
+PyObject *verify_draft(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    KRK_NARGS(13, "verify_draft")
+    KRK_TRY
+    Args g{a};
+    const at::Tensor *x = g.t(0), *start = g.t(1), *draft = g.t(2), *au = g.t(3), *su = g.t(4), *q = g.t_or_none(5), *temp = g.t_or_none(6), *qt = g.t_or_none(7),
+                     *tokens = g.t_or_none(8), *count = g.t_or_none(9), *lp = g.t_or_none(10), *ws = g.t_or_none(11);
+    void *st = a[12] == Py_None ? nullptr : g.stream(12);
+    if (!g.ok || !tabled(x, x, at::kFloat, -1, "logits")) return nullptr;
+    const int64_t rows = x->size(0), vocab = x->size(1);
+    if (!listed(start, x, at::kInt, -1, "row_start")) return nullptr;
+    const int64_t n_seq = start->numel() - 1;
+    if (n_seq < 0 || n_seq > INT32_MAX) return refuse("row_start: expected one more element than there are sequences"), nullptr;
+    if (!listed(draft, x, at::kInt, rows, "draft") || !listed(au, x, at::kFloat, rows, "accept_u") || !listed(su, x, at::kFloat, n_seq, "sample_u") ||
+        !tabled(q, x, at::kFloat, rows, "draft_logits") || !listed(temp, x, at::kFloat, n_seq, "temp") || !listed(qt, x, at::kFloat, n_seq, "draft_temp") ||
+        !listed(tokens, x, at::kInt, rows, "tokens") || !listed(count, x, at::kInt, n_seq, "n_accepted") || !listed(lp, x, at::kFloat, rows, "logprob"))
+        return nullptr;
+    if (q && q->size(1) != vocab) return refuse("draft_logits: expected the shape of logits"), nullptr;
+    Where where(*x, a[12] != Py_None, st);
+    at::Tensor made_t, made_c, made_l, made_ws;
+    if (!tokens) tokens = &(made_t = empty_like_device(*x, {rows}, at::kInt));
+    if (!count) count = &(made_c = empty_like_device(*x, {n_seq}, at::kInt));
+    if (!lp) lp = &(made_l = empty_like_device(*x, {rows}, at::kFloat));
+    krk_cuda_verify v = {};
+    v.row_start = Args::ptr(start), v.draft = Args::ptr(draft), v.accept_u = Args::ptr(au), v.sample_u = Args::ptr(su), v.temp = Args::ptr(temp), v.draft_temp = Args::ptr(qt);
+    v.draft_logits = Args::ptr(q);
+    v.n_rows = rows, v.n_vocab = vocab, v.stride = row_stride(x), v.n_seq = (int)n_seq;
+    if (q) v.draft_stride = row_stride(q);
+    if (ws) {
+        if (!typed(ws, x, at::kByte, "workspace")) return nullptr;
+        if (!ws->is_contiguous()) return refuse("workspace: expected contiguous bytes"), nullptr;
+    } else if (const size_t need = krk_cuda_verify_draft_workspace_bytes(&v)) {
+        ws = &(made_ws = empty_like_device(*x, {(int64_t)need}, at::kByte));
+    }
+    int rc;
+    Py_BEGIN_ALLOW_THREADS rc = krk_cuda_verify_draft(Args::ptr(tokens), Args::ptr(count), Args::ptr(lp), Args::ptr(x), &v, Args::ptr(ws), ws ? (size_t)ws->numel() : 0, where.stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return fail(rc, "verify_draft");
+    PyObject *ot = given_or_made(a[8], made_t), *oc = given_or_made(a[9], made_c), *ol = given_or_made(a[10], made_l);
+    PyObject *all = ot && oc && ol ? PyTuple_Pack(3, ot, oc, ol) : nullptr;
+    Py_XDECREF(ot);
+    Py_XDECREF(oc);
+    Py_XDECREF(ol);
+    return all;
+    KRK_CATCH
+}
+
 #define KRK_FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"set_raise", set_raise, METH_O, nullptr},
                          {"set_address", set_address, METH_O, nullptr},
@@ -788,6 +996,10 @@ PyMethodDef methods[] = {{"set_raise", set_raise, METH_O, nullptr},
                          KRK_FAST(kv_read),
                          KRK_FAST(attention_tree),
                          KRK_FAST(logits_adjust),
+                         KRK_FAST(attention_chunk),
+                         KRK_FAST(step_plan),
+                         KRK_FAST(block_norm),
+                         KRK_FAST(verify_draft),
                          KRK_FAST(moe_ffn),
                          KRK_FAST(moe_ffn_routed),
                          KRK_FAST(backend_upload),
