@@ -821,8 +821,7 @@ PyObject *attention_chunk(PyObject *, PyObject *const *a, Py_ssize_t n) {
         ws = &(made_ws = empty_like_device(*q, {(int64_t)need}, at::kByte));
     }
     int rc;
-    Py_BEGIN_ALLOW_THREADS rc =
-        krk_cuda_attention_chunk(Args::ptr(out), x_dtype(out), Args::ptr(q), x_dtype(q), c, &t, Args::ptr(ws), ws ? (size_t)ws->numel() : 0, where.stream);
+    Py_BEGIN_ALLOW_THREADS rc = krk_cuda_attention_chunk(Args::ptr(out), x_dtype(out), Args::ptr(q), x_dtype(q), c, &t, Args::ptr(ws), ws ? (size_t)ws->numel() : 0, where.stream);
     Py_END_ALLOW_THREADS
     if (rc != 0) return fail(rc, "attention_chunk");
     return given_or_made(a[11], made);
