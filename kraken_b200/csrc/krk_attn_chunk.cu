@@ -1,113 +1,130 @@
-// krk_cuda_attention_chunk, its simplest form: a warp for each (token, query head), one position after the other with the running maximum and sum.
-#include "krk_attn_kernel.cuh"
+// krk_cuda_attention_chunk: the choice of a launch's form, and the kernel that adds up the partial sums of divided items.
+#include "krk_attn_chunk.cuh"
 
 namespace krk_cuda {
 namespace attn {
 namespace {
 
-struct ChunkParams {
-    const void *q;
-    void *out;
-    int64_t q_stride, out_stride;
-    const uint8_t *k, *v;
-    const __half *k_scale, *v_scale;
-    const int32_t *table, *q_start, *kv_len;
-    const float *sinks;
-    int64_t n_pages;
-    int table_width, page_size, max_len, n_seq, n_heads, n_kv, group, max_q, window, type, q_half, out_half;
-    float scale, softcap;
-};
-
-template <int D>
-__device__ __forceinline__ void row_values(float (&x)[D / 32], const uint8_t *pool, const __half *scale, int type, int64_t row) {
-    const int lane = threadIdx.x & 31;
+// CTA (b, y): the item that CTA b + 1 of the first kernel went on with as the second one to have a part of it, if there is one; a warp a row. The parts are
+// added in the order of the CTAs.
+template <int D, bool HALF>
+__global__ void __launch_bounds__(128)
+chunk_merge_kernel(const __grid_constant__ ChunkParams p) {
+    constexpr int NB = D / 32, R = chunk_rows(D);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int lane = threadIdx.x & 31, b = blockIdx.x + 1;
+    const Shared it = p.shared[b];
+    if (it.parts == 0) return;
+    constexpr size_t kPitch = (size_t)2 * R * (D + 2);   // from a CTA's parts to the next one's
+    for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < it.n_rows; r += gridDim.y * 4) {
+        const float *first = p.part + (size_t)(b - 1) * kPitch + (size_t)(R + r) * (D + 2), *others = p.part + (size_t)(b - 1) * kPitch + (size_t)r * (D + 2);
+        float x[NB], m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int c = 0; c < D / 32; c++) {
-        if (type == KRK_CUDA_KV_F16) x[c] = __half2float(reinterpret_cast<const __half *>(pool)[row * D + 32 * c + lane]);
-        else {
-            const float d = __half2float(scale[row * (D / 32) + c]);
-            if (type == KRK_CUDA_KV_Q8) x[c] = d * (float)(int8_t)pool[row * D + 32 * c + lane];
-            else {
-                const int b = pool[row * (D / 2) + 16 * c + (lane & 15)];
-                x[c] = d * (float)((lane < 16 ? b & 15 : b >> 4) - 8);
-            }
+        for (int c = 0; c < NB; c++) x[c] = 0.0f;
+#pragma unroll 2
+        for (int i = 0; i < it.parts; i++) {
+            const float *from = i == 0 ? first : others + i * kPitch;
+            float y[NB];
+#pragma unroll
+            for (int c = 0; c < NB; c++) y[c] = from[32 * c + lane];
+            const float2 ml = *reinterpret_cast<const float2 *>(from + D);
+            if (ml.x == -INFINITY) continue;
+            const float top = fmaxf(m, ml.x), old = m == -INFINITY ? 0.0f : exp2f(m - top), now = exp2f(ml.x - top);
+            m = top;
+            l = l * old + ml.y * now;
+#pragma unroll
+            for (int c = 0; c < NB; c++) x[c] = x[c] * old + y[c] * now;
+        }
+        const int rr = it.row0 + r, token = rr / p.group, head = it.kvh * p.group + rr % p.group;
+        float keep = 1.0f;
+        if (p.sinks) {
+            const float sink = p.sinks[head] * 1.44269504f, top = fmaxf(m, sink);
+            keep = m == -INFINITY ? 0.0f : exp2f(m - top);
+            l = l * keep + (sink == -INFINITY ? 0.0f : sink == top ? 1.0f : exp2f(sink - top));
+        }
+        const float f = l == 0.0f ? 0.0f : keep / l;
+        const int64_t to = (int64_t)(it.q0 + token) * p.out_stride + (int64_t)head * D + lane;
+#pragma unroll
+        for (int c = 0; c < NB; c++) {
+            if constexpr (HALF) static_cast<__half *>(p.out)[to + 32 * c] = __float2half_rn(x[c] * f);
+            else static_cast<float *>(p.out)[to + 32 * c] = x[c] * f;
         }
     }
 }
 
-template <int D>
-__global__ void __launch_bounds__(128)
-attn_chunk_simple(const __grid_constant__ ChunkParams p) {
-    constexpr int NB = D / 32;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int lane = threadIdx.x & 31, head = blockIdx.y, s = blockIdx.z, i = blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int q0 = p.q_start[s], n_q = min(max(p.q_start[s + 1] - q0, 0), p.max_q);
-    if (i >= n_q) return;
-    const int len = min(max(p.kv_len[s], 0), 1 << 30), own = len - n_q + i, kvh = head / p.group;
-    float q[NB], o[NB], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int c = 0; c < NB; c++) {
-        const int64_t at = (int64_t)(q0 + i) * p.q_stride + head * D + 32 * c + lane;
-        q[c] = p.q_half ? __half2float(static_cast<const __half *>(p.q)[at]) : static_cast<const float *>(p.q)[at];
-        o[c] = 0.0f;
+int launch_chunk_merge(const ChunkParams &p, int d, bool half, int rows, cudaStream_t st) {
+    auto kernel = half ? (d == 64 ? chunk_merge_kernel<64, true> : d == 96 ? chunk_merge_kernel<96, true> : d == 128 ? chunk_merge_kernel<128, true>
+                          : d == 192 ? chunk_merge_kernel<192, true> : chunk_merge_kernel<256, true>)
+                       : (d == 64 ? chunk_merge_kernel<64, false> : d == 96 ? chunk_merge_kernel<96, false> : d == 128 ? chunk_merge_kernel<128, false>
+                          : d == 192 ? chunk_merge_kernel<192, false> : chunk_merge_kernel<256, false>);
+    return launched(launch_overlapped(kernel, dim3((unsigned)(p.grid - 1), (unsigned)(rows < 32 ? (rows + 3) / 4 : 8)), dim3(128), st, p));
+}
+
+struct ChunkForm {
+    bool tree;          // the kernel of attention_tree, over pieces of 64 tokens
+    int grid, whole, rows, parts;   // parts: pieces of a sequence at most
+    size_t bytes;
+};
+ChunkForm form_of(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, int out_dtype) {
+    ChunkForm f = {};
+    const int d = cache.head_dim, r = chunk_rows(d), tp = chunk_positions(d);
+    const int64_t rows = (int64_t)a.max_q * (a.n_heads / cache.n_kv_heads), blocks = (rows + r - 1) / r;
+    // f32 results over 8- and 4-bit caches: keys and values of 18 bits, which the products of tree attention take as whole numbers and scales
+    f.tree = out_dtype == KRK_CUDA_X_F32 && cache.type != KRK_CUDA_KV_F16;
+    if (f.tree) {
+        f.parts = (a.max_q + KRK_CUDA_MAX_DRAFT - 1) / KRK_CUDA_MAX_DRAFT;
+        return f;
     }
-    const int end = min(min(own + 1, len), p.max_len);
-    for (int pos = p.window > 0 ? max(0, own - p.window + 1) : 0; pos < end; pos++) {
-        const int page = p.table[(size_t)s * p.table_width + pos / p.page_size];
-        if (page < 0 || page >= p.n_pages) continue;
-        const int64_t row = ((int64_t)page * p.n_kv + kvh) * p.page_size + pos % p.page_size;
-        float x[NB], sum = 0.0f;
-        row_values<D>(x, p.k, p.k_scale, p.type, row);
-#pragma unroll
-        for (int c = 0; c < NB; c++) sum = fmaf(q[c], x[c], sum);
-#pragma unroll
-        for (int b = 16; b > 0; b >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, b);
-        sum *= p.scale;
-        sum = p.softcap > 0.0f ? capped(sum, p.softcap) : sum * 1.44269504f;
-        const float top = fmaxf(m, sum);
-        if (top == -INFINITY) continue;
-        const float corr = exp2f(m - top), w = exp2f(sum - top);
-        m = top;
-        l = l * corr + w;
-        row_values<D>(x, p.v, p.v_scale, p.type, row);
-#pragma unroll
-        for (int c = 0; c < NB; c++) o[c] = o[c] * corr + w * x[c];
-    }
-    float keep = 1.0f;
-    if (p.sinks) {
-        const float sink = p.sinks[head] * 1.44269504f, top = fmaxf(m, sink);
-        keep = m == -INFINITY ? 0.0f : exp2f(m - top);
-        l = l * keep + (sink == -INFINITY ? 0.0f : exp2f(sink - top));
-    }
-    const float f = l == 0.0f ? 0.0f : keep / l;
-#pragma unroll
-    for (int c = 0; c < NB; c++) {
-        const int64_t at = (int64_t)(q0 + i) * p.out_stride + head * D + 32 * c + lane;
-        if (p.out_half) static_cast<__half *>(p.out)[at] = __float2half_rn(o[c] * f);
-        else static_cast<float *>(p.out)[at] = o[c] * f;
-    }
+    f.whole = a.max_kv_len <= (int64_t)kChunkWholeTiles * tp / 2;
+    const int64_t items = (int64_t)a.n_seq * cache.n_kv_heads * blocks, units = f.whole ? items : items * ((a.max_kv_len + tp - 1) / tp);
+    f.grid = (int)(units < sm_count() ? units : sm_count());
+    f.rows = (int)(rows < r ? rows : r);
+    f.bytes = f.whole ? 0 : shared_bytes(f.grid) + (size_t)f.grid * 2 * r * (d + 2) * sizeof(float);
+    return f;
+}
+// One piece of 64 tokens of every sequence that has so many is a sequence of tree attention.
+krk_cuda_attention pieces_of(const krk_cuda_attention &a, int parts) {
+    krk_cuda_attention t = a;
+    t.n_seq = a.n_seq * parts;
+    t.max_q = a.max_q < KRK_CUDA_MAX_DRAFT ? a.max_q : KRK_CUDA_MAX_DRAFT;
+    return t;
 }
 
 }   // namespace
 }   // namespace attn
 
-size_t attention_chunk_workspace_bytes(const krk_cuda_kv_cache &, const krk_cuda_attention &, int) { return 0; }
+size_t attention_chunk_workspace_bytes(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, int out_dtype) {
+    const attn::ChunkForm f = attn::form_of(cache, a, out_dtype);
+    return f.tree ? attention_tree_workspace_bytes(cache, attn::pieces_of(a, f.parts)) : f.bytes;
+}
 
-int launch_attention_chunk(void *out, int out_dtype, const void *q, int q_dtype, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, void *, cudaStream_t st) {
+int launch_attention_chunk(void *out, int out_dtype, const void *q, int q_dtype, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, void *workspace, cudaStream_t st) {
+    const attn::ChunkForm f = attn::form_of(cache, a, out_dtype);
+    const int d = cache.head_dim, r = attn::chunk_rows(d);
+    if (f.tree) {
+        if ((int64_t)a.n_seq * f.parts > INT32_MAX) return KRK_CUDA_ESHAPE;
+        return launch_attention_pieces(static_cast<float *>(out), static_cast<const float *>(q), cache, attn::pieces_of(a, f.parts), f.parts, a.max_q, workspace, st);
+    }
     attn::ChunkParams p;
     p.q = q, p.out = out, p.q_stride = a.q_stride, p.out_stride = a.out_stride;
     p.k = static_cast<const uint8_t *>(cache.k), p.v = static_cast<const uint8_t *>(cache.v);
     p.k_scale = static_cast<const __half *>(cache.k_scale), p.v_scale = static_cast<const __half *>(cache.v_scale);
     p.table = static_cast<const int32_t *>(a.page_table), p.q_start = static_cast<const int32_t *>(a.q_start), p.kv_len = static_cast<const int32_t *>(a.kv_len);
     p.sinks = static_cast<const float *>(a.sinks);
+    p.shared = static_cast<attn::Shared *>(workspace);
+    p.part = f.whole ? nullptr : reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + attn::shared_bytes(f.grid));
     p.n_pages = cache.n_pages, p.table_width = a.table_width, p.page_size = cache.page_size, p.max_len = (int)a.max_kv_len, p.n_seq = a.n_seq, p.n_heads = a.n_heads;
-    p.n_kv = cache.n_kv_heads, p.group = a.n_heads / cache.n_kv_heads, p.max_q = a.max_q, p.window = a.window, p.type = cache.type;
+    p.n_kv = cache.n_kv_heads, p.group = a.n_heads / cache.n_kv_heads, p.max_q = a.max_q, p.window = a.window, p.whole = f.whole, p.grid = f.grid;
     p.q_half = q_dtype == KRK_CUDA_X_F16, p.out_half = out_dtype == KRK_CUDA_X_F16, p.scale = a.scale, p.softcap = a.softcap;
-    if (a.n_seq > 65535 || a.n_heads > 65535) return KRK_CUDA_ESHAPE;
-    const int d = cache.head_dim;
-    auto kernel = d == 64 ? attn::attn_chunk_simple<64> : d == 96 ? attn::attn_chunk_simple<96> : d == 128 ? attn::attn_chunk_simple<128> : d == 192 ? attn::attn_chunk_simple<192> : attn::attn_chunk_simple<256>;
-    return launched(launch_overlapped(kernel, dim3((unsigned)((a.max_q + 3) / 4), (unsigned)a.n_heads, (unsigned)a.n_seq), dim3(128), st, p));
+    p.status = device_status_word();
+    if (!p.status) return KRK_CUDA_EDEVICE;
+    // units of work are counted in 64 bits
+    const double blocks = ((double)a.max_q * p.group + r - 1) / r, all = (double)a.n_seq * p.n_kv * blocks * 4.0 * p.group * ((double)a.max_kv_len + 2.0 * r + 1024.0);
+    if (all > 4e18) return KRK_CUDA_ESHAPE;
+    int rc = cache.type == KRK_CUDA_KV_F16 ? launch_attn_chunk_f16(p, d, p.out_half, st) : cache.type == KRK_CUDA_KV_Q8 ? launch_attn_chunk_q8(p, d, st) : launch_attn_chunk_q4(p, d, st);
+    if (rc == KRK_CUDA_OK && !f.whole && f.grid > 1) rc = attn::launch_chunk_merge(p, d, p.out_half, f.rows, st);
+    return rc;
 }
 
 } // namespace krk_cuda

@@ -1,0 +1,985 @@
+// krk_cuda_attention_chunk: the kernel on tcgen05, instantiated per cache type in krk_attn_chunk_f16.cu / _q8.cu / _q4.cu; the entry point is in
+// krk_attn_chunk.cu.
+//
+//   out[r] = sum_p w_rp v_p / sum_p w_rp,   w_rp = exp(score_rp - max),   score = scale * q_r . k_p,   p up to r's own position
+//
+// A row is a (token, query head) pair; the `group` query heads of a key head are rows of one product. A block of threads has two tiles of 128 rows (one, for
+// heads of more than 128 values) and goes through tiles of positions: S = Q K^T with the rows as the lanes of tensor memory, so that a thread of the
+// softmax has a row to itself; the weights go back to the place of the scores as the operand of O += P V. While one tile of rows is in its softmax the
+// products of the other one run. Keys and values lie in shared memory in the 128-byte swizzle, keys as rows (K-major), values read across (MN-major).
+#pragma once
+
+#include "krk_attn_wide.cuh"
+
+namespace krk_cuda {
+namespace attn {
+
+struct ChunkParams {
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;         // elements from a token to the next
+    const uint8_t *k, *v;
+    const __half *k_scale, *v_scale;
+    const int32_t *table, *q_start, *kv_len;
+    const float *sinks;
+    Shared *shared;                       // [grid]
+    float *part;                          // [grid][2][R][D + 2]
+    int64_t n_pages;
+    int table_width, page_size, max_len, n_seq, n_heads, n_kv, group, max_q, window, whole, grid, q_half, out_half;
+    float scale, softcap;
+    int *status;
+};
+
+constexpr int kChunkCopyWarps = 4;
+__host__ __device__ constexpr int chunk_tiles_of(int d) { return d <= 128 ? 2 : 1; }           // of rows, 128 each
+__host__ __device__ constexpr int chunk_positions(int d) { return d <= 128 ? 128 : 64; }       // of a tile
+__host__ __device__ constexpr int chunk_rows(int d) { return 128 * chunk_tiles_of(d); }
+constexpr int kChunkSetup = 3;        // an item beside its tiles, in tiles
+constexpr int kChunkWholeTiles = 8;   // contexts of up to so many tiles of positions are not divided
+constexpr float kLetBe = 8.0f;        // log2: a reference stands until a score is more than this above it
+constexpr float kUp = 128.0f;         // of weights: times 2^8 they stay below the f16 range
+
+struct ChunkSeq {
+    int q0, n_q, len, before, blocks;
+};
+// Blocks of R rows of a sequence, and what they cost: prefix(b) the units of its first b blocks, a closed formula (positions that a block's rows see, times the
+// group, rather than its tiles), the same wherever it is worked out. An item's units a tile are bounded, see ChunkWalk::start.
+__host__ __device__ __forceinline__ int64_t clamped_sum(int64_t x, int64_t step, int64_t cap, int64_t b) {   // of clamp(x + i step, 0, cap) over i < b
+    const int64_t n0 = min(b, x >= 0 ? 0 : (-x + step - 1) / step), n1 = min(b, max(n0, cap <= x ? 0 : (cap - x + step - 1) / step)), n = n1 - n0;
+    return n * x + step * ((n0 + n1 - 1) * n / 2) + (b - n1) * cap;
+}
+template <int R, int TP>
+struct ChunkCost {
+    int64_t ends, starts, cap, k0, last, head;   // group times: the end of block 0, its start, the positions there are
+    bool window;
+    __host__ __device__ __forceinline__ int64_t prefix(int64_t b) const { return b * k0 + 4 * (clamped_sum(ends, R, cap, b) - (window ? clamped_sum(starts, R, cap, b) : 0)); }
+};
+template <int R>
+__host__ __device__ __forceinline__ ChunkSeq chunk_sequence(const ChunkParams &p, int s) {
+    ChunkSeq q;
+    q.q0 = p.q_start[s];
+    q.n_q = min(max(p.q_start[s + 1] - q.q0, 0), p.max_q);
+    const int len = min(max(p.kv_len[s], 0), 1 << 30);
+    q.len = min(len, p.max_len);
+    q.before = len - q.n_q;
+    q.blocks = (int)(((int64_t)q.n_q * p.group + R - 1) / R);
+    return q;
+}
+template <int R, int TP>
+__host__ __device__ __forceinline__ ChunkCost<R, TP> chunk_cost(const ChunkParams &p, const ChunkSeq &q) {
+    ChunkCost<R, TP> c;
+    const int64_t g = p.group;
+    c.ends = g * q.before + R;
+    c.starts = g * ((int64_t)q.before - p.window + 1);
+    c.cap = g * q.len;
+    c.window = p.window > 0;
+    c.k0 = 4 * g * TP * kChunkSetup;
+    c.head = c.last = 0;
+    if (q.blocks > 0) {
+        const int64_t done = (int64_t)(q.blocks - 1) * R, left = q.n_q * g - done;
+        const int64_t end = min(max(g * ((int64_t)q.before + q.n_q), (int64_t)0), c.cap), start = c.window ? min(max(c.starts + done, (int64_t)0), c.cap) : 0;
+        c.last = c.k0 + (left > 128 ? 4 : 3) * max(end - start, (int64_t)0);
+        c.head = c.prefix(q.blocks - 1) + c.last;
+    }
+    return c;
+}
+// The tiles of positions that some row of block b sees (one at least).
+template <int R, int TP>
+__host__ __device__ __forceinline__ void chunk_tiles(const ChunkParams &p, const ChunkSeq &q, int b, int &tile0, int &tiles) {
+    const int64_t rows = (int64_t)q.n_q * p.group;
+    const int t0 = (int)((int64_t)b * R / p.group), t1 = (int)((min(rows, (int64_t)(b + 1) * R) - 1) / p.group);
+    const int end = max(min(q.len, q.before + t1 + 1), 0), start = p.window > 0 ? max(0, q.before + t0 - p.window + 1) : 0;
+    tile0 = min(start, max(end - 1, 0)) / TP;
+    tiles = max(1, (end + TP - 1) / TP - tile0);
+}
+
+// A place in the work: a tile of a block of rows of a key head of a sequence.
+struct ChunkPlace {
+    int s, kvh, b, tile;
+};
+template <int R, int TP>
+struct ChunkWalk {
+    ChunkPlace at, end;    // at.tile: the first tile of the current item that is this CTA's
+    ChunkSeq sq;
+    int64_t total, base;   // units in all, and before the first item's sequence
+    int64_t first_unit, behind_unit;
+    int grid, cta;
+    bool first, over;
+    // of the current item; parts: see Shared
+    int kvh, block, s, n_rows, tile0, tiles, parts;
+    bool begins, ends;
+
+    __host__ __device__ __forceinline__ static int64_t unit_of(int64_t total, int grid, int b) { return total / grid * b + total % grid * b / grid; }
+    // The tile that a border lies at, `off` units into an item of `cost`: borders near an item's ends are at them.
+    __host__ __device__ __forceinline__ static int tile_at(int64_t off, int64_t cost, int tiles, int whole) {
+        if (whole) return 2 * off < cost ? 0 : tiles;
+        const int t = (int)((double)off / (double)cost * tiles);
+        return t < 2 ? 0 : t > tiles - 2 ? tiles : t;
+    }
+    __host__ __device__ __forceinline__ ChunkPlace place(const ChunkParams &p, int s, int64_t in_seq) const {
+        ChunkPlace r;
+        const ChunkSeq q = chunk_sequence<R>(p, s);
+        const ChunkCost<R, TP> c = chunk_cost<R, TP>(p, q);
+        r.s = s;
+        r.kvh = (int)min(in_seq / c.head, (int64_t)p.n_kv - 1);
+        const int64_t in_head = in_seq - r.kvh * c.head;
+        int lo = 0, hi = q.blocks - 1;   // the last block that begins at or before it
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (c.prefix(mid) <= in_head) lo = mid;
+            else hi = mid - 1;
+        }
+        r.b = lo;
+        int t0, tiles;
+        chunk_tiles<R, TP>(p, q, lo, t0, tiles);
+        const int64_t from = c.prefix(lo);
+        r.tile = tile_at(in_head - from, (lo == q.blocks - 1 ? c.last : c.prefix(lo + 1) - from), tiles, p.whole);
+        return r;
+    }
+    // By the whole CTA, of 128 threads or more.
+    __device__ __forceinline__ void start(const ChunkParams &p) {
+        __shared__ int64_t s_sum[4], s_before[2];
+        __shared__ int s_found[2];
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+        int64_t lo = 0, mine = 0;
+        auto scan = [&](int s0, int64_t from) {
+            const int i = s0 + tid;
+            mine = tid < 128 && i < p.n_seq ? p.n_kv * chunk_cost<R, TP>(p, chunk_sequence<R>(p, i)).head : 0;
+            int64_t upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            if (lane == 31 && warp < 4) s_sum[warp] = upto;
+            __syncthreads();
+            int64_t all = 0;
+            lo = from + upto - mine;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                if (w < warp) lo += s_sum[w];
+                all += s_sum[w];
+            }
+            __syncthreads();
+            return all;
+        };
+        total = 0;
+        for (int s0 = 0; s0 < p.n_seq; s0 += 128) total += scan(s0, total);
+        share(p, (int)blockIdx.x);
+        const int64_t u[2] = {first_unit, behind_unit};
+        if (tid < 2) s_found[tid] = p.n_seq, s_before[tid] = total;
+        __syncthreads();
+        int64_t from = 0;
+        for (int s0 = 0; s0 < p.n_seq; s0 += 128) {
+            if (p.n_seq > 128) from += scan(s0, from);   // (up to 128 sequences the first scan's values stand)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                if (u[i] >= lo && u[i] < lo + mine) s_found[i] = s0 + tid, s_before[i] = lo;
+        }
+        __syncthreads();
+        begin(p, s_found[0], s_before[0], s_found[1], s_before[1]);
+    }
+    // Of CTA b, with the total of units: how many share them, and its own.
+    __host__ __device__ __forceinline__ void share(const ChunkParams &p, int b) {
+        // A share is longer than what an item costs beside its tiles and two tiles: no two borders lie at one tile inside an item, whose units a tile are at most
+        // 4 group (TP kChunkSetup / tiles + TP + 2).
+        const int64_t least = (int64_t)4 * p.group * TP * (kChunkSetup + 3);
+        cta = b;
+        grid = (int)max(min((int64_t)p.grid, total / least), (int64_t)1);
+        first_unit = unit_of(total, grid, min(b, grid));
+        behind_unit = unit_of(total, grid, min(b + 1, grid));
+    }
+    // The sequences in which its first unit and the one behind its last lie (n_seq: none), and the units before each.
+    __host__ __device__ __forceinline__ void begin(const ChunkParams &p, int s0, int64_t before0, int s1, int64_t before1) {
+        over = first_unit >= behind_unit || s0 >= p.n_seq;
+        base = before0;
+        at = end = {p.n_seq, 0, 0, 0};
+        if (!over) {
+            at = place(p, s0, first_unit - before0);
+            if (s1 < p.n_seq) end = place(p, s1, behind_unit - before1);
+            sq = chunk_sequence<R>(p, at.s);
+        }
+        first = true;
+        kvh = block = s = n_rows = tile0 = tiles = parts = 0;
+        begins = ends = false;
+    }
+    // Parts of the item that this CTA has the second one of, 0 if it has not.
+    __host__ __device__ __forceinline__ int count_parts(const ChunkParams &p, int all) const {
+        const ChunkCost<R, TP> c = chunk_cost<R, TP>(p, sq);
+        const int64_t from = base + at.kvh * c.head + c.prefix(at.b), cost = at.b == sq.blocks - 1 ? c.last : c.prefix(at.b + 1) - c.prefix(at.b);
+        const int me = cta;
+        if (me == 0) return 0;
+        const int64_t before = unit_of(total, grid, me - 1) - from;
+        if (before >= 0 && tile_at(before, cost, all, p.whole) > 0) return 0;
+        // the last border that lies in the item
+        int e = (int)min((int64_t)grid - 1, (int64_t)((double)(from + cost) / (double)total * grid) + 1);
+        while (e > me && (unit_of(total, grid, e) - from >= cost || tile_at(unit_of(total, grid, e) - from, cost, all, p.whole) >= all)) e--;
+        return e - me + 2;
+    }
+    __host__ __device__ __forceinline__ bool next(const ChunkParams &p) {
+        while (!over) {
+            int t0, all;
+            chunk_tiles<R, TP>(p, sq, at.b, t0, all);
+            const bool last = at.s == end.s && at.kvh == end.kvh && at.b == end.b;
+            const int from = at.tile, upto = last ? min(end.tile, all) : all;
+            const bool some = upto > from;
+            if (some) {
+                kvh = at.kvh, block = at.b, s = at.s;
+                n_rows = (int)min((int64_t)R, (int64_t)sq.n_q * p.group - (int64_t)at.b * R);
+                tile0 = t0 + from, tiles = upto - from;
+                begins = from == 0, ends = upto == all;
+                parts = first && from > 0 ? count_parts(p, all) : 0;
+            }
+            const ChunkSeq was = sq;
+            first = false;
+            at.tile = 0;
+            if (last) over = true;
+            else if (++at.b >= sq.blocks) {
+                at.b = 0;
+                if (++at.kvh >= p.n_kv) {
+                    at.kvh = 0;
+                    do {
+                        if (++at.s >= p.n_seq) {
+                            over = true;
+                            break;
+                        }
+                        sq = chunk_sequence<R>(p, at.s);
+                    } while (sq.blocks == 0);
+                    if (!over && at.s > end.s) over = true;
+                }
+            }
+            if (some) {
+                now = was;
+                return true;
+            }
+        }
+        return false;
+    }
+    ChunkSeq now;   // the current item's sequence
+    __host__ __device__ __forceinline__ void note(const ChunkParams &p) const {   // by one thread
+        Shared it;
+        it.parts = parts;
+        it.n_rows = n_rows;
+        it.kvh = kvh;
+        it.row0 = block * R;
+        it.q0 = now.q0;
+        it.pad[0] = it.pad[1] = it.pad[2] = 0;
+        p.shared[blockIdx.x] = it;
+    }
+};
+
+template <int D, int NT>
+struct Chunk {
+    static constexpr int NQ = chunk_tiles_of(D), TP = chunk_positions(D), R = chunk_rows(D);
+    static constexpr int kMetaBytes = 1920;
+    static constexpr int kPanels = (D + 63) / 64;                    // blocks of 64 values
+    static constexpr int kTerm = kPanels * 128 * 128, kQTile = NT * kTerm;
+    static constexpr int kSlot = kPanels * TP * 128;                 // half a tile: keys or values
+    static constexpr int kRoom = 227 * 1024 - 1024 - kMetaBytes - 64 - NQ * kQTile;   // (64: ChunkWalk::start)
+    static constexpr int kSlots = kRoom / kSlot > 6 ? 6 : kRoom / kSlot;
+    static constexpr int kQ = kSlots * kSlot, kMeta = kQ + NQ * kQTile, kBytes = kMeta + kMetaBytes + 1024;   // (begins on a 1024-byte boundary)
+    static constexpr int kSoft = 4 * NQ, kWarps = kSoft + kChunkCopyWarps + 1, kThreads = 32 * kWarps;
+    static constexpr uint32_t kO = 256;                              // column of the sums; of the second tile's: 128 more
+    static constexpr uint32_t kS = NQ == 2 ? 128 : 64;               // from a place of scores to the next
+    static_assert(kSlots >= 3, "a half tile of values and one of keys at work, one on its way");
+    static_assert(kBytes + 64 <= 227 * 1024, "shared memory");
+    using Walk = ChunkWalk<R, TP>;
+};
+
+template <int R, int TP>
+struct ChunkMeta {
+    unsigned long long kv_full[6], kv_empty[6], s_full[2], p_full[2], pv_done[2], q_full[2], drained;
+    float scale[R];
+    uint32_t odd[2][8];       // of a tile of rows, an item in turn: values of a tile that not all rows see are no numbers
+    uint8_t there[8];         // of a tile of positions, in turn: bit c: chunk c is a page's
+    int goes_on[2];
+    uint32_t tmem;
+    int gave_up;
+    ChunkWalk<R, TP> walk[2];
+};
+
+__device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t *v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, "
+                 "%26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
+                   "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+                   "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(at) : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t *v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, "
+                 "%27, %28, %29, %30, %31, %32};"
+                 ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
+                   "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]),
+                   "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+}
+// The same with A in tensor memory (lane = row, a column two f16).
+__device__ __forceinline__ void product_from(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t onto, uint32_t elected) {
+    asm volatile("{\n .reg .pred p, q;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %7, 0;\n mov.b64 b, {%2, %3};\n"
+                 " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, {%6, %6, %6, %6}, p;\n}\n"
+                 ::"r"(d), "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(onto), "r"(0u), "r"(elected) : "memory");
+}
+// Bytes I and J of w, as `halves` in krk_attn_kernel.cuh.
+template <int I, int J>
+__device__ __forceinline__ uint32_t halves_of(uint32_t w, uint32_t off) { return halves<I, J>(w, off); }
+__device__ __forceinline__ float capped_half(float x, float cap) {   // as capped, through one exponential: 2^-22 of the cap off, f16 weights take no more
+    const float e = ex2(x * (2.0f * 1.44269504f) / cap);
+    return cap * (1.44269504f - 2.0f * 1.44269504f * __frcp_rn(1.0f + e));
+}
+// A value of a cache as f16 products see it, by a slow path.
+template <int CT, int D>
+__device__ __forceinline__ float value_at(const uint8_t *pool, const __half *scale, int64_t row, int c) {
+    if constexpr (CT == KRK_CUDA_KV_F16) return __half2float(reinterpret_cast<const __half *>(pool)[row * D + c]);
+    const __half d = scale[row * (D / 32) + c / 32];
+    int q;
+    if constexpr (CT == KRK_CUDA_KV_Q8) q = (int8_t)pool[row * D + c];
+    else {
+        const int b = pool[row * (D / 2) + c / 32 * 16 + c % 16];
+        q = ((c & 16) ? b >> 4 : b & 15) - 8;
+    }
+    return __half2float(__hmul(d, __int2half_rn(q)));
+}
+
+// HALF: f16 out, one term of each query and weight (NT), else f32 and two.
+template <int D, int CT, bool HALF>
+__global__ void __launch_bounds__((Chunk<D, HALF ? 1 : 2>::kThreads), 1)
+attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
+    constexpr int NT = HALF ? 1 : 2;
+    using C = Chunk<D, NT>;
+    using Walk = typename C::Walk;
+    constexpr int NQ = C::NQ, TP = C::TP, R = C::R, RB = row_bytes_of(CT, D), kChunks = TP / kChunk;
+    constexpr bool kQuant = CT != KRK_CUDA_KV_F16;
+    extern __shared__ uint8_t raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t base = smem_addr(smem);
+    using Meta = ChunkMeta<R, TP>;
+    static_assert(sizeof(Meta) <= C::kMetaBytes, "Chunk::kMeta");
+    Meta &meta = *reinterpret_cast<Meta *>(smem + C::kMeta);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    volatile int *gave_up = &meta.gave_up;
+    auto bar = [&](unsigned long long &b) { return smem_addr(&b); };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int i = 0; i < C::kSlots; i++) {
+                bar_init(bar(meta.kv_full[i]), kChunkCopyWarps);
+                bar_init(bar(meta.kv_empty[i]), 1);
+            }
+            for (int i = 0; i < 2; i++) {
+                bar_init(bar(meta.s_full[i]), 1);
+                bar_init(bar(meta.p_full[i]), 4);
+                bar_init(bar(meta.pv_done[i]), 1);
+                bar_init(bar(meta.q_full[i]), 4);
+            }
+            bar_init(bar(meta.drained), 1);
+            meta.gave_up = 0;
+        }
+        if (lane < 16) meta.odd[lane >> 3][lane & 7] = 0;
+        __syncwarp();
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        async_fence();
+    }
+    if (warp == C::kWarps - 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&meta.tmem)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_before();
+    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    Walk walk;
+    walk.start(p);   // (its barriers publish those above)
+    if (!p.whole && tid == 0) p.shared[blockIdx.x].parts = 0;
+    if (warp < C::kSoft && (tid & 127) == 0) meta.walk[warp >> 2] = walk;
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = meta.tmem;
+    // tiles of an item that rows of tile q see; those of the first tile of rows end earlier
+    auto tiles_of = [&](const Walk &w, int q) {
+        if (q * 128 >= w.n_rows) return 0;
+        const int t1 = (int)(((int64_t)w.block * R + min(w.n_rows, (q + 1) * 128) - 1) / p.group), end = min(w.now.len, w.now.before + t1 + 1);
+        return min(w.tiles, max((end + TP - 1) / TP - w.tile0, 1));
+    };
+
+    if (warp < C::kSoft) {
+        // ===== softmax: thread = row
+        const int tq = warp >> 2, r_in = tid & 127, quarter = warp & 3;
+        const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16), t_o = t_lane + C::kO + 128 * tq;
+        uint8_t *q_tile = smem + C::kQ + tq * C::kQTile;
+        uint32_t n_tile = 0, n_item = 0, n_all = 0;   // tiles of this tile of rows, items, tiles of all items
+        for (;;) {
+            if ((tid & 127) == 0) {
+                Walk w = meta.walk[tq];
+                meta.goes_on[tq] = w.next(p);
+                if (tq == 0 && meta.goes_on[tq] && w.parts > 0) w.note(p);
+                meta.walk[tq] = w;
+            }
+            group_sync(tq);
+            if (!meta.goes_on[tq]) break;
+            const Walk &walk = meta.walk[tq];
+            const int n_rows = walk.n_rows, tiles = tiles_of(walk, tq), tile0 = walk.tile0, before = walk.now.before, len = walk.now.len, kvh = walk.kvh, q0 = walk.now.q0;
+            const int64_t row0 = (int64_t)walk.block * R + 128 * tq;   // among the key head's
+            const bool whole = walk.begins && walk.ends;
+            const int place_of_part = walk.begins ? 1 : 0;
+            const int mine_rows = min(128, n_rows - 128 * tq);
+            const uint32_t n_before = n_all;
+            n_all += walk.tiles;
+            if (mine_rows <= 0) {
+                n_item++;
+                group_sync(tq);
+                continue;
+            }
+            // ---- queries, four values a lane, eight rows at a time, under a power of two of their own: the largest value in [2^10, 2^11)
+            constexpr int NL = (D + 127) / 128;
+            const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+#pragma unroll 1
+            for (int j0 = 0; j0 < 32; j0 += 8) {
+                float x[8][NL][4], most[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int r = 32 * quarter + j0 + j;
+                    const int64_t rr = row0 + r;
+                    const int i = (int)(rr / p.group), h = kvh * p.group + (int)(rr - (int64_t)i * p.group);
+                    const int64_t from = (int64_t)(q0 + i) * p.q_stride + (int64_t)h * D;
+#pragma unroll
+                    for (int c = 0; c < NL; c++) {
+                        const int d = 128 * c + 4 * lane;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[j][c][e] = 0.0f;
+                        if (r < mine_rows && (D % 128 == 0 || d < D)) {
+                            if (p.q_half) {
+                                const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const __half *>(p.q) + from + d);
+                                const float2 a = __half22float2(half2_of(w.x)), b = __half22float2(half2_of(w.y));
+                                x[j][c][0] = a.x, x[j][c][1] = a.y, x[j][c][2] = b.x, x[j][c][3] = b.y;
+                            } else {
+                                *reinterpret_cast<float4 *>(x[j][c]) = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + from + d);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    most[j] = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < NL; c++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) most[j] = fmaxf(most[j], fabsf(x[j][c][e]));
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) most[j] = fmaxf(most[j], __shfl_xor_sync(0xFFFFFFFFu, most[j], o));
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int r = 32 * quarter + j0 + j;
+                    const int e = most[j] > 0.0f && most[j] <= 3.4028234e38f ? 10 - max((int)(__float_as_uint(most[j]) >> 23) - 127, -110) : 0;
+                    const float up = sign * __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+                    for (int c = 0; c < NL; c++) {
+                        const int d = 128 * c + 4 * lane;
+                        if (D % 128 == 0 || d < D) {
+                            uint32_t hi[2], lo[2];
+                            split(x[j][c][0] * up, x[j][c][1] * up, hi[0], lo[0]);
+                            split(x[j][c][2] * up, x[j][c][3] * up, hi[1], lo[1]);
+                            uint8_t *to = q_tile + (d >> 6) * (128 * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + 2 * (d & 7);
+                            *reinterpret_cast<uint2 *>(to) = make_uint2(hi[0], hi[1]);
+                            if constexpr (NT == 2) *reinterpret_cast<uint2 *>(to + C::kTerm) = make_uint2(lo[0], lo[1]);
+                        }
+                    }
+                    if (lane == 0) meta.scale[128 * tq + r] = fabsf(p.scale) * (p.softcap > 0.0f ? 1.0f : 1.44269504f) * __uint_as_float((uint32_t)(127 - e) << 23);
+                }
+            }
+            async_fence();
+            __syncwarp();
+            if (lane == 0) bar_arrive(bar(meta.q_full[tq]));
+
+            const float sc = meta.scale[128 * tq + r_in];
+            const int64_t rr = row0 + min(r_in, mine_rows - 1);
+            const int token = (int)(rr / p.group), head = kvh * p.group + (int)(rr - (int64_t)token * p.group);
+            const int behind = min(len, before + token + 1), from = p.window > 0 ? max(0, before + token - p.window + 1) : 0;   // what the row sees: [from, behind)
+            // every row of this tile of rows sees [all_from, all_to)
+            const int all_to = min(len, before + (int)(row0 / p.group) + 1), all_from = p.window > 0 ? before + (int)((row0 + mine_rows - 1) / p.group) - p.window + 1 : 0;
+            float m = -INFINITY, l = 0.0f;
+            for (int i = 0; i < tiles; i++, n_tile++) {
+                const int pos0 = (tile0 + i) * TP;
+                const int sb = NQ == 2 ? tq : (int)(n_tile & 1);
+                const uint32_t s_phase = NQ == 2 ? n_tile & 1 : (n_tile >> 1) & 1, t_s = t_lane + C::kS * sb;
+                bar_wait(bar(meta.s_full[sb]), s_phase, gave_up, p.status);
+                tc_after();
+                const uint32_t there = *reinterpret_cast<volatile uint8_t *>(&meta.there[(n_before + i) & 7]);
+                const bool masked = pos0 + TP > all_to || pos0 < all_from || there != (1u << kChunks) - 1u;
+                float f = sc, top = -INFINITY;
+                if (masked || p.softcap > 0.0f) {
+                    // log2 scores in place of the products
+                    f = 1.0f;
+                    const int lo = from - pos0, hi = behind - pos0;
+#pragma unroll 1
+                    for (int c = 0; c < TP; c += 32) {
+                        uint32_t v[32];
+                        tmem_load32(t_s + c, v);
+                        tmem_loaded();
+                        const uint32_t ok = (there >> (c / 16)) & 3u, seen16 = (ok & 1u ? 0xFFFFu : 0u) | (ok & 2u ? 0xFFFF0000u : 0u);
+                        const int a = max(lo - c, 0), b = hi - c;
+                        const uint32_t seen = (a >= 32 ? 0u : 0xFFFFFFFFu << a) & (b >= 32 ? 0xFFFFFFFFu : b <= 0 ? 0u : 0xFFFFFFFFu >> (32 - b)) & seen16;
+#pragma unroll
+                        for (int j = 0; j < 32; j++) {
+                            float x = __uint_as_float(v[j]) * sc;
+                            if (p.softcap > 0.0f) x = HALF ? capped_half(x, p.softcap) : capped(x, p.softcap);
+                            if (!((seen >> j) & 1)) x = -INFINITY;
+                            top = fmaxf(top, x);
+                            v[j] = __float_as_uint(x);
+                        }
+                        tmem_store32(t_s + c, v);
+                    }
+                    tmem_stored();
+                } else {
+#pragma unroll
+                    for (int c = 0; c < TP; c += 64) {
+                        uint32_t v[64];
+                        tmem_load32(t_s + c, v);
+                        tmem_load32(t_s + c + 32, v + 32);
+                        tmem_loaded();
+#pragma unroll
+                        for (int j = 0; j < 64; j += 2) top = fmaxf(top, fmaxf(__uint_as_float(v[j]), __uint_as_float(v[j + 1])));
+                    }
+                    top *= sc;
+                }
+                if (__any_sync(0xFFFFFFFFu, top > m + kLetBe || (m == -INFINITY && top != -INFINITY))) {
+                    const float now = fmaxf(m, top), corr = now == -INFINITY ? 1.0f : ex2(m - now);
+                    m = now;
+                    l *= corr;
+                    if (i > 0) {
+                        bar_wait(bar(meta.pv_done[tq]), (n_tile - 1) & 1, gave_up, p.status);
+                        tc_after();
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            tmem_load32(t_o + c, o);
+                            tmem_loaded();
+#pragma unroll
+                            for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                            tmem_store32(t_o + c, o);
+                        }
+                        tmem_stored();
+                    }
+                }
+                const float less = m == -INFINITY ? 0.0f : -m;
+#pragma unroll
+                for (int c = 0; c < TP; c += 32) {
+                    uint32_t v[32];
+                    tmem_load32(t_s + c, v);
+                    tmem_loaded();
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    uint32_t w[NT * 16];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        float a, b;
+                        if constexpr (HALF) {
+                            a = ex2(fmaf(__uint_as_float(v[j]), f, less + 7.0f)), b = ex2(fmaf(__uint_as_float(v[j + 1]), f, less + 7.0f));
+                            w[j / 2] = bits(__floats2half2_rn(a, b));
+                        } else {
+                            a = kUp * ex2(fmaf(__uint_as_float(v[j]), f, less)), b = kUp * ex2(fmaf(__uint_as_float(v[j + 1]), f, less));
+                            split(a, b, w[j / 2], w[16 + j / 2]);
+                        }
+                        sum[j & 2] += a;
+                        sum[(j & 2) + 1] += b;
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    // (first terms in 16 columns, then the second ones: the place of the scores that were just read, or before it)
+                    if constexpr (HALF) tmem_store16(t_s + c / 2, w);
+                    else tmem_store32(t_s + c, w);
+                }
+                tmem_stored();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(bar(meta.p_full[sb]));
+            }
+
+            // ---- the row's factor, and its outputs through shared memory, in the place of the queries: 32 columns at a time, rows by the warp that has them
+            const float all = l * (1.0f / kUp);
+            float keep, out_f = 1.0f / kUp;
+            if (whole) {
+                float lw = all;
+                keep = 1.0f;
+                if (p.sinks) {
+                    const float sink = p.sinks[head] * 1.44269504f, t = fmaxf(m, sink);
+                    keep = m == -INFINITY ? 0.0f : exp2f(m - t);
+                    lw = lw * keep + (sink == -INFINITY ? 0.0f : sink == t ? 1.0f : exp2f(sink - t));
+                }
+                out_f *= lw == 0.0f ? 0.0f : keep / lw;
+            } else if (r_in < mine_rows) {
+                float *to = p.part + (((size_t)blockIdx.x * 2 + place_of_part) * R + 128 * tq + r_in) * (D + 2);
+                *reinterpret_cast<float2 *>(to + D) = make_float2(m, all);
+            }
+            if (NQ == 1 && tiles > 1) bar_wait(bar(meta.pv_done[tq]), (n_tile - 2) & 1, gave_up, p.status);   // (the products of two tiles may be in flight: a parity tells one from the next)
+            bar_wait(bar(meta.pv_done[tq]), (n_tile - 1) & 1, gave_up, p.status);
+            tc_after();
+            const bool any_odd = *reinterpret_cast<volatile uint32_t *>(&meta.odd[tq][n_item & 7]) != 0;
+            uint8_t *stage = q_tile + quarter * (32 * 128);
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                tmem_load32(t_o + c, o);
+                tmem_loaded();
+                if (any_odd) {
+                    // values that are no numbers, in tiles that not all rows see, were taken out of the products: here are they for the rows that see them
+                    const int first_token = (int)((int64_t)walk.block * R / p.group), last_token = (int)(((int64_t)walk.block * R + n_rows - 1) / p.group);
+                    const int end = min(behind, (tile0 + tiles) * TP);
+                    for (int pos = max(from, tile0 * TP); pos < end; pos++) {
+                        const int t0 = pos / TP * TP;
+                        if (!(t0 + TP > min(len, before + first_token + 1) || (p.window > 0 && t0 < before + last_token - p.window + 1))) {
+                            pos = t0 + TP - 1;
+                            continue;
+                        }
+                        const int page = p.table[(size_t)walk.s * p.table_width + pos / p.page_size];
+                        if (page < 0 || page >= p.n_pages) continue;
+                        const int64_t row = ((int64_t)page * p.n_kv + kvh) * p.page_size + pos % p.page_size;
+                        for (int j = 0; j < 32; j++) {
+                            const float y = value_at<CT, D>(p.v, p.v_scale, row, c + j);
+                            if (fabsf(y) <= 65504.0f) continue;
+#pragma unroll
+                            for (int k = 0; k < 32; k++)
+                                if (k == j) o[k] = __float_as_uint(__uint_as_float(o[k]) + y);
+                        }
+                    }
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int j = 0; j < 32; j += 4)
+                    *reinterpret_cast<float4 *>(stage + lane * 128 + (((j / 4) ^ (lane & 7)) << 4)) =
+                        make_float4(__uint_as_float(o[j]) * out_f, __uint_as_float(o[j + 1]) * out_f, __uint_as_float(o[j + 2]) * out_f, __uint_as_float(o[j + 3]) * out_f);
+                __syncwarp();
+#pragma unroll 2
+                for (int r0 = 0; r0 < 32; r0 += 4) {
+                    const int r = r0 + lane / 8, rw = 32 * quarter + r, at = c + 4 * (lane & 7);
+                    if (rw >= mine_rows) continue;
+                    const float4 x = *reinterpret_cast<const float4 *>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+                    if (whole) {
+                        const int64_t g = row0 + rw;
+                        const int t = (int)(g / p.group), h = kvh * p.group + (int)(g - (int64_t)t * p.group);
+                        const int64_t to = (int64_t)(q0 + t) * p.out_stride + (int64_t)h * D + at;
+                        if constexpr (HALF) {
+                            *reinterpret_cast<uint2 *>(static_cast<__half *>(p.out) + to) = make_uint2(bits(__floats2half2_rn(x.x, x.y)), bits(__floats2half2_rn(x.z, x.w)));
+                        } else {
+                            *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to) = x;
+                        }
+                    } else {
+                        float *to = p.part + (((size_t)blockIdx.x * 2 + place_of_part) * R + 128 * tq + rw) * (D + 2) + at;
+                        *reinterpret_cast<float2 *>(to) = make_float2(x.x, x.y);
+                        *reinterpret_cast<float2 *>(to + 2) = make_float2(x.z, x.w);
+                    }
+                }
+                __syncwarp();
+            }
+            tc_before();
+            group_sync(tq);
+            if (any_odd && (tid & 127) == 0) meta.odd[tq][n_item & 7] = 0;
+            n_item++;
+        }
+    } else if (warp < C::kSoft + kChunkCopyWarps) {
+        // ===== keys and values into a ring of half tiles (keys, values in turn); a warp has the chunks w, w + 4 of 16 positions
+        constexpr int kMine = kChunks / kChunkCopyWarps, kAhead = 32 / kChunks;   // chunks of a warp; tiles whose rows the lanes hold
+        const int w = warp - C::kSoft;
+        int n_item = 0, h = 0;
+        auto take_out = [&](uint32_t &x) {   // of two f16, those that are no numbers
+            bool bad = false;
+            if ((x & 0x7C00u) == 0x7C00u) x &= 0xFFFF0000u, bad = true;
+            if ((x & 0x7C000000u) == 0x7C000000u) x &= 0xFFFFu, bad = true;
+            return bad;
+        };
+        auto tell_odd = [&](int item) {
+            atomicOr(&meta.odd[0][item & 7], 1u);
+            atomicOr(&meta.odd[1][item & 7], 1u);
+        };
+        int64_t pool_rows = 0;   // lane: of chunk lane % kChunks of tile i + lane / kChunks, -1: none
+        int told = 0, tag = -1;  // f16: half tiles told of; lane h % 32: of half tile h, the item whose values are looked at, -1: not
+        constexpr int kPieces = RB / 16, kCopies = (kChunk * kPieces + 31) / 32;
+        // f16: 16-byte pieces asynchronously, where a lane's go: the pattern repeats every eight rows
+        uint32_t to[kQuant ? 1 : kCopies / 2];
+        if constexpr (!kQuant) {
+#pragma unroll
+            for (int j = 0; j < kCopies / 2; j++) {
+                const int c = lane + 32 * j, row = c / kPieces, piece = c % kPieces;
+                to[j] = (piece >> 3) * (TP * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+            }
+        }
+        auto tell = [&](int n) {   // all but the n last ones have arrived
+            if (n == 0) copies_wait<0>();
+            else copies_wait<2>();
+            for (; told < h - n; told++) {
+                const int item = __shfl_sync(0xFFFFFFFFu, tag, told & 31);
+                if (item >= 0) {
+                    bool bad = false;
+                    for (int m = 0; m < kMine; m++)
+#pragma unroll
+                        for (int j = 0; j < kCopies; j++) {
+                            const uint32_t off = to[kQuant ? 0 : j % (kCopies / 2)] + (j / (kCopies / 2)) * 1024;
+                            uint4 *at = reinterpret_cast<uint4 *>(smem + told % C::kSlots * C::kSlot + (w + kChunkCopyWarps * m) * (kChunk * 128) + off);
+                            uint4 v = *at;
+                            const bool b0 = take_out(v.x), b1 = take_out(v.y), b2 = take_out(v.z), b3 = take_out(v.w);
+                            if (b0 || b1 || b2 || b3) *at = v, bad = true;
+                        }
+                    if (bad) tell_odd(item);
+                }
+                async_fence();
+                __syncwarp();
+                if (lane == 0) bar_arrive(bar(meta.kv_full[told % C::kSlots]));
+            }
+        };
+        while (walk.next(p)) {
+            const ChunkSeq &sq = walk.now;
+            const int32_t *table = p.table + (size_t)walk.s * p.table_width;
+            const int first_token = (int)((int64_t)walk.block * R / p.group), last_token = (int)(((int64_t)walk.block * R + walk.n_rows - 1) / p.group);
+            const int all_to = min(sq.len, sq.before + first_token + 1), all_from = p.window > 0 ? sq.before + last_token - p.window + 1 : 0;
+            auto looked_at = [&](int i) { return (walk.tile0 + i) * TP + TP > all_to || (walk.tile0 + i) * TP < all_from; };
+            auto find_rows = [&](int i) -> int64_t {
+                const int tile = i + lane / kChunks, position = (walk.tile0 + tile) * TP + lane % kChunks * kChunk;
+                if (tile >= walk.tiles || position >= sq.len) return -1;
+                const int page = table[position / p.page_size];
+                return page < 0 || page >= p.n_pages ? -1 : ((int64_t)page * p.n_kv + walk.kvh) * p.page_size + position % p.page_size;
+            };
+            // of tile i: its rows, and which chunks there are, for the softmax. `tile_no`: of all tiles
+            auto begin_tile = [&](int i, int tile_no) {
+                if (i % kAhead == 0) pool_rows = find_rows(i);
+                const uint32_t there = __ballot_sync(0xFFFFFFFFu, pool_rows >= 0) >> (kChunks * (i % kAhead)) & ((1u << kChunks) - 1u);
+                if (w == 0 && lane == 0) meta.there[tile_no & 7] = (uint8_t)there;
+            };
+            auto row_of = [&](int i, int m) { return __shfl_sync(0xFFFFFFFFu, pool_rows, kChunks * (i % kAhead) + w + kChunkCopyWarps * m); };
+            if constexpr (!kQuant) {
+#pragma unroll 1
+                for (int i = 0; i < walk.tiles; i++) {
+                    begin_tile(i, h >> 1);
+#pragma unroll 1
+                    for (int kv = 0; kv < 2; kv++) {
+                        const int slot = h % C::kSlots;
+                        const uint32_t empty = bar(meta.kv_empty[slot]), parity = ((h / C::kSlots) & 1) ^ 1;
+                        if (!bar_test(empty, parity)) {
+                            tell(0);   // (who frees the place may wait for these)
+                            bar_wait(empty, parity, gave_up, p.status);
+                        }
+#pragma unroll
+                        for (int m = 0; m < kMine; m++) {
+                            const int chunk = w + kChunkCopyWarps * m, position = (walk.tile0 + i) * TP + chunk * kChunk;
+                            const int64_t row0 = row_of(i, m);
+                            const int left = row0 < 0 ? 0 : sq.len - position;   // rows that are not there come in as zeros
+                            const uint8_t *src = (kv ? p.v : p.k) + row0 * RB + 16 * lane;   // (no row: not looked at, a cache without pages has no memory)
+                            const uint32_t at = base + slot * C::kSlot + chunk * (kChunk * 128);
+                            if (left >= kChunk) {
+#pragma unroll
+                                for (int j = 0; j < kCopies; j++) copy16(to[j % (kCopies / 2)] + at + (j / (kCopies / 2)) * 1024, src + 512 * j, true);
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < kCopies; j++) copy16(to[j % (kCopies / 2)] + at + (j / (kCopies / 2)) * 1024, row0 < 0 ? static_cast<const uint8_t *>(p.q) : src + 512 * j, (lane + 32 * j) / kPieces < left);
+                            }
+                        }
+                        copies_commit();
+                        if (lane == (h & 31)) tag = kv && looked_at(i) ? n_item : -1;
+                        h++;
+                        if (h - told > 2) tell(2);
+                    }
+                }
+            } else {
+                // 8 and 4 bits: through registers, a piece of 16 bytes at a time; a half tile's pieces are asked for while the one before it is unpacked
+                uint4 x[kMine * kCopies];
+                __half d[kMine * kCopies];
+                const int halves = 2 * walk.tiles;
+                auto piece = [&](int t, int m, int j, int64_t row0, uint4 &v, __half &scale) {
+                    const int i = t >> 1, c = lane + 32 * j, row = c / kPieces, position = (walk.tile0 + i) * TP + (w + kChunkCopyWarps * m) * kChunk + row;
+                    v = make_uint4(0u, 0u, 0u, 0u);
+                    scale = __float2half_rn(0.0f);
+                    if (row0 >= 0 && c < kChunk * kPieces && position < sq.len) {
+                        v = *reinterpret_cast<const uint4 *>((t & 1 ? p.v : p.k) + row0 * RB + 16 * c);
+                        scale = (t & 1 ? p.v_scale : p.k_scale)[(row0 + row) * (D / 32) + c % kPieces / (CT == KRK_CUDA_KV_Q8 ? 2 : 1)];
+                    }
+                };
+                begin_tile(0, h >> 1);
+#pragma unroll
+                for (int m = 0; m < kMine; m++) {
+                    const int64_t row0 = row_of(0, m);
+#pragma unroll
+                    for (int j = 0; j < kCopies; j++) piece(0, m, j, row0, x[m * kCopies + j], d[m * kCopies + j]);
+                }
+#pragma unroll 1
+                for (int t = 0; t < halves; t++, h++) {
+                    const int slot = h % C::kSlots;
+                    bar_wait(bar(meta.kv_empty[slot]), ((h / C::kSlots) & 1) ^ 1, gave_up, p.status);
+                    const bool look = (t & 1) && looked_at(t >> 1);
+                    bool bad = false;
+                    if (t + 1 < halves && (t & 1)) begin_tile((t + 1) >> 1, (h + 1) >> 1);
+#pragma unroll
+                    for (int m = 0; m < kMine; m++) {
+                        const int64_t row0 = t + 1 < halves ? row_of((t + 1) >> 1, m) : -1;
+                        uint8_t *chunk_at = smem + slot * C::kSlot + (w + kChunkCopyWarps * m) * (kChunk * 128);
+#pragma unroll
+                        for (int j = 0; j < kCopies; j++) {
+                            const int c = lane + 32 * j, row = c / kPieces, pc = c % kPieces;
+                            uint4 v = x[m * kCopies + j];
+                            const __half2 s2 = __half2half2(d[m * kCopies + j]);
+                            if (t + 1 < halves) piece(t + 1, m, j, row0, x[m * kCopies + j], d[m * kCopies + j]);
+                            if (kChunk * kPieces % 32 != 0 && c >= kChunk * kPieces) continue;
+                            constexpr int kUnits = CT == KRK_CUDA_KV_Q8 ? 2 : 4;   // of eight values
+                            uint32_t y[4 * kUnits];
+                            const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                if constexpr (CT == KRK_CUDA_KV_Q8) {
+                                    const uint32_t u = words[k] ^ 0x80808080u;
+                                    y[2 * k] = bits(__hmul2(half2_of(halves_of<0, 1>(u, 0x64806480u)), s2));
+                                    y[2 * k + 1] = bits(__hmul2(half2_of(halves_of<2, 3>(u, 0x64806480u)), s2));
+                                } else {
+                                    const uint32_t u = words[k] & 0x0F0F0F0Fu, u2 = (words[k] >> 4) & 0x0F0F0F0Fu;
+                                    y[2 * k] = bits(__hmul2(half2_of(halves_of<0, 1>(u, 0x64086408u)), s2));
+                                    y[2 * k + 1] = bits(__hmul2(half2_of(halves_of<2, 3>(u, 0x64086408u)), s2));
+                                    y[8 + 2 * k] = bits(__hmul2(half2_of(halves_of<0, 1>(u2, 0x64086408u)), s2));
+                                    y[8 + 2 * k + 1] = bits(__hmul2(half2_of(halves_of<2, 3>(u2, 0x64086408u)), s2));
+                                }
+                            }
+                            if (look) {
+#pragma unroll
+                                for (int k = 0; k < 4 * kUnits; k++) bad |= take_out(y[k]);
+                            }
+#pragma unroll
+                            for (int k = 0; k < kUnits; k++) {
+                                const int unit = kUnits * pc + k;
+                                *reinterpret_cast<uint4 *>(chunk_at + (unit >> 3) * (TP * 128) + row * 128 + (((unit & 7) ^ (row & 7)) << 4)) =
+                                    make_uint4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
+                            }
+                        }
+                    }
+                    if (bad) tell_odd(n_item);
+                    async_fence();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(bar(meta.kv_full[slot]));
+                }
+            }
+            n_item++;
+        }
+        if constexpr (!kQuant) tell(0);
+    } else {
+        // ===== products
+        const uint32_t elected = elected_lane();
+        uint32_t n_done[2] = {0, 0}, n_item[2] = {0, 0};   // of a tile of rows: tiles so far, items
+        int h0 = 0;   // half tiles before this item
+        constexpr uint32_t qk = (1u << 4) | (uint32_t)(TP >> 3) << 17 | (128u >> 4) << 24, pv = (1u << 4) | 1u << 16 | (uint32_t)(D >> 3) << 17 | (128u >> 4) << 24;
+        while (walk.next(p)) {
+            const int n[2] = {tiles_of(walk, 0), NQ == 2 ? tiles_of(walk, 1) : 0}, all = walk.tiles;
+            auto wait_half = [&](int h) { bar_wait(bar(meta.kv_full[h % C::kSlots]), (h / C::kSlots) & 1, gave_up, p.status); };
+            auto place_of = [&](int q, int i) { return NQ == 2 ? q : (int)((n_done[0] + i) & 1); };
+            auto scores = [&](int q, int i) {
+                const int slot = (h0 + 2 * i) % C::kSlots, sb = place_of(q, i);
+                const uint32_t keys = base + slot * C::kSlot, rows = base + C::kQ + q * C::kQTile, d = tmem + C::kS * sb;
+                tc_after();
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int k = 0; k < D / 16; k++)
+                        product(d, desc_lo(rows + t * C::kTerm + (k >> 2) * (128 * 128) + 32 * (k & 3), 16), kDescHi, desc_lo(keys + (k >> 2) * (TP * 128) + 32 * (k & 3), 16), kDescHi, qk,
+                                t > 0 || k > 0, elected);
+                products_commit(bar(meta.s_full[sb]), elected);
+            };
+            auto sums = [&](int q, int i) {
+                const int slot = (h0 + 2 * i + 1) % C::kSlots, sb = place_of(q, i);
+                const uint32_t values = base + slot * C::kSlot, from = tmem + C::kS * sb, d = tmem + C::kO + 128 * q;
+                bar_wait(bar(meta.p_full[sb]), (NQ == 2 ? n_done[q] + i : (n_done[0] + i) >> 1) & 1, gave_up, p.status);
+                tc_after();
+#pragma unroll
+                for (int k = 0; k < TP / 16; k++)
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+                        product_from(d, from + (NT == 2 ? 32 * (k >> 1) + 16 * t + 8 * (k & 1) : 8 * k), desc_lo(values + 2048 * k, TP * 128), kDescHi, pv, i > 0 || k > 0 || t > 0, elected);
+                products_commit(bar(meta.pv_done[q]), elected);
+            };
+            wait_half(h0);
+#pragma unroll
+            for (int q = 0; q < NQ; q++)
+                if (n[q] > 0) {
+                    bar_wait(bar(meta.q_full[q]), n_item[q] & 1, gave_up, p.status);
+                    scores(q, 0);
+                }
+            products_commit(bar(meta.kv_empty[h0 % C::kSlots]), elected);
+#pragma unroll 1
+            for (int i = 0; i < all; i++) {
+                const bool more = i + 1 < all;
+                if constexpr (NQ == 1) {
+                    if (more) {
+                        wait_half(h0 + 2 * i + 2);
+                        scores(0, i + 1);
+                        products_commit(bar(meta.kv_empty[(h0 + 2 * i + 2) % C::kSlots]), elected);
+                    }
+                    wait_half(h0 + 2 * i + 1);
+                    sums(0, i);
+                    products_commit(bar(meta.kv_empty[(h0 + 2 * i + 1) % C::kSlots]), elected);
+                } else {
+                    wait_half(h0 + 2 * i + 1);
+#pragma unroll
+                    for (int q = 0; q < NQ; q++) {
+                        if (i < n[q]) sums(q, i);
+                        if (q == 1) products_commit(bar(meta.kv_empty[(h0 + 2 * i + 1) % C::kSlots]), elected);
+                        if (i + 1 < n[q]) {
+                            wait_half(h0 + 2 * i + 2);
+                            scores(q, i + 1);
+                        }
+                    }
+                    if (more) products_commit(bar(meta.kv_empty[(h0 + 2 * i + 2) % C::kSlots]), elected);
+                }
+            }
+            h0 += 2 * all;
+#pragma unroll
+            for (int q = 0; q < 2; q++)
+                if (n[q] > 0) n_done[q] += n[q], n_item[q]++;
+        }
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (warp == C::kWarps - 1 && *gave_up) {   // (nobody waits any more, so this is the last word on it)
+        products_commit(bar(meta.drained), elected_lane());
+        bar_wait_drained(bar(meta.drained));
+    }
+    if (warp == C::kWarps - 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+template <int D, int CT, bool HALF>
+int launch_chunk_one(const ChunkParams &p, cudaStream_t st) {
+    using C = Chunk<D, HALF ? 1 : 2>;
+    static std::atomic<uint64_t> ready{0};   // devices whose limit of shared memory is raised for this kernel
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && !((ready.load(std::memory_order_acquire) >> dev) & 1)) {
+        e = cudaFuncSetAttribute(attn_chunk_kernel<D, CT, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
+        if (e == cudaSuccess) ready.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    if (e != cudaSuccess) {
+        note_cuda_error(e);
+        return KRK_CUDA_ELAUNCH;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.grid);
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return launched(cudaLaunchKernelEx(&cfg, attn_chunk_kernel<D, CT, HALF>, p));
+}
+template <int CT, bool HALF>
+int launch_chunk_type(const ChunkParams &p, int d, cudaStream_t st) {
+    switch (d) {
+    case 64: return launch_chunk_one<64, CT, HALF>(p, st);
+    case 96: return launch_chunk_one<96, CT, HALF>(p, st);
+    case 128: return launch_chunk_one<128, CT, HALF>(p, st);
+    case 192: return launch_chunk_one<192, CT, HALF>(p, st);
+    default: return launch_chunk_one<256, CT, HALF>(p, st);
+    }
+}
+
+}   // namespace attn
+
+int launch_attn_chunk_f16(const attn::ChunkParams &p, int head_dim, int half, cudaStream_t st);
+int launch_attn_chunk_f16_half(const attn::ChunkParams &p, int head_dim, cudaStream_t st);
+int launch_attn_chunk_q8(const attn::ChunkParams &p, int head_dim, cudaStream_t st);   // f16 out
+int launch_attn_chunk_q4(const attn::ChunkParams &p, int head_dim, cudaStream_t st);
+
+}   // namespace krk_cuda

@@ -233,7 +233,7 @@ attn_kernel(const __grid_constant__ Params p) {
 
         // ---- pages of this warp's chunks: lane l holds that of the l-th from the last refill on, as a row of the pool
         const int chunk0 = tile0 * kWarps + warp, n_chunks = tile1 - tile0;
-        const int32_t *table = p.table + (size_t)s * p.table_width;
+        const int32_t *table = p.table + (size_t)(s / p.pieces) * p.table_width;
         auto find_row = [&](int i) -> int64_t {   // -1: behind the last position, or not a page
             const int pos = (chunk0 + i * kWarps) * kChunk;
             if (i >= n_chunks || pos >= sq.len) return -1;
@@ -305,7 +305,8 @@ attn_kernel(const __grid_constant__ Params p) {
         if (lane < kPer) {
             const int r = warp + kWarps * lane, rr = block * R + r, i = rr / p.group;
             const bool ok = r < n_rows;
-            const uint64_t mask = !ok ? 0 : p.tree ? p.tree[sq.q0 + i] : (2ull << i) - 1ull;
+            uint64_t mask = !ok ? 0 : p.tree ? p.tree[sq.q0 + i] : (2ull << i) - 1ull;
+            if (p.window > 0 && i >= p.window) mask &= ~0ull << (i + 1 - p.window);   // (trees: the window begins before them)
             Rows row;
             row.scale = ldexpf(p.scale * (p.softcap > 0.0f ? 1.0f : 1.44269504f), -exponent);
             row.first = !ok ? INT32_MAX : p.window > 0 ? sq.before + __popcll(mask) - p.window : 0;

@@ -104,7 +104,7 @@ size_t attention_tree_workspace_bytes(const krk_cuda_kv_cache &cache, const krk_
     return f.whole ? 0 : attn::shared_bytes(f.grid) + (size_t)f.grid * 2 * f.block * (cache.head_dim + 2) * sizeof(float);
 }
 
-int launch_attention_tree(float *out, const float *q, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, void *workspace, cudaStream_t st) {
+int launch_attention_pieces(float *out, const float *q, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, int pieces, int piece_q, void *workspace, cudaStream_t st) {
     const attn::Form f = attn::form_of(cache, a);
     attn::Params p;
     p.q = q;
@@ -132,6 +132,8 @@ int launch_attention_tree(float *out, const float *q, const krk_cuda_kv_cache &c
     p.group = a.n_heads / cache.n_kv_heads;
     p.max_q = a.max_q;
     p.window = a.window;
+    p.pieces = pieces;
+    p.piece_q = piece_q;
     p.whole = f.whole;
     p.grid = f.grid;
     p.scale = a.scale;
@@ -142,6 +144,10 @@ int launch_attention_tree(float *out, const float *q, const krk_cuda_kv_cache &c
              : cache.type == KRK_CUDA_KV_Q8 ? launch_attn_q8(p, cache.head_dim, f.block, st) : launch_attn_q4(p, cache.head_dim, f.block, st);
     if (rc == KRK_CUDA_OK && !f.whole && f.grid > 1) rc = attn::launch_merge(p, cache.head_dim, f.block, f.rows, st);
     return rc;
+}
+
+int launch_attention_tree(float *out, const float *q, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, void *workspace, cudaStream_t st) {
+    return launch_attention_pieces(out, q, cache, a, 1, a.max_q, workspace, st);
 }
 
 } // namespace krk_cuda

@@ -48,6 +48,7 @@ struct Params {
     float *part;                          // [grid][2][R][D + 2]: see part_row
     int64_t n_pages;
     int table_width, page_size, max_len, n_seq, n_heads, n_kv, group, max_q, window, whole, grid;
+    int pieces, piece_q;                  // a chunk of up to piece_q tokens is so many sequences of max_q; trees: 1
     float scale, softcap;
     int *status;                          // raised where a bounded wait gives up
 };
@@ -64,9 +65,18 @@ struct Seq {
 template <int R>
 __device__ __forceinline__ Seq sequence(const Params &p, int s) {
     Seq q;
-    q.q0 = p.q_start[s];
-    q.n_q = min(max(p.q_start[s + 1] - q.q0, 0), p.max_q);
-    const int len = min(max(p.kv_len[s], 0), 1 << 30);
+    int len;
+    if (p.pieces == 1) {
+        q.q0 = p.q_start[s];
+        q.n_q = min(max(p.q_start[s + 1] - q.q0, 0), p.max_q);
+        len = min(max(p.kv_len[s], 0), 1 << 30);
+    } else {
+        // sequence s is piece s % pieces of a chunk: what is behind it in the chunk is not there for it
+        const int of = s / p.pieces, first = (s - of * p.pieces) * p.max_q, q0 = p.q_start[of], n_q = min(max(p.q_start[of + 1] - q0, 0), p.piece_q);
+        q.q0 = q0 + first;
+        q.n_q = min(max(n_q - first, 0), p.max_q);
+        len = min(max(p.kv_len[of], 0), 1 << 30) - max(n_q - first - q.n_q, 0);
+    }
     q.len = min(len, p.max_len);
     q.before = len - q.n_q;
     q.blocks = (q.n_q * p.group + R - 1) / R;
