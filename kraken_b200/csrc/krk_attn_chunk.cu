@@ -117,6 +117,7 @@ int launch_attention_chunk(void *out, int out_dtype, const void *q, int q_dtype,
     p.n_pages = cache.n_pages, p.table_width = a.table_width, p.page_size = cache.page_size, p.max_len = (int)a.max_kv_len, p.n_seq = a.n_seq, p.n_heads = a.n_heads;
     p.n_kv = cache.n_kv_heads, p.group = a.n_heads / cache.n_kv_heads, p.max_q = a.max_q, p.window = a.window, p.whole = f.whole, p.grid = f.grid;
     p.q_half = q_dtype == KRK_CUDA_X_F16, p.out_half = out_dtype == KRK_CUDA_X_F16, p.scale = a.scale, p.softcap = a.softcap;
+    attn::divide_by(p.group, p.group_mul, p.group_shift);
     p.status = device_status_word();
     if (!p.status) return KRK_CUDA_EDEVICE;
     // units of work are counted in 64 bits

@@ -26,9 +26,18 @@ struct ChunkParams {
     float *part;                          // [grid][2][R][D + 2]
     int64_t n_pages;
     int table_width, page_size, max_len, n_seq, n_heads, n_kv, group, max_q, window, whole, grid, q_half, out_half;
+    uint32_t group_mul, group_shift;      // row / group = row * group_mul >> group_shift, rows below 2^30
     float scale, softcap;
     int *status;
 };
+// n / d for n below 2^31: with 2^(s - 1) < d <= 2^s the factor ceil(2^(31 + s) / d) is less than one above the quotient, which n times it is at most 2^31 off.
+inline void divide_by(int d, uint32_t &mul, uint32_t &shift) {
+    int s = 0;
+    while ((1ll << s) < d) s++;
+    mul = (uint32_t)(((1ull << (31 + s)) + d - 1) / d);
+    shift = 31 + s;
+}
+__host__ __device__ __forceinline__ int token_of(const ChunkParams &p, int row) { return (int)(((uint64_t)(uint32_t)row * p.group_mul) >> p.group_shift); }
 
 constexpr int kChunkCopyWarps = 4;
 __host__ __device__ constexpr int chunk_tiles_of(int d) { return d <= 128 ? 2 : 1; }           // of rows, 128 each
@@ -62,7 +71,7 @@ __host__ __device__ __forceinline__ ChunkSeq chunk_sequence(const ChunkParams &p
     const int len = min(max(p.kv_len[s], 0), 1 << 30);
     q.len = min(len, p.max_len);
     q.before = len - q.n_q;
-    q.blocks = (int)(((int64_t)q.n_q * p.group + R - 1) / R);
+    q.blocks = (q.n_q * p.group + R - 1) / R;   // (fewer than 2^30 rows)
     return q;
 }
 template <int R, int TP>
@@ -86,8 +95,7 @@ __host__ __device__ __forceinline__ ChunkCost<R, TP> chunk_cost(const ChunkParam
 // The tiles of positions that some row of block b sees (one at least).
 template <int R, int TP>
 __host__ __device__ __forceinline__ void chunk_tiles(const ChunkParams &p, const ChunkSeq &q, int b, int &tile0, int &tiles) {
-    const int64_t rows = (int64_t)q.n_q * p.group;
-    const int t0 = (int)((int64_t)b * R / p.group), t1 = (int)((min(rows, (int64_t)(b + 1) * R) - 1) / p.group);
+    const int rows = q.n_q * p.group, t0 = token_of(p, b * R), t1 = token_of(p, min(rows, (b + 1) * R) - 1);
     const int end = max(min(q.len, q.before + t1 + 1), 0), start = p.window > 0 ? max(0, q.before + t0 - p.window + 1) : 0;
     tile0 = min(start, max(end - 1, 0)) / TP;
     tiles = max(1, (end + TP - 1) / TP - tile0);
@@ -136,7 +144,7 @@ struct ChunkWalk {
         r.tile = tile_at(in_head - from, (lo == q.blocks - 1 ? c.last : c.prefix(lo + 1) - from), tiles, p.whole);
         return r;
     }
-    // By the whole CTA, of 128 threads or more.
+    // By the whole CTA, of 128 threads or more; warp 0 has the result.
     __device__ __forceinline__ void start(const ChunkParams &p) {
         __shared__ int64_t s_sum[4], s_before[2];
         __shared__ int s_found[2];
@@ -177,7 +185,7 @@ struct ChunkWalk {
                 if (u[i] >= lo && u[i] < lo + mine) s_found[i] = s0 + tid, s_before[i] = lo;
         }
         __syncthreads();
-        begin(p, s_found[0], s_before[0], s_found[1], s_before[1]);
+        if (warp == 0) begin(p, s_found[0], s_before[0], s_found[1], s_before[1]);   // (of all warps it took 5 us: quotients of 64 bits)
     }
     // Of CTA b, with the total of units: how many share them, and its own.
     __host__ __device__ __forceinline__ void share(const ChunkParams &p, int b) {
@@ -216,6 +224,7 @@ struct ChunkWalk {
         while (e > me && (unit_of(total, grid, e) - from >= cost || tile_at(unit_of(total, grid, e) - from, cost, all, p.whole) >= all)) e--;
         return e - me + 2;
     }
+    template <bool PARTS = false>
     __host__ __device__ __forceinline__ bool next(const ChunkParams &p) {
         while (!over) {
             int t0, all;
@@ -225,10 +234,10 @@ struct ChunkWalk {
             const bool some = upto > from;
             if (some) {
                 kvh = at.kvh, block = at.b, s = at.s;
-                n_rows = (int)min((int64_t)R, (int64_t)sq.n_q * p.group - (int64_t)at.b * R);
+                n_rows = min(R, sq.n_q * p.group - at.b * R);
                 tile0 = t0 + from, tiles = upto - from;
                 begins = from == 0, ends = upto == all;
-                parts = first && from > 0 ? count_parts(p, all) : 0;
+                if constexpr (PARTS) parts = first && from > 0 ? count_parts(p, all) : 0;
             }
             const ChunkSeq was = sq;
             first = false;
@@ -388,15 +397,19 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     Walk walk;
     walk.start(p);   // (its barriers publish those above)
-    if (!p.whole && tid == 0) p.shared[blockIdx.x].parts = 0;
-    if (warp < C::kSoft && (tid & 127) == 0) meta.walk[warp >> 2] = walk;
+    if (tid == 0) {
+        if (!p.whole) p.shared[blockIdx.x].parts = 0;
+        meta.walk[0] = meta.walk[1] = walk;
+    }
     __syncthreads();
+    walk = meta.walk[0];
+    __syncthreads();   // (the softmax goes on with it)
     tc_after();
     const uint32_t tmem = meta.tmem;
     // tiles of an item that rows of tile q see; those of the first tile of rows end earlier
     auto tiles_of = [&](const Walk &w, int q) {
         if (q * 128 >= w.n_rows) return 0;
-        const int t1 = (int)(((int64_t)w.block * R + min(w.n_rows, (q + 1) * 128) - 1) / p.group), end = min(w.now.len, w.now.before + t1 + 1);
+        const int t1 = token_of(p, w.block * R + min(w.n_rows, (q + 1) * 128) - 1), end = min(w.now.len, w.now.before + t1 + 1);
         return min(w.tiles, max((end + TP - 1) / TP - w.tile0, 1));
     };
 
@@ -409,7 +422,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
         for (;;) {
             if ((tid & 127) == 0) {
                 Walk w = meta.walk[tq];
-                meta.goes_on[tq] = w.next(p);
+                meta.goes_on[tq] = tq == 0 ? w.template next<true>(p) : w.next(p);
                 if (tq == 0 && meta.goes_on[tq] && w.parts > 0) w.note(p);
                 meta.walk[tq] = w;
             }
@@ -417,7 +430,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             if (!meta.goes_on[tq]) break;
             const Walk &walk = meta.walk[tq];
             const int n_rows = walk.n_rows, tiles = tiles_of(walk, tq), tile0 = walk.tile0, before = walk.now.before, len = walk.now.len, kvh = walk.kvh, q0 = walk.now.q0;
-            const int64_t row0 = (int64_t)walk.block * R + 128 * tq;   // among the key head's
+            const int row0 = walk.block * R + 128 * tq;   // among the key head's
             const bool whole = walk.begins && walk.ends;
             const int place_of_part = walk.begins ? 1 : 0;
             const int mine_rows = min(128, n_rows - 128 * tq);
@@ -437,8 +450,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int r = 32 * quarter + j0 + j;
-                    const int64_t rr = row0 + r;
-                    const int i = (int)(rr / p.group), h = kvh * p.group + (int)(rr - (int64_t)i * p.group);
+                    const int i = token_of(p, row0 + r), h = kvh * p.group + row0 + r - i * p.group;
                     const int64_t from = (int64_t)(q0 + i) * p.q_stride + (int64_t)h * D;
 #pragma unroll
                     for (int c = 0; c < NL; c++) {
@@ -493,11 +505,10 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             if (lane == 0) bar_arrive(bar(meta.q_full[tq]));
 
             const float sc = meta.scale[128 * tq + r_in];
-            const int64_t rr = row0 + min(r_in, mine_rows - 1);
-            const int token = (int)(rr / p.group), head = kvh * p.group + (int)(rr - (int64_t)token * p.group);
+            const int rr = row0 + min(r_in, mine_rows - 1), token = token_of(p, rr), head = kvh * p.group + rr - token * p.group;
             const int behind = min(len, before + token + 1), from = p.window > 0 ? max(0, before + token - p.window + 1) : 0;   // what the row sees: [from, behind)
             // every row of this tile of rows sees [all_from, all_to)
-            const int all_to = min(len, before + (int)(row0 / p.group) + 1), all_from = p.window > 0 ? before + (int)((row0 + mine_rows - 1) / p.group) - p.window + 1 : 0;
+            const int all_to = min(len, before + token_of(p, row0) + 1), all_from = p.window > 0 ? before + token_of(p, row0 + mine_rows - 1) - p.window + 1 : 0;
             float m = -INFINITY, l = 0.0f;
             for (int i = 0; i < tiles; i++, n_tile++) {
                 const int pos0 = (tile0 + i) * TP;
@@ -590,6 +601,8 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 }
                 tmem_stored();
                 tc_before();
+                // (one tile of rows: the products of two tiles may be in flight, which a parity does not tell apart behind the last one)
+                if (NQ == 1 && i > 0 && i == tiles - 1) bar_wait(bar(meta.pv_done[tq]), (n_tile - 1) & 1, gave_up, p.status);
                 __syncwarp();
                 if (lane == 0) bar_arrive(bar(meta.p_full[sb]));
             }
@@ -610,7 +623,6 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 float *to = p.part + (((size_t)blockIdx.x * 2 + place_of_part) * R + 128 * tq + r_in) * (D + 2);
                 *reinterpret_cast<float2 *>(to + D) = make_float2(m, all);
             }
-            if (NQ == 1 && tiles > 1) bar_wait(bar(meta.pv_done[tq]), (n_tile - 2) & 1, gave_up, p.status);   // (the products of two tiles may be in flight: a parity tells one from the next)
             bar_wait(bar(meta.pv_done[tq]), (n_tile - 1) & 1, gave_up, p.status);
             tc_after();
             const bool any_odd = *reinterpret_cast<volatile uint32_t *>(&meta.odd[tq][n_item & 7]) != 0;
@@ -622,7 +634,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 tmem_loaded();
                 if (any_odd) {
                     // values that are no numbers, in tiles that not all rows see, were taken out of the products: here are they for the rows that see them
-                    const int first_token = (int)((int64_t)walk.block * R / p.group), last_token = (int)(((int64_t)walk.block * R + n_rows - 1) / p.group);
+                    const int first_token = token_of(p, walk.block * R), last_token = token_of(p, walk.block * R + n_rows - 1);
                     const int end = min(behind, (tile0 + tiles) * TP);
                     for (int pos = max(from, tile0 * TP); pos < end; pos++) {
                         const int t0 = pos / TP * TP;
@@ -654,8 +666,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     if (rw >= mine_rows) continue;
                     const float4 x = *reinterpret_cast<const float4 *>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
                     if (whole) {
-                        const int64_t g = row0 + rw;
-                        const int t = (int)(g / p.group), h = kvh * p.group + (int)(g - (int64_t)t * p.group);
+                        const int t = token_of(p, row0 + rw), h = kvh * p.group + row0 + rw - t * p.group;
                         const int64_t to = (int64_t)(q0 + t) * p.out_stride + (int64_t)h * D + at;
                         if constexpr (HALF) {
                             *reinterpret_cast<uint2 *>(static_cast<__half *>(p.out) + to) = make_uint2(bits(__floats2half2_rn(x.x, x.y)), bits(__floats2half2_rn(x.z, x.w)));
@@ -728,7 +739,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
         while (walk.next(p)) {
             const ChunkSeq &sq = walk.now;
             const int32_t *table = p.table + (size_t)walk.s * p.table_width;
-            const int first_token = (int)((int64_t)walk.block * R / p.group), last_token = (int)(((int64_t)walk.block * R + walk.n_rows - 1) / p.group);
+            const int first_token = token_of(p, walk.block * R), last_token = token_of(p, walk.block * R + walk.n_rows - 1);
             const int all_to = min(sq.len, sq.before + first_token + 1), all_from = p.window > 0 ? sq.before + last_token - p.window + 1 : 0;
             auto looked_at = [&](int i) { return (walk.tile0 + i) * TP + TP > all_to || (walk.tile0 + i) * TP < all_from; };
             auto find_rows = [&](int i) -> int64_t {

@@ -324,7 +324,7 @@ attn_kernel(const __grid_constant__ Params p) {
             __syncwarp();
         }
         // every row sees [all_from, before), none what is before any_from
-        const int all_from = p.window > 0 ? sq.before + KRK_CUDA_MAX_DRAFT - p.window : 0, any_from = p.window > 0 ? sq.before - p.window : 0;
+        const int all_from = p.window > 0 ? sq.before + KRK_CUDA_MAX_DRAFT - p.window : 0, any_from = p.window > 0 ? sq.before - p.window + (p.piece_q > 0) : 0;   // (chunks have no empty masks)
 
         // Sums of a lane: tile of 16 values m, tile of columns n, [2 h + c]: value value_of(m, g, h) of row 8 n + 2 t + c; with kPair row t, c the
         // term of the weight. Scores and maxima: rows 8 n + 2 t + c (row t), positions g and g + 8.

@@ -147,7 +147,7 @@ int launch_attention_pieces(float *out, const float *q, const krk_cuda_kv_cache 
 }
 
 int launch_attention_tree(float *out, const float *q, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, void *workspace, cudaStream_t st) {
-    return launch_attention_pieces(out, q, cache, a, 1, a.max_q, workspace, st);
+    return launch_attention_pieces(out, q, cache, a, 1, 0, workspace, st);
 }
 
 } // namespace krk_cuda

@@ -48,7 +48,7 @@ struct Params {
     float *part;                          // [grid][2][R][D + 2]: see part_row
     int64_t n_pages;
     int table_width, page_size, max_len, n_seq, n_heads, n_kv, group, max_q, window, whole, grid;
-    int pieces, piece_q;                  // a chunk of up to piece_q tokens is so many sequences of max_q; trees: 1
+    int pieces, piece_q;                  // a chunk of up to piece_q tokens is so many sequences of max_q; trees: 1 and 0
     float scale, softcap;
     int *status;                          // raised where a bounded wait gives up
 };

@@ -28,6 +28,9 @@ static void check_plan(const std::vector<int> &count, const std::vector<int> &le
     ChunkParams p = {};
     p.q_start = start.data(), p.kv_len = len.data(), p.n_seq = (int)count.size(), p.group = group, p.n_kv = n_kv, p.window = window, p.max_len = max_len, p.max_q = max_q, p.grid = grid;
     p.whole = whole;
+    divide_by(group, p.group_mul, p.group_shift);
+    for (int64_t n : {0ll, 1ll, (long long)group - 1, (long long)group, 5ll * group - 1, 5ll * group, (1ll << 30), (1ll << 30) / group * group, (1ll << 30) / group * group - 1})
+        check(token_of(p, (int)n) == n / group, "quotient", group, (int)n);
     std::vector<int64_t> before(1, 0);
     std::map<std::tuple<int, int, int>, std::vector<int>> owner;   // of an item's tiles
     for (int s = 0; s < p.n_seq; s++) {
@@ -51,7 +54,6 @@ static void check_plan(const std::vector<int> &count, const std::vector<int> &le
                 owner[{s, h, b}] = std::vector<int>(tiles, -1);
             }
     }
-    std::vector<ChunkWalk<R, TP>> noted(grid);
     std::map<std::tuple<int, int, int>, int> notes;
     for (int cta = 0; cta < grid; cta++) {
         ChunkWalk<R, TP> w;
@@ -66,7 +68,7 @@ static void check_plan(const std::vector<int> &count, const std::vector<int> &le
         w.begin(p, s0, before[s0], s1, before[s1]);
         int items = 0;
         bool went_on = false;
-        while (w.next(p)) {
+        while (w.template next<true>(p)) {
             auto &o = owner[{w.s, w.kvh, w.block}];
             int t0, tiles;
             chunk_tiles<R, TP>(p, w.now, w.block, t0, tiles);
