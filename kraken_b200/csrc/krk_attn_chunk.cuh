@@ -46,7 +46,7 @@ __host__ __device__ constexpr int chunk_rows(int d) { return 128 * chunk_tiles_o
 constexpr int kChunkSetup = 3;        // an item beside its tiles, in tiles
 constexpr int kChunkWholeTiles = 8;   // contexts of up to so many tiles of positions are not divided
 constexpr float kLetBe = 8.0f;        // log2: a reference stands until a score is more than this above it
-constexpr float kUp = 128.0f;         // of weights: times 2^8 they stay below the f16 range
+constexpr float kUp = 128.0f, kUpLog2 = 7.0f;   // of weights: times 2^8 they stay below the f16 range
 
 struct ChunkSeq {
     int q0, n_q, len, before, blocks;
@@ -111,13 +111,15 @@ struct ChunkWalk {
     ChunkSeq sq;
     int64_t total, base;   // units in all, and before the first item's sequence
     int64_t first_unit, behind_unit;
+    double per_cta;
     int grid, cta;
     bool first, over;
     // of the current item; parts: see Shared
     int kvh, block, s, n_rows, tile0, tiles, parts;
     bool begins, ends;
 
-    __host__ __device__ __forceinline__ static int64_t unit_of(int64_t total, int grid, int b) { return total / grid * b + total % grid * b / grid; }
+    // (in f64, the same in every CTA and rising with b; quotients of 64 bits take a thread some 400 clocks)
+    __host__ __device__ __forceinline__ int64_t unit_of(int b) const { return b >= grid ? total : (int64_t)(per_cta * (double)b); }
     // The tile that a border lies at, `off` units into an item of `cost`: borders near an item's ends are at them.
     __host__ __device__ __forceinline__ static int tile_at(int64_t off, int64_t cost, int tiles, int whole) {
         if (whole) return 2 * off < cost ? 0 : tiles;
@@ -129,14 +131,25 @@ struct ChunkWalk {
         const ChunkSeq q = chunk_sequence<R>(p, s);
         const ChunkCost<R, TP> c = chunk_cost<R, TP>(p, q);
         r.s = s;
-        r.kvh = (int)min(in_seq / c.head, (int64_t)p.n_kv - 1);
+        r.kvh = min((int)((double)in_seq / (double)c.head), p.n_kv - 1);
+        if (r.kvh * c.head > in_seq) r.kvh--;
+        else if (r.kvh + 1 < p.n_kv && (r.kvh + 1) * c.head <= in_seq) r.kvh++;
         const int64_t in_head = in_seq - r.kvh * c.head;
-        int lo = 0, hi = q.blocks - 1;   // the last block that begins at or before it
-        while (lo < hi) {
+        int lo = 0;   // the last block that begins at or before it
+#ifdef __CUDA_ARCH__
+        for (int n = q.blocks; n > 1;) {   // by a warp
+            const int step = (n + 31) / 32, lane = threadIdx.x & 31, i = lane * step;
+            const int ahead = __popc(__ballot_sync(0xFFFFFFFFu, i < n && c.prefix(lo + i) <= in_head)) - 1;
+            lo += ahead * step;
+            n = min(step, n - ahead * step);
+        }
+#else
+        for (int hi = q.blocks - 1; lo < hi;) {
             const int mid = (lo + hi + 1) / 2;
             if (c.prefix(mid) <= in_head) lo = mid;
             else hi = mid - 1;
         }
+#endif
         r.b = lo;
         int t0, tiles;
         chunk_tiles<R, TP>(p, q, lo, t0, tiles);
@@ -185,7 +198,15 @@ struct ChunkWalk {
                 if (u[i] >= lo && u[i] < lo + mine) s_found[i] = s0 + tid, s_before[i] = lo;
         }
         __syncthreads();
-        if (warp == 0) begin(p, s_found[0], s_before[0], s_found[1], s_before[1]);   // (of all warps it took 5 us: quotients of 64 bits)
+        // warps 0 and 1 find the two ends (of all warps it took 5 us)
+        __shared__ ChunkPlace s_end;
+        if (warp == 1 && s_found[1] < p.n_seq) {
+            const ChunkPlace e = place(p, s_found[1], u[1] - s_before[1]);
+            if (lane == 0) s_end = e;
+        }
+        if (warp == 0) begin(p, s_found[0], s_before[0]);
+        __syncthreads();
+        if (s_found[1] < p.n_seq) end = s_end;
     }
     // Of CTA b, with the total of units: how many share them, and its own.
     __host__ __device__ __forceinline__ void share(const ChunkParams &p, int b) {
@@ -193,18 +214,18 @@ struct ChunkWalk {
         // 4 group (TP kChunkSetup / tiles + TP + 2).
         const int64_t least = (int64_t)4 * p.group * TP * (kChunkSetup + 3);
         cta = b;
-        grid = (int)max(min((int64_t)p.grid, total / least), (int64_t)1);
-        first_unit = unit_of(total, grid, min(b, grid));
-        behind_unit = unit_of(total, grid, min(b + 1, grid));
+        grid = (int)fmax(fmin((double)p.grid, floor((double)total / (double)least)), 1.0);
+        per_cta = (double)total / (double)grid;
+        first_unit = unit_of(b);
+        behind_unit = unit_of(b + 1);
     }
-    // The sequences in which its first unit and the one behind its last lie (n_seq: none), and the units before each.
-    __host__ __device__ __forceinline__ void begin(const ChunkParams &p, int s0, int64_t before0, int s1, int64_t before1) {
+    // The sequence in which its first unit lies (n_seq: none), and the units before it. `end` is the place of the one behind its last.
+    __host__ __device__ __forceinline__ void begin(const ChunkParams &p, int s0, int64_t before0) {
         over = first_unit >= behind_unit || s0 >= p.n_seq;
         base = before0;
         at = end = {p.n_seq, 0, 0, 0};
         if (!over) {
             at = place(p, s0, first_unit - before0);
-            if (s1 < p.n_seq) end = place(p, s1, behind_unit - before1);
             sq = chunk_sequence<R>(p, at.s);
         }
         first = true;
@@ -217,11 +238,11 @@ struct ChunkWalk {
         const int64_t from = base + at.kvh * c.head + c.prefix(at.b), cost = at.b == sq.blocks - 1 ? c.last : c.prefix(at.b + 1) - c.prefix(at.b);
         const int me = cta;
         if (me == 0) return 0;
-        const int64_t before = unit_of(total, grid, me - 1) - from;
+        const int64_t before = unit_of(me - 1) - from;
         if (before >= 0 && tile_at(before, cost, all, p.whole) > 0) return 0;
         // the last border that lies in the item
         int e = (int)min((int64_t)grid - 1, (int64_t)((double)(from + cost) / (double)total * grid) + 1);
-        while (e > me && (unit_of(total, grid, e) - from >= cost || tile_at(unit_of(total, grid, e) - from, cost, all, p.whole) >= all)) e--;
+        while (e > me && (unit_of(e) - from >= cost || tile_at(unit_of(e) - from, cost, all, p.whole) >= all)) e--;
         return e - me + 2;
     }
     template <bool PARTS = false>
@@ -277,7 +298,7 @@ struct ChunkWalk {
     }
 };
 
-template <int D, int NT>
+template <int D, int NT, bool QUANT>
 struct Chunk {
     static constexpr int NQ = chunk_tiles_of(D), TP = chunk_positions(D), R = chunk_rows(D);
     static constexpr int kMetaBytes = 1920;
@@ -287,7 +308,10 @@ struct Chunk {
     static constexpr int kRoom = 227 * 1024 - 1024 - kMetaBytes - 64 - NQ * kQTile;   // (64: ChunkWalk::start)
     static constexpr int kSlots = kRoom / kSlot > 6 ? 6 : kRoom / kSlot;
     static constexpr int kQ = kSlots * kSlot, kMeta = kQ + NQ * kQTile, kBytes = kMeta + kMetaBytes + 1024;   // (begins on a 1024-byte boundary)
-    static constexpr int kSoft = 4 * NQ, kWarps = kSoft + kChunkCopyWarps + 1, kThreads = 32 * kWarps;
+    static constexpr int kSoft = 4 * NQ, kProduct = kSoft + kChunkCopyWarps, kWarps = kProduct + 4, kThreads = 32 * kWarps;   // (of the last four one works)
+    // registers of a thread: 512 threads are launched with 128 each; the copies unpack 8 and 4 bits in theirs
+    static constexpr int kSoftRegs = QUANT ? 168 : 184, kOtherRegs = QUANT ? 88 : 72;
+    static_assert(256 * kSoftRegs + 256 * kOtherRegs <= 65536, "registers of a launch");
     static constexpr uint32_t kO = 256;                              // column of the sums; of the second tile's: 128 more
     static constexpr uint32_t kS = NQ == 2 ? 128 : 64;               // from a place of scores to the next
     static_assert(kSlots >= 3, "a half tile of values and one of keys at work, one on its way");
@@ -295,15 +319,19 @@ struct Chunk {
     using Walk = ChunkWalk<R, TP>;
 };
 
+struct ChunkItem {
+    int goes_on, q0, len, before, s, kvh, block, n_rows, tile0, all, tiles;   // all: tiles of the item, tiles: that the rows of this tile see
+    bool whole, begins;
+};
 template <int R, int TP>
 struct ChunkMeta {
-    unsigned long long kv_full[6], kv_empty[6], s_full[2], p_full[2], pv_done[2], q_full[2], drained;
+    unsigned long long kv_full[6], kv_empty[6], s_full[2], p_half[2], p_full[2], pv_done[2], q_full[2], drained;
     float scale[R];
     uint32_t odd[2][8];       // of a tile of rows, an item in turn: values of a tile that not all rows see are no numbers
     uint8_t there[8];         // of a tile of positions, in turn: bit c: chunk c is a page's
-    int goes_on[2];
     uint32_t tmem;
     int gave_up;
+    ChunkItem item[2][2];     // of a tile of rows: this item and the next
     ChunkWalk<R, TP> walk[2];
 };
 
@@ -322,7 +350,18 @@ __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t *v) {
                    "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]),
                    "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
 }
-// The same with A in tensor memory (lane = row, a column two f16).
+// As bar_wait, without a call: a kernel whose warps trade registers has none.
+__device__ __forceinline__ void bar_wait_here(uint32_t bar, uint32_t parity, volatile int *gave_up, int *status) {
+    if (bar_try(bar, parity)) return;
+    const long long t0 = clock64();
+#pragma unroll 1
+    while (!*gave_up && !bar_try(bar, parity))
+        if (clock64() - t0 > kWaitLimit) {
+            *gave_up = 1;
+            atomicExch(status, KRK_CUDA_ETIMEOUT);
+        }
+}
+// A product as above with A in tensor memory (lane = row, a column two f16).
 __device__ __forceinline__ void product_from(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t onto, uint32_t elected) {
     asm volatile("{\n .reg .pred p, q;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %7, 0;\n mov.b64 b, {%2, %3};\n"
                  " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, {%6, %6, %6, %6}, p;\n}\n"
@@ -331,9 +370,16 @@ __device__ __forceinline__ void product_from(uint32_t d, uint32_t a, uint32_t b_
 // Bytes I and J of w, as `halves` in krk_attn_kernel.cuh.
 template <int I, int J>
 __device__ __forceinline__ uint32_t halves_of(uint32_t w, uint32_t off) { return halves<I, J>(w, off); }
-__device__ __forceinline__ float capped_half(float x, float cap) {   // as capped, through one exponential: 2^-22 of the cap off, f16 weights take no more
-    const float e = ex2(x * (2.0f * 1.44269504f) / cap);
-    return cap * (1.44269504f - 2.0f * 1.44269504f * __frcp_rn(1.0f + e));
+// As capped, without a call: the hyperbolic tangent from one exponential (2^-22 off), f32: near zero from its series, whose next term is 2^-26 of it there.
+template <bool HALF>
+__device__ __forceinline__ float capped_here(float x, float cap) {
+    const float y = x / cap, e = ex2(y * (2.0f * 1.44269504f));
+    float t = 1.0f - 2.0f * __frcp_rn(1.0f + e);
+    if constexpr (!HALF) {
+        const float z = y * y;
+        if (z < 0.0625f) t = fmaf(y * z, fmaf(z, fmaf(z, fmaf(z, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), y);
+    }
+    return cap * (1.44269504f * t);
 }
 // A value of a cache as f16 products see it, by a slow path.
 template <int CT, int D>
@@ -349,12 +395,58 @@ __device__ __forceinline__ float value_at(const uint8_t *pool, const __half *sca
     return __half2float(__hmul(d, __int2half_rn(q)));
 }
 
+// Log2 scores under a soft limit in place of products.
+template <bool HALF, int TP>
+__device__ __forceinline__ void soft_limit(uint32_t t_s, float sc, float cap) {
+#pragma unroll 1
+    for (int c = 0; c < TP; c += 16) {
+        uint32_t v[16];
+        tmem_load16(t_s + c, v);
+        tmem_loaded();
+#pragma unroll
+        for (int j = 0; j < 16; j++) v[j] = __float_as_uint(capped_here<HALF>(__uint_as_float(v[j]) * sc, cap));
+        tmem_store16(t_s + c, v);
+    }
+    tmem_stored();
+}
+// Values that are no numbers, in tiles that not all rows of an item see, were taken out of the products: here they are, for the rows that see them. A thread's
+// row sees [pos, end); tiles inside [all_from, all_to) were left as they are.
+template <int CT, int D, int TP>
+__device__ __forceinline__ void add_odd(const ChunkParams &p, const ChunkItem &it, uint32_t t_o, int pos0, int end, int all_to, int all_from) {
+#pragma unroll 1
+    for (int c = 0; c < D; c += 16) {
+        uint32_t o[16];
+        tmem_load16(t_o + c, o);
+        tmem_loaded();
+        for (int pos = pos0; pos < end; pos++) {
+            const int t0 = pos / TP * TP;
+            if (t0 + TP <= all_to && t0 >= all_from) {
+                pos = t0 + TP - 1;
+                continue;
+            }
+            const int page = p.table[(size_t)it.s * p.table_width + pos / p.page_size];
+            if (page < 0 || page >= p.n_pages) continue;
+            const int64_t row = ((int64_t)page * p.n_kv + it.kvh) * p.page_size + pos % p.page_size;
+            for (int j = 0; j < 16; j++) {
+                const float y = value_at<CT, D>(p.v, p.v_scale, row, c + j);
+                if (fabsf(y) <= 65504.0f) continue;
+#pragma unroll
+                for (int k = 0; k < 16; k++)
+                    if (k == j) o[k] = __float_as_uint(__uint_as_float(o[k]) + y);
+            }
+        }
+        __syncwarp();
+        tmem_store16(t_o + c, o);
+    }
+    tmem_stored();
+}
+
 // HALF: f16 out, one term of each query and weight (NT), else f32 and two.
 template <int D, int CT, bool HALF>
-__global__ void __launch_bounds__((Chunk<D, HALF ? 1 : 2>::kThreads), 1)
+__global__ void __launch_bounds__((Chunk<D, HALF ? 1 : 2, CT != KRK_CUDA_KV_F16>::kThreads), 1)
 attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
     constexpr int NT = HALF ? 1 : 2;
-    using C = Chunk<D, NT>;
+    using C = Chunk<D, NT, CT != KRK_CUDA_KV_F16>;
     using Walk = typename C::Walk;
     constexpr int NQ = C::NQ, TP = C::TP, R = C::R, RB = row_bytes_of(CT, D), kChunks = TP / kChunk;
     constexpr bool kQuant = CT != KRK_CUDA_KV_F16;
@@ -376,6 +468,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             }
             for (int i = 0; i < 2; i++) {
                 bar_init(bar(meta.s_full[i]), 1);
+                bar_init(bar(meta.p_half[i]), 4);
                 bar_init(bar(meta.p_full[i]), 4);
                 bar_init(bar(meta.pv_done[i]), 1);
                 bar_init(bar(meta.q_full[i]), 4);
@@ -388,7 +481,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         async_fence();
     }
-    if (warp == C::kWarps - 1) {
+    if (warp == C::kProduct) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&meta.tmem)), "r"(kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         tc_before();
@@ -415,94 +508,103 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
 
     if (warp < C::kSoft) {
         // ===== softmax: thread = row
+        if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
         const int tq = warp >> 2, r_in = tid & 127, quarter = warp & 3;
         const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16), t_o = t_lane + C::kO + 128 * tq;
         uint8_t *q_tile = smem + C::kQ + tq * C::kQTile;
+        auto find_item = [&](uint32_t n) {   // by one thread
+            Walk w = meta.walk[tq];
+            ChunkItem it;
+            it.goes_on = tq == 0 ? w.template next<true>(p) : w.next(p);
+            if (tq == 0 && it.goes_on && w.parts > 0) w.note(p);
+            it.q0 = w.now.q0, it.len = w.now.len, it.before = w.now.before, it.s = w.s, it.kvh = w.kvh, it.block = w.block, it.n_rows = w.n_rows;
+            it.tile0 = w.tile0, it.all = w.tiles, it.tiles = tiles_of(w, tq), it.whole = w.begins && w.ends, it.begins = w.begins;
+            meta.item[tq][n & 1] = it;
+            meta.walk[tq] = w;
+        };
         uint32_t n_tile = 0, n_item = 0, n_all = 0;   // tiles of this tile of rows, items, tiles of all items
-        for (;;) {
-            if ((tid & 127) == 0) {
-                Walk w = meta.walk[tq];
-                meta.goes_on[tq] = tq == 0 ? w.template next<true>(p) : w.next(p);
-                if (tq == 0 && meta.goes_on[tq] && w.parts > 0) w.note(p);
-                meta.walk[tq] = w;
-            }
+        if (r_in == 0) find_item(0);
+        for (;; n_item++) {
             group_sync(tq);
-            if (!meta.goes_on[tq]) break;
-            const Walk &walk = meta.walk[tq];
-            const int n_rows = walk.n_rows, tiles = tiles_of(walk, tq), tile0 = walk.tile0, before = walk.now.before, len = walk.now.len, kvh = walk.kvh, q0 = walk.now.q0;
-            const int row0 = walk.block * R + 128 * tq;   // among the key head's
-            const bool whole = walk.begins && walk.ends;
-            const int place_of_part = walk.begins ? 1 : 0;
+            const ChunkItem &it = meta.item[tq][n_item & 1];
+            if (!it.goes_on) break;
+            const int n_rows = it.n_rows, tiles = it.tiles, tile0 = it.tile0, before = it.before, len = it.len, kvh = it.kvh, q0 = it.q0;
+            const int row0 = it.block * R + 128 * tq;   // among the key head's
             const int mine_rows = min(128, n_rows - 128 * tq);
             const uint32_t n_before = n_all;
-            n_all += walk.tiles;
+            n_all += it.all;
             if (mine_rows <= 0) {
-                n_item++;
                 group_sync(tq);
+                if (r_in == 0) find_item(n_item + 1);
                 continue;
             }
-            // ---- queries, four values a lane, eight rows at a time, under a power of two of their own: the largest value in [2^10, 2^11)
-            constexpr int NL = (D + 127) / 128;
-            const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+            // ---- queries, four values a lane, some rows at a time, under a power of two of their own: the largest value in [2^10, 2^11)
+            const float sign = p.scale < 0.0f ? -1.0f : 1.0f, row_scale = fabsf(p.scale) * (p.softcap > 0.0f ? 1.0f : 1.44269504f);
+            auto queries = [&](auto half_q) {
+                constexpr bool kHalfQ = decltype(half_q)::value;
+                constexpr int NL = (D + 127) / 128, kRows = NL == 1 ? 16 : 8;
+                using Raw = std::conditional_t<kHalfQ, uint2, uint4>;
 #pragma unroll 1
-            for (int j0 = 0; j0 < 32; j0 += 8) {
-                float x[8][NL][4], most[8];
+                for (int j0 = 0; j0 < 32; j0 += kRows) {
+                    Raw x[kRows][NL];
+                    // (a row's place: its token and head, walked from the first one's)
+                    int r = 32 * quarter + j0, i = token_of(p, row0 + r), h = row0 + r - i * p.group;
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int r = 32 * quarter + j0 + j;
-                    const int i = token_of(p, row0 + r), h = kvh * p.group + row0 + r - i * p.group;
-                    const int64_t from = (int64_t)(q0 + i) * p.q_stride + (int64_t)h * D;
+                    for (int j = 0; j < kRows; j++) {
+                        const int64_t from = (int64_t)(q0 + i) * p.q_stride + (int64_t)(kvh * p.group + h) * D;
 #pragma unroll
-                    for (int c = 0; c < NL; c++) {
-                        const int d = 128 * c + 4 * lane;
+                        for (int c = 0; c < NL; c++) {
+                            const int d = 128 * c + 4 * lane;
+                            x[j][c] = Raw{};
+                            if (r + j < mine_rows && (D % 128 == 0 || d < D)) x[j][c] = *reinterpret_cast<const Raw *>(static_cast<const uint8_t *>(p.q) + (from + d) * (kHalfQ ? 2 : 4));
+                        }
+                        if (++h == p.group) h = 0, i++;
+                    }
+                    auto value = [&](int j, int c, int e) {
+                        if constexpr (kHalfQ) {
+                            const float2 two = __half22float2(half2_of(e < 2 ? x[j][c].x : x[j][c].y));
+                            return e & 1 ? two.y : two.x;
+                        } else {
+                            return __uint_as_float(e == 0 ? x[j][c].x : e == 1 ? x[j][c].y : e == 2 ? x[j][c].z : x[j][c].w);
+                        }
+                    };
+                    float most[kRows];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) x[j][c][e] = 0.0f;
-                        if (r < mine_rows && (D % 128 == 0 || d < D)) {
-                            if (p.q_half) {
-                                const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const __half *>(p.q) + from + d);
-                                const float2 a = __half22float2(half2_of(w.x)), b = __half22float2(half2_of(w.y));
-                                x[j][c][0] = a.x, x[j][c][1] = a.y, x[j][c][2] = b.x, x[j][c][3] = b.y;
-                            } else {
-                                *reinterpret_cast<float4 *>(x[j][c]) = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + from + d);
+                    for (int j = 0; j < kRows; j++) {
+                        most[j] = 0.0f;
+#pragma unroll
+                        for (int c = 0; c < NL; c++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) most[j] = fmaxf(most[j], fabsf(value(j, c, e)));
+                    }
+#pragma unroll
+                    for (int j = 0; j < kRows; j++) most[j] = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most[j])));   // (not negative: bits in order)
+#pragma unroll
+                    for (int j = 0; j < kRows; j++) {
+                        const int rr = r + j, e = most[j] > 0.0f && most[j] <= 3.4028234e38f ? 10 - max((int)(__float_as_uint(most[j]) >> 23) - 127, -110) : 0;
+                        const float up = sign * __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+                        for (int c = 0; c < NL; c++) {
+                            const int d = 128 * c + 4 * lane;
+                            if (D % 128 == 0 || d < D) {
+                                uint32_t hi[2], lo[2];
+                                split(value(j, c, 0) * up, value(j, c, 1) * up, hi[0], lo[0]);
+                                split(value(j, c, 2) * up, value(j, c, 3) * up, hi[1], lo[1]);
+                                uint8_t *to = q_tile + (d >> 6) * (128 * 128) + rr * 128 + ((((d & 63) >> 3) ^ (rr & 7)) << 4) + 2 * (d & 7);
+                                *reinterpret_cast<uint2 *>(to) = make_uint2(hi[0], hi[1]);
+                                if constexpr (NT == 2) *reinterpret_cast<uint2 *>(to + C::kTerm) = make_uint2(lo[0], lo[1]);
                             }
                         }
+                        if (lane == 0) meta.scale[128 * tq + rr] = row_scale * __uint_as_float((uint32_t)(127 - e) << 23);
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    most[j] = 0.0f;
-#pragma unroll
-                    for (int c = 0; c < NL; c++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) most[j] = fmaxf(most[j], fabsf(x[j][c][e]));
-                }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) most[j] = fmaxf(most[j], __shfl_xor_sync(0xFFFFFFFFu, most[j], o));
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int r = 32 * quarter + j0 + j;
-                    const int e = most[j] > 0.0f && most[j] <= 3.4028234e38f ? 10 - max((int)(__float_as_uint(most[j]) >> 23) - 127, -110) : 0;
-                    const float up = sign * __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll
-                    for (int c = 0; c < NL; c++) {
-                        const int d = 128 * c + 4 * lane;
-                        if (D % 128 == 0 || d < D) {
-                            uint32_t hi[2], lo[2];
-                            split(x[j][c][0] * up, x[j][c][1] * up, hi[0], lo[0]);
-                            split(x[j][c][2] * up, x[j][c][3] * up, hi[1], lo[1]);
-                            uint8_t *to = q_tile + (d >> 6) * (128 * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + 2 * (d & 7);
-                            *reinterpret_cast<uint2 *>(to) = make_uint2(hi[0], hi[1]);
-                            if constexpr (NT == 2) *reinterpret_cast<uint2 *>(to + C::kTerm) = make_uint2(lo[0], lo[1]);
-                        }
-                    }
-                    if (lane == 0) meta.scale[128 * tq + r] = fabsf(p.scale) * (p.softcap > 0.0f ? 1.0f : 1.44269504f) * __uint_as_float((uint32_t)(127 - e) << 23);
-                }
-            }
+            };
+            if (HALF && p.q_half) queries(std::true_type{});
+            else queries(std::false_type{});
             async_fence();
             __syncwarp();
             if (lane == 0) bar_arrive(bar(meta.q_full[tq]));
+            if (r_in == 0) find_item(n_item + 1);
 
             const float sc = meta.scale[128 * tq + r_in];
             const int rr = row0 + min(r_in, mine_rows - 1), token = token_of(p, rr), head = kvh * p.group + rr - token * p.group;
@@ -510,109 +612,105 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             // every row of this tile of rows sees [all_from, all_to)
             const int all_to = min(len, before + token_of(p, row0) + 1), all_from = p.window > 0 ? before + token_of(p, row0 + mine_rows - 1) - p.window + 1 : 0;
             float m = -INFINITY, l = 0.0f;
+#pragma unroll 1
             for (int i = 0; i < tiles; i++, n_tile++) {
                 const int pos0 = (tile0 + i) * TP;
                 const int sb = NQ == 2 ? tq : (int)(n_tile & 1);
                 const uint32_t s_phase = NQ == 2 ? n_tile & 1 : (n_tile >> 1) & 1, t_s = t_lane + C::kS * sb;
-                bar_wait(bar(meta.s_full[sb]), s_phase, gave_up, p.status);
+                bar_wait_here(bar(meta.s_full[sb]), s_phase, gave_up, p.status);
                 tc_after();
                 const uint32_t there = *reinterpret_cast<volatile uint8_t *>(&meta.there[(n_before + i) & 7]);
                 const bool masked = pos0 + TP > all_to || pos0 < all_from || there != (1u << kChunks) - 1u;
-                float f = sc, top = -INFINITY;
-                if (masked || p.softcap > 0.0f) {
-                    // log2 scores in place of the products
+                float f = sc;
+                // What is rarely done has code of its own, and no more of it than has to be: code that is jumped over, or met for the first time, is fetched at
+                // the pace of thousands of clocks.
+                if (p.softcap > 0.0f) {   // log2 scores in place of the products
+                    soft_limit<HALF, TP>(t_s, sc, p.softcap);
                     f = 1.0f;
-                    const int lo = from - pos0, hi = behind - pos0;
-#pragma unroll 1
-                    for (int c = 0; c < TP; c += 32) {
-                        uint32_t v[32];
-                        tmem_load32(t_s + c, v);
-                        tmem_loaded();
-                        const uint32_t ok = (there >> (c / 16)) & 3u, seen16 = (ok & 1u ? 0xFFFFu : 0u) | (ok & 2u ? 0xFFFF0000u : 0u);
-                        const int a = max(lo - c, 0), b = hi - c;
-                        const uint32_t seen = (a >= 32 ? 0u : 0xFFFFFFFFu << a) & (b >= 32 ? 0xFFFFFFFFu : b <= 0 ? 0u : 0xFFFFFFFFu >> (32 - b)) & seen16;
-#pragma unroll
-                        for (int j = 0; j < 32; j++) {
-                            float x = __uint_as_float(v[j]) * sc;
-                            if (p.softcap > 0.0f) x = HALF ? capped_half(x, p.softcap) : capped(x, p.softcap);
-                            if (!((seen >> j) & 1)) x = -INFINITY;
-                            top = fmaxf(top, x);
-                            v[j] = __float_as_uint(x);
-                        }
-                        tmem_store32(t_s + c, v);
-                    }
-                    tmem_stored();
-                } else {
-#pragma unroll
-                    for (int c = 0; c < TP; c += 64) {
-                        uint32_t v[64];
-                        tmem_load32(t_s + c, v);
-                        tmem_load32(t_s + c + 32, v + 32);
-                        tmem_loaded();
-#pragma unroll
-                        for (int j = 0; j < 64; j += 2) top = fmaxf(top, fmaxf(__uint_as_float(v[j]), __uint_as_float(v[j + 1])));
-                    }
-                    top *= sc;
                 }
+                uint32_t v[TP];
+#pragma unroll
+                for (int c = 0; c < TP; c += 32) tmem_load32(t_s + c, v + c);
+                tmem_loaded();
+                if (masked) {
+                    const int lo = from - pos0, hi = behind - pos0;
+#pragma unroll
+                    for (int c = 0; c < TP; c += 32) {
+                        const uint32_t ok = (there >> (c / 16)) & 3u;
+                        const int a = max(lo - c, 0), b = hi - c;
+                        const uint32_t seen = (a >= 32 ? 0u : 0xFFFFFFFFu << a) & (b >= 32 ? 0xFFFFFFFFu : b <= 0 ? 0u : 0xFFFFFFFFu >> (32 - b)) & ((ok & 1u ? 0xFFFFu : 0u) | (ok & 2u ? 0xFFFF0000u : 0u));
+#pragma unroll
+                        for (int j = 0; j < 32; j++) v[c + j] = seen & (1u << j) ? v[c + j] : 0xFF800000u;
+                    }
+                }
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < TP; j += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) tops[k] = fmaxf(tops[k], fmaxf(__uint_as_float(v[j + 2 * k]), __uint_as_float(v[j + 2 * k + 1])));
+                const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * f;
                 if (__any_sync(0xFFFFFFFFu, top > m + kLetBe || (m == -INFINITY && top != -INFINITY))) {
                     const float now = fmaxf(m, top), corr = now == -INFINITY ? 1.0f : ex2(m - now);
                     m = now;
                     l *= corr;
                     if (i > 0) {
-                        bar_wait(bar(meta.pv_done[tq]), (n_tile - 1) & 1, gave_up, p.status);
+                        bar_wait_here(bar(meta.pv_done[tq]), (n_tile - 1) & 1, gave_up, p.status);
                         tc_after();
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 32) {
-                            uint32_t o[32];
-                            tmem_load32(t_o + c, o);
+                        for (int c = 0; c < D; c += 16) {
+                            uint32_t o[16];
+                            tmem_load16(t_o + c, o);
                             tmem_loaded();
 #pragma unroll
-                            for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
-                            tmem_store32(t_o + c, o);
+                            for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                            tmem_store16(t_o + c, o);
                         }
                         tmem_stored();
                     }
                 }
-                const float less = m == -INFINITY ? 0.0f : -m;
+                // (one tile of rows: the products of two tiles may be in flight, which a parity does not tell apart behind the last one)
+                if (NQ == 1 && i > 0 && i == tiles - 1) bar_wait_here(bar(meta.pv_done[tq]), (n_tile - 1) & 1, gave_up, p.status);
+                const float less = (m == -INFINITY ? 0.0f : -m) + (HALF ? kUpLog2 : 0.0f);
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int c = 0; c < TP; c += 32) {
-                    uint32_t v[32];
-                    tmem_load32(t_s + c, v);
-                    tmem_loaded();
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                     uint32_t w[NT * 16];
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
-                        float a, b;
+                        float a = ex2(fmaf(__uint_as_float(v[c + j]), f, less)), b = ex2(fmaf(__uint_as_float(v[c + j + 1]), f, less));
                         if constexpr (HALF) {
-                            a = ex2(fmaf(__uint_as_float(v[j]), f, less + 7.0f)), b = ex2(fmaf(__uint_as_float(v[j + 1]), f, less + 7.0f));
                             w[j / 2] = bits(__floats2half2_rn(a, b));
                         } else {
-                            a = kUp * ex2(fmaf(__uint_as_float(v[j]), f, less)), b = kUp * ex2(fmaf(__uint_as_float(v[j + 1]), f, less));
+                            a *= kUp, b *= kUp;   // (in the exponent it would take bits of the greatest ones)
                             split(a, b, w[j / 2], w[16 + j / 2]);
                         }
                         sum[j & 2] += a;
                         sum[(j & 2) + 1] += b;
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     // (first terms in 16 columns, then the second ones: the place of the scores that were just read, or before it)
                     if constexpr (HALF) tmem_store16(t_s + c / 2, w);
                     else tmem_store32(t_s + c, w);
+                    if (c + 32 == TP / 2) {   // the first half's products begin
+                        tmem_stored();
+                        tc_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(bar(meta.p_half[sb]));
+                    }
                 }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_stored();
                 tc_before();
-                // (one tile of rows: the products of two tiles may be in flight, which a parity does not tell apart behind the last one)
-                if (NQ == 1 && i > 0 && i == tiles - 1) bar_wait(bar(meta.pv_done[tq]), (n_tile - 1) & 1, gave_up, p.status);
                 __syncwarp();
                 if (lane == 0) bar_arrive(bar(meta.p_full[sb]));
             }
 
             // ---- the row's factor, and its outputs through shared memory, in the place of the queries: 32 columns at a time, rows by the warp that has them
             const float all = l * (1.0f / kUp);
-            float keep, out_f = 1.0f / kUp;
+            float out_f = 1.0f / kUp;
+            const bool whole = it.whole;
+            const int place_of_part = it.begins ? 1 : 0;
             if (whole) {
-                float lw = all;
-                keep = 1.0f;
+                float lw = all, keep = 1.0f;
                 if (p.sinks) {
                     const float sink = p.sinks[head] * 1.44269504f, t = fmaxf(m, sink);
                     keep = m == -INFINITY ? 0.0f : exp2f(m - t);
@@ -623,70 +721,57 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 float *to = p.part + (((size_t)blockIdx.x * 2 + place_of_part) * R + 128 * tq + r_in) * (D + 2);
                 *reinterpret_cast<float2 *>(to + D) = make_float2(m, all);
             }
-            bar_wait(bar(meta.pv_done[tq]), (n_tile - 1) & 1, gave_up, p.status);
+            // rows of a lane on their way out: 32 quarter + lane / 8 + 4 j, columns 4 (lane % 8)
+            int64_t to_row[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int rw = 32 * quarter + lane / 8 + 4 * j;
+                if (whole) {
+                    const int t = token_of(p, row0 + rw), h = kvh * p.group + row0 + rw - t * p.group;
+                    to_row[j] = (int64_t)(q0 + t) * p.out_stride + (int64_t)h * D + 4 * (lane & 7);
+                } else {
+                    to_row[j] = (((int64_t)blockIdx.x * 2 + place_of_part) * R + 128 * tq + rw) * (D + 2) + 4 * (lane & 7);
+                }
+            }
+            bar_wait_here(bar(meta.pv_done[tq]), (n_tile - 1) & 1, gave_up, p.status);
             tc_after();
-            const bool any_odd = *reinterpret_cast<volatile uint32_t *>(&meta.odd[tq][n_item & 7]) != 0;
+            if (*reinterpret_cast<volatile uint32_t *>(&meta.odd[tq][n_item & 7]) != 0)
+                add_odd<CT, D, TP>(p, it, t_o, max(from, tile0 * TP), min(behind, (tile0 + tiles) * TP), min(len, before + token_of(p, it.block * R) + 1),
+                                   p.window > 0 ? before + token_of(p, it.block * R + n_rows - 1) - p.window + 1 : 0);
             uint8_t *stage = q_tile + quarter * (32 * 128);
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
                 tmem_load32(t_o + c, o);
                 tmem_loaded();
-                if (any_odd) {
-                    // values that are no numbers, in tiles that not all rows see, were taken out of the products: here are they for the rows that see them
-                    const int first_token = token_of(p, walk.block * R), last_token = token_of(p, walk.block * R + n_rows - 1);
-                    const int end = min(behind, (tile0 + tiles) * TP);
-                    for (int pos = max(from, tile0 * TP); pos < end; pos++) {
-                        const int t0 = pos / TP * TP;
-                        if (!(t0 + TP > min(len, before + first_token + 1) || (p.window > 0 && t0 < before + last_token - p.window + 1))) {
-                            pos = t0 + TP - 1;
-                            continue;
-                        }
-                        const int page = p.table[(size_t)walk.s * p.table_width + pos / p.page_size];
-                        if (page < 0 || page >= p.n_pages) continue;
-                        const int64_t row = ((int64_t)page * p.n_kv + kvh) * p.page_size + pos % p.page_size;
-                        for (int j = 0; j < 32; j++) {
-                            const float y = value_at<CT, D>(p.v, p.v_scale, row, c + j);
-                            if (fabsf(y) <= 65504.0f) continue;
-#pragma unroll
-                            for (int k = 0; k < 32; k++)
-                                if (k == j) o[k] = __float_as_uint(__uint_as_float(o[k]) + y);
-                        }
-                    }
-                    __syncwarp();
-                }
 #pragma unroll
                 for (int j = 0; j < 32; j += 4)
                     *reinterpret_cast<float4 *>(stage + lane * 128 + (((j / 4) ^ (lane & 7)) << 4)) =
                         make_float4(__uint_as_float(o[j]) * out_f, __uint_as_float(o[j + 1]) * out_f, __uint_as_float(o[j + 2]) * out_f, __uint_as_float(o[j + 3]) * out_f);
                 __syncwarp();
-#pragma unroll 2
-                for (int r0 = 0; r0 < 32; r0 += 4) {
-                    const int r = r0 + lane / 8, rw = 32 * quarter + r, at = c + 4 * (lane & 7);
-                    if (rw >= mine_rows) continue;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int r = lane / 8 + 4 * j;
+                    if (32 * quarter + r >= mine_rows) continue;
                     const float4 x = *reinterpret_cast<const float4 *>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-                    if (whole) {
-                        const int t = token_of(p, row0 + rw), h = kvh * p.group + row0 + rw - t * p.group;
-                        const int64_t to = (int64_t)(q0 + t) * p.out_stride + (int64_t)h * D + at;
-                        if constexpr (HALF) {
-                            *reinterpret_cast<uint2 *>(static_cast<__half *>(p.out) + to) = make_uint2(bits(__floats2half2_rn(x.x, x.y)), bits(__floats2half2_rn(x.z, x.w)));
-                        } else {
-                            *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to) = x;
-                        }
-                    } else {
-                        float *to = p.part + (((size_t)blockIdx.x * 2 + place_of_part) * R + 128 * tq + rw) * (D + 2) + at;
+                    if (!whole) {
+                        float *to = p.part + to_row[j] + c;
                         *reinterpret_cast<float2 *>(to) = make_float2(x.x, x.y);
                         *reinterpret_cast<float2 *>(to + 2) = make_float2(x.z, x.w);
+                    } else if constexpr (HALF) {
+                        *reinterpret_cast<uint2 *>(static_cast<__half *>(p.out) + to_row[j] + c) = make_uint2(bits(__floats2half2_rn(x.x, x.y)), bits(__floats2half2_rn(x.z, x.w)));
+                    } else {
+                        *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to_row[j] + c) = x;
                     }
                 }
                 __syncwarp();
             }
             tc_before();
             group_sync(tq);
-            if (any_odd && (tid & 127) == 0) meta.odd[tq][n_item & 7] = 0;
-            n_item++;
+            if (r_in == 0) meta.odd[tq][n_item & 7] = 0;
         }
-    } else if (warp < C::kSoft + kChunkCopyWarps) {
+    } else if (warp < C::kProduct) {
+        if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
         // ===== keys and values into a ring of half tiles (keys, values in turn); a warp has the chunks w, w + 4 of 16 positions
         constexpr int kMine = kChunks / kChunkCopyWarps, kAhead = 32 / kChunks;   // chunks of a warp; tiles whose rows the lanes hold
         const int w = warp - C::kSoft;
@@ -765,7 +850,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                         const uint32_t empty = bar(meta.kv_empty[slot]), parity = ((h / C::kSlots) & 1) ^ 1;
                         if (!bar_test(empty, parity)) {
                             tell(0);   // (who frees the place may wait for these)
-                            bar_wait(empty, parity, gave_up, p.status);
+                            bar_wait_here(empty, parity, gave_up, p.status);
                         }
 #pragma unroll
                         for (int m = 0; m < kMine; m++) {
@@ -812,7 +897,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
 #pragma unroll 1
                 for (int t = 0; t < halves; t++, h++) {
                     const int slot = h % C::kSlots;
-                    bar_wait(bar(meta.kv_empty[slot]), ((h / C::kSlots) & 1) ^ 1, gave_up, p.status);
+                    bar_wait_here(bar(meta.kv_empty[slot]), ((h / C::kSlots) & 1) ^ 1, gave_up, p.status);
                     const bool look = (t & 1) && looked_at(t >> 1);
                     bool bad = false;
                     if (t + 1 < halves && (t & 1)) begin_tile((t + 1) >> 1, (h + 1) >> 1);
@@ -867,13 +952,15 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
         if constexpr (!kQuant) tell(0);
     } else {
         // ===== products
+        if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+        if (warp == C::kProduct) {
         const uint32_t elected = elected_lane();
         uint32_t n_done[2] = {0, 0}, n_item[2] = {0, 0};   // of a tile of rows: tiles so far, items
         int h0 = 0;   // half tiles before this item
         constexpr uint32_t qk = (1u << 4) | (uint32_t)(TP >> 3) << 17 | (128u >> 4) << 24, pv = (1u << 4) | 1u << 16 | (uint32_t)(D >> 3) << 17 | (128u >> 4) << 24;
         while (walk.next(p)) {
             const int n[2] = {tiles_of(walk, 0), NQ == 2 ? tiles_of(walk, 1) : 0}, all = walk.tiles;
-            auto wait_half = [&](int h) { bar_wait(bar(meta.kv_full[h % C::kSlots]), (h / C::kSlots) & 1, gave_up, p.status); };
+            auto wait_half = [&](int h) { bar_wait_here(bar(meta.kv_full[h % C::kSlots]), (h / C::kSlots) & 1, gave_up, p.status); };
             auto place_of = [&](int q, int i) { return NQ == 2 ? q : (int)((n_done[0] + i) & 1); };
             auto scores = [&](int q, int i) {
                 const int slot = (h0 + 2 * i) % C::kSlots, sb = place_of(q, i);
@@ -890,20 +977,26 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             auto sums = [&](int q, int i) {
                 const int slot = (h0 + 2 * i + 1) % C::kSlots, sb = place_of(q, i);
                 const uint32_t values = base + slot * C::kSlot, from = tmem + C::kS * sb, d = tmem + C::kO + 128 * q;
-                bar_wait(bar(meta.p_full[sb]), (NQ == 2 ? n_done[q] + i : (n_done[0] + i) >> 1) & 1, gave_up, p.status);
+                const uint32_t phase = (NQ == 2 ? n_done[q] + i : (n_done[0] + i) >> 1) & 1;
+                bar_wait_here(bar(meta.p_half[sb]), phase, gave_up, p.status);
                 tc_after();
 #pragma unroll
-                for (int k = 0; k < TP / 16; k++)
+                for (int k = 0; k < TP / 16; k++) {
+                    if (k == TP / 32) {
+                        bar_wait_here(bar(meta.p_full[sb]), phase, gave_up, p.status);
+                        tc_after();
+                    }
 #pragma unroll
                     for (int t = 0; t < NT; t++)
                         product_from(d, from + (NT == 2 ? 32 * (k >> 1) + 16 * t + 8 * (k & 1) : 8 * k), desc_lo(values + 2048 * k, TP * 128), kDescHi, pv, i > 0 || k > 0 || t > 0, elected);
+                }
                 products_commit(bar(meta.pv_done[q]), elected);
             };
             wait_half(h0);
 #pragma unroll
             for (int q = 0; q < NQ; q++)
                 if (n[q] > 0) {
-                    bar_wait(bar(meta.q_full[q]), n_item[q] & 1, gave_up, p.status);
+                    bar_wait_here(bar(meta.q_full[q]), n_item[q] & 1, gave_up, p.status);
                     scores(q, 0);
                 }
             products_commit(bar(meta.kv_empty[h0 % C::kSlots]), elected);
@@ -938,20 +1031,21 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             for (int q = 0; q < 2; q++)
                 if (n[q] > 0) n_done[q] += n[q], n_item[q]++;
         }
+        }
     }
     tc_before();
     __syncthreads();
     tc_after();
-    if (warp == C::kWarps - 1 && *gave_up) {   // (nobody waits any more, so this is the last word on it)
+    if (warp == C::kProduct && *gave_up) {   // (nobody waits any more, so this is the last word on it)
         products_commit(bar(meta.drained), elected_lane());
         bar_wait_drained(bar(meta.drained));
     }
-    if (warp == C::kWarps - 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    if (warp == C::kProduct) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
 template <int D, int CT, bool HALF>
 int launch_chunk_one(const ChunkParams &p, cudaStream_t st) {
-    using C = Chunk<D, HALF ? 1 : 2>;
+    using C = Chunk<D, HALF ? 1 : 2, CT != KRK_CUDA_KV_F16>;
     static std::atomic<uint64_t> ready{0};   // devices whose limit of shared memory is raised for this kernel
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
