@@ -157,56 +157,41 @@ struct ChunkWalk {
         r.tile = tile_at(in_head - from, (lo == q.blocks - 1 ? c.last : c.prefix(lo + 1) - from), tiles, p.whole);
         return r;
     }
-    // By the whole CTA, of 128 threads or more; warp 0 has the result.
+    // By a warp.
     __device__ __forceinline__ void start(const ChunkParams &p) {
-        __shared__ int64_t s_sum[4], s_before[2];
-        __shared__ int s_found[2];
-        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-        int64_t lo = 0, mine = 0;
-        auto scan = [&](int s0, int64_t from) {
-            const int i = s0 + tid;
-            mine = tid < 128 && i < p.n_seq ? p.n_kv * chunk_cost<R, TP>(p, chunk_sequence<R>(p, i)).head : 0;
+        const int lane = threadIdx.x & 31;
+        auto units = [&](int s0) { return s0 + lane < p.n_seq ? p.n_kv * chunk_cost<R, TP>(p, chunk_sequence<R>(p, s0 + lane)).head : 0; };
+        int64_t mine = 0;
+        total = 0;
+        for (int s0 = 0; s0 < p.n_seq; s0 += 32) {
+            mine = units(s0);
+            int64_t all = mine;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xFFFFFFFFu, all, o);
+            total += all;
+        }
+        share(p, (int)blockIdx.x);
+        const int64_t u[2] = {first_unit, behind_unit};
+        int found[2] = {p.n_seq, p.n_seq};
+        int64_t before[2] = {total, total}, from = 0;
+        for (int s0 = 0; s0 < p.n_seq && found[1] == p.n_seq; s0 += 32) {
+            if (p.n_seq > 32) mine = units(s0);   // (up to 32 sequences the first ones stand)
             int64_t upto = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int64_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
                 if (lane >= o) upto += v;
             }
-            if (lane == 31 && warp < 4) s_sum[warp] = upto;
-            __syncthreads();
-            int64_t all = 0;
-            lo = from + upto - mine;
+            const int64_t lo = from + upto - mine;
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
-                if (w < warp) lo += s_sum[w];
-                all += s_sum[w];
+            for (int i = 0; i < 2; i++) {
+                const uint32_t here = __ballot_sync(0xFFFFFFFFu, u[i] >= lo && u[i] < lo + mine);
+                if (here) found[i] = s0 + __ffs(here) - 1, before[i] = __shfl_sync(0xFFFFFFFFu, lo, __ffs(here) - 1);
             }
-            __syncthreads();
-            return all;
-        };
-        total = 0;
-        for (int s0 = 0; s0 < p.n_seq; s0 += 128) total += scan(s0, total);
-        share(p, (int)blockIdx.x);
-        const int64_t u[2] = {first_unit, behind_unit};
-        if (tid < 2) s_found[tid] = p.n_seq, s_before[tid] = total;
-        __syncthreads();
-        int64_t from = 0;
-        for (int s0 = 0; s0 < p.n_seq; s0 += 128) {
-            if (p.n_seq > 128) from += scan(s0, from);   // (up to 128 sequences the first scan's values stand)
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-                if (u[i] >= lo && u[i] < lo + mine) s_found[i] = s0 + tid, s_before[i] = lo;
+            from += __shfl_sync(0xFFFFFFFFu, upto, 31);
         }
-        __syncthreads();
-        // warps 0 and 1 find the two ends (of all warps it took 5 us)
-        __shared__ ChunkPlace s_end;
-        if (warp == 1 && s_found[1] < p.n_seq) {
-            const ChunkPlace e = place(p, s_found[1], u[1] - s_before[1]);
-            if (lane == 0) s_end = e;
-        }
-        if (warp == 0) begin(p, s_found[0], s_before[0]);
-        __syncthreads();
-        if (s_found[1] < p.n_seq) end = s_end;
+        begin(p, found[0], before[0]);
+        if (!over && found[1] < p.n_seq) end = place(p, found[1], u[1] - before[1]);
     }
     // Of CTA b, with the total of units: how many share them, and its own.
     __host__ __device__ __forceinline__ void share(const ChunkParams &p, int b) {
@@ -305,34 +290,44 @@ struct Chunk {
     static constexpr int kPanels = (D + 63) / 64;                    // blocks of 64 values
     static constexpr int kTerm = kPanels * 128 * 128, kQTile = NT * kTerm;
     static constexpr int kSlot = kPanels * TP * 128;                 // half a tile: keys or values
-    static constexpr int kRoom = 227 * 1024 - 1024 - kMetaBytes - 64 - NQ * kQTile;   // (64: ChunkWalk::start)
+    static constexpr int kRoom = 227 * 1024 - 1024 - kMetaBytes - NQ * kQTile;
     static constexpr int kSlots = kRoom / kSlot > 6 ? 6 : kRoom / kSlot;
     static constexpr int kQ = kSlots * kSlot, kMeta = kQ + NQ * kQTile, kBytes = kMeta + kMetaBytes + 1024;   // (begins on a 1024-byte boundary)
-    static constexpr int kSoft = 4 * NQ, kProduct = kSoft + kChunkCopyWarps, kWarps = kProduct + 4, kThreads = 32 * kWarps;   // (of the last four one works)
+    // warps: softmax, copies, products (one for each tile of rows), the one that finds items
+    static constexpr int kSoft = 4 * NQ, kProduct = kSoft + kChunkCopyWarps, kFinder = kProduct + 2, kWarps = kProduct + 4, kThreads = 32 * kWarps;
     // registers of a thread: 512 threads are launched with 128 each; the copies unpack 8 and 4 bits in theirs
     static constexpr int kSoftRegs = QUANT ? 168 : 184, kOtherRegs = QUANT ? 88 : 72;
     static_assert(256 * kSoftRegs + 256 * kOtherRegs <= 65536, "registers of a launch");
     static constexpr uint32_t kO = 256;                              // column of the sums; of the second tile's: 128 more
     static constexpr uint32_t kS = NQ == 2 ? 128 : 64;               // from a place of scores to the next
     static_assert(kSlots >= 3, "a half tile of values and one of keys at work, one on its way");
-    static_assert(kBytes + 64 <= 227 * 1024, "shared memory");
+    static_assert(kBytes <= 227 * 1024, "shared memory");
     using Walk = ChunkWalk<R, TP>;
 };
 
 struct ChunkItem {
-    int goes_on, q0, len, before, s, kvh, block, n_rows, tile0, all, tiles;   // all: tiles of the item, tiles: that the rows of this tile see
+    int goes_on, q0, len, before, s, kvh, block, n_rows, tile0, all, tiles[2], all_from, all_to;   // all: its tiles, tiles: that the rows of a tile see; every row sees [all_from, all_to)
     bool whole, begins;
 };
-template <int R, int TP>
+constexpr int kChunkItems = 3;   // found ahead
+template <int R>
 struct ChunkMeta {
-    unsigned long long kv_full[6], kv_empty[6], s_full[2], p_half[2], p_full[2], pv_done[2], q_full[2], drained;
+    unsigned long long kv_full[6], kv_empty[6], s_full[2], p_half[2], p_full[2], pv_done[2], q_full[2], item_full[kChunkItems], item_empty[kChunkItems], drained[2];
     float scale[R];
     uint32_t odd[2][8];       // of a tile of rows, an item in turn: values of a tile that not all rows see are no numbers
     uint8_t there[8];         // of a tile of positions, in turn: bit c: chunk c is a page's
     uint32_t tmem;
     int gave_up;
-    ChunkItem item[2][2];     // of a tile of rows: this item and the next
-    ChunkWalk<R, TP> walk[2];
+    ChunkItem item[kChunkItems], mine[2];   // mine: of a tile of rows, what its first thread has read
+};
+// A place of a ring and the parity of its turn.
+template <int N>
+struct Ring {
+    int at = 0;
+    uint32_t turn = 0;
+    __device__ __forceinline__ void next() {
+        if (++at == N) at = 0, turn ^= 1;
+    }
 };
 
 __device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t *v) {
@@ -361,11 +356,49 @@ __device__ __forceinline__ void bar_wait_here(uint32_t bar, uint32_t parity, vol
             atomicExch(status, KRK_CUDA_ETIMEOUT);
         }
 }
-// A product as above with A in tensor memory (lane = row, a column two f16).
-__device__ __forceinline__ void product_from(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t onto, uint32_t elected) {
-    asm volatile("{\n .reg .pred p, q;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %7, 0;\n mov.b64 b, {%2, %3};\n"
-                 " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, {%6, %6, %6, %6}, p;\n}\n"
-                 ::"r"(d), "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(onto), "r"(0u), "r"(elected) : "memory");
+// N products over 16 values each, both operands from shared memory; the next 16 values are 32 bytes on. Executed as `product`.
+template <int N>
+__device__ __forceinline__ void products_k(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t onto, uint32_t elected) {
+    static_assert(N == 2 || N == 4, "");
+    if constexpr (N == 4)
+        asm volatile("{\n .reg .pred p, q, t;\n .reg .b64 a0, b0, a1, b1, a2, b2, a3, b3;\n .reg .b32 x1, x2, x3, y1, y2, y3;\n"
+                     " setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %6, 0;\n setp.eq.b32 t, 0, 0;\n"
+                     " add.s32 x1, %1, 2;\n add.s32 x2, %1, 4;\n add.s32 x3, %1, 6;\n add.s32 y1, %2, 2;\n add.s32 y2, %2, 4;\n add.s32 y3, %2, 6;\n"
+                     " mov.b64 a0, {%1, %7};\n mov.b64 a1, {x1, %7};\n mov.b64 a2, {x2, %7};\n mov.b64 a3, {x3, %7};\n"
+                     " mov.b64 b0, {%2, %7};\n mov.b64 b1, {y1, %7};\n mov.b64 b2, {y2, %7};\n mov.b64 b3, {y3, %7};\n"
+                     " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a0, b0, %3, {%5, %5, %5, %5}, p;\n"
+                     " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, {%5, %5, %5, %5}, t;\n"
+                     " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, {%5, %5, %5, %5}, t;\n"
+                     " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, {%5, %5, %5, %5}, t;\n}\n"
+                     ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(onto), "r"(0u), "r"(elected), "r"(kDescHi) : "memory");
+    else
+        asm volatile("{\n .reg .pred p, q, t;\n .reg .b64 a0, b0, a1, b1;\n .reg .b32 x1, y1;\n"
+                     " setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %6, 0;\n setp.eq.b32 t, 0, 0;\n add.s32 x1, %1, 2;\n add.s32 y1, %2, 2;\n"
+                     " mov.b64 a0, {%1, %7};\n mov.b64 a1, {x1, %7};\n mov.b64 b0, {%2, %7};\n mov.b64 b1, {y1, %7};\n"
+                     " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a0, b0, %3, {%5, %5, %5, %5}, p;\n"
+                     " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, {%5, %5, %5, %5}, t;\n}\n"
+                     ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(onto), "r"(0u), "r"(elected), "r"(kDescHi) : "memory");
+}
+// The products over 32 positions with the weights in tensor memory (lane = row, a column two f16): 16 columns of first terms, NT 2: 16 of second ones behind
+// them; the next 16 positions of the values are 2048 bytes on.
+template <int NT>
+__device__ __forceinline__ void products_p(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t onto, uint32_t elected) {
+    if constexpr (NT == 1)
+        asm volatile("{\n .reg .pred p, q, t;\n .reg .b64 b0, b1;\n .reg .b32 x1, y1;\n"
+                     " setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %6, 0;\n setp.eq.b32 t, 0, 0;\n add.s32 x1, %1, 8;\n add.s32 y1, %2, 128;\n"
+                     " mov.b64 b0, {%2, %7};\n mov.b64 b1, {y1, %7};\n"
+                     " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b0, %3, {%5, %5, %5, %5}, p;\n"
+                     " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [x1], b1, %3, {%5, %5, %5, %5}, t;\n}\n"
+                     ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(onto), "r"(0u), "r"(elected), "r"(kDescHi) : "memory");
+    else
+        asm volatile("{\n .reg .pred p, q, t;\n .reg .b64 b0, b1;\n .reg .b32 x1, x2, x3, y1;\n"
+                     " setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %6, 0;\n setp.eq.b32 t, 0, 0;\n add.s32 x1, %1, 8;\n add.s32 x2, %1, 16;\n add.s32 x3, %1, 24;\n add.s32 y1, %2, 128;\n"
+                     " mov.b64 b0, {%2, %7};\n mov.b64 b1, {y1, %7};\n"
+                     " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b0, %3, {%5, %5, %5, %5}, p;\n"
+                     " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [x2], b0, %3, {%5, %5, %5, %5}, t;\n"
+                     " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [x1], b1, %3, {%5, %5, %5, %5}, t;\n"
+                     " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [x3], b1, %3, {%5, %5, %5, %5}, t;\n}\n"
+                     ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(onto), "r"(0u), "r"(elected), "r"(kDescHi) : "memory");
 }
 // Bytes I and J of w, as `halves` in krk_attn_kernel.cuh.
 template <int I, int J>
@@ -410,9 +443,9 @@ __device__ __forceinline__ void soft_limit(uint32_t t_s, float sc, float cap) {
     tmem_stored();
 }
 // Values that are no numbers, in tiles that not all rows of an item see, were taken out of the products: here they are, for the rows that see them. A thread's
-// row sees [pos, end); tiles inside [all_from, all_to) were left as they are.
+// row sees [pos0, end); tiles that every row sees were left as they are.
 template <int CT, int D, int TP>
-__device__ __forceinline__ void add_odd(const ChunkParams &p, const ChunkItem &it, uint32_t t_o, int pos0, int end, int all_to, int all_from) {
+__device__ __forceinline__ void add_odd(const ChunkParams &p, const ChunkItem &it, uint32_t t_o, int pos0, int end) {
 #pragma unroll 1
     for (int c = 0; c < D; c += 16) {
         uint32_t o[16];
@@ -420,7 +453,7 @@ __device__ __forceinline__ void add_odd(const ChunkParams &p, const ChunkItem &i
         tmem_loaded();
         for (int pos = pos0; pos < end; pos++) {
             const int t0 = pos / TP * TP;
-            if (t0 + TP <= all_to && t0 >= all_from) {
+            if (t0 + TP <= it.all_to && t0 >= it.all_from) {
                 pos = t0 + TP - 1;
                 continue;
             }
@@ -453,18 +486,19 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
     extern __shared__ uint8_t raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t base = smem_addr(smem);
-    using Meta = ChunkMeta<R, TP>;
+    using Meta = ChunkMeta<R>;
     static_assert(sizeof(Meta) <= C::kMetaBytes, "Chunk::kMeta");
     Meta &meta = *reinterpret_cast<Meta *>(smem + C::kMeta);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     volatile int *gave_up = &meta.gave_up;
     auto bar = [&](unsigned long long &b) { return smem_addr(&b); };
+    auto wait = [&](unsigned long long &b, uint32_t parity) { bar_wait_here(bar(b), parity, gave_up, p.status); };
 
     if (warp == 0) {
         if (lane == 0) {
             for (int i = 0; i < C::kSlots; i++) {
                 bar_init(bar(meta.kv_full[i]), kChunkCopyWarps);
-                bar_init(bar(meta.kv_empty[i]), 1);
+                bar_init(bar(meta.kv_empty[i]), NQ);
             }
             for (int i = 0; i < 2; i++) {
                 bar_init(bar(meta.s_full[i]), 1);
@@ -472,8 +506,12 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 bar_init(bar(meta.p_full[i]), 4);
                 bar_init(bar(meta.pv_done[i]), 1);
                 bar_init(bar(meta.q_full[i]), 4);
+                bar_init(bar(meta.drained[i]), 1);
             }
-            bar_init(bar(meta.drained), 1);
+            for (int i = 0; i < kChunkItems; i++) {
+                bar_init(bar(meta.item_full[i]), 1);
+                bar_init(bar(meta.item_empty[i]), 2 * NQ + kChunkCopyWarps);
+            }
             meta.gave_up = 0;
         }
         if (lane < 16) meta.odd[lane >> 3][lane & 7] = 0;
@@ -487,24 +525,10 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
         tc_before();
     }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    Walk walk;
-    walk.start(p);   // (its barriers publish those above)
-    if (tid == 0) {
-        if (!p.whole) p.shared[blockIdx.x].parts = 0;
-        meta.walk[0] = meta.walk[1] = walk;
-    }
     __syncthreads();
-    walk = meta.walk[0];
-    __syncthreads();   // (the softmax goes on with it)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     tc_after();
     const uint32_t tmem = meta.tmem;
-    // tiles of an item that rows of tile q see; those of the first tile of rows end earlier
-    auto tiles_of = [&](const Walk &w, int q) {
-        if (q * 128 >= w.n_rows) return 0;
-        const int t1 = token_of(p, w.block * R + min(w.n_rows, (q + 1) * 128) - 1), end = min(w.now.len, w.now.before + t1 + 1);
-        return min(w.tiles, max((end + TP - 1) / TP - w.tile0, 1));
-    };
 
     if (warp < C::kSoft) {
         // ===== softmax: thread = row
@@ -512,101 +536,142 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
         const int tq = warp >> 2, r_in = tid & 127, quarter = warp & 3;
         const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16), t_o = t_lane + C::kO + 128 * tq;
         uint8_t *q_tile = smem + C::kQ + tq * C::kQTile;
-        auto find_item = [&](uint32_t n) {   // by one thread
-            Walk w = meta.walk[tq];
-            ChunkItem it;
-            it.goes_on = tq == 0 ? w.template next<true>(p) : w.next(p);
-            if (tq == 0 && it.goes_on && w.parts > 0) w.note(p);
-            it.q0 = w.now.q0, it.len = w.now.len, it.before = w.now.before, it.s = w.s, it.kvh = w.kvh, it.block = w.block, it.n_rows = w.n_rows;
-            it.tile0 = w.tile0, it.all = w.tiles, it.tiles = tiles_of(w, tq), it.whole = w.begins && w.ends, it.begins = w.begins;
-            meta.item[tq][n & 1] = it;
-            meta.walk[tq] = w;
-        };
         uint32_t n_tile = 0, n_item = 0, n_all = 0;   // tiles of this tile of rows, items, tiles of all items
-        if (r_in == 0) find_item(0);
-        for (;; n_item++) {
+        Ring<kChunkItems> found;
+        for (;; n_item++, found.next()) {
+            if (r_in == 0) {   // (one thread decides for its barriers' 128)
+                wait(meta.item_full[found.at], found.turn);
+                ChunkItem it = meta.item[found.at];
+                if (*gave_up) it.goes_on = 0;
+                meta.mine[tq] = it;
+                bar_arrive(bar(meta.item_empty[found.at]));
+            }
             group_sync(tq);
-            const ChunkItem &it = meta.item[tq][n_item & 1];
+            const ChunkItem &it = meta.mine[tq];
             if (!it.goes_on) break;
-            const int n_rows = it.n_rows, tiles = it.tiles, tile0 = it.tile0, before = it.before, len = it.len, kvh = it.kvh, q0 = it.q0;
+            const int n_rows = it.n_rows, tiles = it.tiles[tq], tile0 = it.tile0, before = it.before, len = it.len, kvh = it.kvh, q0 = it.q0;
             const int row0 = it.block * R + 128 * tq;   // among the key head's
             const int mine_rows = min(128, n_rows - 128 * tq);
             const uint32_t n_before = n_all;
             n_all += it.all;
             if (mine_rows <= 0) {
                 group_sync(tq);
-                if (r_in == 0) find_item(n_item + 1);
                 continue;
             }
-            // ---- queries, four values a lane, some rows at a time, under a power of two of their own: the largest value in [2^10, 2^11)
+            // ---- queries. f16 ones as they are, else under a power of two of their row: the largest value in [2^10, 2^11)
             const float sign = p.scale < 0.0f ? -1.0f : 1.0f, row_scale = fabsf(p.scale) * (p.softcap > 0.0f ? 1.0f : 1.44269504f);
-            auto queries = [&](auto half_q) {
-                constexpr bool kHalfQ = decltype(half_q)::value;
-                constexpr int NL = (D + 127) / 128, kRows = NL == 1 ? 16 : 8;
-                using Raw = std::conditional_t<kHalfQ, uint2, uint4>;
+            // (a row's place in q, and in the tile of shared memory)
+            auto q_at = [&](int r) {
+                const int i = token_of(p, row0 + r);
+                return (int64_t)(q0 + i) * p.q_stride + (int64_t)(kvh * p.group + row0 + r - i * p.group) * D;
+            };
+            auto power_of = [](float most) { return most > 0.0f && most <= 3.4028234e38f ? 10 - max((int)(__float_as_uint(most) >> 23) - 127, -110) : 0; };
+            auto put = [&](int r, int d, const float (&x)[4], int e) {   // four values of a row, under 2^e
+                const float up = sign * __uint_as_float((uint32_t)(127 + e) << 23);
+                uint32_t hi[2], lo[2];
+                split(x[0] * up, x[1] * up, hi[0], lo[0]);
+                split(x[2] * up, x[3] * up, hi[1], lo[1]);
+                uint8_t *to = q_tile + (d >> 6) * (128 * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + 2 * (d & 7);
+                *reinterpret_cast<uint2 *>(to) = make_uint2(hi[0], hi[1]);
+                if constexpr (NT == 2) *reinterpret_cast<uint2 *>(to + C::kTerm) = make_uint2(lo[0], lo[1]);
+            };
+            constexpr int NL = (D + 127) / 128;
+            const bool as_they_are = HALF && p.q_half && p.scale >= 0.0f;
+            if (as_they_are) {
+                constexpr int kPer = D / 8;   // pieces of 16 bytes
+#pragma unroll 4
+                for (int j = 0; j < kPer; j++) {
+                    const int c = lane + 32 * j, r = 32 * quarter + c / kPer, piece = c % kPer;
+                    const bool there = r < mine_rows;
+                    copy16(base + C::kQ + tq * C::kQTile + (piece >> 3) * (128 * 128) + r * 128 + (((piece & 7) ^ (r & 7)) << 4),
+                           there ? static_cast<const __half *>(p.q) + q_at(r) + 8 * piece : p.q, there);
+                }
+                copies_commit();
+                copies_wait<0>();
+            } else if constexpr (!HALF) {
+                // all of a warp's rows first, as they are, each in the 128-byte places that its terms will have
+                constexpr int kPer = D / 4;
+#pragma unroll 4
+                for (int j = 0; j < kPer; j++) {
+                    const int c = lane + 32 * j, r = 32 * quarter + c / kPer, piece = c % kPer, place = piece >> 3;
+                    const bool there = r < mine_rows;
+                    copy16(base + C::kQ + tq * C::kQTile + place / C::kPanels * C::kTerm + place % C::kPanels * (128 * 128) + r * 128 + ((piece & 7) << 4),
+                           there ? static_cast<const float *>(p.q) + q_at(r) + 4 * piece : p.q, there);
+                }
+                copies_commit();
+                copies_wait<0>();
+                __syncwarp();
 #pragma unroll 1
-                for (int j0 = 0; j0 < 32; j0 += kRows) {
-                    Raw x[kRows][NL];
-                    // (a row's place: its token and head, walked from the first one's)
-                    int r = 32 * quarter + j0, i = token_of(p, row0 + r), h = row0 + r - i * p.group;
+                for (int j0 = 0; j0 < 32; j0 += 4) {
+                    float x[4][NL][4], most[4];
 #pragma unroll
-                    for (int j = 0; j < kRows; j++) {
-                        const int64_t from = (int64_t)(q0 + i) * p.q_stride + (int64_t)(kvh * p.group + h) * D;
-#pragma unroll
-                        for (int c = 0; c < NL; c++) {
-                            const int d = 128 * c + 4 * lane;
-                            x[j][c] = Raw{};
-                            if (r + j < mine_rows && (D % 128 == 0 || d < D)) x[j][c] = *reinterpret_cast<const Raw *>(static_cast<const uint8_t *>(p.q) + (from + d) * (kHalfQ ? 2 : 4));
-                        }
-                        if (++h == p.group) h = 0, i++;
-                    }
-                    auto value = [&](int j, int c, int e) {
-                        if constexpr (kHalfQ) {
-                            const float2 two = __half22float2(half2_of(e < 2 ? x[j][c].x : x[j][c].y));
-                            return e & 1 ? two.y : two.x;
-                        } else {
-                            return __uint_as_float(e == 0 ? x[j][c].x : e == 1 ? x[j][c].y : e == 2 ? x[j][c].z : x[j][c].w);
-                        }
-                    };
-                    float most[kRows];
-#pragma unroll
-                    for (int j = 0; j < kRows; j++) {
+                    for (int j = 0; j < 4; j++) {
+                        const int r = 32 * quarter + j0 + j;
                         most[j] = 0.0f;
 #pragma unroll
-                        for (int c = 0; c < NL; c++)
+                        for (int c = 0; c < NL; c++) {
+                            const int piece = 32 * c + lane, place = piece >> 3;
+                            if (D % 128 == 0 || piece < kPer)
+                                *reinterpret_cast<float4 *>(x[j][c]) = *reinterpret_cast<const float4 *>(q_tile + place / C::kPanels * C::kTerm + place % C::kPanels * (128 * 128) + r * 128 + ((piece & 7) << 4));
+                            else x[j][c][0] = x[j][c][1] = x[j][c][2] = x[j][c][3] = 0.0f;
 #pragma unroll
-                            for (int e = 0; e < 4; e++) most[j] = fmaxf(most[j], fabsf(value(j, c, e)));
+                            for (int e = 0; e < 4; e++) most[j] = fmaxf(most[j], fabsf(x[j][c][e]));
+                        }
                     }
 #pragma unroll
-                    for (int j = 0; j < kRows; j++) most[j] = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most[j])));   // (not negative: bits in order)
+                    for (int j = 0; j < 4; j++) most[j] = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most[j])));   // (not negative: bits in order)
 #pragma unroll
-                    for (int j = 0; j < kRows; j++) {
-                        const int rr = r + j, e = most[j] > 0.0f && most[j] <= 3.4028234e38f ? 10 - max((int)(__float_as_uint(most[j]) >> 23) - 127, -110) : 0;
-                        const float up = sign * __uint_as_float((uint32_t)(127 + e) << 23);
+                    for (int j = 0; j < 4; j++) {
+                        const int r = 32 * quarter + j0 + j, e = power_of(most[j]);
+#pragma unroll
+                        for (int c = 0; c < NL; c++)
+                            if (D % 128 == 0 || 32 * c + lane < kPer) put(r, 128 * c + 4 * lane, x[j][c], e);
+                        if (lane == 0) meta.scale[128 * tq + r] = row_scale * __uint_as_float((uint32_t)(127 - e) << 23);
+                    }
+                }
+            } else {
+#pragma unroll 1
+                for (int j0 = 0; j0 < 32; j0 += 4) {
+                    float x[4][NL][4], most[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int r = 32 * quarter + j0 + j;
+                        const int64_t from = q_at(r);
+                        most[j] = 0.0f;
 #pragma unroll
                         for (int c = 0; c < NL; c++) {
                             const int d = 128 * c + 4 * lane;
-                            if (D % 128 == 0 || d < D) {
-                                uint32_t hi[2], lo[2];
-                                split(value(j, c, 0) * up, value(j, c, 1) * up, hi[0], lo[0]);
-                                split(value(j, c, 2) * up, value(j, c, 3) * up, hi[1], lo[1]);
-                                uint8_t *to = q_tile + (d >> 6) * (128 * 128) + rr * 128 + ((((d & 63) >> 3) ^ (rr & 7)) << 4) + 2 * (d & 7);
-                                *reinterpret_cast<uint2 *>(to) = make_uint2(hi[0], hi[1]);
-                                if constexpr (NT == 2) *reinterpret_cast<uint2 *>(to + C::kTerm) = make_uint2(lo[0], lo[1]);
+                            x[j][c][0] = x[j][c][1] = x[j][c][2] = x[j][c][3] = 0.0f;
+                            if (r < mine_rows && (D % 128 == 0 || d < D)) {
+                                if (p.q_half) {
+                                    const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const __half *>(p.q) + from + d);
+                                    const float2 a = __half22float2(half2_of(w.x)), b = __half22float2(half2_of(w.y));
+                                    x[j][c][0] = a.x, x[j][c][1] = a.y, x[j][c][2] = b.x, x[j][c][3] = b.y;
+                                } else {
+                                    *reinterpret_cast<float4 *>(x[j][c]) = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + from + d);
+                                }
                             }
+#pragma unroll
+                            for (int e = 0; e < 4; e++) most[j] = fmaxf(most[j], fabsf(x[j][c][e]));
                         }
-                        if (lane == 0) meta.scale[128 * tq + rr] = row_scale * __uint_as_float((uint32_t)(127 - e) << 23);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; j++) most[j] = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most[j])));
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int r = 32 * quarter + j0 + j, e = power_of(most[j]);
+#pragma unroll
+                        for (int c = 0; c < NL; c++)
+                            if (D % 128 == 0 || 128 * c + 4 * lane < D) put(r, 128 * c + 4 * lane, x[j][c], e);
+                        if (lane == 0) meta.scale[128 * tq + r] = row_scale * __uint_as_float((uint32_t)(127 - e) << 23);
                     }
                 }
-            };
-            if (HALF && p.q_half) queries(std::true_type{});
-            else queries(std::false_type{});
+            }
             async_fence();
             __syncwarp();
             if (lane == 0) bar_arrive(bar(meta.q_full[tq]));
-            if (r_in == 0) find_item(n_item + 1);
 
-            const float sc = meta.scale[128 * tq + r_in];
+            const float sc = as_they_are ? row_scale : meta.scale[128 * tq + r_in];
             const int rr = row0 + min(r_in, mine_rows - 1), token = token_of(p, rr), head = kvh * p.group + rr - token * p.group;
             const int behind = min(len, before + token + 1), from = p.window > 0 ? max(0, before + token - p.window + 1) : 0;   // what the row sees: [from, behind)
             // every row of this tile of rows sees [all_from, all_to)
@@ -617,7 +682,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 const int pos0 = (tile0 + i) * TP;
                 const int sb = NQ == 2 ? tq : (int)(n_tile & 1);
                 const uint32_t s_phase = NQ == 2 ? n_tile & 1 : (n_tile >> 1) & 1, t_s = t_lane + C::kS * sb;
-                bar_wait_here(bar(meta.s_full[sb]), s_phase, gave_up, p.status);
+                wait(meta.s_full[sb], s_phase);
                 tc_after();
                 const uint32_t there = *reinterpret_cast<volatile uint8_t *>(&meta.there[(n_before + i) & 7]);
                 const bool masked = pos0 + TP > all_to || pos0 < all_from || there != (1u << kChunks) - 1u;
@@ -654,7 +719,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     m = now;
                     l *= corr;
                     if (i > 0) {
-                        bar_wait_here(bar(meta.pv_done[tq]), (n_tile - 1) & 1, gave_up, p.status);
+                        wait(meta.pv_done[tq], (n_tile - 1) & 1);
                         tc_after();
 #pragma unroll 1
                         for (int c = 0; c < D; c += 16) {
@@ -669,7 +734,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     }
                 }
                 // (one tile of rows: the products of two tiles may be in flight, which a parity does not tell apart behind the last one)
-                if (NQ == 1 && i > 0 && i == tiles - 1) bar_wait_here(bar(meta.pv_done[tq]), (n_tile - 1) & 1, gave_up, p.status);
+                if (NQ == 1 && i > 0 && i == tiles - 1) wait(meta.pv_done[tq], (n_tile - 1) & 1);
                 const float less = (m == -INFINITY ? 0.0f : -m) + (HALF ? kUpLog2 : 0.0f);
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -708,7 +773,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             const float all = l * (1.0f / kUp);
             float out_f = 1.0f / kUp;
             const bool whole = it.whole;
-            const int place_of_part = it.begins ? 1 : 0;
+            float *part = p.part + (((size_t)blockIdx.x * 2 + it.begins) * R + 128 * tq + 32 * quarter) * (D + 2);   // of the warp's rows
             if (whole) {
                 float lw = all, keep = 1.0f;
                 if (p.sinks) {
@@ -718,27 +783,22 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 }
                 out_f *= lw == 0.0f ? 0.0f : keep / lw;
             } else if (r_in < mine_rows) {
-                float *to = p.part + (((size_t)blockIdx.x * 2 + place_of_part) * R + 128 * tq + r_in) * (D + 2);
-                *reinterpret_cast<float2 *>(to + D) = make_float2(m, all);
+                *reinterpret_cast<float2 *>(part + lane * (D + 2) + D) = make_float2(m, all);
             }
-            // rows of a lane on their way out: 32 quarter + lane / 8 + 4 j, columns 4 (lane % 8)
+            const int out_rows = mine_rows - 32 * quarter - lane / 8;   // a lane's rows: lane / 8 + 4 j below 32, while 4 j is less than this
             int64_t to_row[8];
+            if (whole) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int rw = 32 * quarter + lane / 8 + 4 * j;
-                if (whole) {
-                    const int t = token_of(p, row0 + rw), h = kvh * p.group + row0 + rw - t * p.group;
-                    to_row[j] = (int64_t)(q0 + t) * p.out_stride + (int64_t)h * D + 4 * (lane & 7);
-                } else {
-                    to_row[j] = (((int64_t)blockIdx.x * 2 + place_of_part) * R + 128 * tq + rw) * (D + 2) + 4 * (lane & 7);
+                for (int j = 0; j < 8; j++) {
+                    const int g = row0 + 32 * quarter + lane / 8 + 4 * j, t = token_of(p, g);
+                    to_row[j] = (int64_t)(q0 + t) * p.out_stride + (int64_t)(kvh * p.group + g - t * p.group) * D + 4 * (lane & 7);
                 }
             }
-            bar_wait_here(bar(meta.pv_done[tq]), (n_tile - 1) & 1, gave_up, p.status);
+            wait(meta.pv_done[tq], (n_tile - 1) & 1);
             tc_after();
-            if (*reinterpret_cast<volatile uint32_t *>(&meta.odd[tq][n_item & 7]) != 0)
-                add_odd<CT, D, TP>(p, it, t_o, max(from, tile0 * TP), min(behind, (tile0 + tiles) * TP), min(len, before + token_of(p, it.block * R) + 1),
-                                   p.window > 0 ? before + token_of(p, it.block * R + n_rows - 1) - p.window + 1 : 0);
+            if (*reinterpret_cast<volatile uint32_t *>(&meta.odd[tq][n_item & 7]) != 0) add_odd<CT, D, TP>(p, it, t_o, max(from, tile0 * TP), min(behind, (tile0 + tiles) * TP));
             uint8_t *stage = q_tile + quarter * (32 * 128);
+            const uint8_t *mine = stage + (lane / 8) * 128;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
@@ -749,19 +809,23 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     *reinterpret_cast<float4 *>(stage + lane * 128 + (((j / 4) ^ (lane & 7)) << 4)) =
                         make_float4(__uint_as_float(o[j]) * out_f, __uint_as_float(o[j + 1]) * out_f, __uint_as_float(o[j + 2]) * out_f, __uint_as_float(o[j + 3]) * out_f);
                 __syncwarp();
+                float4 x[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int r = lane / 8 + 4 * j;
-                    if (32 * quarter + r >= mine_rows) continue;
-                    const float4 x = *reinterpret_cast<const float4 *>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-                    if (!whole) {
-                        float *to = p.part + to_row[j] + c;
-                        *reinterpret_cast<float2 *>(to) = make_float2(x.x, x.y);
-                        *reinterpret_cast<float2 *>(to + 2) = make_float2(x.z, x.w);
-                    } else if constexpr (HALF) {
-                        *reinterpret_cast<uint2 *>(static_cast<__half *>(p.out) + to_row[j] + c) = make_uint2(bits(__floats2half2_rn(x.x, x.y)), bits(__floats2half2_rn(x.z, x.w)));
-                    } else {
-                        *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to_row[j] + c) = x;
+                for (int j = 0; j < 8; j++) x[j] = *reinterpret_cast<const float4 *>(mine + j * 512 + (((lane & 7) ^ ((lane / 8 + 4 * j) & 7)) << 4));
+                if (whole) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        if (4 * j >= out_rows) continue;
+                        if constexpr (HALF) *reinterpret_cast<uint2 *>(static_cast<__half *>(p.out) + to_row[j] + c) = make_uint2(bits(__floats2half2_rn(x[j].x, x[j].y)), bits(__floats2half2_rn(x[j].z, x[j].w)));
+                        else *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to_row[j] + c) = x[j];
+                    }
+                } else {
+                    float *to = part + (lane / 8) * (D + 2) + 4 * (lane & 7) + c;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        if (4 * j >= out_rows) continue;
+                        *reinterpret_cast<float2 *>(to + 4 * j * (D + 2)) = make_float2(x[j].x, x[j].y);
+                        *reinterpret_cast<float2 *>(to + 4 * j * (D + 2) + 2) = make_float2(x[j].z, x[j].w);
                     }
                 }
                 __syncwarp();
@@ -771,11 +835,13 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             if (r_in == 0) meta.odd[tq][n_item & 7] = 0;
         }
     } else if (warp < C::kProduct) {
-        if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
         // ===== keys and values into a ring of half tiles (keys, values in turn); a warp has the chunks w, w + 4 of 16 positions
+        if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
         constexpr int kMine = kChunks / kChunkCopyWarps, kAhead = 32 / kChunks;   // chunks of a warp; tiles whose rows the lanes hold
         const int w = warp - C::kSoft;
-        int n_item = 0, h = 0;
+        int n_item = 0, n_tile = 0;
+        Ring<kChunkItems> found;
+        Ring<C::kSlots> to_slot;
         auto take_out = [&](uint32_t &x) {   // of two f16, those that are no numbers
             bool bad = false;
             if ((x & 0x7C00u) == 0x7C00u) x &= 0xFFFF0000u, bad = true;
@@ -787,7 +853,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             atomicOr(&meta.odd[1][item & 7], 1u);
         };
         int64_t pool_rows = 0;   // lane: of chunk lane % kChunks of tile i + lane / kChunks, -1: none
-        int told = 0, tag = -1;  // f16: half tiles told of; lane h % 32: of half tile h, the item whose values are looked at, -1: not
+        int asked = 0, told = 0, told_slot = 0, tag = -1;  // f16: half tiles asked for and told of; lane h % 32: of half tile h, the item whose values are looked at, -1: not
         constexpr int kPieces = RB / 16, kCopies = (kChunk * kPieces + 31) / 32;
         // f16: 16-byte pieces asynchronously, where a lane's go: the pattern repeats every eight rows
         uint32_t to[kQuant ? 1 : kCopies / 2];
@@ -801,15 +867,16 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
         auto tell = [&](int n) {   // all but the n last ones have arrived
             if (n == 0) copies_wait<0>();
             else copies_wait<2>();
-            for (; told < h - n; told++) {
+            for (; told < asked - n; told++) {
                 const int item = __shfl_sync(0xFFFFFFFFu, tag, told & 31);
                 if (item >= 0) {
                     bool bad = false;
+#pragma unroll 1
                     for (int m = 0; m < kMine; m++)
 #pragma unroll
                         for (int j = 0; j < kCopies; j++) {
                             const uint32_t off = to[kQuant ? 0 : j % (kCopies / 2)] + (j / (kCopies / 2)) * 1024;
-                            uint4 *at = reinterpret_cast<uint4 *>(smem + told % C::kSlots * C::kSlot + (w + kChunkCopyWarps * m) * (kChunk * 128) + off);
+                            uint4 *at = reinterpret_cast<uint4 *>(smem + told_slot * C::kSlot + (w + kChunkCopyWarps * m) * (kChunk * 128) + off);
                             uint4 v = *at;
                             const bool b0 = take_out(v.x), b1 = take_out(v.y), b2 = take_out(v.z), b3 = take_out(v.w);
                             if (b0 || b1 || b2 || b3) *at = v, bad = true;
@@ -818,47 +885,52 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 }
                 async_fence();
                 __syncwarp();
-                if (lane == 0) bar_arrive(bar(meta.kv_full[told % C::kSlots]));
+                if (lane == 0) bar_arrive(bar(meta.kv_full[told_slot]));
+                if (++told_slot == C::kSlots) told_slot = 0;
             }
         };
-        while (walk.next(p)) {
-            const ChunkSeq &sq = walk.now;
-            const int32_t *table = p.table + (size_t)walk.s * p.table_width;
-            const int first_token = token_of(p, walk.block * R), last_token = token_of(p, walk.block * R + walk.n_rows - 1);
-            const int all_to = min(sq.len, sq.before + first_token + 1), all_from = p.window > 0 ? sq.before + last_token - p.window + 1 : 0;
-            auto looked_at = [&](int i) { return (walk.tile0 + i) * TP + TP > all_to || (walk.tile0 + i) * TP < all_from; };
+        for (;; n_item++, found.next()) {
+            if constexpr (!kQuant) {
+                if (!bar_test(bar(meta.item_full[found.at]), found.turn)) tell(0);   // (before the item may come others' work with these)
+            }
+            wait(meta.item_full[found.at], found.turn);
+            const ChunkItem it = meta.item[found.at];
+            __syncwarp();
+            if (lane == 0) bar_arrive(bar(meta.item_empty[found.at]));
+            if (!it.goes_on || *gave_up) break;
+            const int32_t *table = p.table + (size_t)it.s * p.table_width;
+            auto looked_at = [&](int i) { return (it.tile0 + i) * TP + TP > it.all_to || (it.tile0 + i) * TP < it.all_from; };
             auto find_rows = [&](int i) -> int64_t {
-                const int tile = i + lane / kChunks, position = (walk.tile0 + tile) * TP + lane % kChunks * kChunk;
-                if (tile >= walk.tiles || position >= sq.len) return -1;
+                const int tile = i + lane / kChunks, position = (it.tile0 + tile) * TP + lane % kChunks * kChunk;
+                if (tile >= it.all || position >= it.len) return -1;
                 const int page = table[position / p.page_size];
-                return page < 0 || page >= p.n_pages ? -1 : ((int64_t)page * p.n_kv + walk.kvh) * p.page_size + position % p.page_size;
+                return page < 0 || page >= p.n_pages ? -1 : ((int64_t)page * p.n_kv + it.kvh) * p.page_size + position % p.page_size;
             };
-            // of tile i: its rows, and which chunks there are, for the softmax. `tile_no`: of all tiles
-            auto begin_tile = [&](int i, int tile_no) {
+            // of tile i: its rows, and which chunks there are, for the softmax
+            auto begin_tile = [&](int i) {
                 if (i % kAhead == 0) pool_rows = find_rows(i);
                 const uint32_t there = __ballot_sync(0xFFFFFFFFu, pool_rows >= 0) >> (kChunks * (i % kAhead)) & ((1u << kChunks) - 1u);
-                if (w == 0 && lane == 0) meta.there[tile_no & 7] = (uint8_t)there;
+                if (w == 0 && lane == 0) meta.there[n_tile & 7] = (uint8_t)there;
+                n_tile++;
             };
             auto row_of = [&](int i, int m) { return __shfl_sync(0xFFFFFFFFu, pool_rows, kChunks * (i % kAhead) + w + kChunkCopyWarps * m); };
             if constexpr (!kQuant) {
 #pragma unroll 1
-                for (int i = 0; i < walk.tiles; i++) {
-                    begin_tile(i, h >> 1);
+                for (int i = 0; i < it.all; i++) {
+                    begin_tile(i);
 #pragma unroll 1
                     for (int kv = 0; kv < 2; kv++) {
-                        const int slot = h % C::kSlots;
-                        const uint32_t empty = bar(meta.kv_empty[slot]), parity = ((h / C::kSlots) & 1) ^ 1;
-                        if (!bar_test(empty, parity)) {
+                        if (!bar_test(bar(meta.kv_empty[to_slot.at]), to_slot.turn ^ 1)) {
                             tell(0);   // (who frees the place may wait for these)
-                            bar_wait_here(empty, parity, gave_up, p.status);
+                            wait(meta.kv_empty[to_slot.at], to_slot.turn ^ 1);
                         }
 #pragma unroll
                         for (int m = 0; m < kMine; m++) {
-                            const int chunk = w + kChunkCopyWarps * m, position = (walk.tile0 + i) * TP + chunk * kChunk;
+                            const int chunk = w + kChunkCopyWarps * m, position = (it.tile0 + i) * TP + chunk * kChunk;
                             const int64_t row0 = row_of(i, m);
-                            const int left = row0 < 0 ? 0 : sq.len - position;   // rows that are not there come in as zeros
+                            const int left = row0 < 0 ? 0 : it.len - position;   // rows that are not there come in as zeros
                             const uint8_t *src = (kv ? p.v : p.k) + row0 * RB + 16 * lane;   // (no row: not looked at, a cache without pages has no memory)
-                            const uint32_t at = base + slot * C::kSlot + chunk * (kChunk * 128);
+                            const uint32_t at = base + to_slot.at * C::kSlot + chunk * (kChunk * 128);
                             if (left >= kChunk) {
 #pragma unroll
                                 for (int j = 0; j < kCopies; j++) copy16(to[j % (kCopies / 2)] + at + (j / (kCopies / 2)) * 1024, src + 512 * j, true);
@@ -868,53 +940,54 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                             }
                         }
                         copies_commit();
-                        if (lane == (h & 31)) tag = kv && looked_at(i) ? n_item : -1;
-                        h++;
-                        if (h - told > 2) tell(2);
+                        if (lane == (asked & 31)) tag = kv && looked_at(i) ? n_item : -1;
+                        asked++;
+                        to_slot.next();
+                        if (asked - told > 2) tell(2);
                     }
                 }
             } else {
-                // 8 and 4 bits: through registers, a piece of 16 bytes at a time; a half tile's pieces are asked for while the one before it is unpacked
-                uint4 x[kMine * kCopies];
-                __half d[kMine * kCopies];
-                const int halves = 2 * walk.tiles;
-                auto piece = [&](int t, int m, int j, int64_t row0, uint4 &v, __half &scale) {
-                    const int i = t >> 1, c = lane + 32 * j, row = c / kPieces, position = (walk.tile0 + i) * TP + (w + kChunkCopyWarps * m) * kChunk + row;
-                    v = make_uint4(0u, 0u, 0u, 0u);
-                    scale = __float2half_rn(0.0f);
-                    if (row0 >= 0 && c < kChunk * kPieces && position < sq.len) {
-                        v = *reinterpret_cast<const uint4 *>((t & 1 ? p.v : p.k) + row0 * RB + 16 * c);
-                        scale = (t & 1 ? p.v_scale : p.k_scale)[(row0 + row) * (D / 32) + c % kPieces / (CT == KRK_CUDA_KV_Q8 ? 2 : 1)];
-                    }
+                // 8 and 4 bits: through registers, a piece of 16 bytes at a time; a half tile's pieces are asked for while the one before it is unpacked. What is not
+                // there comes from other rows of the page (or from the queries, without a page) under a scale of zero.
+                constexpr int kSets = kMine * kCopies;
+                uint4 x[kSets];
+                uint16_t d[kSets];
+                const int halves = 2 * it.all;
+                auto ask = [&](int t, int m, int j, int64_t row0, uint4 &v, uint16_t &scale) {
+                    const int c = lane + 32 * j, row = c / kPieces;
+                    const bool none = row0 < 0 || (kChunk * kPieces % 32 != 0 && c >= kChunk * kPieces);
+                    const uint8_t *from = none ? static_cast<const uint8_t *>(p.q) : (t & 1 ? p.v : p.k) + row0 * RB + 16 * c;
+                    const __half *s_from = none ? static_cast<const __half *>(p.q) : (t & 1 ? p.v_scale : p.k_scale) + (row0 + row) * (D / 32) + c % kPieces / (CT == KRK_CUDA_KV_Q8 ? 2 : 1);
+                    v = *reinterpret_cast<const uint4 *>(from);
+                    scale = *reinterpret_cast<const uint16_t *>(s_from);
                 };
-                begin_tile(0, h >> 1);
+                begin_tile(0);
+                int64_t rows[kMine];   // of the half tile that is unpacked
 #pragma unroll
                 for (int m = 0; m < kMine; m++) {
-                    const int64_t row0 = row_of(0, m);
+                    rows[m] = row_of(0, m);
 #pragma unroll
-                    for (int j = 0; j < kCopies; j++) piece(0, m, j, row0, x[m * kCopies + j], d[m * kCopies + j]);
+                    for (int j = 0; j < kCopies; j++) ask(0, m, j, rows[m], x[m * kCopies + j], d[m * kCopies + j]);
                 }
 #pragma unroll 1
-                for (int t = 0; t < halves; t++, h++) {
-                    const int slot = h % C::kSlots;
-                    bar_wait_here(bar(meta.kv_empty[slot]), ((h / C::kSlots) & 1) ^ 1, gave_up, p.status);
-                    const bool look = (t & 1) && looked_at(t >> 1);
+                for (int t = 0; t < halves; t++) {
+                    const int i = t >> 1;
+                    const bool look = (t & 1) && looked_at(i), more = t + 1 < halves;
                     bool bad = false;
-                    if (t + 1 < halves && (t & 1)) begin_tile((t + 1) >> 1, (h + 1) >> 1);
+                    if (more && (t & 1)) begin_tile(i + 1);
+                    wait(meta.kv_empty[to_slot.at], to_slot.turn ^ 1);
 #pragma unroll
                     for (int m = 0; m < kMine; m++) {
-                        const int64_t row0 = t + 1 < halves ? row_of((t + 1) >> 1, m) : -1;
-                        uint8_t *chunk_at = smem + slot * C::kSlot + (w + kChunkCopyWarps * m) * (kChunk * 128);
+                        const int chunk = w + kChunkCopyWarps * m, left = rows[m] < 0 ? 0 : it.len - ((it.tile0 + i) * TP + chunk * kChunk);
+                        rows[m] = more ? row_of((t + 1) >> 1, m) : -1;
+                        uint8_t *chunk_at = smem + to_slot.at * C::kSlot + chunk * (kChunk * 128);
 #pragma unroll
                         for (int j = 0; j < kCopies; j++) {
-                            const int c = lane + 32 * j, row = c / kPieces, pc = c % kPieces;
-                            uint4 v = x[m * kCopies + j];
-                            const __half2 s2 = __half2half2(d[m * kCopies + j]);
-                            if (t + 1 < halves) piece(t + 1, m, j, row0, x[m * kCopies + j], d[m * kCopies + j]);
-                            if (kChunk * kPieces % 32 != 0 && c >= kChunk * kPieces) continue;
+                            const int c = lane + 32 * j, row = c / kPieces, pc = c % kPieces, n = m * kCopies + j;
+                            const uint32_t words[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
+                            const __half2 s2 = half2_of(row < left ? d[n] * 0x10001u : 0u);
                             constexpr int kUnits = CT == KRK_CUDA_KV_Q8 ? 2 : 4;   // of eight values
                             uint32_t y[4 * kUnits];
-                            const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                             for (int k = 0; k < 4; k++) {
                                 if constexpr (CT == KRK_CUDA_KV_Q8) {
@@ -929,10 +1002,12 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                                     y[8 + 2 * k + 1] = bits(__hmul2(half2_of(halves_of<2, 3>(u2, 0x64086408u)), s2));
                                 }
                             }
+                            if (more) ask(t + 1, m, j, rows[m], x[n], d[n]);
                             if (look) {
 #pragma unroll
                                 for (int k = 0; k < 4 * kUnits; k++) bad |= take_out(y[k]);
                             }
+                            if (kChunk * kPieces % 32 != 0 && c >= kChunk * kPieces) continue;
 #pragma unroll
                             for (int k = 0; k < kUnits; k++) {
                                 const int unit = kUnits * pc + k;
@@ -944,102 +1019,131 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     if (bad) tell_odd(n_item);
                     async_fence();
                     __syncwarp();
-                    if (lane == 0) bar_arrive(bar(meta.kv_full[slot]));
+                    if (lane == 0) bar_arrive(bar(meta.kv_full[to_slot.at]));
+                    to_slot.next();
                 }
             }
-            n_item++;
         }
         if constexpr (!kQuant) tell(0);
     } else {
-        // ===== products
         if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
-        if (warp == C::kProduct) {
-        const uint32_t elected = elected_lane();
-        uint32_t n_done[2] = {0, 0}, n_item[2] = {0, 0};   // of a tile of rows: tiles so far, items
-        int h0 = 0;   // half tiles before this item
-        constexpr uint32_t qk = (1u << 4) | (uint32_t)(TP >> 3) << 17 | (128u >> 4) << 24, pv = (1u << 4) | 1u << 16 | (uint32_t)(D >> 3) << 17 | (128u >> 4) << 24;
-        while (walk.next(p)) {
-            const int n[2] = {tiles_of(walk, 0), NQ == 2 ? tiles_of(walk, 1) : 0}, all = walk.tiles;
-            auto wait_half = [&](int h) { bar_wait_here(bar(meta.kv_full[h % C::kSlots]), (h / C::kSlots) & 1, gave_up, p.status); };
-            auto place_of = [&](int q, int i) { return NQ == 2 ? q : (int)((n_done[0] + i) & 1); };
-            auto scores = [&](int q, int i) {
-                const int slot = (h0 + 2 * i) % C::kSlots, sb = place_of(q, i);
-                const uint32_t keys = base + slot * C::kSlot, rows = base + C::kQ + q * C::kQTile, d = tmem + C::kS * sb;
-                tc_after();
+        if (warp < C::kProduct + NQ) {
+            // ===== products of a tile of rows
+            const int q = warp - C::kProduct;
+            const uint32_t elected = elected_lane();
+            constexpr uint32_t qk = (1u << 4) | (uint32_t)(TP >> 3) << 17 | (128u >> 4) << 24, pv = (1u << 4) | 1u << 16 | (uint32_t)(D >> 3) << 17 | (128u >> 4) << 24;
+            const uint32_t rows = desc_lo(base + C::kQ + q * C::kQTile, 16), slots_k = desc_lo(base, 16), slots_v = desc_lo(base, TP * 128), t_o = tmem + C::kO + 128 * q;
+            uint32_t n_tile = 0, n_item = 0;    // of this tile of rows
+            Ring<kChunkItems> found;
+            Ring<C::kSlots> keys, values;   // half tiles 2 i and 2 i + 1
+            values.next();
+            auto free = [&](const Ring<C::kSlots> &r) { products_commit(bar(meta.kv_empty[r.at]), elected); };
+            auto two_on = [&](Ring<C::kSlots> &r) { r.next(), r.next(); };
+            for (;; found.next()) {
+                wait(meta.item_full[found.at], found.turn);
+                const int goes_on = meta.item[found.at].goes_on, all = meta.item[found.at].all, n = meta.item[found.at].tiles[q];
+                __syncwarp();
+                if (lane == 0) bar_arrive(bar(meta.item_empty[found.at]));
+                if (!goes_on || *gave_up) break;
+                auto place_of = [&](uint32_t t) { return NQ == 2 ? (uint32_t)q : t & 1; };
+                auto scores = [&](uint32_t t) {   // of tile t of all
+                    wait(meta.kv_full[keys.at], keys.turn);
+                    tc_after();
+                    const uint32_t at = slots_k + keys.at * (C::kSlot >> 4), d = tmem + C::kS * place_of(t);
 #pragma unroll
-                for (int t = 0; t < NT; t++)
+                    for (int term = 0; term < NT; term++)
 #pragma unroll
-                    for (int k = 0; k < D / 16; k++)
-                        product(d, desc_lo(rows + t * C::kTerm + (k >> 2) * (128 * 128) + 32 * (k & 3), 16), kDescHi, desc_lo(keys + (k >> 2) * (TP * 128) + 32 * (k & 3), 16), kDescHi, qk,
-                                t > 0 || k > 0, elected);
-                products_commit(bar(meta.s_full[sb]), elected);
-            };
-            auto sums = [&](int q, int i) {
-                const int slot = (h0 + 2 * i + 1) % C::kSlots, sb = place_of(q, i);
-                const uint32_t values = base + slot * C::kSlot, from = tmem + C::kS * sb, d = tmem + C::kO + 128 * q;
-                const uint32_t phase = (NQ == 2 ? n_done[q] + i : (n_done[0] + i) >> 1) & 1;
-                bar_wait_here(bar(meta.p_half[sb]), phase, gave_up, p.status);
-                tc_after();
-#pragma unroll
-                for (int k = 0; k < TP / 16; k++) {
-                    if (k == TP / 32) {
-                        bar_wait_here(bar(meta.p_full[sb]), phase, gave_up, p.status);
-                        tc_after();
-                    }
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-                        product_from(d, from + (NT == 2 ? 32 * (k >> 1) + 16 * t + 8 * (k & 1) : 8 * k), desc_lo(values + 2048 * k, TP * 128), kDescHi, pv, i > 0 || k > 0 || t > 0, elected);
-                }
-                products_commit(bar(meta.pv_done[q]), elected);
-            };
-            wait_half(h0);
-#pragma unroll
-            for (int q = 0; q < NQ; q++)
-                if (n[q] > 0) {
-                    bar_wait_here(bar(meta.q_full[q]), n_item[q] & 1, gave_up, p.status);
-                    scores(q, 0);
-                }
-            products_commit(bar(meta.kv_empty[h0 % C::kSlots]), elected);
-#pragma unroll 1
-            for (int i = 0; i < all; i++) {
-                const bool more = i + 1 < all;
-                if constexpr (NQ == 1) {
-                    if (more) {
-                        wait_half(h0 + 2 * i + 2);
-                        scores(0, i + 1);
-                        products_commit(bar(meta.kv_empty[(h0 + 2 * i + 2) % C::kSlots]), elected);
-                    }
-                    wait_half(h0 + 2 * i + 1);
-                    sums(0, i);
-                    products_commit(bar(meta.kv_empty[(h0 + 2 * i + 1) % C::kSlots]), elected);
-                } else {
-                    wait_half(h0 + 2 * i + 1);
-#pragma unroll
-                    for (int q = 0; q < NQ; q++) {
-                        if (i < n[q]) sums(q, i);
-                        if (q == 1) products_commit(bar(meta.kv_empty[(h0 + 2 * i + 1) % C::kSlots]), elected);
-                        if (i + 1 < n[q]) {
-                            wait_half(h0 + 2 * i + 2);
-                            scores(q, i + 1);
+                        for (int c = 0; c < D; c += 64) {
+                            const uint32_t a = rows + term * (C::kTerm >> 4) + (c >> 6) * (128 * 128 >> 4), b = at + (c >> 6) * (TP * 128 >> 4);
+                            if (D - c >= 64) products_k<4>(d, a, b, qk, term > 0 || c > 0, elected);
+                            else products_k<2>(d, a, b, qk, term > 0 || c > 0, elected);
                         }
+                    products_commit(bar(meta.s_full[place_of(t)]), elected);
+                    free(keys);
+                    two_on(keys);
+                };
+                auto sums = [&](uint32_t t, bool onto) {
+                    wait(meta.kv_full[values.at], values.turn);
+                    const uint32_t at = slots_v + values.at * (C::kSlot >> 4), from = tmem + C::kS * place_of(t), phase = (NQ == 2 ? t : t >> 1) & 1;
+#pragma unroll
+                    for (int c = 0; c < TP; c += 32) {
+                        if (c == 0) {
+                            wait(meta.p_half[place_of(t)], phase);
+                            tc_after();
+                        } else if (c == TP / 2) {
+                            wait(meta.p_full[place_of(t)], phase);
+                            tc_after();
+                        }
+                        products_p<NT>(t_o, from + c * NT / 2, at + c * 8, pv, onto || c > 0, elected);
                     }
-                    if (more) products_commit(bar(meta.kv_empty[(h0 + 2 * i + 2) % C::kSlots]), elected);
+                    products_commit(bar(meta.pv_done[q]), elected);
+                    free(values);
+                    two_on(values);
+                };
+                if (n > 0) {
+                    wait(meta.q_full[q], n_item & 1);
+                    n_item++;
+                    scores(n_tile);
+#pragma unroll 1
+                    for (int i = 0; i < n; i++) {
+                        if (NQ == 1 && i + 1 < n) scores(n_tile + i + 1);
+                        sums(n_tile + i, i > 0);
+                        if (NQ == 2 && i + 1 < n) scores(n_tile + i + 1);
+                    }
+                    n_tile += n;
+                }
+                // what only the other tile's rows see
+#pragma unroll 1
+                for (int i = n; i < all; i++) {
+                    wait(meta.kv_full[keys.at], keys.turn);
+                    free(keys);
+                    two_on(keys);
+                    wait(meta.kv_full[values.at], values.turn);
+                    free(values);
+                    two_on(values);
                 }
             }
-            h0 += 2 * all;
-#pragma unroll
-            for (int q = 0; q < 2; q++)
-                if (n[q] > 0) n_done[q] += n[q], n_item[q]++;
-        }
+        } else if (warp == C::kFinder) {
+            // ===== items
+            Walk walk;
+            walk.start(p);
+            if (!p.whole && lane == 0) p.shared[blockIdx.x].parts = 0;
+            Ring<kChunkItems> found;
+            for (;; found.next()) {
+                const bool more = walk.template next<true>(p);
+                wait(meta.item_empty[found.at], found.turn ^ 1);
+                if (*gave_up) break;
+                if (lane == 0) {
+                    ChunkItem &it = meta.item[found.at];
+                    it.goes_on = more;
+                    if (more) {
+                        const ChunkSeq &q = walk.now;
+                        const int first = walk.block * R, last = first + walk.n_rows - 1;
+                        it.q0 = q.q0, it.len = q.len, it.before = q.before, it.s = walk.s, it.kvh = walk.kvh, it.block = walk.block, it.n_rows = walk.n_rows, it.tile0 = walk.tile0, it.all = walk.tiles;
+                        it.whole = walk.begins && walk.ends, it.begins = walk.begins;
+                        it.all_to = min(q.len, q.before + token_of(p, first) + 1), it.all_from = p.window > 0 ? q.before + token_of(p, last) - p.window + 1 : 0;
+                        // tiles that rows of the first tile of rows see: they end earlier
+                        const int end = min(q.len, q.before + token_of(p, min(last, first + 127)) + 1);
+                        it.tiles[0] = min(walk.tiles, max((end + TP - 1) / TP - walk.tile0, 1));
+                        it.tiles[1] = walk.n_rows > 128 ? walk.tiles : 0;
+                        if (walk.parts > 0) walk.note(p);
+                    }
+                    bar_arrive(bar(meta.item_full[found.at]));
+                }
+                __syncwarp();
+                if (!more) break;
+            }
         }
     }
     tc_before();
     __syncthreads();
     tc_after();
-    if (warp == C::kProduct && *gave_up) {   // (nobody waits any more, so this is the last word on it)
-        products_commit(bar(meta.drained), elected_lane());
-        bar_wait_drained(bar(meta.drained));
+    if (*gave_up && warp >= C::kProduct && warp < C::kProduct + NQ) {   // (nobody waits any more, so this is the last word on it)
+        products_commit(bar(meta.drained[warp - C::kProduct]), elected_lane());
+        const long long t0 = clock64();
+        while (!bar_try(bar(meta.drained[warp - C::kProduct]), 0) && clock64() - t0 <= kWaitLimit) __nanosleep(32);
     }
+    __syncthreads();
     if (warp == C::kProduct) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
