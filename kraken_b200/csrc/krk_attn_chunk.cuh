@@ -45,6 +45,7 @@ __host__ __device__ constexpr int chunk_positions(int d) { return d <= 128 ? 128
 __host__ __device__ constexpr int chunk_rows(int d) { return 128 * chunk_tiles_of(d); }
 constexpr int kChunkSetup = 3;        // an item beside its tiles, in tiles
 constexpr int kChunkWholeTiles = 8;   // contexts of up to so many tiles of positions are not divided
+constexpr int kPolyOf8 = 2;           // f16: of eight exponentials, those by a polynomial
 constexpr float kLetBe = 8.0f;        // log2: a reference stands until a score is more than this above it
 constexpr float kUp = 128.0f, kUpLog2 = 7.0f;   // of weights: times 2^8 they stay below the f16 range
 
@@ -119,27 +120,29 @@ struct ChunkWalk {
     bool begins, ends;
 
     // (in f64, the same in every CTA and rising with b; quotients of 64 bits take a thread some 400 clocks)
-    __host__ __device__ __forceinline__ int64_t unit_of(int b) const { return b >= grid ? total : (int64_t)(per_cta * (double)b); }
-    // The tile that a border lies at, `off` units into an item of `cost`: borders near an item's ends are at them.
+    __host__ __device__ __forceinline__ int64_t unit_of(int b) const { return b >= grid ? total : min((int64_t)(per_cta * (double)b), total); }
+    // The tile that a border lies at, `off` units into an item of `cost`: borders near an item's ends are at them. (f32: off by a tile at most, of millions.)
     __host__ __device__ __forceinline__ static int tile_at(int64_t off, int64_t cost, int tiles, int whole) {
         if (whole) return 2 * off < cost ? 0 : tiles;
-        const int t = (int)((double)off / (double)cost * tiles);
+        const int t = (int)((float)off / (float)cost * (float)tiles);
         return t < 2 ? 0 : t > tiles - 2 ? tiles : t;
     }
-    __host__ __device__ __forceinline__ ChunkPlace place(const ChunkParams &p, int s, int64_t in_seq) const {
+    // Where unit in_seq of sequence s lies. On the device by a warp, whose halves may ask for two units.
+    __host__ __device__ __forceinline__ static ChunkPlace place(const ChunkParams &p, int s, int64_t in_seq) {
         ChunkPlace r;
         const ChunkSeq q = chunk_sequence<R>(p, s);
         const ChunkCost<R, TP> c = chunk_cost<R, TP>(p, q);
         r.s = s;
-        r.kvh = min((int)((double)in_seq / (double)c.head), p.n_kv - 1);
+        r.kvh = min((int)((float)in_seq / (float)c.head), p.n_kv - 1);
         if (r.kvh * c.head > in_seq) r.kvh--;
         else if (r.kvh + 1 < p.n_kv && (r.kvh + 1) * c.head <= in_seq) r.kvh++;
         const int64_t in_head = in_seq - r.kvh * c.head;
         int lo = 0;   // the last block that begins at or before it
 #ifdef __CUDA_ARCH__
-        for (int n = q.blocks; n > 1;) {   // by a warp
-            const int step = (n + 31) / 32, lane = threadIdx.x & 31, i = lane * step;
-            const int ahead = __popc(__ballot_sync(0xFFFFFFFFu, i < n && c.prefix(lo + i) <= in_head)) - 1;
+        const int lane = threadIdx.x & 31;
+        for (int n = q.blocks; __any_sync(0xFFFFFFFFu, n > 1);) {
+            const int step = (n + 15) / 16, i = (lane & 15) * step;
+            const int ahead = __popc(__ballot_sync(0xFFFFFFFFu, i < n && c.prefix(lo + i) <= in_head) >> (lane & 16) & 0xFFFFu) - 1;
             lo += ahead * step;
             n = min(step, n - ahead * step);
         }
@@ -190,29 +193,34 @@ struct ChunkWalk {
             }
             from += __shfl_sync(0xFFFFFFFFu, upto, 31);
         }
-        begin(p, found[0], before[0]);
-        if (!over && found[1] < p.n_seq) end = place(p, found[1], u[1] - before[1]);
+        ChunkPlace mine_at = {p.n_seq, 0, 0, 0};
+        if (found[0] < p.n_seq) {
+            const int half = lane >> 4, s0 = half ? found[1] : found[0];
+            const ChunkPlace r = place(p, min(s0, p.n_seq - 1), s0 < p.n_seq ? (half ? u[1] - before[1] : u[0] - before[0]) : 0);
+            mine_at = {s0, r.kvh, r.b, r.tile};
+        }
+        auto from_lane = [&](int l) {
+            return ChunkPlace{__shfl_sync(0xFFFFFFFFu, mine_at.s, l), __shfl_sync(0xFFFFFFFFu, mine_at.kvh, l), __shfl_sync(0xFFFFFFFFu, mine_at.b, l), __shfl_sync(0xFFFFFFFFu, mine_at.tile, l)};
+        };
+        begin(p, from_lane(0), from_lane(16), before[0]);
     }
     // Of CTA b, with the total of units: how many share them, and its own.
     __host__ __device__ __forceinline__ void share(const ChunkParams &p, int b) {
         // A share is longer than what an item costs beside its tiles and two tiles: no two borders lie at one tile inside an item, whose units a tile are at most
         // 4 group (TP kChunkSetup / tiles + TP + 2).
-        const int64_t least = (int64_t)4 * p.group * TP * (kChunkSetup + 3);
+        const int64_t least = (int64_t)4 * p.group * TP * (kChunkSetup + 4);
         cta = b;
-        grid = (int)fmax(fmin((double)p.grid, floor((double)total / (double)least)), 1.0);
-        per_cta = (double)total / (double)grid;
+        const int most = (int)fminf((float)p.grid, (float)total / (float)least);
+        grid = max(most, 1);
+        per_cta = (double)total * (double)(1.0f / (float)grid);   // (to f32: shares are so far from equal, and the last one ends at the total)
         first_unit = unit_of(b);
         behind_unit = unit_of(b + 1);
     }
-    // The sequence in which its first unit lies (n_seq: none), and the units before it. `end` is the place of the one behind its last.
-    __host__ __device__ __forceinline__ void begin(const ChunkParams &p, int s0, int64_t before0) {
-        over = first_unit >= behind_unit || s0 >= p.n_seq;
-        base = before0;
-        at = end = {p.n_seq, 0, 0, 0};
-        if (!over) {
-            at = place(p, s0, first_unit - before0);
-            sq = chunk_sequence<R>(p, at.s);
-        }
+    // From the places of its first unit and of the one behind its last (s n_seq: none), and the units before the first one's sequence.
+    __host__ __device__ __forceinline__ void begin(const ChunkParams &p, const ChunkPlace &from, const ChunkPlace &upto, int64_t units_before) {
+        at = from, end = upto, base = units_before;
+        over = first_unit >= behind_unit || at.s >= p.n_seq;
+        if (!over) sq = chunk_sequence<R>(p, at.s);
         first = true;
         kvh = block = s = n_rows = tile0 = tiles = parts = 0;
         begins = ends = false;
@@ -225,10 +233,22 @@ struct ChunkWalk {
         if (me == 0) return 0;
         const int64_t before = unit_of(me - 1) - from;
         if (before >= 0 && tile_at(before, cost, all, p.whole) > 0) return 0;
-        // the last border that lies in the item
-        int e = (int)min((int64_t)grid - 1, (int64_t)((double)(from + cost) / (double)total * grid) + 1);
-        while (e > me && (unit_of(e) - from >= cost || tile_at(unit_of(e) - from, cost, all, p.whole) >= all)) e--;
-        return e - me + 2;
+        // the borders behind it that lie in the item, one behind the other
+        int n = 0;
+        auto inside = [&](int e) {
+            const int64_t off = unit_of(e) - from;
+            return e < grid && off < cost && tile_at(off, cost, all, p.whole) < all;
+        };
+#ifdef __CUDA_ARCH__
+        for (int e = me + 1;; e += 32) {
+            const uint32_t some = __ballot_sync(0xFFFFFFFFu, inside(e + (int)(threadIdx.x & 31)));
+            n += __popc(some);
+            if (some != 0xFFFFFFFFu) break;
+        }
+#else
+        while (inside(me + 1 + n)) n++;
+#endif
+        return n + 2;
     }
     template <bool PARTS = false>
     __host__ __device__ __forceinline__ bool next(const ChunkParams &p) {
@@ -293,11 +313,11 @@ struct Chunk {
     static constexpr int kRoom = 227 * 1024 - 1024 - kMetaBytes - NQ * kQTile;
     static constexpr int kSlots = kRoom / kSlot > 6 ? 6 : kRoom / kSlot;
     static constexpr int kQ = kSlots * kSlot, kMeta = kQ + NQ * kQTile, kBytes = kMeta + kMetaBytes + 1024;   // (begins on a 1024-byte boundary)
-    // warps: softmax, copies, products (one for each tile of rows), the one that finds items
-    static constexpr int kSoft = 4 * NQ, kProduct = kSoft + kChunkCopyWarps, kFinder = kProduct + 2, kWarps = kProduct + 4, kThreads = 32 * kWarps;
+    // warps: softmax, copies, products, the one that finds items
+    static constexpr int kSoft = 4 * NQ, kProduct = kSoft + kChunkCopyWarps, kFinder = kProduct + 1, kWarps = kProduct + 4, kThreads = 32 * kWarps;
     // registers of a thread: 512 threads are launched with 128 each; the copies unpack 8 and 4 bits in theirs
-    static constexpr int kSoftRegs = QUANT ? 168 : 184, kOtherRegs = QUANT ? 88 : 72;
-    static_assert(256 * kSoftRegs + 256 * kOtherRegs <= 65536, "registers of a launch");
+    static constexpr int kSoftRegs = QUANT ? 168 : 184, kCopyRegs = QUANT ? 112 : 72, kOtherRegs = QUANT ? 64 : 72;
+    static_assert(256 * kSoftRegs + 128 * (kCopyRegs + kOtherRegs) <= 65536, "registers of a launch");
     static constexpr uint32_t kO = 256;                              // column of the sums; of the second tile's: 128 more
     static constexpr uint32_t kS = NQ == 2 ? 128 : 64;               // from a place of scores to the next
     static_assert(kSlots >= 3, "a half tile of values and one of keys at work, one on its way");
@@ -312,7 +332,7 @@ struct ChunkItem {
 constexpr int kChunkItems = 3;   // found ahead
 template <int R>
 struct ChunkMeta {
-    unsigned long long kv_full[6], kv_empty[6], s_full[2], p_half[2], p_full[2], pv_done[2], q_full[2], item_full[kChunkItems], item_empty[kChunkItems], drained[2];
+    unsigned long long kv_full[6], kv_empty[6], s_full[2], p_half[2], p_full[2], pv_done[2], q_full[2], item_full[kChunkItems], item_empty[kChunkItems], drained;
     float scale[R];
     uint32_t odd[2][8];       // of a tile of rows, an item in turn: values of a tile that not all rows see are no numbers
     uint8_t there[8];         // of a tile of positions, in turn: bit c: chunk c is a page's
@@ -414,6 +434,14 @@ __device__ __forceinline__ float capped_here(float x, float cap) {
     }
     return cap * (1.44269504f * t);
 }
+// 2^x to 7.5e-5 of itself (x up to 15; an f16 weight's rounding is 2.4e-4 on average): the whole part goes to the exponent, the rest, in +-1/2, to the polynomial of
+// third degree whose greatest relative error is least. Below 2^-40 it is 2^-40, which f16 does not hold; a NaN stays one.
+__device__ __forceinline__ float exp2_poly(float x) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-40.0f));
+    const float t = x + 12582912.0f, r = x - (t - 12582912.0f);   // 1.5 * 2^23: to whole numbers
+    const float y = fmaf(fmaf(fmaf(0.055171668f, r, 0.242611122f), r, 0.693260986f), r, 0.999928074f);
+    return __int_as_float(__float_as_int(y) + (__float_as_int(t) << 23));
+}
 // A value of a cache as f16 products see it, by a slow path.
 template <int CT, int D>
 __device__ __forceinline__ float value_at(const uint8_t *pool, const __half *scale, int64_t row, int c) {
@@ -498,7 +526,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
         if (lane == 0) {
             for (int i = 0; i < C::kSlots; i++) {
                 bar_init(bar(meta.kv_full[i]), kChunkCopyWarps);
-                bar_init(bar(meta.kv_empty[i]), NQ);
+                bar_init(bar(meta.kv_empty[i]), 1);
             }
             for (int i = 0; i < 2; i++) {
                 bar_init(bar(meta.s_full[i]), 1);
@@ -506,11 +534,11 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 bar_init(bar(meta.p_full[i]), 4);
                 bar_init(bar(meta.pv_done[i]), 1);
                 bar_init(bar(meta.q_full[i]), 4);
-                bar_init(bar(meta.drained[i]), 1);
             }
+            bar_init(bar(meta.drained), 1);
             for (int i = 0; i < kChunkItems; i++) {
                 bar_init(bar(meta.item_full[i]), 1);
-                bar_init(bar(meta.item_empty[i]), 2 * NQ + kChunkCopyWarps);
+                bar_init(bar(meta.item_empty[i]), NQ + kChunkCopyWarps + 1);
             }
             meta.gave_up = 0;
         }
@@ -742,10 +770,14 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     uint32_t w[NT * 16];
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
-                        float a = ex2(fmaf(__uint_as_float(v[c + j]), f, less)), b = ex2(fmaf(__uint_as_float(v[c + j + 1]), f, less));
+                        float a = fmaf(__uint_as_float(v[c + j]), f, less), b = fmaf(__uint_as_float(v[c + j + 1]), f, less);
                         if constexpr (HALF) {
+                            // (the exponential unit takes a warp eight clocks a value, as long as the products of one tile of rows: some go another way)
+                            if (j % 8 < kPolyOf8) a = exp2_poly(a), b = exp2_poly(b);
+                            else a = ex2(a), b = ex2(b);
                             w[j / 2] = bits(__floats2half2_rn(a, b));
                         } else {
+                            a = ex2(a), b = ex2(b);
                             a *= kUp, b *= kUp;   // (in the exponent it would take bits of the greatest ones)
                             split(a, b, w[j / 2], w[16 + j / 2]);
                         }
@@ -836,7 +868,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
         }
     } else if (warp < C::kProduct) {
         // ===== keys and values into a ring of half tiles (keys, values in turn); a warp has the chunks w, w + 4 of 16 positions
-        if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+        if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kCopyRegs));
         constexpr int kMine = kChunks / kChunkCopyWarps, kAhead = 32 / kChunks;   // chunks of a warp; tiles whose rows the lanes hold
         const int w = warp - C::kSoft;
         int n_item = 0, n_tile = 0;
@@ -1027,81 +1059,91 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
         if constexpr (!kQuant) tell(0);
     } else {
         if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
-        if (warp < C::kProduct + NQ) {
-            // ===== products of a tile of rows
-            const int q = warp - C::kProduct;
+        if (warp == C::kProduct) {
+            // ===== products, of the two tiles of rows in turn: while one is in its softmax the other one's run. (A warp each: both came to be in their softmax, and
+            // both waited for products, at the same time.)
             const uint32_t elected = elected_lane();
             constexpr uint32_t qk = (1u << 4) | (uint32_t)(TP >> 3) << 17 | (128u >> 4) << 24, pv = (1u << 4) | 1u << 16 | (uint32_t)(D >> 3) << 17 | (128u >> 4) << 24;
-            const uint32_t rows = desc_lo(base + C::kQ + q * C::kQTile, 16), slots_k = desc_lo(base, 16), slots_v = desc_lo(base, TP * 128), t_o = tmem + C::kO + 128 * q;
-            uint32_t n_tile = 0, n_item = 0;    // of this tile of rows
+            const uint32_t rows = desc_lo(base + C::kQ, 16), slots_k = desc_lo(base, 16), slots_v = desc_lo(base, TP * 128), t_o = tmem + C::kO;
+            uint32_t n_tile[2] = {0, 0}, n_item[2] = {0, 0};   // of a tile of rows
             Ring<kChunkItems> found;
             Ring<C::kSlots> keys, values;   // half tiles 2 i and 2 i + 1
             values.next();
-            auto free = [&](const Ring<C::kSlots> &r) { products_commit(bar(meta.kv_empty[r.at]), elected); };
-            auto two_on = [&](Ring<C::kSlots> &r) { r.next(), r.next(); };
+            auto free = [&](Ring<C::kSlots> &r) {
+                products_commit(bar(meta.kv_empty[r.at]), elected);
+                r.next(), r.next();
+            };
+            auto place_of = [&](int q, uint32_t t) { return NQ == 2 ? (uint32_t)q : t & 1; };
+            auto scores = [&](int q, uint32_t t) {   // of the t-th tile of all
+                const uint32_t at = slots_k + keys.at * (C::kSlot >> 4), d = tmem + C::kS * place_of(q, t);
+#pragma unroll
+                for (int term = 0; term < NT; term++)
+#pragma unroll
+                    for (int c = 0; c < D; c += 64) {
+                        const uint32_t a = rows + q * (C::kQTile >> 4) + term * (C::kTerm >> 4) + (c >> 6) * (128 * 128 >> 4), b = at + (c >> 6) * (TP * 128 >> 4);
+                        if (D - c >= 64) products_k<4>(d, a, b, qk, term > 0 || c > 0, elected);
+                        else products_k<2>(d, a, b, qk, term > 0 || c > 0, elected);
+                    }
+                products_commit(bar(meta.s_full[place_of(q, t)]), elected);
+            };
+            auto sums = [&](int q, uint32_t t, bool onto) {
+                const uint32_t at = slots_v + values.at * (C::kSlot >> 4), from = tmem + C::kS * place_of(q, t), phase = (NQ == 2 ? t : t >> 1) & 1;
+#pragma unroll
+                for (int c = 0; c < TP; c += 32) {
+                    if (c == 0) {
+                        wait(meta.p_half[place_of(q, t)], phase);
+                        tc_after();
+                    } else if (c == TP / 2) {
+                        wait(meta.p_full[place_of(q, t)], phase);
+                        tc_after();
+                    }
+                    products_p<NT>(t_o + 128 * q, from + c * NT / 2, at + c * 8, pv, onto || c > 0, elected);
+                }
+                products_commit(bar(meta.pv_done[q]), elected);
+            };
+            auto keys_there = [&] { wait(meta.kv_full[keys.at], keys.turn); };
+            auto values_there = [&] { wait(meta.kv_full[values.at], values.turn); };
             for (;; found.next()) {
                 wait(meta.item_full[found.at], found.turn);
-                const int goes_on = meta.item[found.at].goes_on, all = meta.item[found.at].all, n = meta.item[found.at].tiles[q];
+                const int goes_on = meta.item[found.at].goes_on, all = meta.item[found.at].all, n[2] = {meta.item[found.at].tiles[0], NQ == 2 ? meta.item[found.at].tiles[1] : 0};
                 __syncwarp();
                 if (lane == 0) bar_arrive(bar(meta.item_empty[found.at]));
                 if (!goes_on || *gave_up) break;
-                auto place_of = [&](uint32_t t) { return NQ == 2 ? (uint32_t)q : t & 1; };
-                auto scores = [&](uint32_t t) {   // of tile t of all
-                    wait(meta.kv_full[keys.at], keys.turn);
-                    tc_after();
-                    const uint32_t at = slots_k + keys.at * (C::kSlot >> 4), d = tmem + C::kS * place_of(t);
+                keys_there();
 #pragma unroll
-                    for (int term = 0; term < NT; term++)
-#pragma unroll
-                        for (int c = 0; c < D; c += 64) {
-                            const uint32_t a = rows + term * (C::kTerm >> 4) + (c >> 6) * (128 * 128 >> 4), b = at + (c >> 6) * (TP * 128 >> 4);
-                            if (D - c >= 64) products_k<4>(d, a, b, qk, term > 0 || c > 0, elected);
-                            else products_k<2>(d, a, b, qk, term > 0 || c > 0, elected);
-                        }
-                    products_commit(bar(meta.s_full[place_of(t)]), elected);
-                    free(keys);
-                    two_on(keys);
-                };
-                auto sums = [&](uint32_t t, bool onto) {
-                    wait(meta.kv_full[values.at], values.turn);
-                    const uint32_t at = slots_v + values.at * (C::kSlot >> 4), from = tmem + C::kS * place_of(t), phase = (NQ == 2 ? t : t >> 1) & 1;
-#pragma unroll
-                    for (int c = 0; c < TP; c += 32) {
-                        if (c == 0) {
-                            wait(meta.p_half[place_of(t)], phase);
-                            tc_after();
-                        } else if (c == TP / 2) {
-                            wait(meta.p_full[place_of(t)], phase);
-                            tc_after();
-                        }
-                        products_p<NT>(t_o, from + c * NT / 2, at + c * 8, pv, onto || c > 0, elected);
+                for (int q = 0; q < NQ; q++)
+                    if (n[q] > 0) {
+                        wait(meta.q_full[q], n_item[q]++ & 1);
+                        tc_after();
+                        scores(q, n_tile[q]);
                     }
-                    products_commit(bar(meta.pv_done[q]), elected);
-                    free(values);
-                    two_on(values);
-                };
-                if (n > 0) {
-                    wait(meta.q_full[q], n_item & 1);
-                    n_item++;
-                    scores(n_tile);
+                free(keys);
 #pragma unroll 1
-                    for (int i = 0; i < n; i++) {
-                        if (NQ == 1 && i + 1 < n) scores(n_tile + i + 1);
-                        sums(n_tile + i, i > 0);
-                        if (NQ == 2 && i + 1 < n) scores(n_tile + i + 1);
+                for (int i = 0; i < all; i++) {
+                    const bool more = i + 1 < all;
+                    if constexpr (NQ == 1) {
+                        if (more) {
+                            keys_there();
+                            tc_after();
+                            scores(0, n_tile[0] + i + 1);
+                            free(keys);
+                        }
+                        values_there();
+                        sums(0, n_tile[0] + i, i > 0);
+                    } else {
+                        values_there();
+#pragma unroll
+                        for (int q = 0; q < NQ; q++) {
+                            if (i < n[q]) sums(q, n_tile[q] + i, i > 0);
+                            if (q == 0 && more) keys_there();
+                            if (i + 1 < n[q]) scores(q, n_tile[q] + i + 1);
+                        }
+                        if (more) free(keys);
                     }
-                    n_tile += n;
-                }
-                // what only the other tile's rows see
-#pragma unroll 1
-                for (int i = n; i < all; i++) {
-                    wait(meta.kv_full[keys.at], keys.turn);
-                    free(keys);
-                    two_on(keys);
-                    wait(meta.kv_full[values.at], values.turn);
                     free(values);
-                    two_on(values);
                 }
+#pragma unroll
+                for (int q = 0; q < NQ; q++) n_tile[q] += n[q];
             }
         } else if (warp == C::kFinder) {
             // ===== items
@@ -1138,12 +1180,11 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
     tc_before();
     __syncthreads();
     tc_after();
-    if (*gave_up && warp >= C::kProduct && warp < C::kProduct + NQ) {   // (nobody waits any more, so this is the last word on it)
-        products_commit(bar(meta.drained[warp - C::kProduct]), elected_lane());
+    if (warp == C::kProduct && *gave_up) {   // (nobody waits any more, so this is the last word on it)
+        products_commit(bar(meta.drained), elected_lane());
         const long long t0 = clock64();
-        while (!bar_try(bar(meta.drained[warp - C::kProduct]), 0) && clock64() - t0 <= kWaitLimit) __nanosleep(32);
+        while (!bar_try(bar(meta.drained), 0) && clock64() - t0 <= kWaitLimit) __nanosleep(32);
     }
-    __syncthreads();
     if (warp == C::kProduct) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 

@@ -65,8 +65,8 @@ static void check_plan(const std::vector<int> &count, const std::vector<int> &le
             return p.n_seq;
         };
         const int s0 = find(w.first_unit), s1 = find(w.behind_unit);
-        w.begin(p, s0, before[s0]);
-        if (!w.over && s1 < p.n_seq) w.end = w.place(p, s1, w.behind_unit - before[s1]);
+        const ChunkPlace none = {p.n_seq, 0, 0, 0};
+        w.begin(p, s0 < p.n_seq ? w.place(p, s0, w.first_unit - before[s0]) : none, s1 < p.n_seq ? w.place(p, s1, w.behind_unit - before[s1]) : none, before[s0]);
         int items = 0;
         bool went_on = false;
         while (w.template next<true>(p)) {
