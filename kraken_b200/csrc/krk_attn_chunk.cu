@@ -18,7 +18,7 @@ chunk_merge_kernel(const __grid_constant__ ChunkParams p) {
     if (it.parts == 0) return;
     constexpr size_t kPitch = (size_t)2 * R * (D + 2);   // from a CTA's parts to the next one's
     for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < it.n_rows; r += gridDim.y * 4) {
-        const float *first = p.part + (size_t)(b - 1) * kPitch + (size_t)(R + r) * (D + 2), *others = p.part + (size_t)(b - 1) * kPitch + (size_t)r * (D + 2);
+        const float *others = p.part + (size_t)(b - 1) * kPitch, *first = others + (size_t)R * (D + 2);   // of part 0, of the others
         float x[NB], m = -INFINITY, l = 0.0f;
 #pragma unroll
         for (int c = 0; c < NB; c++) x[c] = 0.0f;
@@ -27,8 +27,8 @@ chunk_merge_kernel(const __grid_constant__ ChunkParams p) {
             const float *from = i == 0 ? first : others + i * kPitch;
             float y[NB];
 #pragma unroll
-            for (int c = 0; c < NB; c++) y[c] = from[32 * c + lane];
-            const float2 ml = *reinterpret_cast<const float2 *>(from + D);
+            for (int c = 0; c < NB; c++) y[c] = from[r * D + 32 * c + lane];
+            const float2 ml = reinterpret_cast<const float2 *>(from + R * D)[r];
             if (ml.x == -INFINITY) continue;
             const float top = fmaxf(m, ml.x), old = m == -INFINITY ? 0.0f : exp2f(m - top), now = exp2f(ml.x - top);
             m = top;
@@ -51,6 +51,37 @@ chunk_merge_kernel(const __grid_constant__ ChunkParams p) {
             else static_cast<float *>(p.out)[to + 32 * c] = x[c] * f;
         }
     }
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {   // looked up once: the library does not link the driver
+    static const EncodeTiled fn = [] {
+        void *ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) ptr = nullptr;
+        return reinterpret_cast<EncodeTiled>(ptr);
+    }();
+    return fn;
+}
+// The rows of an f16 pool, in boxes of 64 values (the 128-byte swizzle) of as many positions of a tile as lie in one page.
+bool encode_pools(ChunkParams &p, int d) {
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return false;
+    p.box_rows = chunk_positions(d);
+    while (p.page_size % p.box_rows) p.box_rows /= 2;
+    // (a cache without pages has no memory: a row of the queries, which no copy names)
+    const int64_t rows = p.n_pages * p.n_kv * p.page_size;
+    p.pool_rows = (int)(rows > 0 ? rows : 1);
+    for (int kv = 0; kv < 2; kv++) {
+        const cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)p.pool_rows}, strides[1] = {(cuuint64_t)(2 * d)};
+        const cuuint32_t box[2] = {64, (cuuint32_t)p.box_rows}, step[2] = {1, 1};
+        const void *from = rows > 0 ? static_cast<const void *>(kv ? p.v : p.k) : p.q;
+        if (encode(kv ? &p.v_map : &p.k_map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(from), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return false;
+    }
+    return true;
 }
 
 int launch_chunk_merge(const ChunkParams &p, int d, bool half, int rows, cudaStream_t st) {
@@ -80,7 +111,7 @@ ChunkForm form_of(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, i
     const int64_t items = (int64_t)a.n_seq * cache.n_kv_heads * blocks, units = f.whole ? items : items * ((a.max_kv_len + tp - 1) / tp);
     f.grid = (int)(units < sm_count() ? units : sm_count());
     f.rows = (int)(rows < r ? rows : r);
-    f.bytes = f.whole ? 0 : shared_bytes(f.grid) + (size_t)f.grid * 2 * r * (d + 2) * sizeof(float);
+    f.bytes = f.whole ? 0 : shared_bytes(f.grid) + 32 + (size_t)f.grid * 2 * r * (d + 2) * sizeof(float);
     return f;
 }
 // One piece of 64 tokens of every sequence that has so many is a sequence of tree attention.
@@ -113,13 +144,15 @@ int launch_attention_chunk(void *out, int out_dtype, const void *q, int q_dtype,
     p.table = static_cast<const int32_t *>(a.page_table), p.q_start = static_cast<const int32_t *>(a.q_start), p.kv_len = static_cast<const int32_t *>(a.kv_len);
     p.sinks = static_cast<const float *>(a.sinks);
     p.shared = static_cast<attn::Shared *>(workspace);
-    p.part = f.whole ? nullptr : reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + attn::shared_bytes(f.grid));
+    p.part = f.whole ? nullptr : reinterpret_cast<float *>((reinterpret_cast<uintptr_t>(workspace) + attn::shared_bytes(f.grid) + 31) & ~(uintptr_t)31);
     p.n_pages = cache.n_pages, p.table_width = a.table_width, p.page_size = cache.page_size, p.max_len = (int)a.max_kv_len, p.n_seq = a.n_seq, p.n_heads = a.n_heads;
     p.n_kv = cache.n_kv_heads, p.group = a.n_heads / cache.n_kv_heads, p.max_q = a.max_q, p.window = a.window, p.whole = f.whole, p.grid = f.grid;
+    p.out_wide = (reinterpret_cast<uintptr_t>(out) | (uintptr_t)(a.out_stride * (out_dtype == KRK_CUDA_X_F16 ? 2 : 4))) % 32 == 0;
     p.q_half = q_dtype == KRK_CUDA_X_F16, p.out_half = out_dtype == KRK_CUDA_X_F16, p.scale = a.scale, p.softcap = a.softcap;
     attn::divide_by(p.group, p.group_mul, p.group_shift);
     p.status = device_status_word();
     if (!p.status) return KRK_CUDA_EDEVICE;
+    if (cache.type == KRK_CUDA_KV_F16 && !attn::encode_pools(p, d)) return KRK_CUDA_ELAUNCH;
     // units of work are counted in 64 bits
     const double blocks = ((double)a.max_q * p.group + r - 1) / r, all = (double)a.n_seq * p.n_kv * blocks * 4.0 * p.group * ((double)a.max_kv_len + 2.0 * r + 1024.0);
     if (all > 4e18) return KRK_CUDA_ESHAPE;

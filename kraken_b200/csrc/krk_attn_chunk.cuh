@@ -9,6 +9,8 @@
 // products of the other one run. Keys and values lie in shared memory in the 128-byte swizzle, keys as rows (K-major), values read across (MN-major).
 #pragma once
 
+#include <cuda.h>
+
 #include "krk_attn_wide.cuh"
 
 namespace krk_cuda {
@@ -23,12 +25,15 @@ struct ChunkParams {
     const int32_t *table, *q_start, *kv_len;
     const float *sinks;
     Shared *shared;                       // [grid]
-    float *part;                          // [grid][2][R][D + 2]
+    float *part;                          // [grid][2]: sums [R][D], maxima (log2) and weights [R][2], on 32-byte boundaries
     int64_t n_pages;
-    int table_width, page_size, max_len, n_seq, n_heads, n_kv, group, max_q, window, whole, grid, q_half, out_half;
+    int table_width, page_size, max_len, n_seq, n_heads, n_kv, group, max_q, window, whole, grid, q_half, out_half, out_wide;   // out_wide: rows of out begin on 32-byte boundaries
     uint32_t group_mul, group_shift;      // row / group = row * group_mul >> group_shift, rows below 2^30
     float scale, softcap;
     int *status;
+    // f16 caches: the pool's rows as boxes of 64 values of box_rows positions, a part of one page; behind the last row zeros come in
+    int box_rows, pool_rows;
+    alignas(64) CUtensorMap k_map, v_map;
 };
 // n / d for n below 2^31: with 2^(s - 1) < d <= 2^s the factor ceil(2^(31 + s) / d) is less than one above the quotient, which n times it is at most 2^31 off.
 inline void divide_by(int d, uint32_t &mul, uint32_t &shift) {
@@ -39,7 +44,6 @@ inline void divide_by(int d, uint32_t &mul, uint32_t &shift) {
 }
 __host__ __device__ __forceinline__ int token_of(const ChunkParams &p, int row) { return (int)(((uint64_t)(uint32_t)row * p.group_mul) >> p.group_shift); }
 
-constexpr int kChunkCopyWarps = 4;
 __host__ __device__ constexpr int chunk_tiles_of(int d) { return d <= 128 ? 2 : 1; }           // of rows, 128 each
 __host__ __device__ constexpr int chunk_positions(int d) { return d <= 128 ? 128 : 64; }       // of a tile
 __host__ __device__ constexpr int chunk_rows(int d) { return 128 * chunk_tiles_of(d); }
@@ -309,15 +313,17 @@ struct Chunk {
     static constexpr int kMetaBytes = 1920;
     static constexpr int kPanels = (D + 63) / 64;                    // blocks of 64 values
     static constexpr int kTerm = kPanels * 128 * 128, kQTile = NT * kTerm;
+    static constexpr int kQSets = NT == 1 ? 2 : 1, kQSet = NQ * kQTile;   // the queries of this item and, where there is room, of the next one
     static constexpr int kSlot = kPanels * TP * 128;                 // half a tile: keys or values
-    static constexpr int kRoom = 227 * 1024 - 1024 - kMetaBytes - NQ * kQTile;
+    static constexpr int kRoom = 227 * 1024 - 1024 - kMetaBytes - kQSets * kQSet;
     static constexpr int kSlots = kRoom / kSlot > 6 ? 6 : kRoom / kSlot;
-    static constexpr int kQ = kSlots * kSlot, kMeta = kQ + NQ * kQTile, kBytes = kMeta + kMetaBytes + 1024;   // (begins on a 1024-byte boundary)
+    static constexpr int kQ = kSlots * kSlot, kMeta = kQ + kQSets * kQSet, kBytes = kMeta + kMetaBytes + 1024;   // (begins on a 1024-byte boundary)
     // warps: softmax, copies, products, the one that finds items
-    static constexpr int kSoft = 4 * NQ, kProduct = kSoft + kChunkCopyWarps, kFinder = kProduct + 1, kWarps = kProduct + 4, kThreads = 32 * kWarps;
-    // registers of a thread: 512 threads are launched with 128 each; the copies unpack 8 and 4 bits in theirs
-    static constexpr int kSoftRegs = QUANT ? 168 : 184, kCopyRegs = QUANT ? 112 : 72, kOtherRegs = QUANT ? 64 : 72;
-    static_assert(256 * kSoftRegs + 128 * (kCopyRegs + kOtherRegs) <= 65536, "registers of a launch");
+    static constexpr int kSoft = 4 * NQ, kCopies = QUANT ? 4 : 2, kProduct = kSoft + kCopies, kFinder = kProduct + 1, kWarps = kSoft + (QUANT ? 8 : 4), kThreads = 32 * kWarps;
+    // Registers of a thread, traded between groups of four warps (a spill goes to level 2: shared memory has what level 1 had). Launched with: 384 threads 168, 512 128.
+    static constexpr bool kTrade = NQ == 2;
+    static constexpr int kSoftRegs = QUANT ? 168 : 200, kCopyRegs = 104, kOtherRegs = QUANT ? 72 : 104;
+    static_assert(256 * kSoftRegs + 128 * (kCopyRegs + (QUANT ? kOtherRegs : 0)) <= (QUANT ? 512 * 128 : 384 * 168) , "registers of a launch");
     static constexpr uint32_t kO = 256;                              // column of the sums; of the second tile's: 128 more
     static constexpr uint32_t kS = NQ == 2 ? 128 : 64;               // from a place of scores to the next
     static_assert(kSlots >= 3, "a half tile of values and one of keys at work, one on its way");
@@ -327,13 +333,12 @@ struct Chunk {
 
 struct ChunkItem {
     int goes_on, q0, len, before, s, kvh, block, n_rows, tile0, all, tiles[2], all_from, all_to;   // all: its tiles, tiles: that the rows of a tile see; every row sees [all_from, all_to)
+    int rows_from[2], rows_to[2];   // every row of a tile of rows sees [rows_from, rows_to)
     bool whole, begins;
 };
 constexpr int kChunkItems = 3;   // found ahead
-template <int R>
 struct ChunkMeta {
-    unsigned long long kv_full[6], kv_empty[6], s_full[2], p_half[2], p_full[2], pv_done[2], q_full[2], item_full[kChunkItems], item_empty[kChunkItems], drained;
-    float scale[R];
+    unsigned long long kv_full[6], kv_empty[6], s_full[2], p_half[2], p_full[2], pv_done[2], q_full[2][2], q_empty[2], item_full[kChunkItems], item_empty[kChunkItems], drained;
     uint32_t odd[2][8];       // of a tile of rows, an item in turn: values of a tile that not all rows see are no numbers
     uint8_t there[8];         // of a tile of positions, in turn: bit c: chunk c is a page's
     uint32_t tmem;
@@ -365,6 +370,12 @@ __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t *v) {
                    "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]),
                    "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
 }
+__device__ __forceinline__ bool take_out(uint32_t &x) {   // of two f16, those that are no numbers
+    bool bad = false;
+    if ((x & 0x7C00u) == 0x7C00u) x &= 0xFFFF0000u, bad = true;
+    if ((x & 0x7C000000u) == 0x7C000000u) x &= 0xFFFFu, bad = true;
+    return bad;
+}
 // As bar_wait, without a call: a kernel whose warps trade registers has none.
 __device__ __forceinline__ void bar_wait_here(uint32_t bar, uint32_t parity, volatile int *gave_up, int *status) {
     if (bar_try(bar, parity)) return;
@@ -375,6 +386,20 @@ __device__ __forceinline__ void bar_wait_here(uint32_t bar, uint32_t parity, vol
             *gave_up = 1;
             atomicExch(status, KRK_CUDA_ETIMEOUT);
         }
+}
+__device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t *v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+// 32 bytes of a thread: a sector (wide: on its boundary).
+__device__ __forceinline__ void store32(void *to, const uint32_t *w, int wide) {
+    if (wide)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                     ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+    else {
+        reinterpret_cast<uint4 *>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4 *>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
 }
 // N products over 16 values each, both operands from shared memory; the next 16 values are 32 bytes on. Executed as `product`.
 template <int N>
@@ -473,7 +498,7 @@ __device__ __forceinline__ void soft_limit(uint32_t t_s, float sc, float cap) {
 // Values that are no numbers, in tiles that not all rows of an item see, were taken out of the products: here they are, for the rows that see them. A thread's
 // row sees [pos0, end); tiles that every row sees were left as they are.
 template <int CT, int D, int TP>
-__device__ __forceinline__ void add_odd(const ChunkParams &p, const ChunkItem &it, uint32_t t_o, int pos0, int end) {
+__device__ __forceinline__ void add_odd(const ChunkParams &p, const volatile ChunkItem &it, uint32_t t_o, int pos0, int end) {
 #pragma unroll 1
     for (int c = 0; c < D; c += 16) {
         uint32_t o[16];
@@ -514,7 +539,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
     extern __shared__ uint8_t raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t base = smem_addr(smem);
-    using Meta = ChunkMeta<R>;
+    using Meta = ChunkMeta;
     static_assert(sizeof(Meta) <= C::kMetaBytes, "Chunk::kMeta");
     Meta &meta = *reinterpret_cast<Meta *>(smem + C::kMeta);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -522,10 +547,12 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
     auto bar = [&](unsigned long long &b) { return smem_addr(&b); };
     auto wait = [&](unsigned long long &b, uint32_t parity) { bar_wait_here(bar(b), parity, gave_up, p.status); };
 
+    // f16 queries enter as they are, and are copied ahead
+    const bool as_they_are = HALF && p.q_half && p.scale >= 0.0f;
     if (warp == 0) {
         if (lane == 0) {
             for (int i = 0; i < C::kSlots; i++) {
-                bar_init(bar(meta.kv_full[i]), kChunkCopyWarps);
+                bar_init(bar(meta.kv_full[i]), kQuant ? C::kCopies : 1);
                 bar_init(bar(meta.kv_empty[i]), 1);
             }
             for (int i = 0; i < 2; i++) {
@@ -533,12 +560,13 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 bar_init(bar(meta.p_half[i]), 4);
                 bar_init(bar(meta.p_full[i]), 4);
                 bar_init(bar(meta.pv_done[i]), 1);
-                bar_init(bar(meta.q_full[i]), 4);
+                for (int j = 0; j < 2; j++) bar_init(bar(meta.q_full[i][j]), as_they_are ? (kQuant ? C::kCopies : 1) : 4);   // [set][tile of rows]
+                bar_init(bar(meta.q_empty[i]), 1);
             }
             bar_init(bar(meta.drained), 1);
             for (int i = 0; i < kChunkItems; i++) {
                 bar_init(bar(meta.item_full[i]), 1);
-                bar_init(bar(meta.item_empty[i]), NQ + kChunkCopyWarps + 1);
+                bar_init(bar(meta.item_empty[i]), NQ + C::kCopies + 1);
             }
             meta.gave_up = 0;
         }
@@ -560,10 +588,9 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
 
     if (warp < C::kSoft) {
         // ===== softmax: thread = row
-        if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
+        if constexpr (C::kTrade) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
         const int tq = warp >> 2, r_in = tid & 127, quarter = warp & 3;
         const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16), t_o = t_lane + C::kO + 128 * tq;
-        uint8_t *q_tile = smem + C::kQ + tq * C::kQTile;
         uint32_t n_tile = 0, n_item = 0, n_all = 0;   // tiles of this tile of rows, items, tiles of all items
         Ring<kChunkItems> found;
         for (;; n_item++, found.next()) {
@@ -575,145 +602,111 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 bar_arrive(bar(meta.item_empty[found.at]));
             }
             group_sync(tq);
-            const ChunkItem &it = meta.mine[tq];
+            // (read again where it is wanted, not kept beside a tile's scores: registers)
+            const volatile ChunkItem &it = meta.mine[tq];
             if (!it.goes_on) break;
-            const int n_rows = it.n_rows, tiles = it.tiles[tq], tile0 = it.tile0, before = it.before, len = it.len, kvh = it.kvh, q0 = it.q0;
-            const int row0 = it.block * R + 128 * tq;   // among the key head's
-            const int mine_rows = min(128, n_rows - 128 * tq);
-            const uint32_t n_before = n_all;
+            const int tiles = it.tiles[tq];
             n_all += it.all;
-            if (mine_rows <= 0) {
+            if (it.n_rows <= 128 * tq) {
                 group_sync(tq);
                 continue;
             }
-            // ---- queries. f16 ones as they are, else under a power of two of their row: the largest value in [2^10, 2^11)
-            const float sign = p.scale < 0.0f ? -1.0f : 1.0f, row_scale = fabsf(p.scale) * (p.softcap > 0.0f ? 1.0f : 1.44269504f);
-            // (a row's place in q, and in the tile of shared memory)
-            auto q_at = [&](int r) {
-                const int i = token_of(p, row0 + r);
-                return (int64_t)(q0 + i) * p.q_stride + (int64_t)(kvh * p.group + row0 + r - i * p.group) * D;
-            };
-            auto power_of = [](float most) { return most > 0.0f && most <= 3.4028234e38f ? 10 - max((int)(__float_as_uint(most) >> 23) - 127, -110) : 0; };
-            auto put = [&](int r, int d, const float (&x)[4], int e) {   // four values of a row, under 2^e
-                const float up = sign * __uint_as_float((uint32_t)(127 + e) << 23);
-                uint32_t hi[2], lo[2];
-                split(x[0] * up, x[1] * up, hi[0], lo[0]);
-                split(x[2] * up, x[3] * up, hi[1], lo[1]);
-                uint8_t *to = q_tile + (d >> 6) * (128 * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + 2 * (d & 7);
-                *reinterpret_cast<uint2 *>(to) = make_uint2(hi[0], hi[1]);
-                if constexpr (NT == 2) *reinterpret_cast<uint2 *>(to + C::kTerm) = make_uint2(lo[0], lo[1]);
-            };
-            constexpr int NL = (D + 127) / 128;
-            const bool as_they_are = HALF && p.q_half && p.scale >= 0.0f;
-            if (as_they_are) {
-                constexpr int kPer = D / 8;   // pieces of 16 bytes
+            float sc;             // takes a row's products to its log2 scores (with a soft limit: to the scores)
+            int from, behind;     // what the row sees: [from, behind)
+            const float row_scale = fabsf(p.scale) * (p.softcap > 0.0f ? 1.0f : 1.44269504f);
+            {
+                const int row0 = it.block * R + 128 * tq, token = token_of(p, row0 + min(r_in, min(128, it.n_rows - 128 * tq) - 1));   // row0: among the key head's
+                behind = min((int)it.len, it.before + token + 1), from = p.window > 0 ? max(0, it.before + token - p.window + 1) : 0;
+            }
+            sc = row_scale;
+            if (!as_they_are) {
+                // ---- queries under a power of two of their row: the largest value in [2^10, 2^11)
+                const int kvh = it.kvh, q0 = it.q0, row0 = it.block * R + 128 * tq, mine_rows = min(128, it.n_rows - 128 * tq);
+                const uint32_t q_off = C::kQ + (C::kQSets == 2 ? n_item & 1 : 0) * C::kQSet + tq * C::kQTile;
+                uint8_t *q_tile = smem + q_off;
+                const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+                auto power_of = [](float most) { return most > 0.0f && most <= 3.4028234e38f ? 10 - max((int)(__float_as_uint(most) >> 23) - 127, -110) : 0; };
+                auto put = [&](int r, int d, float4 x, int e) {   // four values of a row, under 2^e
+                    const float up = sign * __uint_as_float((uint32_t)(127 + e) << 23);
+                    uint32_t hi[2], lo[2];
+                    split(x.x * up, x.y * up, hi[0], lo[0]);
+                    split(x.z * up, x.w * up, hi[1], lo[1]);
+                    uint8_t *to = q_tile + (d >> 6) * (128 * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + 2 * (d & 7);
+                    *reinterpret_cast<uint2 *>(to) = make_uint2(hi[0], hi[1]);
+                    if constexpr (NT == 2) *reinterpret_cast<uint2 *>(to + C::kTerm) = make_uint2(lo[0], lo[1]);
+                };
+                auto greatest = [](float4 x) { return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))); };
+                constexpr int NL = (D + 127) / 128, kPer = D / 4;   // pieces of four values
+                if constexpr (!HALF) {
+                    // all of a warp's rows first, as they are, each in the 128-byte places that its terms will have
 #pragma unroll 4
-                for (int j = 0; j < kPer; j++) {
-                    const int c = lane + 32 * j, r = 32 * quarter + c / kPer, piece = c % kPer;
-                    const bool there = r < mine_rows;
-                    copy16(base + C::kQ + tq * C::kQTile + (piece >> 3) * (128 * 128) + r * 128 + (((piece & 7) ^ (r & 7)) << 4),
-                           there ? static_cast<const __half *>(p.q) + q_at(r) + 8 * piece : p.q, there);
+                    for (int j = 0; j < kPer; j++) {
+                        const int c = lane + 32 * j, r = 32 * quarter + c / kPer, piece = c % kPer, place = piece >> 3, i = token_of(p, row0 + r);
+                        const bool there = r < mine_rows;
+                        const float *src = static_cast<const float *>(p.q) + ((int64_t)(q0 + i) * p.q_stride + (int64_t)(kvh * p.group + row0 + r - i * p.group) * D + 4 * piece);
+                        copy16(base + q_off + place / C::kPanels * C::kTerm + place % C::kPanels * (128 * 128) + r * 128 + ((piece & 7) << 4), there ? static_cast<const void *>(src) : p.q, there);
+                    }
+                    copies_commit();
+                    copies_wait<0>();
+                    __syncwarp();
                 }
-                copies_commit();
-                copies_wait<0>();
-            } else if constexpr (!HALF) {
-                // all of a warp's rows first, as they are, each in the 128-byte places that its terms will have
-                constexpr int kPer = D / 4;
-#pragma unroll 4
-                for (int j = 0; j < kPer; j++) {
-                    const int c = lane + 32 * j, r = 32 * quarter + c / kPer, piece = c % kPer, place = piece >> 3;
-                    const bool there = r < mine_rows;
-                    copy16(base + C::kQ + tq * C::kQTile + place / C::kPanels * C::kTerm + place % C::kPanels * (128 * 128) + r * 128 + ((piece & 7) << 4),
-                           there ? static_cast<const float *>(p.q) + q_at(r) + 4 * piece : p.q, there);
-                }
-                copies_commit();
-                copies_wait<0>();
-                __syncwarp();
+                constexpr int kRows = NL == 1 ? 4 : 2;   // at a time
 #pragma unroll 1
-                for (int j0 = 0; j0 < 32; j0 += 4) {
-                    float x[4][NL][4], most[4];
+                for (int j0 = 0; j0 < 32; j0 += kRows) {
+                    float4 x[kRows][NL];
+                    uint32_t most[kRows];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int r = 32 * quarter + j0 + j;
-                        most[j] = 0.0f;
+                    for (int j = 0; j < kRows; j++) {
+                        const int r = 32 * quarter + j0 + j, i = token_of(p, row0 + r);
+                        const int64_t at = (int64_t)(q0 + i) * p.q_stride + (int64_t)(kvh * p.group + row0 + r - i * p.group) * D;
 #pragma unroll
                         for (int c = 0; c < NL; c++) {
                             const int piece = 32 * c + lane, place = piece >> 3;
-                            if (D % 128 == 0 || piece < kPer)
-                                *reinterpret_cast<float4 *>(x[j][c]) = *reinterpret_cast<const float4 *>(q_tile + place / C::kPanels * C::kTerm + place % C::kPanels * (128 * 128) + r * 128 + ((piece & 7) << 4));
-                            else x[j][c][0] = x[j][c][1] = x[j][c][2] = x[j][c][3] = 0.0f;
-#pragma unroll
-                            for (int e = 0; e < 4; e++) most[j] = fmaxf(most[j], fabsf(x[j][c][e]));
+                            x[j][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (D % 128 != 0 && piece >= kPer) continue;
+                            if constexpr (!HALF) {
+                                x[j][c] = *reinterpret_cast<const float4 *>(q_tile + place / C::kPanels * C::kTerm + place % C::kPanels * (128 * 128) + r * 128 + ((piece & 7) << 4));
+                            } else if (r < mine_rows) {
+                                if (p.q_half) {
+                                    const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const __half *>(p.q) + at + 4 * piece);
+                                    const float2 a = __half22float2(half2_of(w.x)), b = __half22float2(half2_of(w.y));
+                                    x[j][c] = make_float4(a.x, a.y, b.x, b.y);
+                                } else {
+                                    x[j][c] = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + at + 4 * piece);
+                                }
+                            }
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < 4; j++) most[j] = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most[j])));   // (not negative: bits in order)
+                    for (int j = 0; j < kRows; j++) {
+                        float top = greatest(x[j][0]);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int r = 32 * quarter + j0 + j, e = power_of(most[j]);
+                        for (int c = 1; c < NL; c++) top = fmaxf(top, greatest(x[j][c]));
+                        most[j] = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top));   // (not negative: bits in order)
+                    }
+#pragma unroll
+                    for (int j = 0; j < kRows; j++) {
+                        const int r = 32 * quarter + j0 + j, e = power_of(__uint_as_float(most[j]));
 #pragma unroll
                         for (int c = 0; c < NL; c++)
                             if (D % 128 == 0 || 32 * c + lane < kPer) put(r, 128 * c + 4 * lane, x[j][c], e);
-                        if (lane == 0) meta.scale[128 * tq + r] = row_scale * __uint_as_float((uint32_t)(127 - e) << 23);
+                        if (lane == j0 + j) sc = row_scale * __uint_as_float((uint32_t)(127 - e) << 23);
                     }
                 }
-            } else {
-#pragma unroll 1
-                for (int j0 = 0; j0 < 32; j0 += 4) {
-                    float x[4][NL][4], most[4];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int r = 32 * quarter + j0 + j;
-                        const int64_t from = q_at(r);
-                        most[j] = 0.0f;
-#pragma unroll
-                        for (int c = 0; c < NL; c++) {
-                            const int d = 128 * c + 4 * lane;
-                            x[j][c][0] = x[j][c][1] = x[j][c][2] = x[j][c][3] = 0.0f;
-                            if (r < mine_rows && (D % 128 == 0 || d < D)) {
-                                if (p.q_half) {
-                                    const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const __half *>(p.q) + from + d);
-                                    const float2 a = __half22float2(half2_of(w.x)), b = __half22float2(half2_of(w.y));
-                                    x[j][c][0] = a.x, x[j][c][1] = a.y, x[j][c][2] = b.x, x[j][c][3] = b.y;
-                                } else {
-                                    *reinterpret_cast<float4 *>(x[j][c]) = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + from + d);
-                                }
-                            }
-#pragma unroll
-                            for (int e = 0; e < 4; e++) most[j] = fmaxf(most[j], fabsf(x[j][c][e]));
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; j++) most[j] = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most[j])));
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int r = 32 * quarter + j0 + j, e = power_of(most[j]);
-#pragma unroll
-                        for (int c = 0; c < NL; c++)
-                            if (D % 128 == 0 || 128 * c + 4 * lane < D) put(r, 128 * c + 4 * lane, x[j][c], e);
-                        if (lane == 0) meta.scale[128 * tq + r] = row_scale * __uint_as_float((uint32_t)(127 - e) << 23);
-                    }
-                }
+                async_fence();
+                __syncwarp();
+                if (lane == 0) bar_arrive(bar(meta.q_full[C::kQSets == 2 ? n_item & 1 : 0][tq]));
             }
-            async_fence();
-            __syncwarp();
-            if (lane == 0) bar_arrive(bar(meta.q_full[tq]));
-
-            const float sc = as_they_are ? row_scale : meta.scale[128 * tq + r_in];
-            const int rr = row0 + min(r_in, mine_rows - 1), token = token_of(p, rr), head = kvh * p.group + rr - token * p.group;
-            const int behind = min(len, before + token + 1), from = p.window > 0 ? max(0, before + token - p.window + 1) : 0;   // what the row sees: [from, behind)
-            // every row of this tile of rows sees [all_from, all_to)
-            const int all_to = min(len, before + token_of(p, row0) + 1), all_from = p.window > 0 ? before + token_of(p, row0 + mine_rows - 1) - p.window + 1 : 0;
             float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
             for (int i = 0; i < tiles; i++, n_tile++) {
-                const int pos0 = (tile0 + i) * TP;
                 const int sb = NQ == 2 ? tq : (int)(n_tile & 1);
                 const uint32_t s_phase = NQ == 2 ? n_tile & 1 : (n_tile >> 1) & 1, t_s = t_lane + C::kS * sb;
                 wait(meta.s_full[sb], s_phase);
                 tc_after();
-                const uint32_t there = *reinterpret_cast<volatile uint8_t *>(&meta.there[(n_before + i) & 7]);
-                const bool masked = pos0 + TP > all_to || pos0 < all_from || there != (1u << kChunks) - 1u;
+                const uint32_t there = *reinterpret_cast<volatile uint8_t *>(&meta.there[(n_all - it.all + i) & 7]);
+                const int pos0 = (it.tile0 + i) * TP;
+                const bool masked = pos0 + TP > it.rows_to[tq] || pos0 < it.rows_from[tq] || there != (1u << kChunks) - 1u;
                 float f = sc;
                 // What is rarely done has code of its own, and no more of it than has to be: code that is jumped over, or met for the first time, is fetched at
                 // the pace of thousands of clocks.
@@ -761,15 +754,48 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                         tmem_stored();
                     }
                 }
+                // ---- values that are no numbers, where not all rows of the item see all positions: out of the tile (add_odd brings them to those that see them). Told
+                // of before they go, since both tiles of rows look.
+                if (!kQuant && (pos0 + TP > it.all_to || pos0 < it.all_from)) {
+                    const uint32_t h = 2 * (n_all - it.all + i) + 1, slot = h % C::kSlots;
+                    wait(meta.kv_full[slot], h / C::kSlots & 1);
+                    uint8_t *at = smem + slot * C::kSlot + (r_in % TP) * 128;
+                    constexpr int kFrom = 128 / TP;   // threads of a position, which take blocks of 64 values in turn
+                    uint32_t any = 0;
+#pragma unroll 1
+                    for (int c = r_in / TP; c < C::kPanels; c += kFrom)
+#pragma unroll
+                        for (int u = 0; u < 8; u++) {
+                            if (64 * c + 8 * u >= D) continue;
+                            const uint4 w = *reinterpret_cast<const uint4 *>(at + c * (TP * 128) + ((u ^ (r_in & 7)) << 4));
+                            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for (int k = 0; k < 4; k++) any |= ((ws[k] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;   // (an exponent of ones carries into the sign's place)
+                        }
+                    if (any) {
+                        atomicOr(&meta.odd[0][n_item & 7], 1u);
+                        atomicOr(&meta.odd[1][n_item & 7], 1u);
+                        __threadfence_block();
+                        for (int c = r_in / TP; c < C::kPanels; c += kFrom)
+                            for (int u = 0; u < 8; u++) {
+                                uint4 *w = reinterpret_cast<uint4 *>(at + c * (TP * 128) + (u << 4));
+                                uint4 x = *w;
+                                const bool b0 = take_out(x.x), b1 = take_out(x.y), b2 = take_out(x.z), b3 = take_out(x.w);
+                                if (b0 || b1 || b2 || b3) *w = x;
+                            }
+                        async_fence();
+                    }
+                    __syncwarp();
+                }
                 // (one tile of rows: the products of two tiles may be in flight, which a parity does not tell apart behind the last one)
                 if (NQ == 1 && i > 0 && i == tiles - 1) wait(meta.pv_done[tq], (n_tile - 1) & 1);
                 const float less = (m == -INFINITY ? 0.0f : -m) + (HALF ? kUpLog2 : 0.0f);
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int c = 0; c < TP; c += 32) {
-                    uint32_t w[NT * 16];
+                for (int c = 0; c < TP; c += 16) {   // (16 at a time: registers)
+                    uint32_t w[NT * 8];
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
+                    for (int j = 0; j < 16; j += 2) {
                         float a = fmaf(__uint_as_float(v[c + j]), f, less), b = fmaf(__uint_as_float(v[c + j + 1]), f, less);
                         if constexpr (HALF) {
                             // (the exponential unit takes a warp eight clocks a value, as long as the products of one tile of rows: some go another way)
@@ -779,15 +805,15 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                         } else {
                             a = ex2(a), b = ex2(b);
                             a *= kUp, b *= kUp;   // (in the exponent it would take bits of the greatest ones)
-                            split(a, b, w[j / 2], w[16 + j / 2]);
+                            split(a, b, w[j / 2], w[8 + j / 2]);
                         }
                         sum[j & 2] += a;
                         sum[(j & 2) + 1] += b;
                     }
-                    // (first terms in 16 columns, then the second ones: the place of the scores that were just read, or before it)
-                    if constexpr (HALF) tmem_store16(t_s + c / 2, w);
-                    else tmem_store32(t_s + c, w);
-                    if (c + 32 == TP / 2) {   // the first half's products begin
+                    // (of 32 scores first terms in 16 columns, then the second ones: the place of scores that were read before)
+                    tmem_store8(t_s + (HALF ? c / 2 : (c & ~31) + (c & 16) / 2), w);
+                    if constexpr (!HALF) tmem_store8(t_s + (c & ~31) + 16 + (c & 16) / 2, w + 8);
+                    if (c + 16 == TP / 2) {   // the first half's products begin
                         tmem_stored();
                         tc_before();
                         __syncwarp();
@@ -801,63 +827,54 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 if (lane == 0) bar_arrive(bar(meta.p_full[sb]));
             }
 
-            // ---- the row's factor, and its outputs through shared memory, in the place of the queries: 32 columns at a time, rows by the warp that has them
+            // ---- the row's factor, and its outputs, whole sectors at a time
+            const int kvh = it.kvh, q0 = it.q0, row0 = it.block * R + 128 * tq, mine_rows = min(128, it.n_rows - 128 * tq), tile0 = it.tile0;
             const float all = l * (1.0f / kUp);
             float out_f = 1.0f / kUp;
             const bool whole = it.whole;
-            float *part = p.part + (((size_t)blockIdx.x * 2 + it.begins) * R + 128 * tq + 32 * quarter) * (D + 2);   // of the warp's rows
+            float *part = p.part + ((size_t)blockIdx.x * 2 + it.begins) * R * (D + 2);
             if (whole) {
                 float lw = all, keep = 1.0f;
                 if (p.sinks) {
-                    const float sink = p.sinks[head] * 1.44269504f, t = fmaxf(m, sink);
+                    const int rr = row0 + min(r_in, mine_rows - 1);   // (again below: registers)
+                    const float sink = p.sinks[kvh * p.group + rr - token_of(p, rr) * p.group] * 1.44269504f, t = fmaxf(m, sink);
                     keep = m == -INFINITY ? 0.0f : exp2f(m - t);
                     lw = lw * keep + (sink == -INFINITY ? 0.0f : sink == t ? 1.0f : exp2f(sink - t));
                 }
                 out_f *= lw == 0.0f ? 0.0f : keep / lw;
             } else if (r_in < mine_rows) {
-                *reinterpret_cast<float2 *>(part + lane * (D + 2) + D) = make_float2(m, all);
-            }
-            const int out_rows = mine_rows - 32 * quarter - lane / 8;   // a lane's rows: lane / 8 + 4 j below 32, while 4 j is less than this
-            int64_t to_row[8];
-            if (whole) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int g = row0 + 32 * quarter + lane / 8 + 4 * j, t = token_of(p, g);
-                    to_row[j] = (int64_t)(q0 + t) * p.out_stride + (int64_t)(kvh * p.group + g - t * p.group) * D + 4 * (lane & 7);
-                }
+                reinterpret_cast<float2 *>(part + R * D)[128 * tq + r_in] = make_float2(m, all);
             }
             wait(meta.pv_done[tq], (n_tile - 1) & 1);
             tc_after();
             if (*reinterpret_cast<volatile uint32_t *>(&meta.odd[tq][n_item & 7]) != 0) add_odd<CT, D, TP>(p, it, t_o, max(from, tile0 * TP), min(behind, (tile0 + tiles) * TP));
-            uint8_t *stage = q_tile + quarter * (32 * 128);
-            const uint8_t *mine = stage + (lane / 8) * 128;
+            const int rr = row0 + min(r_in, mine_rows - 1), token = token_of(p, rr);
+            const int64_t to = (int64_t)(q0 + token) * p.out_stride + (int64_t)(kvh * p.group + rr - token * p.group) * D;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
                 tmem_load32(t_o + c, o);
                 tmem_loaded();
+                if (r_in < mine_rows) {
+                    if (!HALF || !whole) {
+                        float *at = (whole ? static_cast<float *>(p.out) + to : part + (128 * tq + r_in) * D) + c;
+                        const int wide = whole ? p.out_wide : 1;
 #pragma unroll
-                for (int j = 0; j < 32; j += 4)
-                    *reinterpret_cast<float4 *>(stage + lane * 128 + (((j / 4) ^ (lane & 7)) << 4)) =
-                        make_float4(__uint_as_float(o[j]) * out_f, __uint_as_float(o[j + 1]) * out_f, __uint_as_float(o[j + 2]) * out_f, __uint_as_float(o[j + 3]) * out_f);
-                __syncwarp();
-                float4 x[8];
+                        for (int j = 0; j < 32; j += 8) {
+                            uint32_t w[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = *reinterpret_cast<const float4 *>(mine + j * 512 + (((lane & 7) ^ ((lane / 8 + 4 * j) & 7)) << 4));
-                if (whole) {
+                            for (int k = 0; k < 8; k++) w[k] = __float_as_uint(__uint_as_float(o[j + k]) * out_f);
+                            store32(at + j, w, wide);
+                        }
+                    } else {
+                        __half *at = static_cast<__half *>(p.out) + to + c;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        if (4 * j >= out_rows) continue;
-                        if constexpr (HALF) *reinterpret_cast<uint2 *>(static_cast<__half *>(p.out) + to_row[j] + c) = make_uint2(bits(__floats2half2_rn(x[j].x, x[j].y)), bits(__floats2half2_rn(x[j].z, x[j].w)));
-                        else *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to_row[j] + c) = x[j];
-                    }
-                } else {
-                    float *to = part + (lane / 8) * (D + 2) + 4 * (lane & 7) + c;
+                        for (int j = 0; j < 32; j += 16) {
+                            uint32_t w[8];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        if (4 * j >= out_rows) continue;
-                        *reinterpret_cast<float2 *>(to + 4 * j * (D + 2)) = make_float2(x[j].x, x[j].y);
-                        *reinterpret_cast<float2 *>(to + 4 * j * (D + 2) + 2) = make_float2(x[j].z, x[j].w);
+                            for (int k = 0; k < 8; k++) w[k] = bits(__floats2half2_rn(__uint_as_float(o[j + 2 * k]) * out_f, __uint_as_float(o[j + 2 * k + 1]) * out_f));
+                            store32(at + j, w, p.out_wide);
+                        }
                     }
                 }
                 __syncwarp();
@@ -867,69 +884,50 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             if (r_in == 0) meta.odd[tq][n_item & 7] = 0;
         }
     } else if (warp < C::kProduct) {
-        // ===== keys and values into a ring of half tiles (keys, values in turn); a warp has the chunks w, w + 4 of 16 positions
-        if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kCopyRegs));
-        constexpr int kMine = kChunks / kChunkCopyWarps, kAhead = 32 / kChunks;   // chunks of a warp; tiles whose rows the lanes hold
+        // ===== keys and values into a ring of half tiles (keys, values in turn). f16: one warp, boxes of 64 values; the other one brings queries. 8 and 4 bits: a warp
+        // has the chunks w, w + 4 of 16 positions
+        if constexpr (C::kTrade) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kCopyRegs));
+        constexpr int kMine = kQuant ? kChunks / C::kCopies : 1, kAhead = 32 / kChunks;   // chunks of a warp; tiles whose rows the lanes hold
         const int w = warp - C::kSoft;
         int n_item = 0, n_tile = 0;
         Ring<kChunkItems> found;
         Ring<C::kSlots> to_slot;
-        auto take_out = [&](uint32_t &x) {   // of two f16, those that are no numbers
-            bool bad = false;
-            if ((x & 0x7C00u) == 0x7C00u) x &= 0xFFFF0000u, bad = true;
-            if ((x & 0x7C000000u) == 0x7C000000u) x &= 0xFFFFu, bad = true;
-            return bad;
-        };
         auto tell_odd = [&](int item) {
             atomicOr(&meta.odd[0][item & 7], 1u);
             atomicOr(&meta.odd[1][item & 7], 1u);
         };
         int64_t pool_rows = 0;   // lane: of chunk lane % kChunks of tile i + lane / kChunks, -1: none
-        int asked = 0, told = 0, told_slot = 0, tag = -1;  // f16: half tiles asked for and told of; lane h % 32: of half tile h, the item whose values are looked at, -1: not
         constexpr int kPieces = RB / 16, kCopies = (kChunk * kPieces + 31) / 32;
-        // f16: 16-byte pieces asynchronously, where a lane's go: the pattern repeats every eight rows
-        uint32_t to[kQuant ? 1 : kCopies / 2];
-        if constexpr (!kQuant) {
-#pragma unroll
-            for (int j = 0; j < kCopies / 2; j++) {
-                const int c = lane + 32 * j, row = c / kPieces, piece = c % kPieces;
-                to[j] = (piece >> 3) * (TP * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
-            }
-        }
-        auto tell = [&](int n) {   // all but the n last ones have arrived
-            if (n == 0) copies_wait<0>();
-            else copies_wait<2>();
-            for (; told < asked - n; told++) {
-                const int item = __shfl_sync(0xFFFFFFFFu, tag, told & 31);
-                if (item >= 0) {
-                    bool bad = false;
-#pragma unroll 1
-                    for (int m = 0; m < kMine; m++)
-#pragma unroll
-                        for (int j = 0; j < kCopies; j++) {
-                            const uint32_t off = to[kQuant ? 0 : j % (kCopies / 2)] + (j / (kCopies / 2)) * 1024;
-                            uint4 *at = reinterpret_cast<uint4 *>(smem + told_slot * C::kSlot + (w + kChunkCopyWarps * m) * (kChunk * 128) + off);
-                            uint4 v = *at;
-                            const bool b0 = take_out(v.x), b1 = take_out(v.y), b2 = take_out(v.z), b3 = take_out(v.w);
-                            if (b0 || b1 || b2 || b3) *at = v, bad = true;
-                        }
-                    if (bad) tell_odd(item);
-                }
-                async_fence();
-                __syncwarp();
-                if (lane == 0) bar_arrive(bar(meta.kv_full[told_slot]));
-                if (++told_slot == C::kSlots) told_slot = 0;
-            }
-        };
         for (;; n_item++, found.next()) {
-            if constexpr (!kQuant) {
-                if (!bar_test(bar(meta.item_full[found.at]), found.turn)) tell(0);   // (before the item may come others' work with these)
-            }
             wait(meta.item_full[found.at], found.turn);
             const ChunkItem it = meta.item[found.at];
             __syncwarp();
             if (lane == 0) bar_arrive(bar(meta.item_empty[found.at]));
             if (!it.goes_on || *gave_up) break;
+            if constexpr (HALF) {
+                if (as_they_are && (kQuant || w == 1)) {
+                    // the item's queries, 16 bytes a lane, into the place of the last but one's
+                    const int set = n_item & 1;
+                    wait(meta.q_empty[set], (n_item >> 1 & 1) ^ 1);
+                    constexpr int kWarps = kQuant ? C::kCopies : 1, kPer = D / 8, kAll = R * kPer / (32 * kWarps);
+                    const uint32_t to_set = base + C::kQ + set * C::kQSet;
+#pragma unroll 4
+                    for (int j = 0; j < kAll; j++) {
+                        const int c = lane + 32 * ((kQuant ? w : 0) + kWarps * j), r = c / kPer, piece = c % kPer, g = it.block * R + r, i = token_of(p, g);
+                        const bool there = r < it.n_rows;
+                        const __half *src = static_cast<const __half *>(p.q) + ((int64_t)(it.q0 + i) * p.q_stride + (int64_t)(it.kvh * p.group + g - i * p.group) * D + 8 * piece);
+                        copy16(to_set + (r >> 7) * C::kQTile + (piece >> 3) * (128 * 128) + (r & 127) * 128 + (((piece & 7) ^ (r & 7)) << 4), there ? static_cast<const void *>(src) : p.q, there);
+                    }
+                    copies_commit();
+                    if constexpr (!kQuant) {
+                        copies_wait<0>();
+                        async_fence();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(bar(meta.q_full[set][0]));
+                    }
+                }
+            }
+            if (!kQuant && w == 1) continue;
             const int32_t *table = p.table + (size_t)it.s * p.table_width;
             auto looked_at = [&](int i) { return (it.tile0 + i) * TP + TP > it.all_to || (it.tile0 + i) * TP < it.all_from; };
             auto find_rows = [&](int i) -> int64_t {
@@ -945,37 +943,25 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 if (w == 0 && lane == 0) meta.there[n_tile & 7] = (uint8_t)there;
                 n_tile++;
             };
-            auto row_of = [&](int i, int m) { return __shfl_sync(0xFFFFFFFFu, pool_rows, kChunks * (i % kAhead) + w + kChunkCopyWarps * m); };
+            auto row_of = [&](int i, int m) { return __shfl_sync(0xFFFFFFFFu, pool_rows, kChunks * (i % kAhead) + w + C::kCopies * m); };
             if constexpr (!kQuant) {
+                // a half tile is TP / box_rows boxes for each 64 values, a lane each
+                const int per = p.box_rows / kChunk, boxes = TP / p.box_rows, box = lane / C::kPanels, panel = lane % C::kPanels;
 #pragma unroll 1
                 for (int i = 0; i < it.all; i++) {
                     begin_tile(i);
+                    const int64_t row = __shfl_sync(0xFFFFFFFFu, pool_rows, kChunks * (i % kAhead) + min(box * per, kChunks - 1));
+                    const int y = row < 0 ? p.pool_rows : (int)row;
 #pragma unroll 1
                     for (int kv = 0; kv < 2; kv++) {
-                        if (!bar_test(bar(meta.kv_empty[to_slot.at]), to_slot.turn ^ 1)) {
-                            tell(0);   // (who frees the place may wait for these)
-                            wait(meta.kv_empty[to_slot.at], to_slot.turn ^ 1);
-                        }
-#pragma unroll
-                        for (int m = 0; m < kMine; m++) {
-                            const int chunk = w + kChunkCopyWarps * m, position = (it.tile0 + i) * TP + chunk * kChunk;
-                            const int64_t row0 = row_of(i, m);
-                            const int left = row0 < 0 ? 0 : it.len - position;   // rows that are not there come in as zeros
-                            const uint8_t *src = (kv ? p.v : p.k) + row0 * RB + 16 * lane;   // (no row: not looked at, a cache without pages has no memory)
-                            const uint32_t at = base + to_slot.at * C::kSlot + chunk * (kChunk * 128);
-                            if (left >= kChunk) {
-#pragma unroll
-                                for (int j = 0; j < kCopies; j++) copy16(to[j % (kCopies / 2)] + at + (j / (kCopies / 2)) * 1024, src + 512 * j, true);
-                            } else {
-#pragma unroll
-                                for (int j = 0; j < kCopies; j++) copy16(to[j % (kCopies / 2)] + at + (j / (kCopies / 2)) * 1024, row0 < 0 ? static_cast<const uint8_t *>(p.q) : src + 512 * j, (lane + 32 * j) / kPieces < left);
-                            }
-                        }
-                        copies_commit();
-                        if (lane == (asked & 31)) tag = kv && looked_at(i) ? n_item : -1;
-                        asked++;
+                        wait(meta.kv_empty[to_slot.at], to_slot.turn ^ 1);
+                        const uint32_t full = bar(meta.kv_full[to_slot.at]);
+                        if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "r"((uint32_t)C::kSlot) : "memory");
+                        __syncwarp();
+                        if (box < boxes)
+                            asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                                         ::"r"(base + to_slot.at * C::kSlot + panel * (TP * 128) + box * p.box_rows * 128), "l"(kv ? &p.v_map : &p.k_map), "r"(64 * panel), "r"(y), "r"(full) : "memory");
                         to_slot.next();
-                        if (asked - told > 2) tell(2);
                     }
                 }
             } else {
@@ -1010,7 +996,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     wait(meta.kv_empty[to_slot.at], to_slot.turn ^ 1);
 #pragma unroll
                     for (int m = 0; m < kMine; m++) {
-                        const int chunk = w + kChunkCopyWarps * m, left = rows[m] < 0 ? 0 : it.len - ((it.tile0 + i) * TP + chunk * kChunk);
+                        const int chunk = w + C::kCopies * m, left = rows[m] < 0 ? 0 : it.len - ((it.tile0 + i) * TP + chunk * kChunk);
                         rows[m] = more ? row_of((t + 1) >> 1, m) : -1;
                         uint8_t *chunk_at = smem + to_slot.at * C::kSlot + chunk * (kChunk * 128);
 #pragma unroll
@@ -1049,23 +1035,26 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                         }
                     }
                     if (bad) tell_odd(n_item);
+                    if (HALF && t == 0) copies_wait<0>();
                     async_fence();
                     __syncwarp();
-                    if (lane == 0) bar_arrive(bar(meta.kv_full[to_slot.at]));
+                    if (lane == 0) {
+                        if (HALF && t == 0 && as_they_are) bar_arrive(bar(meta.q_full[n_item & 1][0]));
+                        bar_arrive(bar(meta.kv_full[to_slot.at]));
+                    }
                     to_slot.next();
                 }
             }
         }
-        if constexpr (!kQuant) tell(0);
     } else {
-        if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+        if constexpr (C::kTrade) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
         if (warp == C::kProduct) {
             // ===== products, of the two tiles of rows in turn: while one is in its softmax the other one's run. (A warp each: both came to be in their softmax, and
             // both waited for products, at the same time.)
             const uint32_t elected = elected_lane();
             constexpr uint32_t qk = (1u << 4) | (uint32_t)(TP >> 3) << 17 | (128u >> 4) << 24, pv = (1u << 4) | 1u << 16 | (uint32_t)(D >> 3) << 17 | (128u >> 4) << 24;
             const uint32_t rows = desc_lo(base + C::kQ, 16), slots_k = desc_lo(base, 16), slots_v = desc_lo(base, TP * 128), t_o = tmem + C::kO;
-            uint32_t n_tile[2] = {0, 0}, n_item[2] = {0, 0};   // of a tile of rows
+            uint32_t n_tile[2] = {0, 0}, n_item = 0;   // n_tile: of a tile of rows
             Ring<kChunkItems> found;
             Ring<C::kSlots> keys, values;   // half tiles 2 i and 2 i + 1
             values.next();
@@ -1074,13 +1063,14 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 r.next(), r.next();
             };
             auto place_of = [&](int q, uint32_t t) { return NQ == 2 ? (uint32_t)q : t & 1; };
+            uint32_t set = 0, rows_set = rows, q_turns = 0;   // of the queries; q_turns: bit 2 set + q, of those that the softmax brings
             auto scores = [&](int q, uint32_t t) {   // of the t-th tile of all
                 const uint32_t at = slots_k + keys.at * (C::kSlot >> 4), d = tmem + C::kS * place_of(q, t);
 #pragma unroll
                 for (int term = 0; term < NT; term++)
 #pragma unroll
                     for (int c = 0; c < D; c += 64) {
-                        const uint32_t a = rows + q * (C::kQTile >> 4) + term * (C::kTerm >> 4) + (c >> 6) * (128 * 128 >> 4), b = at + (c >> 6) * (TP * 128 >> 4);
+                        const uint32_t a = rows_set + q * (C::kQTile >> 4) + term * (C::kTerm >> 4) + (c >> 6) * (128 * 128 >> 4), b = at + (c >> 6) * (TP * 128 >> 4);
                         if (D - c >= 64) products_k<4>(d, a, b, qk, term > 0 || c > 0, elected);
                         else products_k<2>(d, a, b, qk, term > 0 || c > 0, elected);
                     }
@@ -1109,11 +1099,17 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 __syncwarp();
                 if (lane == 0) bar_arrive(bar(meta.item_empty[found.at]));
                 if (!goes_on || *gave_up) break;
+                set = C::kQSets == 2 ? n_item & 1 : 0, rows_set = rows + set * (C::kQSet >> 4);
                 keys_there();
 #pragma unroll
                 for (int q = 0; q < NQ; q++)
                     if (n[q] > 0) {
-                        wait(meta.q_full[q], n_item[q]++ & 1);
+                        if (as_they_are) {
+                            if (q == 0) wait(meta.q_full[set][0], n_item >> 1 & 1);
+                        } else {
+                            wait(meta.q_full[set][q], q_turns >> (2 * set + q) & 1);
+                            q_turns ^= 1u << (2 * set + q);
+                        }
                         tc_after();
                         scores(q, n_tile[q]);
                     }
@@ -1142,6 +1138,8 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     }
                     free(values);
                 }
+                if (HALF && as_they_are) products_commit(bar(meta.q_empty[set]), elected);
+                n_item++;
 #pragma unroll
                 for (int q = 0; q < NQ; q++) n_tile[q] += n[q];
             }
@@ -1168,6 +1166,10 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                         const int end = min(q.len, q.before + token_of(p, min(last, first + 127)) + 1);
                         it.tiles[0] = min(walk.tiles, max((end + TP - 1) / TP - walk.tile0, 1));
                         it.tiles[1] = walk.n_rows > 128 ? walk.tiles : 0;
+                        for (int t = 0; t < 2; t++) {
+                            it.rows_to[t] = min(q.len, q.before + token_of(p, min(last, first + 128 * t)) + 1);
+                            it.rows_from[t] = p.window > 0 ? q.before + token_of(p, min(last, first + 128 * t + 127)) - p.window + 1 : 0;
+                        }
                         if (walk.parts > 0) walk.note(p);
                     }
                     bar_arrive(bar(meta.item_full[found.at]));
