@@ -49,7 +49,7 @@ __host__ __device__ constexpr int chunk_positions(int d) { return d <= 128 ? 128
 __host__ __device__ constexpr int chunk_rows(int d) { return 128 * chunk_tiles_of(d); }
 constexpr int kChunkSetup = 3;        // an item beside its tiles, in tiles
 constexpr int kChunkWholeTiles = 8;   // contexts of up to so many tiles of positions are not divided
-constexpr int kPolyOf8 = 2;           // f16: of eight exponentials, those by a polynomial
+constexpr int kPolyOf8 = 4;           // f16: of eight exponentials, those by a polynomial
 constexpr float kLetBe = 8.0f;        // log2: a reference stands until a score is more than this above it
 constexpr float kUp = 128.0f, kUpLog2 = 7.0f;   // of weights: times 2^8 they stay below the f16 range
 
@@ -376,16 +376,26 @@ __device__ __forceinline__ bool take_out(uint32_t &x) {   // of two f16, those t
     if ((x & 0x7C000000u) == 0x7C000000u) x &= 0xFFFFu, bad = true;
     return bad;
 }
-// As bar_wait, without a call: a kernel whose warps trade registers has none.
+// As bar_wait, without a call: a kernel whose warps trade registers has none. Tries that follow each other take the path to shared memory from the other
+// warps' exchanges and loads; a warp with time sleeps between them.
+template <int SLEEP>
 __device__ __forceinline__ void bar_wait_here(uint32_t bar, uint32_t parity, volatile int *gave_up, int *status) {
     if (bar_try(bar, parity)) return;
     const long long t0 = clock64();
 #pragma unroll 1
-    while (!*gave_up && !bar_try(bar, parity))
+    for (;;) {
+#pragma unroll 1
+        for (int i = 0; i < 16; i++) {
+            if (SLEEP > 0) __nanosleep(SLEEP);
+            if (bar_try(bar, parity)) return;
+        }
+        if (*gave_up) return;
         if (clock64() - t0 > kWaitLimit) {
             *gave_up = 1;
             atomicExch(status, KRK_CUDA_ETIMEOUT);
+            return;
         }
+    }
 }
 __device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t *v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
@@ -459,13 +469,38 @@ __device__ __forceinline__ float capped_here(float x, float cap) {
     }
     return cap * (1.44269504f * t);
 }
-// 2^x to 7.5e-5 of itself (x up to 15; an f16 weight's rounding is 2.4e-4 on average): the whole part goes to the exponent, the rest, in +-1/2, to the polynomial of
-// third degree whose greatest relative error is least. Below 2^-40 it is 2^-40, which f16 does not hold; a NaN stays one.
-__device__ __forceinline__ float exp2_poly(float x) {
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-40.0f));
-    const float t = x + 12582912.0f, r = x - (t - 12582912.0f);   // 1.5 * 2^23: to whole numbers
-    const float y = fmaf(fmaf(fmaf(0.055171668f, r, 0.242611122f), r, 0.693260986f), r, 0.999928074f);
-    return __int_as_float(__float_as_int(y) + (__float_as_int(t) << 23));
+// Two f32 at a time.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t x, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^x of two x to 7.5e-5 of itself (x up to 15; an f16 weight's rounding is 2.4e-4 at most): the whole part goes to the exponent, the rest, in +-1/2, to the polynomial
+// of third degree whose greatest relative error is least. Below 2^-40 it is 2^-40, which f16 does not hold; a NaN stays one.
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t xx) {
+    float a, b, ta, tb;
+    unpair(xx, a, b);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-40.0f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-40.0f));
+    const uint64_t x = pair(a, b), t = add2(x, pair(12582912.0f, 12582912.0f)), n = add2(t, pair(-12582912.0f, -12582912.0f));   // 1.5 * 2^23: to whole numbers
+    const uint64_t r = fma2(n, pair(-1.0f, -1.0f), x);
+    uint64_t y = fma2(pair(0.055171668f, 0.055171668f), r, pair(0.242611122f, 0.242611122f));
+    y = fma2(y, r, pair(0.693260986f, 0.693260986f));
+    y = fma2(y, r, pair(0.999928074f, 0.999928074f));
+    unpair(y, a, b);
+    unpair(t, ta, tb);
+    return pair(__int_as_float(__float_as_int(a) + (__float_as_int(ta) << 23)), __int_as_float(__float_as_int(b) + (__float_as_int(tb) << 23)));
 }
 // A value of a cache as f16 products see it, by a slow path.
 template <int CT, int D>
@@ -545,7 +580,8 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     volatile int *gave_up = &meta.gave_up;
     auto bar = [&](unsigned long long &b) { return smem_addr(&b); };
-    auto wait = [&](unsigned long long &b, uint32_t parity) { bar_wait_here(bar(b), parity, gave_up, p.status); };
+    auto wait = [&](unsigned long long &b, uint32_t parity) { bar_wait_here<0>(bar(b), parity, gave_up, p.status); };
+    auto wait_idle = [&](unsigned long long &b, uint32_t parity) { bar_wait_here<100>(bar(b), parity, gave_up, p.status); };
 
     // f16 queries enter as they are, and are copied ahead
     const bool as_they_are = HALF && p.q_half && p.scale >= 0.0f;
@@ -650,11 +686,11 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     copies_wait<0>();
                     __syncwarp();
                 }
-                constexpr int kRows = NL == 1 ? 4 : 2;   // at a time
+                constexpr int kRows = NL == 1 ? 8 : 4;   // at a time
 #pragma unroll 1
                 for (int j0 = 0; j0 < 32; j0 += kRows) {
                     float4 x[kRows][NL];
-                    uint32_t most[kRows];
+                    float most[kRows];
 #pragma unroll
                     for (int j = 0; j < kRows; j++) {
                         const int r = 32 * quarter + j0 + j, i = token_of(p, row0 + r);
@@ -679,14 +715,18 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     }
 #pragma unroll
                     for (int j = 0; j < kRows; j++) {
-                        float top = greatest(x[j][0]);
+                        most[j] = greatest(x[j][0]);
 #pragma unroll
-                        for (int c = 1; c < NL; c++) top = fmaxf(top, greatest(x[j][c]));
-                        most[j] = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top));   // (not negative: bits in order)
+                        for (int c = 1; c < NL; c++) most[j] = fmaxf(most[j], greatest(x[j][c]));
                     }
+                    // (an exchange at a time of all rows: the warp-wide maximum as one instruction took 440 clocks a row)
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                        for (int j = 0; j < kRows; j++) most[j] = fmaxf(most[j], __shfl_xor_sync(0xFFFFFFFFu, most[j], o));
 #pragma unroll
                     for (int j = 0; j < kRows; j++) {
-                        const int r = 32 * quarter + j0 + j, e = power_of(__uint_as_float(most[j]));
+                        const int r = 32 * quarter + j0 + j, e = power_of(most[j]);
 #pragma unroll
                         for (int c = 0; c < NL; c++)
                             if (D % 128 == 0 || 32 * c + lane < kPer) put(r, 128 * c + 4 * lane, x[j][c], e);
@@ -702,11 +742,14 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             for (int i = 0; i < tiles; i++, n_tile++) {
                 const int sb = NQ == 2 ? tq : (int)(n_tile & 1);
                 const uint32_t s_phase = NQ == 2 ? n_tile & 1 : (n_tile >> 1) & 1, t_s = t_lane + C::kS * sb;
+                const int pos0 = (it.tile0 + i) * TP, all_to = it.all_to, all_from = it.all_from, rows_to = it.rows_to[tq], rows_from = it.rows_from[tq];
+                const uint32_t tile_no = n_all - it.all + i;
+                bool masked = (pos0 + TP > rows_to) | (pos0 < rows_from);
+                const bool look = !kQuant && ((pos0 + TP > all_to) | (pos0 < all_from));
                 wait(meta.s_full[sb], s_phase);
                 tc_after();
-                const uint32_t there = *reinterpret_cast<volatile uint8_t *>(&meta.there[(n_all - it.all + i) & 7]);
-                const int pos0 = (it.tile0 + i) * TP;
-                const bool masked = pos0 + TP > it.rows_to[tq] || pos0 < it.rows_from[tq] || there != (1u << kChunks) - 1u;
+                const uint32_t there = *reinterpret_cast<volatile uint8_t *>(&meta.there[tile_no & 7]);
+                masked |= there != (1u << kChunks) - 1u;
                 float f = sc;
                 // What is rarely done has code of its own, and no more of it than has to be: code that is jumped over, or met for the first time, is fetched at
                 // the pace of thousands of clocks.
@@ -756,8 +799,8 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 }
                 // ---- values that are no numbers, where not all rows of the item see all positions: out of the tile (add_odd brings them to those that see them). Told
                 // of before they go, since both tiles of rows look.
-                if (!kQuant && (pos0 + TP > it.all_to || pos0 < it.all_from)) {
-                    const uint32_t h = 2 * (n_all - it.all + i) + 1, slot = h % C::kSlots;
+                if (look) {
+                    const uint32_t h = 2 * tile_no + 1, slot = h % C::kSlots;
                     wait(meta.kv_full[slot], h / C::kSlots & 1);
                     uint8_t *at = smem + slot * C::kSlot + (r_in % TP) * 128;
                     constexpr int kFrom = 128 / TP;   // threads of a position, which take blocks of 64 values in turn
@@ -790,25 +833,28 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 // (one tile of rows: the products of two tiles may be in flight, which a parity does not tell apart behind the last one)
                 if (NQ == 1 && i > 0 && i == tiles - 1) wait(meta.pv_done[tq], (n_tile - 1) & 1);
                 const float less = (m == -INFINITY ? 0.0f : -m) + (HALF ? kUpLog2 : 0.0f);
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint64_t sum[2] = {0, 0};
+                const uint64_t ff = pair(f, f), ll = pair(less, less);
 #pragma unroll
                 for (int c = 0; c < TP; c += 16) {   // (16 at a time: registers)
                     uint32_t w[NT * 8];
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
-                        float a = fmaf(__uint_as_float(v[c + j]), f, less), b = fmaf(__uint_as_float(v[c + j + 1]), f, less);
-                        if constexpr (HALF) {
-                            // (the exponential unit takes a warp eight clocks a value, as long as the products of one tile of rows: some go another way)
-                            if (j % 8 < kPolyOf8) a = exp2_poly(a), b = exp2_poly(b);
-                            else a = ex2(a), b = ex2(b);
-                            w[j / 2] = bits(__floats2half2_rn(a, b));
+                        uint64_t x = fma2(pair(__uint_as_float(v[c + j]), __uint_as_float(v[c + j + 1])), ff, ll);
+                        float a, b;
+                        // (the exponential unit takes a warp eight clocks a value, as long as the products of one tile of rows: some go another way)
+                        if (HALF && j % 8 < kPolyOf8) {
+                            x = exp2_poly(x);
+                            unpair(x, a, b);
                         } else {
+                            unpair(x, a, b);
                             a = ex2(a), b = ex2(b);
-                            a *= kUp, b *= kUp;   // (in the exponent it would take bits of the greatest ones)
-                            split(a, b, w[j / 2], w[8 + j / 2]);
+                            if (!HALF) a *= kUp, b *= kUp;   // (in the exponent it would take bits of the greatest ones)
+                            x = pair(a, b);
                         }
-                        sum[j & 2] += a;
-                        sum[(j & 2) + 1] += b;
+                        if constexpr (HALF) w[j / 2] = bits(__floats2half2_rn(a, b));
+                        else split(a, b, w[j / 2], w[8 + j / 2]);
+                        sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], x);
                     }
                     // (of 32 scores first terms in 16 columns, then the second ones: the place of scores that were read before)
                     tmem_store8(t_s + (HALF ? c / 2 : (c & ~31) + (c & 16) / 2), w);
@@ -820,7 +866,11 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                         if (lane == 0) bar_arrive(bar(meta.p_half[sb]));
                     }
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                {
+                    float a, b;
+                    unpair(add2(sum[0], sum[1]), a, b);
+                    l += a + b;
+                }
                 tmem_stored();
                 tc_before();
                 __syncwarp();
@@ -908,7 +958,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 if (as_they_are && (kQuant || w == 1)) {
                     // the item's queries, 16 bytes a lane, into the place of the last but one's
                     const int set = n_item & 1;
-                    wait(meta.q_empty[set], (n_item >> 1 & 1) ^ 1);
+                    wait_idle(meta.q_empty[set], (n_item >> 1 & 1) ^ 1);
                     constexpr int kWarps = kQuant ? C::kCopies : 1, kPer = D / 8, kAll = R * kPer / (32 * kWarps);
                     const uint32_t to_set = base + C::kQ + set * C::kQSet;
 #pragma unroll 4
@@ -954,7 +1004,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     const int y = row < 0 ? p.pool_rows : (int)row;
 #pragma unroll 1
                     for (int kv = 0; kv < 2; kv++) {
-                        wait(meta.kv_empty[to_slot.at], to_slot.turn ^ 1);
+                        wait_idle(meta.kv_empty[to_slot.at], to_slot.turn ^ 1);
                         const uint32_t full = bar(meta.kv_full[to_slot.at]);
                         if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "r"((uint32_t)C::kSlot) : "memory");
                         __syncwarp();
@@ -993,7 +1043,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     const bool look = (t & 1) && looked_at(i), more = t + 1 < halves;
                     bool bad = false;
                     if (more && (t & 1)) begin_tile(i + 1);
-                    wait(meta.kv_empty[to_slot.at], to_slot.turn ^ 1);
+                    wait_idle(meta.kv_empty[to_slot.at], to_slot.turn ^ 1);
 #pragma unroll
                     for (int m = 0; m < kMine; m++) {
                         const int chunk = w + C::kCopies * m, left = rows[m] < 0 ? 0 : it.len - ((it.tile0 + i) * TP + chunk * kChunk);
@@ -1107,7 +1157,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                         if (as_they_are) {
                             if (q == 0) wait(meta.q_full[set][0], n_item >> 1 & 1);
                         } else {
-                            wait(meta.q_full[set][q], q_turns >> (2 * set + q) & 1);
+                            wait_idle(meta.q_full[set][q], q_turns >> (2 * set + q) & 1);
                             q_turns ^= 1u << (2 * set + q);
                         }
                         tc_after();
@@ -1151,7 +1201,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             Ring<kChunkItems> found;
             for (;; found.next()) {
                 const bool more = walk.template next<true>(p);
-                wait(meta.item_empty[found.at], found.turn ^ 1);
+                wait_idle(meta.item_empty[found.at], found.turn ^ 1);
                 if (*gave_up) break;
                 if (lane == 0) {
                     ChunkItem &it = meta.item[found.at];
