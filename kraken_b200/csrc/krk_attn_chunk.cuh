@@ -401,6 +401,11 @@ __device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t *v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
                  ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
+// The 128 threads of a tile of rows meet. (Warps whole: one whose first thread had been apart stayed in two parts, and took twice its time and 440 clocks an exchange.)
+__device__ __forceinline__ void rows_sync(int tile) {
+    __syncwarp();
+    asm volatile("barrier.cta.sync.aligned %0, 128;" ::"r"(1 + tile) : "memory");
+}
 // 32 bytes of a thread: a sector (wide: on its boundary).
 __device__ __forceinline__ void store32(void *to, const uint32_t *w, int wide) {
     if (wide)
@@ -637,14 +642,14 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 meta.mine[tq] = it;
                 bar_arrive(bar(meta.item_empty[found.at]));
             }
-            group_sync(tq);
+            rows_sync(tq);
             // (read again where it is wanted, not kept beside a tile's scores: registers)
             const volatile ChunkItem &it = meta.mine[tq];
             if (!it.goes_on) break;
             const int tiles = it.tiles[tq];
             n_all += it.all;
             if (it.n_rows <= 128 * tq) {
-                group_sync(tq);
+                rows_sync(tq);
                 continue;
             }
             float sc;             // takes a row's products to its log2 scores (with a soft limit: to the scores)
@@ -930,7 +935,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 __syncwarp();
             }
             tc_before();
-            group_sync(tq);
+            rows_sync(tq);
             if (r_in == 0) meta.odd[tq][n_item & 7] = 0;
         }
     } else if (warp < C::kProduct) {
