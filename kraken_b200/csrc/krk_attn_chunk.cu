@@ -84,6 +84,19 @@ bool encode_pools(ChunkParams &p, int d) {
     return true;
 }
 
+// The queries as [token][head][value], in boxes of 128 bytes of the group's heads of so many tokens as are 128 rows. f16 in the 128-byte swizzle.
+void encode_queries(ChunkParams &p, int d, bool half) {
+    const EncodeTiled encode = encode_tiled();
+    p.q_boxes = 0;
+    if (!encode || 128 % p.group != 0) return;
+    const int bytes = half ? 2 : 4;
+    // (no box names a token that no sequence has: their number is not known here)
+    const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)p.n_heads, 1ull << 30}, strides[2] = {(cuuint64_t)(d * bytes), (cuuint64_t)(p.q_stride * bytes)};
+    const cuuint32_t box[3] = {(cuuint32_t)(128 / bytes), (cuuint32_t)p.group, (cuuint32_t)(128 / p.group)}, step[3] = {1, 1, 1};
+    p.q_boxes = encode(&p.q_map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void *>(p.q), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                       half ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int launch_chunk_merge(const ChunkParams &p, int d, bool half, int rows, cudaStream_t st) {
     auto kernel = half ? (d == 64 ? chunk_merge_kernel<64, true> : d == 96 ? chunk_merge_kernel<96, true> : d == 128 ? chunk_merge_kernel<128, true>
                           : d == 192 ? chunk_merge_kernel<192, true> : chunk_merge_kernel<256, true>)
@@ -153,6 +166,7 @@ int launch_attention_chunk(void *out, int out_dtype, const void *q, int q_dtype,
     p.status = device_status_word();
     if (!p.status) return KRK_CUDA_EDEVICE;
     if (cache.type == KRK_CUDA_KV_F16 && !attn::encode_pools(p, d)) return KRK_CUDA_ELAUNCH;
+    attn::encode_queries(p, d, p.q_half);
     // units of work are counted in 64 bits
     const double blocks = ((double)a.max_q * p.group + r - 1) / r, all = (double)a.n_seq * p.n_kv * blocks * 4.0 * p.group * ((double)a.max_kv_len + 2.0 * r + 1024.0);
     if (all > 4e18) return KRK_CUDA_ESHAPE;

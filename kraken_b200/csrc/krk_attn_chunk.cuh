@@ -33,7 +33,9 @@ struct ChunkParams {
     int *status;
     // f16 caches: the pool's rows as boxes of 64 values of box_rows positions, a part of one page; behind the last row zeros come in
     int box_rows, pool_rows;
-    alignas(64) CUtensorMap k_map, v_map;
+    // queries: boxes of 128 bytes of 128 rows, where that many are whole tokens (q_boxes)
+    int q_boxes;
+    alignas(64) CUtensorMap k_map, v_map, q_map;
 };
 // n / d for n below 2^31: with 2^(s - 1) < d <= 2^s the factor ceil(2^(31 + s) / d) is less than one above the quotient, which n times it is at most 2^31 off.
 inline void divide_by(int d, uint32_t &mul, uint32_t &shift) {
@@ -210,9 +212,9 @@ struct ChunkWalk {
     }
     // Of CTA b, with the total of units: how many share them, and its own.
     __host__ __device__ __forceinline__ void share(const ChunkParams &p, int b) {
-        // A share is longer than what an item costs beside its tiles and two tiles: no two borders lie at one tile inside an item, whose units a tile are at most
-        // 4 group (TP kChunkSetup / tiles + TP + 2).
-        const int64_t least = (int64_t)4 * p.group * TP * (kChunkSetup + 4);
+        // A share is longer than what an item costs beside its tiles: no two borders lie at one tile inside an item, which is not near its ends where it has
+        // four tiles and more, of 4 group (TP kChunkSetup / tiles + TP + 2) units at most. Undivided items have a share each if there are CTAs.
+        const int64_t least = p.whole ? 1 : (int64_t)4 * p.group * TP * (kChunkSetup + 1);
         cta = b;
         const int most = (int)fminf((float)p.grid, (float)total / (float)least);
         grid = max(most, 1);
@@ -338,7 +340,7 @@ struct ChunkItem {
 };
 constexpr int kChunkItems = 3;   // found ahead
 struct ChunkMeta {
-    unsigned long long kv_full[6], kv_empty[6], s_full[2], p_half[2], p_full[2], pv_done[2], q_full[2][2], q_empty[2], item_full[kChunkItems], item_empty[kChunkItems], drained;
+    unsigned long long kv_full[6], kv_empty[6], s_full[2], p_half[2], p_full[2], pv_done[2], q_full[2][2], q_empty[2], q_raw, item_full[kChunkItems], item_empty[kChunkItems], drained;
     uint32_t odd[2][8];       // of a tile of rows, an item in turn: values of a tile that not all rows see are no numbers
     uint8_t there[8];         // of a tile of positions, in turn: bit c: chunk c is a page's
     uint32_t tmem;
@@ -604,6 +606,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 for (int j = 0; j < 2; j++) bar_init(bar(meta.q_full[i][j]), as_they_are ? (kQuant ? C::kCopies : 1) : 4);   // [set][tile of rows]
                 bar_init(bar(meta.q_empty[i]), 1);
             }
+            bar_init(bar(meta.q_raw), 1);
             bar_init(bar(meta.drained), 1);
             for (int i = 0; i < kChunkItems; i++) {
                 bar_init(bar(meta.item_full[i]), 1);
@@ -649,6 +652,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             const int tiles = it.tiles[tq];
             n_all += it.all;
             if (it.n_rows <= 128 * tq) {
+                if (!HALF) wait(meta.q_raw, n_item & 1);   // (a parity tells one turn from the next)
                 rows_sync(tq);
                 continue;
             }
@@ -678,19 +682,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 };
                 auto greatest = [](float4 x) { return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))); };
                 constexpr int NL = (D + 127) / 128, kPer = D / 4;   // pieces of four values
-                if constexpr (!HALF) {
-                    // all of a warp's rows first, as they are, each in the 128-byte places that its terms will have
-#pragma unroll 4
-                    for (int j = 0; j < kPer; j++) {
-                        const int c = lane + 32 * j, r = 32 * quarter + c / kPer, piece = c % kPer, place = piece >> 3, i = token_of(p, row0 + r);
-                        const bool there = r < mine_rows;
-                        const float *src = static_cast<const float *>(p.q) + ((int64_t)(q0 + i) * p.q_stride + (int64_t)(kvh * p.group + row0 + r - i * p.group) * D + 4 * piece);
-                        copy16(base + q_off + place / C::kPanels * C::kTerm + place % C::kPanels * (128 * 128) + r * 128 + ((piece & 7) << 4), there ? static_cast<const void *>(src) : p.q, there);
-                    }
-                    copies_commit();
-                    copies_wait<0>();
-                    __syncwarp();
-                }
+                if constexpr (!HALF) wait(meta.q_raw, n_item & 1);   // (as they are, each row in the 128-byte places that its terms will have)
                 constexpr int kRows = NL == 1 ? 8 : 4;   // at a time
 #pragma unroll 1
                 for (int j0 = 0; j0 < 32; j0 += kRows) {
@@ -959,27 +951,44 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             __syncwarp();
             if (lane == 0) bar_arrive(bar(meta.item_empty[found.at]));
             if (!it.goes_on || *gave_up) break;
-            if constexpr (HALF) {
-                if (as_they_are && (kQuant || w == 1)) {
-                    // the item's queries, 16 bytes a lane, into the place of the last but one's
-                    const int set = n_item & 1;
-                    wait_idle(meta.q_empty[set], (n_item >> 1 & 1) ^ 1);
-                    constexpr int kWarps = kQuant ? C::kCopies : 1, kPer = D / 8, kAll = R * kPer / (32 * kWarps);
-                    const uint32_t to_set = base + C::kQ + set * C::kQSet;
+            if ((kQuant || w == 1) && (!HALF || as_they_are)) {
+                // The item's queries, into the place of the last but one's (f32: of the last one's): f16 as the products take them; f32 for the softmax to divide into terms, each
+                // row in the 128-byte places that its terms will have. Tiles of 128 rows as boxes, others 16 bytes a lane.
+                const int set = C::kQSets == 2 ? n_item & 1 : 0;
+                wait_idle(meta.q_empty[set], ((C::kQSets == 2 ? n_item >> 1 : n_item) & 1) ^ 1);
+                constexpr int kBytes = HALF ? 2 : 4, kPer = D * kBytes / 16, kPlaces = (D * kBytes + 127) / 128, kWarps = kQuant ? C::kCopies : 1, kAll = 128 * kPer / (32 * kWarps);
+                auto place_at = [](int place) { return HALF ? place * (128 * 128) : place / C::kPanels * C::kTerm + place % C::kPanels * (128 * 128); };
+                const uint32_t to_set = base + C::kQ + set * C::kQSet, full = HALF ? bar(meta.q_full[set][0]) : bar(meta.q_raw);
+                uint32_t boxed = 0;   // bytes that come in boxes
+                for (int t = 0; t < NQ; t++)
+                    if (p.q_boxes && it.n_rows >= 128 * (t + 1)) boxed += kPlaces * 128 * 128;
+                const bool tells = !kQuant || w == 0;
+                if (tells && lane == 0 && boxed > 0) asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(full), "r"(boxed) : "memory");
+                __syncwarp();
+#pragma unroll 1
+                for (int t = 0; t < NQ; t++) {
+                    const int rows = it.n_rows - 128 * t, first = it.block * R + 128 * t;
+                    if (rows <= 0) break;
+                    if (p.q_boxes && rows >= 128) {
+                        if (tells && lane < kPlaces)
+                            asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                                         ::"r"(to_set + t * C::kQTile + place_at(lane)), "l"(&p.q_map), "r"(128 / kBytes * lane), "r"(it.kvh * p.group), "r"(it.q0 + token_of(p, first)), "r"(full) : "memory");
+                        continue;
+                    }
 #pragma unroll 4
                     for (int j = 0; j < kAll; j++) {
-                        const int c = lane + 32 * ((kQuant ? w : 0) + kWarps * j), r = c / kPer, piece = c % kPer, g = it.block * R + r, i = token_of(p, g);
-                        const bool there = r < it.n_rows;
-                        const __half *src = static_cast<const __half *>(p.q) + ((int64_t)(it.q0 + i) * p.q_stride + (int64_t)(it.kvh * p.group + g - i * p.group) * D + 8 * piece);
-                        copy16(to_set + (r >> 7) * C::kQTile + (piece >> 3) * (128 * 128) + (r & 127) * 128 + (((piece & 7) ^ (r & 7)) << 4), there ? static_cast<const void *>(src) : p.q, there);
+                        const int c = lane + 32 * ((kQuant ? w : 0) + kWarps * j), r = c / kPer, piece = c % kPer, g = first + r, i = token_of(p, g);
+                        const bool there = r < rows;
+                        const uint8_t *src = static_cast<const uint8_t *>(p.q) + ((int64_t)(it.q0 + i) * p.q_stride + (int64_t)(it.kvh * p.group + g - i * p.group) * D) * kBytes + 16 * piece;
+                        copy16(to_set + t * C::kQTile + place_at(piece >> 3) + r * 128 + (((piece & 7) ^ (HALF ? r & 7 : 0)) << 4), there ? static_cast<const void *>(src) : p.q, there);
                     }
-                    copies_commit();
-                    if constexpr (!kQuant) {
-                        copies_wait<0>();
-                        async_fence();
-                        __syncwarp();
-                        if (lane == 0) bar_arrive(bar(meta.q_full[set][0]));
-                    }
+                }
+                copies_commit();
+                if constexpr (!kQuant) {
+                    copies_wait<0>();
+                    async_fence();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(full);
                 }
             }
             if (!kQuant && w == 1) continue;
@@ -1169,6 +1178,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                         scores(q, n_tile[q]);
                     }
                 free(keys);
+                if (all == 1) products_commit(bar(meta.q_empty[set]), elected);
 #pragma unroll 1
                 for (int i = 0; i < all; i++) {
                     const bool more = i + 1 < all;
@@ -1178,6 +1188,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                             tc_after();
                             scores(0, n_tile[0] + i + 1);
                             free(keys);
+                            if (i + 2 == all) products_commit(bar(meta.q_empty[set]), elected);
                         }
                         values_there();
                         sums(0, n_tile[0] + i, i > 0);
@@ -1190,10 +1201,10 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                             if (i + 1 < n[q]) scores(q, n_tile[q] + i + 1);
                         }
                         if (more) free(keys);
+                        if (i + 2 == all) products_commit(bar(meta.q_empty[set]), elected);
                     }
                     free(values);
                 }
-                if (HALF && as_they_are) products_commit(bar(meta.q_empty[set]), elected);
                 n_item++;
 #pragma unroll
                 for (int q = 0; q < NQ; q++) n_tile[q] += n[q];
