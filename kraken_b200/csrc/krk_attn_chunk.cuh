@@ -309,17 +309,19 @@ struct ChunkWalk {
     }
 };
 
-template <int D, int NT, bool QUANT>
+template <int D, int NT, int CT>
 struct Chunk {
+    static constexpr bool QUANT = CT != KRK_CUDA_KV_F16;
     static constexpr int NQ = chunk_tiles_of(D), TP = chunk_positions(D), R = chunk_rows(D);
     static constexpr int kMetaBytes = 1920;
     static constexpr int kPanels = (D + 63) / 64;                    // blocks of 64 values
     static constexpr int kTerm = kPanels * 128 * 128, kQTile = NT * kTerm;
-    static constexpr int kQSets = NT == 1 ? 2 : 1, kQSet = NQ * kQTile;   // the queries of this item and, where there is room, of the next one
+    static constexpr int kQSets = NT == 1 && !QUANT ? 2 : 1, kQSet = NQ * kQTile;   // the queries of this item and, where there is room, of the next one
     static constexpr int kSlot = kPanels * TP * 128;                 // half a tile: keys or values
-    static constexpr int kRoom = 227 * 1024 - 1024 - kMetaBytes - kQSets * kQSet;
+    static constexpr int kRawChunk = QUANT ? kChunk * (row_bytes_of(CT, D) + scale_bytes_of(CT, D)) : 0, kRaws = 3, kRaw = TP / kChunk * kRawChunk;   // 8 and 4 bits as they are: quants and scales of a half tile
+    static constexpr int kRoom = 227 * 1024 - 1024 - kMetaBytes - kQSets * kQSet - kRaws * kRaw;
     static constexpr int kSlots = kRoom / kSlot > 6 ? 6 : kRoom / kSlot;
-    static constexpr int kQ = kSlots * kSlot, kMeta = kQ + kQSets * kQSet, kBytes = kMeta + kMetaBytes + 1024;   // (begins on a 1024-byte boundary)
+    static constexpr int kQ = kSlots * kSlot, kRawAt = kQ + kQSets * kQSet, kMeta = kRawAt + kRaws * kRaw, kBytes = kMeta + kMetaBytes + 1024;   // (begins on a 1024-byte boundary)
     // warps: softmax, copies, products, the one that finds items
     static constexpr int kSoft = 4 * NQ, kCopies = QUANT ? 4 : 2, kProduct = kSoft + kCopies, kFinder = kProduct + 1, kWarps = kSoft + (QUANT ? 8 : 4), kThreads = 32 * kWarps;
     // Registers of a thread, traded between groups of four warps (a spill goes to level 2: shared memory has what level 1 had). Launched with: 384 threads 168, 512 128.
@@ -571,10 +573,10 @@ __device__ __forceinline__ void add_odd(const ChunkParams &p, const volatile Chu
 
 // HALF: f16 out, one term of each query and weight (NT), else f32 and two.
 template <int D, int CT, bool HALF>
-__global__ void __launch_bounds__((Chunk<D, HALF ? 1 : 2, CT != KRK_CUDA_KV_F16>::kThreads), 1)
+__global__ void __launch_bounds__((Chunk<D, HALF ? 1 : 2, CT>::kThreads), 1)
 attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
     constexpr int NT = HALF ? 1 : 2;
-    using C = Chunk<D, NT, CT != KRK_CUDA_KV_F16>;
+    using C = Chunk<D, NT, CT>;
     using Walk = typename C::Walk;
     constexpr int NQ = C::NQ, TP = C::TP, R = C::R, RB = row_bytes_of(CT, D), kChunks = TP / kChunk;
     constexpr bool kQuant = CT != KRK_CUDA_KV_F16;
@@ -932,7 +934,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
         }
     } else if (warp < C::kProduct) {
         // ===== keys and values into a ring of half tiles (keys, values in turn). f16: one warp, boxes of 64 values; the other one brings queries. 8 and 4 bits: a warp
-        // has the chunks w, w + 4 of 16 positions
+        // has a quarter of the chunks of 16 positions
         if constexpr (C::kTrade) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kCopyRegs));
         constexpr int kMine = kQuant ? kChunks / C::kCopies : 1, kAhead = 32 / kChunks;   // chunks of a warp; tiles whose rows the lanes hold
         const int w = warp - C::kSoft;
@@ -947,10 +949,12 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
         constexpr int kPieces = RB / 16, kCopies = (kChunk * kPieces + 31) / 32;
         for (;; n_item++, found.next()) {
             wait(meta.item_full[found.at], found.turn);
-            const ChunkItem it = meta.item[found.at];
-            __syncwarp();
-            if (lane == 0) bar_arrive(bar(meta.item_empty[found.at]));
+            const volatile ChunkItem &it = meta.item[found.at];   // (read where it is wanted: registers)
             if (!it.goes_on || *gave_up) break;
+            auto done = [&] {
+                __syncwarp();
+                if (lane == 0) bar_arrive(bar(meta.item_empty[found.at]));
+            };
             if ((kQuant || w == 1) && (!HALF || as_they_are)) {
                 // The item's queries, into the place of the last but one's (f32: of the last one's): f16 as the products take them; f32 for the softmax to divide into terms, each
                 // row in the 128-byte places that its terms will have. Tiles of 128 rows as boxes, others 16 bytes a lane.
@@ -991,7 +995,10 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     if (lane == 0) bar_arrive(full);
                 }
             }
-            if (!kQuant && w == 1) continue;
+            if (!kQuant && w == 1) {
+                done();
+                continue;
+            }
             const int32_t *table = p.table + (size_t)it.s * p.table_width;
             auto looked_at = [&](int i) { return (it.tile0 + i) * TP + TP > it.all_to || (it.tile0 + i) * TP < it.all_from; };
             auto find_rows = [&](int i) -> int64_t {
@@ -1007,7 +1014,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 if (w == 0 && lane == 0) meta.there[n_tile & 7] = (uint8_t)there;
                 n_tile++;
             };
-            auto row_of = [&](int i, int m) { return __shfl_sync(0xFFFFFFFFu, pool_rows, kChunks * (i % kAhead) + w + C::kCopies * m); };
+            auto row_of = [&](int i, int m) { return __shfl_sync(0xFFFFFFFFu, pool_rows, kChunks * (i % kAhead) + w * kMine + m); };
             if constexpr (!kQuant) {
                 // a half tile is TP / box_rows boxes for each 64 values, a lane each
                 const int per = p.box_rows / kChunk, boxes = TP / p.box_rows, box = lane / C::kPanels, panel = lane % C::kPanels;
@@ -1029,45 +1036,65 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     }
                 }
             } else {
-                // 8 and 4 bits: through registers, a piece of 16 bytes at a time; a half tile's pieces are asked for while the one before it is unpacked. What is not
-                // there comes from other rows of the page (or from the queries, without a page) under a scale of zero.
-                constexpr int kSets = kMine * kCopies;
-                uint4 x[kSets];
-                uint16_t d[kSets];
+                // 8 and 4 bits: quants and scales of a warp's chunks come asynchronously, two half tiles ahead, and are unpacked to f16. (Through registers the loads' own
+                // took so many that others went to level 2.) What is not there has a scale of zero.
+                constexpr int SB = scale_bytes_of(CT, D);
                 const int halves = 2 * it.all;
-                auto ask = [&](int t, int m, int j, int64_t row0, uint4 &v, uint16_t &scale) {
-                    const int c = lane + 32 * j, row = c / kPieces;
-                    const bool none = row0 < 0 || (kChunk * kPieces % 32 != 0 && c >= kChunk * kPieces);
-                    const uint8_t *from = none ? static_cast<const uint8_t *>(p.q) : (t & 1 ? p.v : p.k) + row0 * RB + 16 * c;
-                    const __half *s_from = none ? static_cast<const __half *>(p.q) : (t & 1 ? p.v_scale : p.k_scale) + (row0 + row) * (D / 32) + c % kPieces / (CT == KRK_CUDA_KV_Q8 ? 2 : 1);
-                    v = *reinterpret_cast<const uint4 *>(from);
-                    scale = *reinterpret_cast<const uint16_t *>(s_from);
+                uint8_t *raw_mem = smem + C::kRawAt + w * kMine * C::kRawChunk;
+                const uint32_t raw_at = base + C::kRawAt + w * kMine * C::kRawChunk;
+                uint32_t there = 0;   // kMine bits of a half tile, the last asked for lowest
+                auto ask = [&](int t, int raw) {
+                    const int i = t >> 1;
+                    if ((t & 1) == 0) begin_tile(i);
+#pragma unroll
+                    for (int m = 0; m < kMine; m++) {
+                        const int64_t row0 = row_of(i, m);
+                        there = there << 1 | (uint32_t)(row0 >= 0);
+                        if (row0 < 0) continue;
+                        const uint8_t *from = (t & 1 ? p.v : p.k) + row0 * RB + 16 * lane;
+                        const uint32_t to = raw_at + raw * C::kRaw + m * C::kRawChunk + 16 * lane;
+#pragma unroll
+                        for (int j = 0; j < kCopies; j++)
+                            if (kChunk * kPieces % 32 == 0 || lane + 32 * j < kChunk * kPieces) copy16(to + 512 * j, from + 512 * j, true);
+                        if (lane < SB) copy16(to + kChunk * RB, reinterpret_cast<const uint8_t *>(t & 1 ? p.v_scale : p.k_scale) + row0 * SB + 16 * lane, true);
+                    }
                 };
-                begin_tile(0);
-                int64_t rows[kMine];   // of the half tile that is unpacked
-#pragma unroll
-                for (int m = 0; m < kMine; m++) {
-                    rows[m] = row_of(0, m);
-#pragma unroll
-                    for (int j = 0; j < kCopies; j++) ask(0, m, j, rows[m], x[m * kCopies + j], d[m * kCopies + j]);
-                }
+                Ring<C::kRaws> raw;
+                ask(0, 0);
+                copies_commit();
+                ask(1, 1);
+                copies_commit();
 #pragma unroll 1
                 for (int t = 0; t < halves; t++) {
                     const int i = t >> 1;
-                    const bool look = (t & 1) && looked_at(i), more = t + 1 < halves;
+                    if (t + 2 < halves) ask(t + 2, raw.at == 0 ? 2 : raw.at - 1);
+                    else there <<= kMine;
+                    copies_commit();
+                    copies_wait<2>();
+                    const bool look = (t & 1) && looked_at(i);
                     bool bad = false;
-                    if (more && (t & 1)) begin_tile(i + 1);
+                    __syncwarp();
                     wait_idle(meta.kv_empty[to_slot.at], to_slot.turn ^ 1);
-#pragma unroll
+#pragma unroll 1
                     for (int m = 0; m < kMine; m++) {
-                        const int chunk = w + C::kCopies * m, left = rows[m] < 0 ? 0 : it.len - ((it.tile0 + i) * TP + chunk * kChunk);
-                        rows[m] = more ? row_of((t + 1) >> 1, m) : -1;
+                        const int chunk = w * kMine + m, left = there >> (3 * kMine - 1 - m) & 1 ? it.len - ((it.tile0 + i) * TP + chunk * kChunk) : 0;
                         uint8_t *chunk_at = smem + to_slot.at * C::kSlot + chunk * (kChunk * 128);
+                        const uint8_t *from = raw_mem + raw.at * C::kRaw + m * C::kRawChunk;
+                        uint4 x[kCopies];
+                        uint32_t d[kCopies];
 #pragma unroll
                         for (int j = 0; j < kCopies; j++) {
-                            const int c = lane + 32 * j, row = c / kPieces, pc = c % kPieces, n = m * kCopies + j;
-                            const uint32_t words[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
-                            const __half2 s2 = half2_of(row < left ? d[n] * 0x10001u : 0u);
+                            const int c = lane + 32 * j, row = c / kPieces;
+                            x[j] = make_uint4(0u, 0u, 0u, 0u), d[j] = 0;
+                            if (kChunk * kPieces % 32 != 0 && c >= kChunk * kPieces) continue;
+                            x[j] = *reinterpret_cast<const uint4 *>(from + 16 * c);
+                            d[j] = *reinterpret_cast<const uint16_t *>(from + kChunk * RB + row * SB + 2 * (c % kPieces / (CT == KRK_CUDA_KV_Q8 ? 2 : 1)));
+                        }
+#pragma unroll
+                        for (int j = 0; j < kCopies; j++) {
+                            const int c = lane + 32 * j, row = c / kPieces, pc = c % kPieces;
+                            const uint32_t words[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+                            const __half2 s2 = half2_of(row < left ? d[j] * 0x10001u : 0u);
                             constexpr int kUnits = CT == KRK_CUDA_KV_Q8 ? 2 : 4;   // of eight values
                             uint32_t y[4 * kUnits];
 #pragma unroll
@@ -1084,7 +1111,6 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                                     y[8 + 2 * k + 1] = bits(__hmul2(half2_of(halves_of<2, 3>(u2, 0x64086408u)), s2));
                                 }
                             }
-                            if (more) ask(t + 1, m, j, rows[m], x[n], d[n]);
                             if (look) {
 #pragma unroll
                                 for (int k = 0; k < 4 * kUnits; k++) bad |= take_out(y[k]);
@@ -1099,16 +1125,18 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                         }
                     }
                     if (bad) tell_odd(n_item);
-                    if (HALF && t == 0) copies_wait<0>();
                     async_fence();
                     __syncwarp();
                     if (lane == 0) {
-                        if (HALF && t == 0 && as_they_are) bar_arrive(bar(meta.q_full[n_item & 1][0]));
+                        if (HALF && t == 0 && as_they_are) bar_arrive(bar(meta.q_full[0][0]));   // (their copies were asked for before the second half tile's)
                         bar_arrive(bar(meta.kv_full[to_slot.at]));
                     }
                     to_slot.next();
+                    raw.next();
                 }
+                copies_wait<0>();
             }
+            done();
         }
     } else {
         if constexpr (C::kTrade) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
@@ -1169,7 +1197,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 for (int q = 0; q < NQ; q++)
                     if (n[q] > 0) {
                         if (as_they_are) {
-                            if (q == 0) wait(meta.q_full[set][0], n_item >> 1 & 1);
+                            if (q == 0) wait(meta.q_full[set][0], (C::kQSets == 2 ? n_item >> 1 : n_item) & 1);
                         } else {
                             wait_idle(meta.q_full[set][q], q_turns >> (2 * set + q) & 1);
                             q_turns ^= 1u << (2 * set + q);
@@ -1258,7 +1286,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
 
 template <int D, int CT, bool HALF>
 int launch_chunk_one(const ChunkParams &p, cudaStream_t st) {
-    using C = Chunk<D, HALF ? 1 : 2, CT != KRK_CUDA_KV_F16>;
+    using C = Chunk<D, HALF ? 1 : 2, CT>;
     static std::atomic<uint64_t> ready{0};   // devices whose limit of shared memory is raised for this kernel
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
