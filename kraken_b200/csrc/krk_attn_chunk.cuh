@@ -326,7 +326,7 @@ struct Chunk {
     static constexpr int kSoft = 4 * NQ, kCopies = QUANT ? 4 : 2, kProduct = kSoft + kCopies, kFinder = kProduct + 1, kWarps = kSoft + (QUANT ? 8 : 4), kThreads = 32 * kWarps;
     // Registers of a thread, traded between groups of four warps (a spill goes to level 2: shared memory has what level 1 had). Launched with: 384 threads 168, 512 128.
     static constexpr bool kTrade = NQ == 2;
-    static constexpr int kSoftRegs = QUANT ? 168 : 200, kCopyRegs = 104, kOtherRegs = QUANT ? 72 : 104;
+    static constexpr int kSoftRegs = QUANT ? 168 : 200, kCopyRegs = QUANT ? 88 : 104, kOtherRegs = QUANT ? 88 : 104;
     static_assert(256 * kSoftRegs + 128 * (kCopyRegs + (QUANT ? kOtherRegs : 0)) <= (QUANT ? 512 * 128 : 384 * 168) , "registers of a launch");
     static constexpr uint32_t kO = 256;                              // column of the sums; of the second tile's: 128 more
     static constexpr uint32_t kS = NQ == 2 ? 128 : 64;               // from a place of scores to the next
