@@ -37,7 +37,7 @@ struct VerifyParams {
     float *logprob;
     Part *part;               // [1 or 2][n_rows][slices]
     int64_t p_stride, q_stride;
-    int n_rows, n_vocab, n_seq, slices;
+    int n_rows, n_vocab, n_seq, slices, vec;   // vec: rows begin on 16-byte boundaries
 };
 
 // The reciprocal of a temperature; greedy requests: 1.
@@ -119,17 +119,38 @@ verify_stats_kernel(const __grid_constant__ VerifyParams p) {
     }
 }
 
+// e^(x k ln 2 / 64 - ...): exponentials as 2^(t / 64), t = x k + b up to about 0, to 4e-14 of themselves: the whole part of t from a table of 2^(j / 64) and the
+// exponent, the rest, in +-1/2, by the series of e^(r ln 2 / 64) to the fourth power. Below 2^-1000: 0; a NaN stays one.
+constexpr double kSteps = 92.332482616893657;   // 64 / ln 2
+__device__ __forceinline__ double exp_step(double t, const double *table) {
+    constexpr double c = 0.010830424696249145;   // ln 2 / 64
+    const double whole = t + 6755399441055744.0;   // 1.5 * 2^52
+    const double r = t - (whole - 6755399441055744.0);
+    const int n = __double2loint(whole);
+    const double e = fma(r, fma(r, fma(r, fma(r, c * c * c * c / 24.0, c * c * c / 6.0), c * c / 2.0), c), 1.0) * table[n & 63];
+    const double y = __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
+    return t >= -64000.0 ? y : t < -64000.0 ? 0.0 : t;
+}
+__device__ __forceinline__ double exp_of(double a, const double *table) { return exp_step(a * kSteps, table); }
+// log z, z >= 1, from the f32 one by a step of Newton's.
+__device__ __forceinline__ double log_of(double z, const double *table) {
+    const double y = (double)logf((float)z);
+    return y + (z * exp_of(-y, table) - 1.0);
+}
+
 // A row's slices together, by a warp: the maximum, its lowest place, the sum of exponentials.
 struct Row {
     float m;
     int at;
     double sum;
 };
-__device__ __forceinline__ Row row_of(const VerifyParams &p, int item, double inv) {
+__device__ __forceinline__ Row row_of(const VerifyParams &p, int item, double inv, const double *table) {
     const int lane = threadIdx.x & 31;
     const Part *part = p.part + (size_t)item * p.slices;
-    Row r = {-INFINITY, INT32_MAX, 0.0};
-    for (int i = lane; i < p.slices; i += 32) {
+    Part first = {-INFINITY, -1, 0.0};
+    if (lane < p.slices) first = part[lane];
+    Row r = {first.m, first.at >= 0 ? first.at : INT32_MAX, 0.0};
+    for (int i = lane + 32; i < p.slices; i += 32) {
         const Part o = part[i];
         if (o.at >= 0 && (o.m > r.m || r.at == INT32_MAX)) r.at = o.at;
         r.m = fmaxf(r.m, o.m);
@@ -141,23 +162,13 @@ __device__ __forceinline__ Row row_of(const VerifyParams &p, int item, double in
         if (om > r.m || (om == r.m && oa < r.at)) r.m = om, r.at = oa;
     }
     for (int i = lane; i < p.slices; i += 32) {
-        const Part o = part[i];
-        if (o.m != -INFINITY || o.sum != 0.0) r.sum += o.m == -INFINITY ? o.sum : o.sum * exp(((double)o.m - (double)r.m) * inv);
+        const Part o = i == lane ? first : part[i];
+        if (o.m != -INFINITY || o.sum != 0.0) r.sum += o.m == -INFINITY ? o.sum : o.sum * exp_of(((double)o.m - (double)r.m) * inv, table);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) r.sum += __shfl_xor_sync(0xFFFFFFFFu, r.sum, o);
     if (r.m == -INFINITY) r.at = -1;
     return r;
-}
-
-// exp(a), a <= 0, to 4e-14 of itself: 2^(n / 64) from a table, the rest by its series to the fourth power; below e^-700: 0.
-__device__ __forceinline__ double exp_of(double a, const double *table) {
-    if (!(a >= -700.0)) return isnan(a) ? a : 0.0;
-    const double t = rint(a * 92.332482616893657);   // 64 / ln 2
-    const int n = (int)t;
-    const double r = fma(t, -0.010830424696249145, a);   // ln 2 / 64
-    const double e = fma(r, fma(r, fma(r, fma(r, 1.0 / 24.0, 1.0 / 6.0), 0.5), 1.0), 1.0) * table[n & 63];
-    return __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
 }
 
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads)
@@ -166,7 +177,7 @@ verify_draw_kernel(const __grid_constant__ VerifyParams p) {
     __shared__ int s_stop, s_token;
     const cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cluster.block_rank(), s = blockIdx.x / kCluster;
-    if (tid < 64) table[tid] = exp2((double)tid / 64.0);
+    if (tid < 64) table[tid] = exp2((double)tid / 64.0);   // (published by the cluster's meeting)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int r0 = p.row_start[s], r1 = p.row_start[s + 1], rows = r0 >= 0 && r1 <= p.n_rows ? r1 - r0 : 0;
@@ -179,29 +190,27 @@ verify_draw_kernel(const __grid_constant__ VerifyParams p) {
     const double inv_p = fmin(per_temp(p.temp, s), 1e37), inv_q = fmin(per_temp(p.draft_temp ? p.draft_temp : p.temp, s), 1e37);
     if (tid == 0) s_stop = rows - 1, s_token = -1;
     cluster.sync();   // (all blocks are there to be written to)
-    // ---- the drafted tokens, a row a warp
+    // ---- the drafted tokens, a row a warp.
     for (int j = warp; j < rows - 1; j += kDrawWarps) {
         if (j > __shfl_sync(0xFFFFFFFFu, *(volatile int *)&s_stop, 0)) break;   // (an earlier one has been refused)
         const int row = r0 + j, token = p.draft[row];
-        const Row pr = row_of(p, row, inv_p);
+        const Row pr = row_of(p, row, inv_p, table);
         bool ok = token >= 0 && token < p.n_vocab;
-        double lp = 0.0;
         if (ok) {
             const double a = ((double)p.p[row * p.p_stride + token] - (double)pr.m) * inv_p;
-            lp = a - log(pr.sum);
             if (greedy) {
                 ok = pr.at == token;
             } else {
                 double qt = 1.0;
                 if (p.q) {
-                    const Row qr = row_of(p, p.n_rows + row, inv_q);
-                    qt = exp(((double)p.q[row * p.q_stride + token] - (double)qr.m) * inv_q) / qr.sum;
+                    const Row qr = row_of(p, p.n_rows + row, inv_q, table);
+                    qt = exp_of(((double)p.q[row * p.q_stride + token] - (double)qr.m) * inv_q, table) / qr.sum;
                 }
-                ok = (double)p.accept_u[row] * qt < exp(a) / pr.sum;   // (no number: refused)
+                ok = (double)p.accept_u[row] * qt < exp_of(a, table) / pr.sum;   // (no number: refused)
             }
+            if (ok && rank == 0 && p.logprob && lane == 0) p.logprob[row] = (float)(a - log_of(pr.sum, table));
         }
         if (!ok && lane == 0) atomicMin(&s_stop, j);
-        if (ok && lane == 0 && rank == 0 && p.logprob) p.logprob[row] = (float)lp;
     }
     __syncthreads();
     const int stop = s_stop, row = r0 + stop;
@@ -211,16 +220,24 @@ verify_draw_kernel(const __grid_constant__ VerifyParams p) {
     const bool two = p.q && !last;
     int token = -1;
     // (every warp for itself: they all find the same)
-    const Row pr = row_of(p, row, inv_p);
+    const Row pr = row_of(p, row, inv_p, table);
     if (greedy) {
         token = pr.at;
     } else {
-        const Row qr = two ? row_of(p, p.n_rows + row, inv_q) : Row{0.0f, 0, 1.0};
-        // ---- the sums of exponentials in 64 bits: each warp of the cluster has a part of the row
-        const int per = ((p.n_vocab + kParts - 1) / kParts + 31) / 32 * 32, part = rank * kDrawWarps + warp;
+        const Row qr = two ? row_of(p, p.n_rows + row, inv_q, table) : Row{0.0f, 0, 1.0};
+        // ---- the sums of exponentials in 64 bits: each warp of the cluster has a part of the row, a lane eight values of 256 that follow each other
+        const int per = ((p.n_vocab + kParts - 1) / kParts + 7) / 8 * 8, part = rank * kDrawWarps + warp;
         const int lo = min(p.n_vocab, part * per), hi = min(p.n_vocab, lo + per);
-        auto e_p = [&](int i) { return exp_of(((double)x[i] - (double)pr.m) * inv_p, table); };
-        auto e_q = [&](int i) { return exp_of(((double)y[i] - (double)qr.m) * inv_q, table); };
+        const double k_p = inv_p * kSteps, b_p = -(double)pr.m * k_p, k_q = inv_q * kSteps, b_q = -(double)qr.m * k_q;
+        auto load = [&](const float *row, int i0, float (&v)[8]) {
+            if (p.vec && i0 + 8 <= hi) {
+                *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(row + i0);
+                *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(row + i0 + 4);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = i0 + j < hi ? row[i0 + j] : -INFINITY;
+            }
+        };
         auto warp_sum = [&](double v) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
@@ -241,24 +258,46 @@ verify_draw_kernel(const __grid_constant__ VerifyParams p) {
         };
         auto total = [&](const double *v) { return __shfl_sync(0xFFFFFFFFu, upto(v), 31); };
         double a = 0.0, b = 0.0;
-        for (int i = lo + lane; i < hi; i += 32) {
-            a += e_p(i);
-            if (two) b += e_q(i);
+        for (int i0 = lo + 8 * lane; i0 < hi; i0 += 256) {
+            float xp[8], xq[8];
+            load(x, i0, xp);
+            if (two) load(y, i0, xq);
+            double s4[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+            for (int j = 0; j < 8; j++) s4[j & 3] += exp_step(fma((double)xp[j], k_p, b_p), table);
+            a += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+            if (two) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) s4[j] = 0.0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) s4[j & 3] += exp_step(fma((double)xq[j], k_q, b_q), table);
+                b += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+            }
         }
         tell(0, warp_sum(a));
         if (two) tell(1, warp_sum(b));
         cluster.sync();
         const double per_p = 1.0 / total(sums[0]), per_q = two ? 1.0 / total(sums[1]) : 0.0;
         bool whole = !two && certain < 0;   // weights are p
-        auto weight = [&](int i) {
-            if (i == certain && !whole) return 0.0;
-            const double w = e_p(i) * per_p;
-            return two && !whole ? fmax(w - e_q(i) * per_q, 0.0) : w;
+        auto weights = [&](int i0, double (&w)[8]) {
+            float xp[8], xq[8];
+            load(x, i0, xp);
+            if (two && !whole) load(y, i0, xq);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                w[j] = exp_step(fma((double)xp[j], k_p, b_p), table) * per_p;
+                if (two && !whole) w[j] = fmax(w[j] - exp_step(fma((double)xq[j], k_q, b_q), table) * per_q, 0.0);
+                if (i0 + j == certain && !whole) w[j] = 0.0;
+            }
         };
         double all = 0.0;
         for (int round = 0; round < 2; round++) {
             double w = 0.0;
-            for (int i = lo + lane; i < hi; i += 32) w += weight(i);
+            for (int i0 = lo + 8 * lane; i0 < hi; i0 += 256) {
+                double v[8];
+                weights(i0, v);
+                w += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            }
             tell(2, warp_sum(w));
             cluster.sync();
             all = total(sums[2]);
@@ -286,19 +325,34 @@ verify_draw_kernel(const __grid_constant__ VerifyParams p) {
         }
         if (found == part) {
             int at = -1, last_at = -1;
-            for (int i0 = lo; i0 < hi && at < 0; i0 += 32) {
-                const int i = i0 + lane;
-                const double w = i < hi ? weight(i) : 0.0;
-                double so_far = w;
+            for (int i0 = lo; i0 < hi && at < 0; i0 += 256) {
+                double v[8] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
+                if (i0 + 8 * lane < hi) weights(i0 + 8 * lane, v);
+                double upto = 0.0;
+                int mine_last = -1;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    upto += v[j];
+                    if (v[j] > 0.0) mine_last = i0 + 8 * lane + j;
+                }
+                const double own = upto;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
-                    const double v = __shfl_up_sync(0xFFFFFFFFu, so_far, o);
-                    if (lane >= o) so_far += v;
+                    const double u = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+                    if (lane >= o) upto += u;
                 }
-                const unsigned over = __ballot_sync(0xFFFFFFFFu, w > 0.0 && before + so_far > goal), some = __ballot_sync(0xFFFFFFFFu, w > 0.0);
-                if (over) at = i0 + __ffs(over) - 1;
-                if (some) last_at = i0 + 31 - __clz(some);
-                before += __shfl_sync(0xFFFFFFFFu, so_far, 31);
+                // the first lane whose sums pass the number, and of its values the first one
+                double here = before + (upto - own);
+                int mine = -1;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    here += v[j];
+                    if (mine < 0 && v[j] > 0.0 && here > goal) mine = i0 + 8 * lane + j;
+                }
+                const unsigned over = __ballot_sync(0xFFFFFFFFu, mine >= 0), some = __ballot_sync(0xFFFFFFFFu, mine_last >= 0);
+                if (over) at = __shfl_sync(0xFFFFFFFFu, mine, __ffs(over) - 1);
+                if (some) last_at = __shfl_sync(0xFFFFFFFFu, mine_last, 31 - __clz(some));
+                before += __shfl_sync(0xFFFFFFFFu, upto, 31);
             }
             if (at < 0) at = last_at;   // (likewise)
             if (lane == 0) *cluster.map_shared_rank(&s_token, 0) = at;
@@ -309,7 +363,7 @@ verify_draw_kernel(const __grid_constant__ VerifyParams p) {
     if (rank != 0) return;
     for (int j = tid; j < rows; j += kDrawThreads) {
         p.tokens[r0 + j] = j < stop ? p.draft[r0 + j] : j == stop ? token : -1;
-        if (p.logprob && j >= stop) p.logprob[r0 + j] = j == stop && token >= 0 ? (float)(((double)x[token] - (double)pr.m) * inv_p - log(pr.sum)) : 0.0f;
+        if (p.logprob && j >= stop) p.logprob[r0 + j] = j == stop && token >= 0 ? (float)(((double)x[token] - (double)pr.m) * inv_p - log_of(pr.sum, table)) : 0.0f;
     }
     if (tid == 0) p.n_accepted[s] = stop;
 }
@@ -343,6 +397,7 @@ int launch_verify_draft(int32_t *tokens, int32_t *n_accepted, float *logprob, co
     const int64_t blocks = (int64_t)(p.q ? 2 : 1) * p.n_rows * p.slices;
     if (blocks > INT32_MAX || (int64_t)v.n_seq * kCluster > INT32_MAX) return KRK_CUDA_ESHAPE;
     const bool vec = ((reinterpret_cast<uintptr_t>(p.p) | reinterpret_cast<uintptr_t>(p.q)) & 15) == 0 && (v.n_rows == 1 || (v.stride % 4 == 0 && (!p.q || v.draft_stride % 4 == 0)));
+    p.vec = vec;
     if (blocks > 0) {
         const int rc = launched(launch_overlapped(vec ? verify_stats_kernel<true> : verify_stats_kernel<false>, dim3((unsigned)blocks), dim3(kStatThreads), st, p));
         if (rc != KRK_CUDA_OK) return rc;
