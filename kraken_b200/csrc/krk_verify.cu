@@ -9,7 +9,7 @@
 //
 // Where the number falls among a hundred thousand weights, most of them of 1e-6 and less, the sums' own rounding decides: with f32 exponentials (6e-8 each, a sum
 // 2e-8 off) one draw in 250 came out as a neighbour. So the drawn row's weights, their sums and the sums before them have 64 bits (weights to 4e-14). The
-// judgement compares two numbers once, for which f32 exponentials summed in 64 bits do (1e-8 of the rows' sums), with the token's own in 64 bits.
+// judgement compares two numbers once, for which sums of f32 exponentials do (their arguments' rounding: under 1e-6 of a sum), with the token's own in 64 bits.
 #include "krk_common.cuh"
 
 #include <cooperative_groups.h>
@@ -119,8 +119,8 @@ verify_stats_kernel(const __grid_constant__ VerifyParams p) {
     }
 }
 
-// e^(x k ln 2 / 64 - ...): exponentials as 2^(t / 64), t = x k + b up to about 0, to 4e-14 of themselves: the whole part of t from a table of 2^(j / 64) and the
-// exponent, the rest, in +-1/2, by the series of e^(r ln 2 / 64) to the fourth power. Below 2^-1000: 0; a NaN stays one.
+// 2^(t / 64), t <= 0, to 4e-14 of itself: t's whole part by a table of 2^(j / 64) and the exponent, the rest, in +-1/2, by the series of e^(r ln 2 / 64) to the
+// fourth power. Below 2^-1000: 0; a NaN stays one.
 constexpr double kSteps = 92.332482616893657;   // 64 / ln 2
 __device__ __forceinline__ double exp_step(double t, const double *table) {
     constexpr double c = 0.010830424696249145;   // ln 2 / 64
@@ -171,7 +171,7 @@ __device__ __forceinline__ Row row_of(const VerifyParams &p, int item, double in
     return r;
 }
 
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads)
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads, 2)
 verify_draw_kernel(const __grid_constant__ VerifyParams p) {
     __shared__ double table[64], sums[3][kParts];   // [sum of p's exponentials, of q's, of weights][warps of the cluster]: this block writes its own to all of them
     __shared__ int s_stop, s_token;
@@ -228,7 +228,9 @@ verify_draw_kernel(const __grid_constant__ VerifyParams p) {
         // ---- the sums of exponentials in 64 bits: each warp of the cluster has a part of the row, a lane eight values of 256 that follow each other
         const int per = ((p.n_vocab + kParts - 1) / kParts + 7) / 8 * 8, part = rank * kDrawWarps + warp;
         const int lo = min(p.n_vocab, part * per), hi = min(p.n_vocab, lo + per);
-        const double k_p = inv_p * kSteps, b_p = -(double)pr.m * k_p, k_q = inv_q * kSteps, b_q = -(double)qr.m * k_q;
+        const double m_p = pr.m, m_q = qr.m, k_p = inv_p * kSteps, k_q = inv_q * kSteps;
+        auto e_p = [&](float v) { return exp_step(((double)v - m_p) * k_p, table); };   // (the difference first: by a small temperature a product would lose it)
+        auto e_q = [&](float v) { return exp_step(((double)v - m_q) * k_q, table); };
         auto load = [&](const float *row, int i0, float (&v)[8]) {
             if (p.vec && i0 + 8 <= hi) {
                 *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(row + i0);
@@ -257,27 +259,24 @@ verify_draw_kernel(const __grid_constant__ VerifyParams p) {
             return a;
         };
         auto total = [&](const double *v) { return __shfl_sync(0xFFFFFFFFu, upto(v), 31); };
-        double a = 0.0, b = 0.0;
-        for (int i0 = lo + 8 * lane; i0 < hi; i0 += 256) {
-            float xp[8], xq[8];
-            load(x, i0, xp);
-            if (two) load(y, i0, xq);
-            double s4[4] = {0.0, 0.0, 0.0, 0.0};
+        // (weights that are p need not be divided by its sum: it scales them all)
+        double per_p = 1.0, per_q = 0.0;
+        if (two) {
+            double a = 0.0, b = 0.0;
+            for (int i0 = lo + 8 * lane; i0 < hi; i0 += 256) {
+                float xp[8], xq[8];
+                load(x, i0, xp);
+                load(y, i0, xq);
+                double a2[2] = {0.0, 0.0}, b2[2] = {0.0, 0.0};
 #pragma unroll
-            for (int j = 0; j < 8; j++) s4[j & 3] += exp_step(fma((double)xp[j], k_p, b_p), table);
-            a += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-            if (two) {
-#pragma unroll
-                for (int j = 0; j < 4; j++) s4[j] = 0.0;
-#pragma unroll
-                for (int j = 0; j < 8; j++) s4[j & 3] += exp_step(fma((double)xq[j], k_q, b_q), table);
-                b += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                for (int j = 0; j < 8; j++) a2[j & 1] += e_p(xp[j]), b2[j & 1] += e_q(xq[j]);
+                a += a2[0] + a2[1], b += b2[0] + b2[1];
             }
+            tell(0, warp_sum(a));
+            tell(1, warp_sum(b));
+            cluster.sync();
+            per_p = 1.0 / total(sums[0]), per_q = 1.0 / total(sums[1]);
         }
-        tell(0, warp_sum(a));
-        if (two) tell(1, warp_sum(b));
-        cluster.sync();
-        const double per_p = 1.0 / total(sums[0]), per_q = two ? 1.0 / total(sums[1]) : 0.0;
         bool whole = !two && certain < 0;   // weights are p
         auto weights = [&](int i0, double (&w)[8]) {
             float xp[8], xq[8];
@@ -285,8 +284,8 @@ verify_draw_kernel(const __grid_constant__ VerifyParams p) {
             if (two && !whole) load(y, i0, xq);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                w[j] = exp_step(fma((double)xp[j], k_p, b_p), table) * per_p;
-                if (two && !whole) w[j] = fmax(w[j] - exp_step(fma((double)xq[j], k_q, b_q), table) * per_q, 0.0);
+                w[j] = e_p(xp[j]) * per_p;
+                if (two && !whole) w[j] = fmax(w[j] - e_q(xq[j]) * per_q, 0.0);
                 if (i0 + j == certain && !whole) w[j] = 0.0;
             }
         };

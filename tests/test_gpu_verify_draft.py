@@ -125,6 +125,19 @@ def test_temperatures(cuda):
     run(cuda, x, start, draft, au, su, temp=temp, q=q, draft_temp=temp[::-1].copy())
 
 
+def test_temperatures_near_zero(cuda):
+    """Positive temperatures down to the smallest normal one: all the weight on the greatest value, or shared by those that tie, wherever the row lies."""
+    for i, t in enumerate((1e-6, 1e-20, 1e-30, 1.2e-38)):
+        x, start, draft, au, su, temp, q = batch(20 + i, [4, 4, 1, 2], 5000)
+        x += np.float32(17.3)
+        q -= np.float32(5.1)
+        x[start[1], [3, 4100]] = 90.0
+        draft[::2] = x.argmax(1)[::2]
+        run(cuda, x, start, draft, au * 0.5, su, temp=0 * temp + np.float32(t), q=q)
+        run(cuda, x, start, draft, au * 0.5, su, temp=0 * temp + np.float32(t))
+        run(cuda, x, start, draft, au, su, temp=temp, draft_temp=0 * temp + np.float32(t), q=q)
+
+
 def test_numbers_at_their_ends(cuda):
     """0 accepts whatever the target has, 1 and the largest number below it draw the last token there is; equal models accept everything."""
     x, start, draft, au, su, temp, q = batch(2, [5, 5], 4000)
