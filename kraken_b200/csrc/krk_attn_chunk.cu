@@ -9,22 +9,22 @@ namespace {
 // added in the order of the CTAs.
 template <int D, bool HALF>
 __global__ void __launch_bounds__(128)
-chunk_merge_kernel(const __grid_constant__ ChunkParams p) {
-    constexpr int NB = D / 32, R = chunk_rows(D);
+chunk_merge_kernel(const __grid_constant__ ChunkParams p, int R) {   // R: rows of an item
+    constexpr int NB = D / 32;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31, b = blockIdx.x + 1;
     const Shared it = p.shared[b];
     if (it.parts == 0) return;
-    constexpr size_t kPitch = (size_t)2 * R * (D + 2);   // from a CTA's parts to the next one's
+    const size_t pitch = (size_t)2 * R * (D + 2);   // from a CTA's parts to the next one's
     for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < it.n_rows; r += gridDim.y * 4) {
-        const float *others = p.part + (size_t)(b - 1) * kPitch, *first = others + (size_t)R * (D + 2);   // of part 0, of the others
+        const float *others = p.part + (size_t)(b - 1) * pitch, *first = others + (size_t)R * (D + 2);   // of part 0, of the others
         float x[NB], m = -INFINITY, l = 0.0f;
 #pragma unroll
         for (int c = 0; c < NB; c++) x[c] = 0.0f;
 #pragma unroll 2
         for (int i = 0; i < it.parts; i++) {
-            const float *from = i == 0 ? first : others + i * kPitch;
+            const float *from = i == 0 ? first : others + i * pitch;
             float y[NB];
 #pragma unroll
             for (int c = 0; c < NB; c++) y[c] = from[r * D + 32 * c + lane];
@@ -68,7 +68,7 @@ EncodeTiled encode_tiled() {   // looked up once: the library does not link the 
 bool encode_pools(ChunkParams &p, int d) {
     const EncodeTiled encode = encode_tiled();
     if (!encode) return false;
-    p.box_rows = chunk_positions(d);
+    p.box_rows = chunk_positions(d, 1);
     while (p.page_size % p.box_rows) p.box_rows /= 2;
     // (a cache without pages has no memory: a row of the queries, which no copy names)
     const int64_t rows = p.n_pages * p.n_kv * p.page_size;
@@ -97,36 +97,14 @@ void encode_queries(ChunkParams &p, int d, bool half) {
                        half ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int launch_chunk_merge(const ChunkParams &p, int d, bool half, int rows, cudaStream_t st) {
+int launch_chunk_merge(const ChunkParams &p, int d, bool half, int r, int rows, cudaStream_t st) {
     auto kernel = half ? (d == 64 ? chunk_merge_kernel<64, true> : d == 96 ? chunk_merge_kernel<96, true> : d == 128 ? chunk_merge_kernel<128, true>
                           : d == 192 ? chunk_merge_kernel<192, true> : chunk_merge_kernel<256, true>)
                        : (d == 64 ? chunk_merge_kernel<64, false> : d == 96 ? chunk_merge_kernel<96, false> : d == 128 ? chunk_merge_kernel<128, false>
                           : d == 192 ? chunk_merge_kernel<192, false> : chunk_merge_kernel<256, false>);
-    return launched(launch_overlapped(kernel, dim3((unsigned)(p.grid - 1), (unsigned)(rows < 32 ? (rows + 3) / 4 : 8)), dim3(128), st, p));
+    return launched(launch_overlapped(kernel, dim3((unsigned)(p.grid - 1), (unsigned)(rows < 32 ? (rows + 3) / 4 : 8)), dim3(128), st, p, r));
 }
 
-struct ChunkForm {
-    bool tree;          // the kernel of attention_tree, over pieces of 64 tokens
-    int grid, whole, rows, parts;   // parts: pieces of a sequence at most
-    size_t bytes;
-};
-ChunkForm form_of(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, int out_dtype) {
-    ChunkForm f = {};
-    const int d = cache.head_dim, r = chunk_rows(d), tp = chunk_positions(d);
-    const int64_t rows = (int64_t)a.max_q * (a.n_heads / cache.n_kv_heads), blocks = (rows + r - 1) / r;
-    // f32 results over 8- and 4-bit caches: keys and values of 18 bits, which the products of tree attention take as whole numbers and scales
-    f.tree = out_dtype == KRK_CUDA_X_F32 && cache.type != KRK_CUDA_KV_F16;
-    if (f.tree) {
-        f.parts = (a.max_q + KRK_CUDA_MAX_DRAFT - 1) / KRK_CUDA_MAX_DRAFT;
-        return f;
-    }
-    f.whole = a.max_kv_len <= (int64_t)kChunkWholeTiles * tp / 2;
-    const int64_t items = (int64_t)a.n_seq * cache.n_kv_heads * blocks, units = f.whole ? items : items * ((a.max_kv_len + tp - 1) / tp);
-    f.grid = (int)(units < sm_count() ? units : sm_count());
-    f.rows = (int)(rows < r ? rows : r);
-    f.bytes = f.whole ? 0 : shared_bytes(f.grid) + 32 + (size_t)f.grid * 2 * r * (d + 2) * sizeof(float);
-    return f;
-}
 // One piece of 64 tokens of every sequence that has so many is a sequence of tree attention.
 krk_cuda_attention pieces_of(const krk_cuda_attention &a, int parts) {
     krk_cuda_attention t = a;
@@ -135,22 +113,53 @@ krk_cuda_attention pieces_of(const krk_cuda_attention &a, int parts) {
     return t;
 }
 
+constexpr int kChunkLeastRows = 0;
+struct ChunkForm {
+    bool chunk, tree;   // the kernel of chunks; that of attention_tree, over pieces of 64 tokens. Both: the second one where the first one met what it cannot hold
+    int terms;          // of keys and values
+    int grid, whole, rows, parts;   // parts: pieces of a sequence at most
+    size_t bytes, beyond_at;
+};
+ChunkForm form_of(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, int out_dtype) {
+    ChunkForm f = {};
+    f.tree = out_dtype == KRK_CUDA_X_F32 && cache.type != KRK_CUDA_KV_F16;
+    f.terms = f.tree ? 2 : 1;
+    const int d = cache.head_dim, r = chunk_rows(d, f.terms), tp = chunk_positions(d, f.terms);
+    const int64_t rows = (int64_t)a.max_q * (a.n_heads / cache.n_kv_heads), blocks = (rows + r - 1) / r;
+    f.chunk = !f.tree || (d <= 128 && rows > kChunkLeastRows);
+    // f32 results over 8- and 4-bit caches: keys and values of 18 bits, which the products of tree attention take as whole numbers and scales
+    if (f.tree) {
+        f.parts = (a.max_q + KRK_CUDA_MAX_DRAFT - 1) / KRK_CUDA_MAX_DRAFT;
+        f.bytes = attention_tree_workspace_bytes(cache, pieces_of(a, f.parts));
+        if (!f.chunk) return f;
+    }
+    f.whole = a.max_kv_len <= (int64_t)kChunkWholeTiles * tp / 2;
+    const int64_t items = (int64_t)a.n_seq * cache.n_kv_heads * blocks, units = f.whole ? items : items * ((a.max_kv_len + tp - 1) / tp);
+    f.grid = (int)(units < sm_count() ? units : sm_count());
+    f.rows = (int)(rows < r ? rows : r);
+    const size_t bytes = f.whole ? 0 : shared_bytes(f.grid) + 32 + (size_t)f.grid * 2 * r * (d + 2) * sizeof(float);
+    f.beyond_at = ((f.bytes > bytes ? f.bytes : bytes) + 15) / 16 * 16;
+    f.bytes = f.tree ? f.beyond_at + f.grid * sizeof(int) : bytes;
+    return f;
+}
 }   // namespace
 }   // namespace attn
 
 size_t attention_chunk_workspace_bytes(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, int out_dtype) {
     const attn::ChunkForm f = attn::form_of(cache, a, out_dtype);
-    return f.tree ? attention_tree_workspace_bytes(cache, attn::pieces_of(a, f.parts)) : f.bytes;
+    return f.bytes;
 }
 
 int launch_attention_chunk(void *out, int out_dtype, const void *q, int q_dtype, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, void *workspace, cudaStream_t st) {
     const attn::ChunkForm f = attn::form_of(cache, a, out_dtype);
-    const int d = cache.head_dim, r = attn::chunk_rows(d);
-    if (f.tree) {
-        if ((int64_t)a.n_seq * f.parts > INT32_MAX) return KRK_CUDA_ESHAPE;
-        return launch_attention_pieces(static_cast<float *>(out), static_cast<const float *>(q), cache, attn::pieces_of(a, f.parts), f.parts, a.max_q, workspace, st);
-    }
+    const int d = cache.head_dim, r = attn::chunk_rows(d, f.terms);
     attn::ChunkParams p;
+    p.beyond = reinterpret_cast<int *>(static_cast<uint8_t *>(workspace) + f.beyond_at);
+    auto pieces = [&]() {
+        if ((int64_t)a.n_seq * f.parts > INT32_MAX) return KRK_CUDA_ESHAPE;
+        return launch_attention_pieces(static_cast<float *>(out), static_cast<const float *>(q), cache, attn::pieces_of(a, f.parts), f.parts, a.max_q, f.chunk ? p.beyond : nullptr, f.grid, workspace, st);
+    };
+    if (!f.chunk) return pieces();
     p.q = q, p.out = out, p.q_stride = a.q_stride, p.out_stride = a.out_stride;
     p.k = static_cast<const uint8_t *>(cache.k), p.v = static_cast<const uint8_t *>(cache.v);
     p.k_scale = static_cast<const __half *>(cache.k_scale), p.v_scale = static_cast<const __half *>(cache.v_scale);
@@ -170,9 +179,9 @@ int launch_attention_chunk(void *out, int out_dtype, const void *q, int q_dtype,
     // units of work are counted in 64 bits
     const double blocks = ((double)a.max_q * p.group + r - 1) / r, all = (double)a.n_seq * p.n_kv * blocks * 4.0 * p.group * ((double)a.max_kv_len + 2.0 * r + 1024.0);
     if (all > 4e18) return KRK_CUDA_ESHAPE;
-    int rc = cache.type == KRK_CUDA_KV_F16 ? launch_attn_chunk_f16(p, d, p.out_half, st) : cache.type == KRK_CUDA_KV_Q8 ? launch_attn_chunk_q8(p, d, st) : launch_attn_chunk_q4(p, d, st);
-    if (rc == KRK_CUDA_OK && !f.whole && f.grid > 1) rc = attn::launch_chunk_merge(p, d, p.out_half, f.rows, st);
-    return rc;
+    int rc = cache.type == KRK_CUDA_KV_F16 ? launch_attn_chunk_f16(p, d, p.out_half, st) : cache.type == KRK_CUDA_KV_Q8 ? launch_attn_chunk_q8(p, d, p.out_half, st) : launch_attn_chunk_q4(p, d, p.out_half, st);
+    if (rc == KRK_CUDA_OK && !f.whole && f.grid > 1) rc = attn::launch_chunk_merge(p, d, p.out_half, r, f.rows, st);
+    return rc == KRK_CUDA_OK && f.tree ? pieces() : rc;
 }
 
 } // namespace krk_cuda

@@ -25,6 +25,7 @@ struct ChunkParams {
     const int32_t *table, *q_start, *kv_len;
     const float *sinks;
     Shared *shared;                       // [grid]
+    int *beyond;                          // [grid]: 1 where a value of keys or values lay beyond f16 (two terms of 8 and 4 bits)
     float *part;                          // [grid][2]: sums [R][D], maxima (log2) and weights [R][2], on 32-byte boundaries
     int64_t n_pages;
     int table_width, page_size, max_len, n_seq, n_heads, n_kv, group, max_q, window, whole, grid, q_half, out_half, out_wide;   // out_wide: rows of out begin on 32-byte boundaries
@@ -46,9 +47,10 @@ inline void divide_by(int d, uint32_t &mul, uint32_t &shift) {
 }
 __host__ __device__ __forceinline__ int token_of(const ChunkParams &p, int row) { return (int)(((uint64_t)(uint32_t)row * p.group_mul) >> p.group_shift); }
 
-__host__ __device__ constexpr int chunk_tiles_of(int d) { return d <= 128 ? 2 : 1; }           // of rows, 128 each
-__host__ __device__ constexpr int chunk_positions(int d) { return d <= 128 ? 128 : 64; }       // of a tile
-__host__ __device__ constexpr int chunk_rows(int d) { return 128 * chunk_tiles_of(d); }
+// kt: terms of keys and values
+__host__ __device__ constexpr int chunk_tiles_of(int d, int kt) { return d <= 128 && kt == 1 ? 2 : 1; }           // of rows, 128 each
+__host__ __device__ constexpr int chunk_positions(int d, int kt) { return d <= 128 && kt == 1 ? 128 : 64; }       // of a tile
+__host__ __device__ constexpr int chunk_rows(int d, int kt) { return 128 * chunk_tiles_of(d, kt); }
 constexpr int kChunkSetup = 3;        // an item beside its tiles, in tiles
 constexpr int kChunkWholeTiles = 8;   // contexts of up to so many tiles of positions are not divided
 constexpr int kPolyOf8 = 4;           // f16: of eight exponentials, those by a polynomial
@@ -312,12 +314,13 @@ struct ChunkWalk {
 template <int D, int NT, int CT>
 struct Chunk {
     static constexpr bool QUANT = CT != KRK_CUDA_KV_F16;
-    static constexpr int NQ = chunk_tiles_of(D), TP = chunk_positions(D), R = chunk_rows(D);
+    static constexpr int KT = QUANT && NT == 2 ? 2 : 1;              // terms of keys and values: quants times their scales have 18 bits
+    static constexpr int NQ = chunk_tiles_of(D, KT), TP = chunk_positions(D, KT), R = chunk_rows(D, KT);
     static constexpr int kMetaBytes = 1920;
     static constexpr int kPanels = (D + 63) / 64;                    // blocks of 64 values
     static constexpr int kTerm = kPanels * 128 * 128, kQTile = NT * kTerm;
     static constexpr int kQSets = NT == 1 && !QUANT ? 2 : 1, kQSet = NQ * kQTile;   // the queries of this item and, where there is room, of the next one
-    static constexpr int kSlot = kPanels * TP * 128;                 // half a tile: keys or values
+    static constexpr int kSlotTerm = kPanels * TP * 128, kSlot = KT * kSlotTerm;   // half a tile: keys or values
     static constexpr int kRawChunk = QUANT ? kChunk * (row_bytes_of(CT, D) + scale_bytes_of(CT, D)) : 0, kRaws = 3, kRaw = TP / kChunk * kRawChunk;   // 8 and 4 bits as they are: quants and scales of a half tile
     static constexpr int kRoom = 227 * 1024 - 1024 - kMetaBytes - kQSets * kQSet - kRaws * kRaw;
     static constexpr int kSlots = kRoom / kSlot > 6 ? 6 : kRoom / kSlot;
@@ -336,7 +339,7 @@ struct Chunk {
 };
 
 struct ChunkItem {
-    int goes_on, q0, len, before, s, kvh, block, n_rows, tile0, all, tiles[2], all_from, all_to;   // all: its tiles, tiles: that the rows of a tile see; every row sees [all_from, all_to)
+    int goes_on, q0, len, before, s, kvh, block, n_rows, tile0, all, tiles[2], all_from, all_to, any_from;   // all: its tiles, tiles: that the rows of a tile see; every row sees [all_from, all_to), none what is before any_from
     int rows_from[2], rows_to[2];   // every row of a tile of rows sees [rows_from, rows_to)
     bool whole, begins;
 };
@@ -346,7 +349,7 @@ struct ChunkMeta {
     uint32_t odd[2][8];       // of a tile of rows, an item in turn: values of a tile that not all rows see are no numbers
     uint8_t there[8];         // of a tile of positions, in turn: bit c: chunk c is a page's
     uint32_t tmem;
-    int gave_up;
+    int gave_up, beyond;
     ChunkItem item[kChunkItems], mine[2];   // mine: of a tile of rows, what its first thread has read
 };
 // A place of a ring and the parity of its turn.
@@ -464,9 +467,6 @@ __device__ __forceinline__ void products_p(uint32_t d, uint32_t a, uint32_t b_lo
                      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [x3], b1, %3, {%5, %5, %5, %5}, t;\n}\n"
                      ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(onto), "r"(0u), "r"(elected), "r"(kDescHi) : "memory");
 }
-// Bytes I and J of w, as `halves` in krk_attn_kernel.cuh.
-template <int I, int J>
-__device__ __forceinline__ uint32_t halves_of(uint32_t w, uint32_t off) { return halves<I, J>(w, off); }
 // As capped, without a call: the hyperbolic tangent from one exponential (2^-22 off), f32: near zero from its series, whose next term is 2^-26 of it there.
 template <bool HALF>
 __device__ __forceinline__ float capped_here(float x, float cap) {
@@ -577,6 +577,7 @@ __global__ void __launch_bounds__((Chunk<D, HALF ? 1 : 2, CT>::kThreads), 1)
 attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
     constexpr int NT = HALF ? 1 : 2;
     using C = Chunk<D, NT, CT>;
+    constexpr int KT = C::KT;
     using Walk = typename C::Walk;
     constexpr int NQ = C::NQ, TP = C::TP, R = C::R, RB = row_bytes_of(CT, D), kChunks = TP / kChunk;
     constexpr bool kQuant = CT != KRK_CUDA_KV_F16;
@@ -608,13 +609,13 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 for (int j = 0; j < 2; j++) bar_init(bar(meta.q_full[i][j]), as_they_are ? (kQuant ? C::kCopies : 1) : 4);   // [set][tile of rows]
                 bar_init(bar(meta.q_empty[i]), 1);
             }
-            bar_init(bar(meta.q_raw), 1);
+            bar_init(bar(meta.q_raw), kQuant ? C::kCopies : 1);
             bar_init(bar(meta.drained), 1);
             for (int i = 0; i < kChunkItems; i++) {
                 bar_init(bar(meta.item_full[i]), 1);
                 bar_init(bar(meta.item_empty[i]), NQ + C::kCopies + 1);
             }
-            meta.gave_up = 0;
+            meta.gave_up = 0, meta.beyond = 0;
         }
         if (lane < 16) meta.odd[lane >> 3][lane & 7] = 0;
         __syncwarp();
@@ -1039,7 +1040,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 // 8 and 4 bits: quants and scales of a warp's chunks come asynchronously, two half tiles ahead, and are unpacked to f16. (Through registers the loads' own
                 // took so many that others went to level 2.) What is not there has a scale of zero.
                 constexpr int SB = scale_bytes_of(CT, D);
-                const int halves = 2 * it.all;
+                const int half_tiles = 2 * it.all;
                 uint8_t *raw_mem = smem + C::kRawAt + w * kMine * C::kRawChunk;
                 const uint32_t raw_at = base + C::kRawAt + w * kMine * C::kRawChunk;
                 uint32_t there = 0;   // kMine bits of a half tile, the last asked for lowest
@@ -1060,14 +1061,15 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     }
                 };
                 Ring<C::kRaws> raw;
+                bool beyond = false;
                 ask(0, 0);
                 copies_commit();
                 ask(1, 1);
                 copies_commit();
 #pragma unroll 1
-                for (int t = 0; t < halves; t++) {
+                for (int t = 0; t < half_tiles; t++) {
                     const int i = t >> 1;
-                    if (t + 2 < halves) ask(t + 2, raw.at == 0 ? 2 : raw.at - 1);
+                    if (t + 2 < half_tiles) ask(t + 2, raw.at == 0 ? 2 : raw.at - 1);
                     else there <<= kMine;
                     copies_commit();
                     copies_wait<2>();
@@ -1078,6 +1080,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
 #pragma unroll 1
                     for (int m = 0; m < kMine; m++) {
                         const int chunk = w * kMine + m, left = there >> (3 * kMine - 1 - m) & 1 ? it.len - ((it.tile0 + i) * TP + chunk * kChunk) : 0;
+                        const int unseen = KT == 2 ? it.any_from - ((it.tile0 + i) * TP + chunk * kChunk) : 0;
                         uint8_t *chunk_at = smem + to_slot.at * C::kSlot + chunk * (kChunk * 128);
                         const uint8_t *from = raw_mem + raw.at * C::kRaw + m * C::kRawChunk;
                         uint4 x[kCopies];
@@ -1094,33 +1097,45 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                         for (int j = 0; j < kCopies; j++) {
                             const int c = lane + 32 * j, row = c / kPieces, pc = c % kPieces;
                             const uint32_t words[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
-                            const __half2 s2 = half2_of(row < left ? d[j] * 0x10001u : 0u);
+                            const uint32_t scale = row < left ? d[j] : 0u;
+                            const __half2 s2 = half2_of(scale * 0x10001u);
+                            // (two terms: a scale that may take a value beyond f16, of a position that some row sees)
+                            if constexpr (KT == 2) beyond |= (scale & 0x7FFFu) > (CT == KRK_CUDA_KV_Q8 ? 0x5FFFu : 0x6FFFu) && (scale & 0x7C00u) != 0x7C00u && row >= unseen;
                             constexpr int kUnits = CT == KRK_CUDA_KV_Q8 ? 2 : 4;   // of eight values
-                            uint32_t y[4 * kUnits];
+                            uint32_t y[4 * kUnits], rest[KT == 2 ? 4 * kUnits : 1];
+                            auto times = [&](int k, uint32_t quants) {   // (what rounds off a product is exact, and has few bits)
+                                const __half2 x = __hmul2(half2_of(quants), s2);
+                                y[k] = bits(x);
+                                if constexpr (KT == 2) rest[k] = bits(__hfma2(half2_of(quants), s2, __hneg2(x)));
+                            };
 #pragma unroll
                             for (int k = 0; k < 4; k++) {
                                 if constexpr (CT == KRK_CUDA_KV_Q8) {
                                     const uint32_t u = words[k] ^ 0x80808080u;
-                                    y[2 * k] = bits(__hmul2(half2_of(halves_of<0, 1>(u, 0x64806480u)), s2));
-                                    y[2 * k + 1] = bits(__hmul2(half2_of(halves_of<2, 3>(u, 0x64806480u)), s2));
+                                    times(2 * k, halves<0, 1>(u, 0x64806480u));
+                                    times(2 * k + 1, halves<2, 3>(u, 0x64806480u));
                                 } else {
                                     const uint32_t u = words[k] & 0x0F0F0F0Fu, u2 = (words[k] >> 4) & 0x0F0F0F0Fu;
-                                    y[2 * k] = bits(__hmul2(half2_of(halves_of<0, 1>(u, 0x64086408u)), s2));
-                                    y[2 * k + 1] = bits(__hmul2(half2_of(halves_of<2, 3>(u, 0x64086408u)), s2));
-                                    y[8 + 2 * k] = bits(__hmul2(half2_of(halves_of<0, 1>(u2, 0x64086408u)), s2));
-                                    y[8 + 2 * k + 1] = bits(__hmul2(half2_of(halves_of<2, 3>(u2, 0x64086408u)), s2));
+                                    times(2 * k, halves<0, 1>(u, 0x64086408u));
+                                    times(2 * k + 1, halves<2, 3>(u, 0x64086408u));
+                                    times(8 + 2 * k, halves<0, 1>(u2, 0x64086408u));
+                                    times(8 + 2 * k + 1, halves<2, 3>(u2, 0x64086408u));
                                 }
                             }
                             if (look) {
 #pragma unroll
-                                for (int k = 0; k < 4 * kUnits; k++) bad |= take_out(y[k]);
+                                for (int k = 0; k < 4 * kUnits; k++) {
+                                    bad |= take_out(y[k]);
+                                    if constexpr (KT == 2) take_out(rest[k]);
+                                }
                             }
                             if (kChunk * kPieces % 32 != 0 && c >= kChunk * kPieces) continue;
 #pragma unroll
                             for (int k = 0; k < kUnits; k++) {
                                 const int unit = kUnits * pc + k;
-                                *reinterpret_cast<uint4 *>(chunk_at + (unit >> 3) * (TP * 128) + row * 128 + (((unit & 7) ^ (row & 7)) << 4)) =
-                                    make_uint4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
+                                uint8_t *to = chunk_at + (unit >> 3) * (TP * 128) + row * 128 + (((unit & 7) ^ (row & 7)) << 4);
+                                *reinterpret_cast<uint4 *>(to) = make_uint4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
+                                if constexpr (KT == 2) *reinterpret_cast<uint4 *>(to + C::kSlotTerm) = make_uint4(rest[4 * k], rest[4 * k + 1], rest[4 * k + 2], rest[4 * k + 3]);
                             }
                         }
                     }
@@ -1128,13 +1143,14 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     async_fence();
                     __syncwarp();
                     if (lane == 0) {
-                        if (HALF && t == 0 && as_they_are) bar_arrive(bar(meta.q_full[0][0]));   // (their copies were asked for before the second half tile's)
+                        if (t == 0 && (!HALF || as_they_are)) bar_arrive(HALF ? bar(meta.q_full[0][0]) : bar(meta.q_raw));   // (their copies were asked for before the second half tile's)
                         bar_arrive(bar(meta.kv_full[to_slot.at]));
                     }
                     to_slot.next();
                     raw.next();
                 }
                 copies_wait<0>();
+                if (KT == 2 && beyond) meta.beyond = 1;
             }
             done();
         }
@@ -1159,10 +1175,11 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             auto scores = [&](int q, uint32_t t) {   // of the t-th tile of all
                 const uint32_t at = slots_k + keys.at * (C::kSlot >> 4), d = tmem + C::kS * place_of(q, t);
 #pragma unroll
-                for (int term = 0; term < NT; term++)
+                for (int term = 0; term < NT + KT - 1; term++)   // (of two second terms the product is left out: 2^-22 of the first ones')
 #pragma unroll
                     for (int c = 0; c < D; c += 64) {
-                        const uint32_t a = rows_set + q * (C::kQTile >> 4) + term * (C::kTerm >> 4) + (c >> 6) * (128 * 128 >> 4), b = at + (c >> 6) * (TP * 128 >> 4);
+                        const uint32_t a = rows_set + q * (C::kQTile >> 4) + (term == 1 ? C::kTerm >> 4 : 0) + (c >> 6) * (128 * 128 >> 4),
+                                       b = at + (term == 2 ? C::kSlotTerm >> 4 : 0) + (c >> 6) * (TP * 128 >> 4);
                         if (D - c >= 64) products_k<4>(d, a, b, qk, term > 0 || c > 0, elected);
                         else products_k<2>(d, a, b, qk, term > 0 || c > 0, elected);
                     }
@@ -1180,6 +1197,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                         tc_after();
                     }
                     products_p<NT>(t_o + 128 * q, from + c * NT / 2, at + c * 8, pv, onto || c > 0, elected);
+                    if constexpr (KT == 2) products_p<1>(t_o + 128 * q, from + c * NT / 2, at + (C::kSlotTerm >> 4) + c * 8, pv, 1u, elected);
                 }
                 products_commit(bar(meta.pv_done[q]), elected);
             };
@@ -1256,6 +1274,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                         it.q0 = q.q0, it.len = q.len, it.before = q.before, it.s = walk.s, it.kvh = walk.kvh, it.block = walk.block, it.n_rows = walk.n_rows, it.tile0 = walk.tile0, it.all = walk.tiles;
                         it.whole = walk.begins && walk.ends, it.begins = walk.begins;
                         it.all_to = min(q.len, q.before + token_of(p, first) + 1), it.all_from = p.window > 0 ? q.before + token_of(p, last) - p.window + 1 : 0;
+                        it.any_from = p.window > 0 ? q.before + token_of(p, first) - p.window + 1 : 0;
                         // tiles that rows of the first tile of rows see: they end earlier
                         const int end = min(q.len, q.before + token_of(p, min(last, first + 127)) + 1);
                         it.tiles[0] = min(walk.tiles, max((end + TP - 1) / TP - walk.tile0, 1));
@@ -1276,6 +1295,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
     tc_before();
     __syncthreads();
     tc_after();
+    if (KT == 2 && tid == 0) p.beyond[blockIdx.x] = meta.beyond;
     if (warp == C::kProduct && *gave_up) {   // (nobody waits any more, so this is the last word on it)
         products_commit(bar(meta.drained), elected_lane());
         const long long t0 = clock64();
@@ -1312,6 +1332,9 @@ int launch_chunk_one(const ChunkParams &p, cudaStream_t st) {
 }
 template <int CT, bool HALF>
 int launch_chunk_type(const ChunkParams &p, int d, cudaStream_t st) {
+    if constexpr (CT != KRK_CUDA_KV_F16 && !HALF)   // (two terms of queries, keys and values: no room for longer heads)
+        return d == 64 ? launch_chunk_one<64, CT, HALF>(p, st) : d == 96 ? launch_chunk_one<96, CT, HALF>(p, st) : launch_chunk_one<128, CT, HALF>(p, st);
+    else
     switch (d) {
     case 64: return launch_chunk_one<64, CT, HALF>(p, st);
     case 96: return launch_chunk_one<96, CT, HALF>(p, st);
@@ -1325,7 +1348,7 @@ int launch_chunk_type(const ChunkParams &p, int d, cudaStream_t st) {
 
 int launch_attn_chunk_f16(const attn::ChunkParams &p, int head_dim, int half, cudaStream_t st);
 int launch_attn_chunk_f16_half(const attn::ChunkParams &p, int head_dim, cudaStream_t st);
-int launch_attn_chunk_q8(const attn::ChunkParams &p, int head_dim, cudaStream_t st);   // f16 out
-int launch_attn_chunk_q4(const attn::ChunkParams &p, int head_dim, cudaStream_t st);
+int launch_attn_chunk_q8(const attn::ChunkParams &p, int head_dim, int half, cudaStream_t st);
+int launch_attn_chunk_q4(const attn::ChunkParams &p, int head_dim, int half, cudaStream_t st);
 
 }   // namespace krk_cuda

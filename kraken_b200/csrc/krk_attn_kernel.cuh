@@ -206,6 +206,7 @@ attn_kernel(const __grid_constant__ Params p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!called_for(p)) return;
 
     Walk<R> walk;
     walk.start(p);

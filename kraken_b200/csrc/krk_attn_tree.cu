@@ -15,6 +15,7 @@ merge_kernel(const __grid_constant__ Params p, int r_block) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!called_for(p)) return;
     const int b = blockIdx.x + 1;
     const Shared it = p.shared[b];
     if (it.parts == 0) return;
@@ -104,7 +105,7 @@ size_t attention_tree_workspace_bytes(const krk_cuda_kv_cache &cache, const krk_
     return f.whole ? 0 : attn::shared_bytes(f.grid) + (size_t)f.grid * 2 * f.block * (cache.head_dim + 2) * sizeof(float);
 }
 
-int launch_attention_pieces(float *out, const float *q, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, int pieces, int piece_q, void *workspace, cudaStream_t st) {
+int launch_attention_pieces(float *out, const float *q, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, int pieces, int piece_q, const int *only_if, int only_ifs, void *workspace, cudaStream_t st) {
     const attn::Form f = attn::form_of(cache, a);
     attn::Params p;
     p.q = q;
@@ -134,6 +135,8 @@ int launch_attention_pieces(float *out, const float *q, const krk_cuda_kv_cache 
     p.window = a.window;
     p.pieces = pieces;
     p.piece_q = piece_q;
+    p.only_if = only_if;
+    p.only_ifs = only_ifs;
     p.whole = f.whole;
     p.grid = f.grid;
     p.scale = a.scale;
@@ -147,7 +150,7 @@ int launch_attention_pieces(float *out, const float *q, const krk_cuda_kv_cache 
 }
 
 int launch_attention_tree(float *out, const float *q, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, void *workspace, cudaStream_t st) {
-    return launch_attention_pieces(out, q, cache, a, 1, 0, workspace, st);
+    return launch_attention_pieces(out, q, cache, a, 1, 0, nullptr, 0, workspace, st);
 }
 
 } // namespace krk_cuda

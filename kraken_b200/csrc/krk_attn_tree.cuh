@@ -51,7 +51,16 @@ struct Params {
     int pieces, piece_q;                  // a chunk of up to piece_q tokens is so many sequences of max_q; trees: 1 and 0
     float scale, softcap;
     int *status;                          // raised where a bounded wait gives up
+    const int *only_if;                   // nothing is done where all only_ifs of them are 0; trees: null
+    int only_ifs;
 };
+// Whether the launch has anything to do: the same for all threads of a block.
+__device__ __forceinline__ bool called_for(const Params &p) {
+    if (!p.only_if) return true;
+    int any = 0;
+    for (int i = threadIdx.x; i < p.only_ifs; i += blockDim.x) any |= p.only_if[i];
+    return __syncthreads_or(any) != 0;
+}
 
 // The work, in the order of its units: sequences, their key heads, blocks of R rows (items), tiles of positions. The CTAs take equal
 // shares of the units, whatever the lengths are, and a tile belongs to the CTA that has its first unit; where items are not

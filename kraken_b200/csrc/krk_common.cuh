@@ -328,7 +328,9 @@ int launch_kv_read(const krk_cuda_kv_cache &cache, float *k, float *v, const int
 size_t attention_tree_workspace_bytes(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a);
 int launch_attention_tree(float *out, const float *q, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, void *workspace, cudaStream_t st);
 // The same where sequences are chunks of up to piece_q tokens, in `pieces` pieces of a.max_q each (a.n_seq counts pieces, lengths and page tables are the chunks').
-int launch_attention_pieces(float *out, const float *q, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, int pieces, int piece_q, void *workspace, cudaStream_t st);
+// only_if: does nothing unless one of so many numbers there, written by the launches before it, is not 0.
+int launch_attention_pieces(float *out, const float *q, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, int pieces, int piece_q, const int *only_if, int only_ifs, void *workspace,
+                            cudaStream_t st);
 size_t attention_chunk_workspace_bytes(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, int out_dtype);
 int launch_attention_chunk(void *out, int out_dtype, const void *q, int q_dtype, const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, void *workspace, cudaStream_t st);
 // Plan of a step (krk_step.cu), norms between blocks (krk_norm.cu), verification of drafted tokens (krk_verify.cu).

@@ -18,9 +18,11 @@ def attention(q, k, v, seen, scale, softcap=0.0, sinks=None, half=False, quants=
     """One sequence. q [rows, heads, d], k and v [positions, kv heads, d] in 64 bits, seen [rows, positions] -> (out, tolerance).
 
     The tolerance counts, against a = sum(w |v|) / sum(w), with s the scores and S = scale sum|q||k| of the largest position that a row sees:
-      f32: queries in two f16 terms 2^-22 of S; half: f32 queries rounded to 11 bits, 2^-11 of S (f16 ones enter as they are), quants' keys and values
+      f32: queries in two f16 terms 2^-22 of S; over quants, whose values are two terms exactly, the product of both second terms (2^-11 each) is left out,
+      2^-22 of S and of a; half: f32 queries rounded to 11 bits, 2^-11 of S (f16 ones enter as they are), quants' keys and values
       rounded to f16, 2^-11 of S and of a, 2^-25 (f16's last step, halved) sum|q| scale and 2^-25 besides
-      products summed in f32 in steps of 16, truncations included: (d / 16 + 4) 2^-23 S (two terms: twice as many)
+      products summed in f32 in steps of 16, truncations included: (d / 16 + 4) 2^-23 S (two terms: twice as many, over quants three times)
+      half: half of the exponentials are a polynomial's, 7.5e-5 < 2^-13 off, in numerator and denominator
       the score times log2(e), its difference from the reference and the exponential: 2^-23 (|s| + |max|) + 2^-21; tanh by 2^-21 of the softcap
       a weight is off by the sum of these, in numerator and denominator; f32: weights in two f16 terms 2^-22; half: rounded to f16, 2^-11; f16 ends in steps of
       2^-24, and weights are times 2^7 or more under the greatest: 2^-25 / 2^7 max|v| for each position that is seen
@@ -58,11 +60,11 @@ def attention(q, k, v, seen, scale, softcap=0.0, sinks=None, half=False, quants=
         for p in torch.nonzero((bad != 0).any(1)).flatten().tolist():
             o = torch.where(seen[:, p:p + 1] & (bad[p] != 0), o + bad[p], o)
         out[:, h] = o
-        off = (2.0 ** -11 * ((not q_half) + quants) if half else 2.0 ** -22) * size + (d_steps(q) * (1 if half else 2)) * 2.0 ** -23 * size
+        off = (2.0 ** -11 * ((not q_half) + quants) if half else 2.0 ** -22 * (1 + quants)) * size + (d_steps(q) * (1 if half else 3 if quants else 2)) * 2.0 ** -23 * size
         if half and quants:
             off = off + 2.0 ** -25 * qq.abs().sum(1, keepdim=True) * abs(scale)
         off = off + 2.0 ** -23 * (most + top.abs()) + 2.0 ** -21 + softcap * 2.0 ** -21
-        t = a * (2 * off + (2.0 ** -11 * (1 + quants) if half else 2.0 ** -21) + (n / 16 + 300) * 2.0 ** -23) + n * 2.0 ** -32 * vmax / safe.clamp(min=1.0)
+        t = a * (2 * off + (2.0 ** -11 * (1 + quants) + 2.0 ** -12 if half else 2.0 ** -22 * (2 + quants)) + (n / 16 + 300) * 2.0 ** -23) + n * 2.0 ** -32 * vmax / safe.clamp(min=1.0)
         if half:
             t = t + 2.0 ** -11 * o.abs() + 2.0 ** -25 * (2 + quants)
         tol[:, h] = torch.where(n > 0, t, 0)

@@ -177,6 +177,26 @@ def test_values_of_unlike_size(cuda, act):
         b.check(scale=1.0 / q_size / 8)
 
 
+@pytest.mark.parametrize("kind", ["q8", "q4"])
+def test_scales_beyond_the_range_of_f16_values(cuda, kind):
+    """f32 results over quants times scales that pass 65504: what no two f16 terms hold."""
+    b = Batch(cuda, 14, KINDS[kind], 128, 2, 4, 16, [90, 40], [700, 300], "f32")
+    clean = b.check()
+    for name, p in (("v", 3), ("k", 200), ("v", 695)):
+        scale = getattr(b.cache, name + "_scale")
+        was = scale.clone()
+        scale[b.table[0, p // 16].long(), 1, p % 16] = 60000.0
+        if name == "k":
+            b.q *= 2.0 ** -16
+        b.check()
+        if name == "k":
+            b.q *= 2.0 ** 16
+        scale.copy_(was)
+    assert (b.check() == clean).all()
+    b.cache.v_scale[b.table[0, 2].long(), :, 5] = 60000.0   # a position before the window
+    b.check(window=300)
+
+
 def test_strides_streams_and_graphs(cuda):
     """Rows of q and out apart, another stream, two captured graphs that share a workspace and replay on other lengths."""
     import torch
