@@ -113,7 +113,6 @@ krk_cuda_attention pieces_of(const krk_cuda_attention &a, int parts) {
     return t;
 }
 
-constexpr int kChunkLeastRows = 0;
 struct ChunkForm {
     bool chunk, tree;   // the kernel of chunks; that of attention_tree, over pieces of 64 tokens. Both: the second one where the first one met what it cannot hold
     int terms;          // of keys and values
@@ -126,7 +125,10 @@ ChunkForm form_of(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, i
     f.terms = f.tree ? 2 : 1;
     const int d = cache.head_dim, r = chunk_rows(d, f.terms), tp = chunk_positions(d, f.terms);
     const int64_t rows = (int64_t)a.max_q * (a.n_heads / cache.n_kv_heads), blocks = (rows + r - 1) / r;
-    f.chunk = !f.tree || (d <= 128 && rows > kChunkLeastRows);
+    // f32 results over 8 and 4 bits: few rows go to the kernel of attention_tree, as all rows of heads longer than 128 (two terms of queries, keys and values have no
+    // room). Behind 2000 positions, eight sequences of 64 tokens (256 rows of 128 values, 8 bits): 61 us here, 68 there, one sequence 57 and 39; of 128 tokens 76 and
+    // 120, 58 and 67; 4 bits and 64 values, 128 tokens 73 and 77, 56 and 45; 300 tokens 124 and 164, 75 and 85; one token 38 and 13.
+    f.chunk = !f.tree || (d <= 128 && rows * d > 256 * 128);
     // f32 results over 8- and 4-bit caches: keys and values of 18 bits, which the products of tree attention take as whole numbers and scales
     if (f.tree) {
         f.parts = (a.max_q + KRK_CUDA_MAX_DRAFT - 1) / KRK_CUDA_MAX_DRAFT;

@@ -326,7 +326,7 @@ struct Chunk {
     static constexpr int kSlots = kRoom / kSlot > 6 ? 6 : kRoom / kSlot;
     static constexpr int kQ = kSlots * kSlot, kRawAt = kQ + kQSets * kQSet, kMeta = kRawAt + kRaws * kRaw, kBytes = kMeta + kMetaBytes + 1024;   // (begins on a 1024-byte boundary)
     // warps: softmax, copies, products, the one that finds items
-    static constexpr int kSoft = 4 * NQ, kCopies = QUANT ? 4 : 2, kProduct = kSoft + kCopies, kFinder = kProduct + 1, kWarps = kSoft + (QUANT ? 8 : 4), kThreads = 32 * kWarps;
+    static constexpr int kSoft = 4 * NQ, kCopies = KT == 2 ? 8 : QUANT ? 4 : 2, kProduct = kSoft + kCopies, kFinder = kProduct + 1, kWarps = KT == 2 ? kFinder + 1 : kSoft + (QUANT ? 8 : 4), kThreads = 32 * kWarps;
     // Registers of a thread, traded between groups of four warps (a spill goes to level 2: shared memory has what level 1 had). Launched with: 384 threads 168, 512 128.
     static constexpr bool kTrade = NQ == 2;
     static constexpr int kSoftRegs = QUANT ? 168 : 200, kCopyRegs = QUANT ? 88 : 104, kOtherRegs = QUANT ? 88 : 104;
@@ -937,20 +937,27 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
         // ===== keys and values into a ring of half tiles (keys, values in turn). f16: one warp, boxes of 64 values; the other one brings queries. 8 and 4 bits: a warp
         // has a quarter of the chunks of 16 positions
         if constexpr (C::kTrade) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kCopyRegs));
-        constexpr int kMine = kQuant ? kChunks / C::kCopies : 1, kAhead = 32 / kChunks;   // chunks of a warp; tiles whose rows the lanes hold
-        const int w = warp - C::kSoft;
+        // chunks of a warp, or warps of a chunk; tiles whose rows the lanes hold
+        constexpr int kPart = kQuant && C::kCopies > kChunks ? C::kCopies / kChunks : 1, kMine = kQuant && kPart == 1 ? kChunks / C::kCopies : 1, kAhead = 32 / kChunks, kRows = kChunk / kPart;
+        const int w = warp - C::kSoft, row_w = kRows * (w % kPart);   // its first row of a chunk
         int n_item = 0, n_tile = 0;
         Ring<kChunkItems> found;
         Ring<C::kSlots> to_slot;
+        // (also where others have given up: a copy in flight has to land before the block ends)
+        auto landed = [&](uint32_t full, uint32_t parity) {
+            const long long t0 = clock64();
+            while (!bar_try(full, parity) && clock64() - t0 <= kWaitLimit) __nanosleep(32);
+        };
         auto tell_odd = [&](int item) {
             atomicOr(&meta.odd[0][item & 7], 1u);
             atomicOr(&meta.odd[1][item & 7], 1u);
         };
         int64_t pool_rows = 0;   // lane: of chunk lane % kChunks of tile i + lane / kChunks, -1: none
-        constexpr int kPieces = RB / 16, kCopies = (kChunk * kPieces + 31) / 32;
+        constexpr int kPieces = RB / 16, kCopies = (kRows * kPieces + 31) / 32;
         for (;; n_item++, found.next()) {
             wait(meta.item_full[found.at], found.turn);
-            const volatile ChunkItem &it = meta.item[found.at];   // (read where it is wanted: registers)
+            // (read where it is wanted, where registers are few)
+            std::conditional_t<KT == 2, const ChunkItem, const volatile ChunkItem &> it = meta.item[found.at];
             if (!it.goes_on || *gave_up) break;
             auto done = [&] {
                 __syncwarp();
@@ -1015,7 +1022,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 if (w == 0 && lane == 0) meta.there[n_tile & 7] = (uint8_t)there;
                 n_tile++;
             };
-            auto row_of = [&](int i, int m) { return __shfl_sync(0xFFFFFFFFu, pool_rows, kChunks * (i % kAhead) + w * kMine + m); };
+            auto row_of = [&](int i, int m) { return __shfl_sync(0xFFFFFFFFu, pool_rows, kChunks * (i % kAhead) + w / kPart * kMine + m); };
             if constexpr (!kQuant) {
                 // a half tile is TP / box_rows boxes for each 64 values, a lane each
                 const int per = p.box_rows / kChunk, boxes = TP / p.box_rows, box = lane / C::kPanels, panel = lane % C::kPanels;
@@ -1041,23 +1048,23 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 // took so many that others went to level 2.) What is not there has a scale of zero.
                 constexpr int SB = scale_bytes_of(CT, D);
                 const int half_tiles = 2 * it.all;
-                uint8_t *raw_mem = smem + C::kRawAt + w * kMine * C::kRawChunk;
-                const uint32_t raw_at = base + C::kRawAt + w * kMine * C::kRawChunk;
+                uint8_t *raw_mem = smem + C::kRawAt + w * kMine * (C::kRawChunk / kPart);
+                const uint32_t raw_at = base + C::kRawAt + w * kMine * (C::kRawChunk / kPart);
                 uint32_t there = 0;   // kMine bits of a half tile, the last asked for lowest
                 auto ask = [&](int t, int raw) {
                     const int i = t >> 1;
                     if ((t & 1) == 0) begin_tile(i);
 #pragma unroll
                     for (int m = 0; m < kMine; m++) {
-                        const int64_t row0 = row_of(i, m);
-                        there = there << 1 | (uint32_t)(row0 >= 0);
-                        if (row0 < 0) continue;
+                        const int64_t chunk_row = row_of(i, m), row0 = chunk_row + row_w;
+                        there = there << 1 | (uint32_t)(chunk_row >= 0);
+                        if (chunk_row < 0) continue;
                         const uint8_t *from = (t & 1 ? p.v : p.k) + row0 * RB + 16 * lane;
                         const uint32_t to = raw_at + raw * C::kRaw + m * C::kRawChunk + 16 * lane;
 #pragma unroll
                         for (int j = 0; j < kCopies; j++)
-                            if (kChunk * kPieces % 32 == 0 || lane + 32 * j < kChunk * kPieces) copy16(to + 512 * j, from + 512 * j, true);
-                        if (lane < SB) copy16(to + kChunk * RB, reinterpret_cast<const uint8_t *>(t & 1 ? p.v_scale : p.k_scale) + row0 * SB + 16 * lane, true);
+                            if (kRows * kPieces % 32 == 0 || lane + 32 * j < kRows * kPieces) copy16(to + 512 * j, from + 512 * j, true);
+                        if (lane < SB / kPart) copy16(to + kRows * RB, reinterpret_cast<const uint8_t *>(t & 1 ? p.v_scale : p.k_scale) + row0 * SB + 16 * lane, true);
                     }
                 };
                 Ring<C::kRaws> raw;
@@ -1079,9 +1086,9 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                     wait_idle(meta.kv_empty[to_slot.at], to_slot.turn ^ 1);
 #pragma unroll 1
                     for (int m = 0; m < kMine; m++) {
-                        const int chunk = w * kMine + m, left = there >> (3 * kMine - 1 - m) & 1 ? it.len - ((it.tile0 + i) * TP + chunk * kChunk) : 0;
-                        const int unseen = KT == 2 ? it.any_from - ((it.tile0 + i) * TP + chunk * kChunk) : 0;
-                        uint8_t *chunk_at = smem + to_slot.at * C::kSlot + chunk * (kChunk * 128);
+                        const int chunk = w / kPart * kMine + m, left = there >> (3 * kMine - 1 - m) & 1 ? it.len - ((it.tile0 + i) * TP + chunk * kChunk + row_w) : 0;
+                        const int unseen = KT == 2 ? it.any_from - ((it.tile0 + i) * TP + chunk * kChunk + row_w) : 0;
+                        uint8_t *chunk_at = smem + to_slot.at * C::kSlot + chunk * (kChunk * 128) + row_w * 128;
                         const uint8_t *from = raw_mem + raw.at * C::kRaw + m * C::kRawChunk;
                         uint4 x[kCopies];
                         uint32_t d[kCopies];
@@ -1089,9 +1096,9 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                         for (int j = 0; j < kCopies; j++) {
                             const int c = lane + 32 * j, row = c / kPieces;
                             x[j] = make_uint4(0u, 0u, 0u, 0u), d[j] = 0;
-                            if (kChunk * kPieces % 32 != 0 && c >= kChunk * kPieces) continue;
+                            if (kRows * kPieces % 32 != 0 && c >= kRows * kPieces) continue;
                             x[j] = *reinterpret_cast<const uint4 *>(from + 16 * c);
-                            d[j] = *reinterpret_cast<const uint16_t *>(from + kChunk * RB + row * SB + 2 * (c % kPieces / (CT == KRK_CUDA_KV_Q8 ? 2 : 1)));
+                            d[j] = *reinterpret_cast<const uint16_t *>(from + kRows * RB + row * SB + 2 * (c % kPieces / (CT == KRK_CUDA_KV_Q8 ? 2 : 1)));
                         }
 #pragma unroll
                         for (int j = 0; j < kCopies; j++) {
@@ -1129,7 +1136,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                                     if constexpr (KT == 2) take_out(rest[k]);
                                 }
                             }
-                            if (kChunk * kPieces % 32 != 0 && c >= kChunk * kPieces) continue;
+                            if (kRows * kPieces % 32 != 0 && c >= kRows * kPieces) continue;
 #pragma unroll
                             for (int k = 0; k < kUnits; k++) {
                                 const int unit = kUnits * pc + k;
@@ -1154,6 +1161,11 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             }
             done();
         }
+        // (what others, having given up, have not waited for)
+        if (*gave_up && !kQuant && w == 0)
+            for (int i = 0; i < C::kSlots; i++) landed(bar(meta.kv_full[i]), i < to_slot.at ? to_slot.turn : to_slot.turn ^ 1);
+        if (*gave_up && w == (kQuant ? 0 : 1) && n_item > 0 && (!HALF || as_they_are))
+            landed(HALF ? bar(meta.q_full[C::kQSets == 2 ? (n_item - 1) & 1 : 0][0]) : bar(meta.q_raw), (C::kQSets == 2 ? (n_item - 1) >> 1 : n_item - 1) & 1);
     } else {
         if constexpr (C::kTrade) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
         if (warp == C::kProduct) {
