@@ -117,7 +117,7 @@ struct ChunkForm {
     bool chunk, tree;   // the kernel of chunks; that of attention_tree, over pieces of 64 tokens. Both: the second one where the first one met what it cannot hold
     int terms;          // of keys and values
     int grid, whole, rows, parts;   // parts: pieces of a sequence at most
-    size_t bytes, beyond_at;
+    size_t bytes, runs_at, beyond_at;
 };
 ChunkForm form_of(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, int out_dtype) {
     ChunkForm f = {};
@@ -139,7 +139,9 @@ ChunkForm form_of(const krk_cuda_kv_cache &cache, const krk_cuda_attention &a, i
     const int64_t items = (int64_t)a.n_seq * cache.n_kv_heads * blocks, units = f.whole ? items : items * ((a.max_kv_len + tp - 1) / tp);
     f.grid = (int)(units < sm_count() ? units : sm_count());
     f.rows = (int)(rows < r ? rows : r);
-    const size_t bytes = f.whole ? 0 : shared_bytes(f.grid) + 32 + (size_t)f.grid * 2 * r * (d + 2) * sizeof(float);
+    size_t bytes = f.whole ? 0 : shared_bytes(f.grid) + 32 + (size_t)f.grid * 2 * r * (d + 2) * sizeof(float);
+    f.runs_at = (bytes + 15) / 16 * 16;
+    if (!f.whole && out_dtype == KRK_CUDA_X_F32) bytes = f.runs_at + (size_t)f.grid * r * (d + 1) * sizeof(float);
     f.beyond_at = ((f.bytes > bytes ? f.bytes : bytes) + 15) / 16 * 16;
     f.bytes = f.tree ? f.beyond_at + f.grid * sizeof(int) : bytes;
     return f;
@@ -169,6 +171,7 @@ int launch_attention_chunk(void *out, int out_dtype, const void *q, int q_dtype,
     p.sinks = static_cast<const float *>(a.sinks);
     p.shared = static_cast<attn::Shared *>(workspace);
     p.part = f.whole ? nullptr : reinterpret_cast<float *>((reinterpret_cast<uintptr_t>(workspace) + attn::shared_bytes(f.grid) + 31) & ~(uintptr_t)31);
+    p.runs = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + f.runs_at), p.run_tops = p.runs + (size_t)f.grid * r * d;
     p.n_pages = cache.n_pages, p.table_width = a.table_width, p.page_size = cache.page_size, p.max_len = (int)a.max_kv_len, p.n_seq = a.n_seq, p.n_heads = a.n_heads;
     p.n_kv = cache.n_kv_heads, p.group = a.n_heads / cache.n_kv_heads, p.max_q = a.max_q, p.window = a.window, p.whole = f.whole, p.grid = f.grid;
     p.out_wide = (reinterpret_cast<uintptr_t>(out) | (uintptr_t)(a.out_stride * (out_dtype == KRK_CUDA_X_F16 ? 2 : 4))) % 32 == 0;

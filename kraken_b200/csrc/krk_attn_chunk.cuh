@@ -27,6 +27,7 @@ struct ChunkParams {
     Shared *shared;                       // [grid]
     int *beyond;                          // [grid]: 1 where a value of keys or values lay beyond f16 (two terms of 8 and 4 bits)
     float *part;                          // [grid][2]: sums [R][D], maxima (log2) and weights [R][2], on 32-byte boundaries
+    float *runs, *run_tops;               // f32: [grid][R][D] sums of the runs of tiles behind an item's last one, [grid][R] their references (log2)
     int64_t n_pages;
     int table_width, page_size, max_len, n_seq, n_heads, n_kv, group, max_q, window, whole, grid, q_half, out_half, out_wide;   // out_wide: rows of out begin on 32-byte boundaries
     uint32_t group_mul, group_shift;      // row / group = row * group_mul >> group_shift, rows below 2^30
@@ -336,6 +337,11 @@ struct Chunk {
     static_assert(kSlots >= 3, "a half tile of values and one of keys at work, one on its way");
     static_assert(kBytes <= 227 * 1024, "shared memory");
     using Walk = ChunkWalk<R, TP>;
+    // f32: tiles whose values are summed in tensor memory. Its sums are cut off, not rounded: a step of 16 positions and a term loses half a last place of the sum on the average,
+    // always towards zero, and behind 5000 positions three terms' steps had lost 1.6e-5. So sums of runs are added up in registers and kept in memory, a row a thread.
+    // Products with second terms have sums of their own where there is room, so that they cut nothing off the others (7.5e-6 against 16,000, runs of 1024; with their own).
+    static constexpr int kRun = 2048 / TP;
+    static constexpr bool kApart = KT == 2;
 };
 
 struct ChunkItem {
@@ -538,6 +544,40 @@ __device__ __forceinline__ void soft_limit(uint32_t t_s, float sc, float cap) {
         tmem_store16(t_s + c, v);
     }
     tmem_stored();
+}
+// A row's sums out of tensor memory, under the reference m, onto those that are kept under another one. Nobody else adds to them: additions in memory come in the
+// order of the runs, and their thread does not wait for them. (Read, added to and written back they took a tenth of the time.)
+template <int D, bool APART>
+__device__ __forceinline__ void add_run(uint32_t t_o, float *kept, float *kept_top, float m, bool onto) {
+    if (onto && __any_sync(0xFFFFFFFFu, *kept_top != m)) {
+        const float top = *kept_top, f = top == -INFINITY ? 0.0f : ex2(top - m);
+#pragma unroll 1
+        for (int c = 0; c < D; c += 4) {
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(kept + c));   // (level 2, where the additions are)
+            *reinterpret_cast<float4 *>(kept + c) = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+        }
+        __syncwarp();
+    }
+#pragma unroll 1
+    for (int c = 0; c < D; c += 16) {
+        uint32_t o[16], rest[APART ? 16 : 1];
+        tmem_load16(t_o + c, o);
+        if constexpr (APART) tmem_load16(t_o + 128 + c, rest);
+        tmem_loaded();
+        if constexpr (APART)
+#pragma unroll
+            for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) + __uint_as_float(rest[j]));
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            if (onto)
+                asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};"
+                             ::"l"(kept + c + j), "f"(__uint_as_float(o[j])), "f"(__uint_as_float(o[j + 1])), "f"(__uint_as_float(o[j + 2])), "f"(__uint_as_float(o[j + 3])) : "memory");
+            else
+                *reinterpret_cast<uint4 *>(kept + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+        }
+    }
+    *kept_top = m;
+    __syncwarp();
 }
 // Values that are no numbers, in tiles that not all rows of an item see, were taken out of the products: here they are, for the rows that see them. A thread's
 // row sees [pos0, end); tiles that every row sees were left as they are.
@@ -751,6 +791,12 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 const uint32_t there = *reinterpret_cast<volatile uint8_t *>(&meta.there[tile_no & 7]);
                 masked |= there != (1u << kChunks) - 1u;
                 float f = sc;
+                if (!HALF && i > 0 && i % C::kRun == 0) {   // a run's sums leave tensor memory (its last products are behind the one before them, whose end s_full has told)
+                    wait(meta.pv_done[tq], (n_tile - 1) & 1);
+                    tc_after();
+                    const size_t at = (size_t)blockIdx.x * R + 128 * tq + r_in;
+                    add_run<D, C::kApart>(t_o, p.runs + at * D, p.run_tops + at, m, i > C::kRun);
+                }
                 // What is rarely done has code of its own, and no more of it than has to be: code that is jumped over, or met for the first time, is fetched at
                 // the pace of thousands of clocks.
                 if (p.softcap > 0.0f) {   // log2 scores in place of the products
@@ -786,7 +832,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                         wait(meta.pv_done[tq], (n_tile - 1) & 1);
                         tc_after();
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 16) {
+                        for (int c = 0; c < (C::kApart ? D + 128 : D); c += 16) {   // (apart: the second terms' 128 columns on; what is between does not matter)
                             uint32_t o[16];
                             tmem_load16(t_o + c, o);
                             tmem_loaded();
@@ -898,17 +944,40 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             wait(meta.pv_done[tq], (n_tile - 1) & 1);
             tc_after();
             if (*reinterpret_cast<volatile uint32_t *>(&meta.odd[tq][n_item & 7]) != 0) add_odd<CT, D, TP>(p, it, t_o, max(from, tile0 * TP), min(behind, (tile0 + tiles) * TP));
+            const float *run = nullptr;   // the sums of the runs before
+            float run_f = 0.0f;
+            if (!HALF && tiles > C::kRun) {
+                const size_t at = (size_t)blockIdx.x * R + 128 * tq + r_in;
+                const float top = p.run_tops[at];
+                run = p.runs + at * D, run_f = top == -INFINITY ? 0.0f : ex2(top - m);
+            }
             const int rr = row0 + min(r_in, mine_rows - 1), token = token_of(p, rr);
             const int64_t to = (int64_t)(q0 + token) * p.out_stride + (int64_t)(kvh * p.group + rr - token * p.group) * D;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
                 tmem_load32(t_o + c, o);
-                tmem_loaded();
+                if constexpr (C::kApart) {
+                    uint32_t rest[32];
+                    tmem_load32(t_o + 128 + c, rest);
+                    tmem_loaded();
+#pragma unroll
+                    for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) + __uint_as_float(rest[j]));
+                } else {
+                    tmem_loaded();
+                }
                 if (r_in < mine_rows) {
                     if (!HALF || !whole) {
                         float *at = (whole ? static_cast<float *>(p.out) + to : part + (128 * tq + r_in) * D) + c;
                         const int wide = whole ? p.out_wide : 1;
+                        if (!HALF && run) {
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4) {
+                                const float4 x = __ldcg(reinterpret_cast<const float4 *>(run + c + j));
+                                o[j] = __float_as_uint(fmaf(x.x, run_f, __uint_as_float(o[j]))), o[j + 1] = __float_as_uint(fmaf(x.y, run_f, __uint_as_float(o[j + 1])));
+                                o[j + 2] = __float_as_uint(fmaf(x.z, run_f, __uint_as_float(o[j + 2]))), o[j + 3] = __float_as_uint(fmaf(x.w, run_f, __uint_as_float(o[j + 3])));
+                            }
+                        }
 #pragma unroll
                         for (int j = 0; j < 32; j += 8) {
                             uint32_t w[8];
@@ -1187,13 +1256,14 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
             auto scores = [&](int q, uint32_t t) {   // of the t-th tile of all
                 const uint32_t at = slots_k + keys.at * (C::kSlot >> 4), d = tmem + C::kS * place_of(q, t);
 #pragma unroll
-                for (int term = 0; term < NT + KT - 1; term++)   // (of two second terms the product is left out: 2^-22 of the first ones')
+                for (int term = NT + KT - 2; term >= 0; term--)   // (those with second terms first: sums lose last places of what they are by then; both second terms' is left out, 2^-22)
 #pragma unroll
                     for (int c = 0; c < D; c += 64) {
                         const uint32_t a = rows_set + q * (C::kQTile >> 4) + (term == 1 ? C::kTerm >> 4 : 0) + (c >> 6) * (128 * 128 >> 4),
                                        b = at + (term == 2 ? C::kSlotTerm >> 4 : 0) + (c >> 6) * (TP * 128 >> 4);
-                        if (D - c >= 64) products_k<4>(d, a, b, qk, term > 0 || c > 0, elected);
-                        else products_k<2>(d, a, b, qk, term > 0 || c > 0, elected);
+                        const uint32_t onto = term < NT + KT - 2 || c > 0;
+                        if (D - c >= 64) products_k<4>(d, a, b, qk, onto, elected);
+                        else products_k<2>(d, a, b, qk, onto, elected);
                     }
                 products_commit(bar(meta.s_full[place_of(q, t)]), elected);
             };
@@ -1208,11 +1278,17 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                         wait(meta.p_full[place_of(q, t)], phase);
                         tc_after();
                     }
-                    products_p<NT>(t_o + 128 * q, from + c * NT / 2, at + c * 8, pv, onto || c > 0, elected);
-                    if constexpr (KT == 2) products_p<1>(t_o + 128 * q, from + c * NT / 2, at + (C::kSlotTerm >> 4) + c * 8, pv, 1u, elected);
+                    if constexpr (C::kApart) {
+                        products_p<1>(t_o, from + c, at + c * 8, pv, onto || c > 0, elected);
+                        products_p<1>(t_o + 128, from + c + 16, at + c * 8, pv, onto || c > 0, elected);
+                        products_p<1>(t_o + 128, from + c, at + (C::kSlotTerm >> 4) + c * 8, pv, 1u, elected);
+                    } else {
+                        products_p<NT>(t_o + 128 * q, from + c * NT / 2, at + c * 8, pv, onto || c > 0, elected);
+                    }
                 }
                 products_commit(bar(meta.pv_done[q]), elected);
             };
+            auto onto = [&](int i) { return HALF ? i > 0 : i % C::kRun != 0; };
             auto keys_there = [&] { wait(meta.kv_full[keys.at], keys.turn); };
             auto values_there = [&] { wait(meta.kv_full[values.at], values.turn); };
             for (;; found.next()) {
@@ -1249,12 +1325,12 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                             if (i + 2 == all) products_commit(bar(meta.q_empty[set]), elected);
                         }
                         values_there();
-                        sums(0, n_tile[0] + i, i > 0);
+                        sums(0, n_tile[0] + i, onto(i));
                     } else {
                         values_there();
 #pragma unroll
                         for (int q = 0; q < NQ; q++) {
-                            if (i < n[q]) sums(q, n_tile[q] + i, i > 0);
+                            if (i < n[q]) sums(q, n_tile[q] + i, onto(i));
                             if (q == 0 && more) keys_there();
                             if (i + 1 < n[q]) scores(q, n_tile[q] + i + 1);
                         }

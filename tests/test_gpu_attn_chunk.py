@@ -197,6 +197,19 @@ def test_scales_beyond_the_range_of_f16_values(cuda, kind):
     b.check(window=300)
 
 
+@pytest.mark.parametrize("kind,d", [("f16", 128), ("f16", 64), ("f16", 256), ("q8", 128), ("q4", 96)])
+def test_sums_over_many_positions(cuda, kind, d):
+    """f32: products' sums are cut off at 2^-23 of what they have come to, which a run of 256 steps' worth of positions bounds at 256 / 2 * 2^-23 (sums that grow evenly,
+    of values of one sign), however many positions there are; 5 * 2^-20 beside that (weights and values in two terms, exponentials of scores below 2)."""
+    b = Batch(cuda, 21, KINDS[kind], d, 1, 4, 64, [200, 64], [20000, 9000], "f32", q_size=0.1, spread=False)
+    torch = b.torch
+    x = torch.randn((2, b.cache.n_pages * 64, 1, d), device="cuda")
+    cuda.kv_append(b.cache, x[0], x[1].abs() + 2, torch.arange(b.cache.n_pages * 64, device="cuda"))
+    got = b.check().double()
+    want, _, rows = b.want(d ** -0.5)
+    assert float(((got - want[:rows]).abs() / want[:rows]).max()) <= 128 * 2.0 ** -23 + 5 * 2.0 ** -20
+
+
 def test_strides_streams_and_graphs(cuda):
     """Rows of q and out apart, another stream, two captured graphs that share a workspace and replay on other lengths."""
     import torch
