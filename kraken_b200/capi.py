@@ -525,6 +525,8 @@ def block_norm(x, weight=None, residual=None, post_weight=None, post_norm=None, 
                h_out=None, out=None, stream=None):
     """Between two blocks: h = residual + alpha * gate * P(x), y = norm(h) * (offset + weight); P(x) the norm of x times (offset + post_weight), or x where there
     is neither post_weight nor post_norm. x, residual f32 [rows, n]; gate f32 [n] or [rows, n]. Returns (y, h), y f32 or (dtype=torch.float16) f16."""
+    if dtype not in (None, torch.float32, torch.float16) or (dtype is not None and out is not None and out.dtype != dtype):
+        raise ValueError("block_norm: dtype is float32 or float16, and that of out")
     return _fc.block_norm(x, weight, residual, post_weight, post_weight is not None if post_norm is None else post_norm, gate, alpha, eps, offset, dtype is torch.float16, h_out,
                           out, stream)
 
