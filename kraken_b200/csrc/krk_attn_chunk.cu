@@ -108,7 +108,7 @@ int launch_chunk_merge(const ChunkParams &p, int d, bool half, int r, int rows, 
 // One piece of 64 tokens of every sequence that has so many is a sequence of tree attention.
 krk_cuda_attention pieces_of(const krk_cuda_attention &a, int parts) {
     krk_cuda_attention t = a;
-    t.n_seq = a.n_seq * parts;
+    t.n_seq = (int)((int64_t)a.n_seq * parts < INT32_MAX ? (int64_t)a.n_seq * parts : INT32_MAX);   // (more are refused)
     t.max_q = a.max_q < KRK_CUDA_MAX_DRAFT ? a.max_q : KRK_CUDA_MAX_DRAFT;
     return t;
 }
@@ -159,8 +159,8 @@ int launch_attention_chunk(void *out, int out_dtype, const void *q, int q_dtype,
     const int d = cache.head_dim, r = attn::chunk_rows(d, f.terms);
     attn::ChunkParams p;
     p.beyond = reinterpret_cast<int *>(static_cast<uint8_t *>(workspace) + f.beyond_at);
+    if (f.tree && (int64_t)a.n_seq * f.parts > INT32_MAX) return KRK_CUDA_ESHAPE;
     auto pieces = [&]() {
-        if ((int64_t)a.n_seq * f.parts > INT32_MAX) return KRK_CUDA_ESHAPE;
         return launch_attention_pieces(static_cast<float *>(out), static_cast<const float *>(q), cache, attn::pieces_of(a, f.parts), f.parts, a.max_q, f.chunk ? p.beyond : nullptr, f.grid, workspace, st);
     };
     if (!f.chunk) return pieces();

@@ -3,10 +3,20 @@
 //
 //   out[r] = sum_p w_rp v_p / sum_p w_rp,   w_rp = exp(score_rp - max),   score = scale * q_r . k_p,   p up to r's own position
 //
-// A row is a (token, query head) pair; the `group` query heads of a key head are rows of one product. A block of threads has two tiles of 128 rows (one, for
-// heads of more than 128 values) and goes through tiles of positions: S = Q K^T with the rows as the lanes of tensor memory, so that a thread of the
-// softmax has a row to itself; the weights go back to the place of the scores as the operand of O += P V. While one tile of rows is in its softmax the
-// products of the other one run. Keys and values lie in shared memory in the 128-byte swizzle, keys as rows (K-major), values read across (MN-major).
+// A row is a (token, query head) pair; the `group` query heads of a key head are rows of one product. A block of threads has two tiles of 128 rows and goes
+// through tiles of 128 positions: S = Q K^T with the rows as the lanes of tensor memory, so that a thread of the softmax has a row to itself; the weights go
+// back to the place of the scores as the operand of O += P V. While one tile of rows is in its softmax the products of the other one run. Where shared memory has
+// no room for that (heads of more than 128 values, two terms of keys and values) it is one tile of rows and tiles of 64 positions, with two places of scores in
+// turn. Keys and values lie in shared memory in the 128-byte swizzle, keys as rows (K-major), values read across (MN-major).
+//
+// The reference that a softmax subtracts stands until a score passes it by 2^8: the sums in tensor memory are rescaled a few times a row, not each tile. The work
+// is divided by what blocks of rows cost (ChunkWalk), partial sums of divided items are added up by a second kernel in the order of the blocks.
+//
+// Bound: tensor pipe and power for f16 results of long chunks: 4096 tokens behind 8192, 32 heads of 128 over 8, 630 to 700 us by the card's temperature (980 to 1090
+// TFLOP/s; cuBLAS sustains 1372 on this card). There the exponential unit is as busy as the tensor pipe, so half of the exponentials are a polynomial's (604 -> 548 us for 8192 tokens).
+// f32 results take two terms of queries and weights, twice the products: 2048 tokens 121 us (2 x 283 TFLOP/s), 8192 tokens 980 to 1040. Over 8 and 4 bits what unpacks
+// the quants is the limit: 24 ragged sequences of up to 512 tokens behind up to 8000, 8 bits, 550 us; 4096 behind 8192 965; f32, three products, two chunks of up to 700
+// behind 5000, 420. Few tokens: a launch, pages, one item's latency: 33 tokens 23 us.
 #pragma once
 
 #include <cuda.h>
@@ -169,9 +179,39 @@ struct ChunkWalk {
         r.tile = tile_at(in_head - from, (lo == q.blocks - 1 ? c.last : c.prefix(lo + 1) - from), tiles, p.whole);
         return r;
     }
+    // Undivided items, no more of them than blocks of threads: each has one, whatever it costs. (Units and places would take 9000 clocks, most of them for fetching code.)
+    __device__ __forceinline__ bool start_with_one(const ChunkParams &p) {
+        const int lane = threadIdx.x & 31, me = (int)blockIdx.x;
+        ChunkPlace mine = {p.n_seq, 0, 0, 0};
+        int64_t before = 0;
+        for (int s0 = 0; s0 < p.n_seq; s0 += 32) {
+            const int blocks = s0 + lane < p.n_seq ? chunk_sequence<R>(p, s0 + lane).blocks : 0;
+            const int64_t items = (int64_t)blocks * p.n_kv;
+            int64_t upto = items;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const int64_t off = me - (before + upto - items);
+            const uint32_t here = __ballot_sync(0xFFFFFFFFu, off >= 0 && off < items);
+            if (here) {
+                const int l = __ffs(here) - 1, n = __shfl_sync(0xFFFFFFFFu, blocks, l), item = (int)__shfl_sync(0xFFFFFFFFu, off, l);
+                mine = {s0 + l, item / n, item % n, 0};
+            }
+            before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+            if (before > (int64_t)gridDim.x) return false;
+        }
+        total = before, grid = (int)before, cta = me, first_unit = 0, behind_unit = 1, per_cta = 1.0;
+        ChunkPlace behind = mine;
+        behind.tile = INT_MAX;
+        begin(p, mine, behind, 0);
+        return true;
+    }
     // By a warp.
     __device__ __forceinline__ void start(const ChunkParams &p) {
         const int lane = threadIdx.x & 31;
+        if (p.whole && start_with_one(p)) return;
         auto units = [&](int s0) { return s0 + lane < p.n_seq ? p.n_kv * chunk_cost<R, TP>(p, chunk_sequence<R>(p, s0 + lane)).head : 0; };
         int64_t mine = 0;
         total = 0;
@@ -337,9 +377,10 @@ struct Chunk {
     static_assert(kSlots >= 3, "a half tile of values and one of keys at work, one on its way");
     static_assert(kBytes <= 227 * 1024, "shared memory");
     using Walk = ChunkWalk<R, TP>;
-    // f32: tiles whose values are summed in tensor memory. Its sums are cut off, not rounded: a step of 16 positions and a term loses half a last place of the sum on the average,
-    // always towards zero, and behind 5000 positions three terms' steps had lost 1.6e-5. So sums of runs are added up in registers and kept in memory, a row a thread.
-    // Products with second terms have sums of their own where there is room, so that they cut nothing off the others (7.5e-6 against 16,000, runs of 1024; with their own).
+    // f32: tiles whose values are summed in tensor memory. Its sums are cut off, not rounded: a step of 16 positions loses up to a last place of what the sum has come to,
+    // always towards zero, and behind 5000 positions three terms' steps had lost 1.6e-5. So the sums of a run go to memory, where runs are added in f32. Products with second
+    // terms have sums of their own where there is room (8 bits, 8600 positions of values of one sign: 5.7e-6; in one sum, with runs of 1024, 7.3e-6). 4096 tokens behind 8192
+    // take 5 to 10 % longer than without.
     static constexpr int kRun = 2048 / TP;
     static constexpr bool kApart = KT == 2;
 };

@@ -4,7 +4,11 @@
 //
 // Bound: reading x and the residual and writing h and y once. A block of threads has a row in registers from its loads to the last store: the two sums of
 // squares are a shuffle and a trip through shared memory each. Sums are f32, a thread's values first, then a tree. Weights and a shared gate come out of level 2.
+// Measured: one row of 4096 5.7 us (a launch; two trips to memory); 2048 rows, f16 out, two norms and a gate 25.4 us, 4.6 TB/s of 6.5. There two groups of four
+// values a thread are best: one (1024 threads a row) 29.5, four 27.6, eight 37.2.
 #include "krk_common.cuh"
+
+#include <atomic>
 
 namespace krk_cuda {
 
@@ -29,6 +33,10 @@ __device__ __forceinline__ float block_sum(float v, float *part) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
     return v;
+}
+
+__device__ __forceinline__ void copy16_ahead(void *to, const void *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
 
 // VEC values at a time, PER times a thread; PER 0: rows wider than the registers of a block, walked again for each step (h and then x from memory).
@@ -167,6 +175,114 @@ block_norm_kernel(const __grid_constant__ NormParams p) {
     }
 }
 
+// Many rows: blocks that stay, two a multiprocessor, each with every gridDim.x-th row. A thread's values of the next two rows are on their way while it works on one
+// (asynchronous copies into places of its own in shared memory, which nobody else reads), weights and a shared gate stay in its registers.
+template <int PER>
+__global__ void __launch_bounds__(512, 2)
+block_norm_rows_kernel(const __grid_constant__ NormParams p, int64_t rows) {
+    constexpr int kStages = 3;
+    __shared__ float part[4][32];
+    extern __shared__ float4 ahead[];   // [stage][x, residual][PER][thread]
+    const int tid = threadIdx.x, threads = (int)blockDim.x, groups = p.n / 4;
+    float4 post[PER], gate[PER], weight[PER];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const bool gated = p.gate != nullptr;
+    auto value = [&](const float *from, int at, float otherwise, float more) {
+        const float4 v = from ? reinterpret_cast<const float4 *>(from)[at] : make_float4(otherwise, otherwise, otherwise, otherwise);
+        return make_float4(v.x + more, v.y + more, v.z + more, v.w + more);
+    };
+    auto ask = [&](int64_t row, int stage) {
+        if (row < rows) {
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int at = tid + i * threads;
+                if (at >= groups) continue;
+                float4 *to = ahead + (stage * 2 * PER + i) * threads + tid;
+                copy16_ahead(to, p.x + row * p.x_stride + 4 * at);
+                if (p.residual) copy16_ahead(to + PER * threads, p.residual + row * p.residual_stride + 4 * at);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    ask(blockIdx.x, 0);
+    ask((int64_t)blockIdx.x + gridDim.x, 1);
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int at = min(tid + i * threads, groups - 1);
+        // (what a norm multiplies by without a weight is 1)
+        post[i] = value(p.post_weight, at, 1.0f, p.post_weight ? p.offset : 0.0f);
+        weight[i] = value(p.weight, at, 1.0f, p.weight ? p.offset : 0.0f);
+        gate[i] = value(p.gate, at, 1.0f, 0.0f);
+    }
+    auto squares = [](float4 v, float sum) { return fmaf(v.w, v.w, fmaf(v.z, v.z, fmaf(v.y, v.y, fmaf(v.x, v.x, sum)))); };
+    auto times = [](float4 a, float4 b) { return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w); };
+    auto factor = [&](float sum) { return 1.0f / sqrtf(sum / (float)p.n + p.eps); };
+    int stage = 0, turn = 0;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 2) {
+        ask(row + 2 * (int64_t)gridDim.x, stage == 0 ? 2 : stage - 1);
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        float4 v[PER];
+        float sum = 0.0f, f = 1.0f;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (tid + i * threads < groups) v[i] = ahead[(stage * 2 * PER + i) * threads + tid];
+            sum = squares(v[i], sum);
+        }
+        if (p.post_norm) f = factor(block_sum(sum, part[turn]));
+        sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int at = tid + i * threads;
+            if (at >= groups) continue;
+            if (p.post_norm) {
+                v[i] = make_float4(v[i].x * f, v[i].y * f, v[i].z * f, v[i].w * f);
+                if (p.post_weight) v[i] = times(v[i], post[i]);
+            }
+            if (gated) v[i] = times(v[i], gate[i]);
+            if (p.residual) {
+                const float4 r = ahead[(stage * 2 * PER + PER + i) * threads + tid];
+                v[i] = make_float4(fmaf(p.alpha, v[i].x, r.x), fmaf(p.alpha, v[i].y, r.y), fmaf(p.alpha, v[i].z, r.z), fmaf(p.alpha, v[i].w, r.w));
+            } else {
+                v[i] = make_float4(p.alpha * v[i].x, p.alpha * v[i].y, p.alpha * v[i].z, p.alpha * v[i].w);
+            }
+            if (p.h) reinterpret_cast<float4 *>(p.h + row * p.h_stride)[at] = v[i];
+            sum = squares(v[i], sum);
+        }
+        f = factor(block_sum(sum, part[turn + 1]));
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int at = tid + i * threads;
+            if (at >= groups) continue;
+            v[i] = make_float4(v[i].x * f, v[i].y * f, v[i].z * f, v[i].w * f);
+            if (p.weight) v[i] = times(v[i], weight[i]);
+            if (p.half) {
+                __half2 two[2] = {__floats2half2_rn(v[i].x, v[i].y), __floats2half2_rn(v[i].z, v[i].w)};
+                reinterpret_cast<uint2 *>(static_cast<__half *>(p.y) + row * p.y_stride)[at] = *reinterpret_cast<uint2 *>(two);
+            } else {
+                reinterpret_cast<float4 *>(static_cast<float *>(p.y) + row * p.y_stride)[at] = v[i];
+            }
+        }
+        stage = stage == 2 ? 0 : stage + 1;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// Once a device and form: the limit of shared memory.
+int raise_shared(int form, void (*kernel)(NormParams, int64_t), int bytes) {
+    static std::atomic<uint64_t> ready[2] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && !((ready[form].load(std::memory_order_acquire) >> dev) & 1)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) ready[form].fetch_or(1ull << dev, std::memory_order_release);
+    }
+    if (e == cudaSuccess) return KRK_CUDA_OK;
+    note_cuda_error(e);
+    return KRK_CUDA_ELAUNCH;
+}
+
 } // namespace
 
 int launch_block_norm(void *y, float *h_out, const float *x, const krk_cuda_norm &m, cudaStream_t st) {
@@ -185,6 +301,20 @@ int launch_block_norm(void *y, float *h_out, const float *x, const krk_cuda_norm
     const int groups = (int)(vec ? m.n / 4 : m.n);
     const int per = groups <= 512 ? 1 : groups <= 1024 ? 2 : groups <= 2048 ? 4 : groups <= 4096 ? 8 : 0;
     const int threads = per == 0 ? 1024 : ((groups + per - 1) / per + 31) / 32 * 32;
+    const int stay = 2 * sm_count();
+    if (vec && (per == 1 || per == 2) && groups >= 256 && m.gate_stride == 0 && m.rows >= 3 * (int64_t)stay) {
+        const size_t shared = (size_t)3 * 2 * per * threads * 16;
+        auto rows_kernel = per == 1 ? block_norm_rows_kernel<1> : block_norm_rows_kernel<2>;
+        const int rc = raise_shared(per == 1 ? 0 : 1, rows_kernel, 3 * 2 * per * 512 * 16);
+        if (rc != KRK_CUDA_OK) return rc;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)stay), cfg.blockDim = dim3((unsigned)threads), cfg.dynamicSmemBytes = shared, cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr, cfg.numAttrs = 1;
+        return launched(cudaLaunchKernelEx(&cfg, rows_kernel, p, (int64_t)m.rows));
+    }
     auto kernel = vec ? (per == 1 ? block_norm_kernel<4, 1> : per == 2 ? block_norm_kernel<4, 2> : per == 4 ? block_norm_kernel<4, 4> : per == 8 ? block_norm_kernel<4, 8> : block_norm_kernel<4, 0>)
                       : (per == 1 ? block_norm_kernel<1, 1> : per == 2 ? block_norm_kernel<1, 2> : per == 4 ? block_norm_kernel<1, 4> : per == 8 ? block_norm_kernel<1, 8> : block_norm_kernel<1, 0>);
     return launched(launch_overlapped(kernel, dim3((unsigned)m.rows), dim3(threads), st, p));

@@ -115,3 +115,35 @@ def test_without_h(cuda):
         m = cuda.Norm(residual=r.data_ptr(), rows=2, n=n, x_stride=n, residual_stride=n, y_stride=n, post_norm=1, alpha=1.0, eps=1e-6)
         assert cuda.lib.krk_cuda_block_norm(y.data_ptr(), None, x.data_ptr(), C.byref(m), torch.cuda.current_stream().cuda_stream) == 0
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("n", [1024, 1540, 2052, 4096, 4100])
+@pytest.mark.parametrize("rows", [887, 1000, 2500])
+def test_many_rows(cuda, n, rows):
+    """The same bits as for a few rows at a time, whatever a row's neighbours are; rows in place, rows apart, without h."""
+    import ctypes as C
+
+    import torch
+    gen = torch.Generator("cuda").manual_seed(n + rows)
+    x, r = (torch.randn((rows, n + 4), device="cuda", generator=gen)[:, :n] for _ in range(2))
+    x *= torch.exp(2 * torch.randn((rows, 1), device="cuda", generator=gen))
+    w, pw, g = (torch.rand(n, device="cuda", generator=gen) + 0.5 for _ in range(3))
+    for more in (dict(), dict(residual=r, weight=w), dict(residual=r, weight=w, post_weight=pw, gate=g, alpha=0.7, dtype=torch.float16), dict(post_norm=True, offset=1.0, weight=w),
+                 dict(residual=r, post_weight=pw, offset=1.0)):
+        y, h = cuda.block_norm(x, **more)
+        for a in range(0, rows, 400):
+            few = {k: v[a:a + 400] if k == "residual" else v for k, v in more.items()}
+            y2, h2 = cuda.block_norm(x[a:a + 400], **few)
+            assert torch.equal(y[a:a + 400], y2) and torch.equal(h[a:a + 400], h2)
+    y, h = cuda.block_norm(x, w, r, pw)
+    for place in (0, 1):
+        args = [x.clone(), r.clone()]
+        y2, h2 = cuda.block_norm(args[0], w, args[1], pw, h_out=args[place])
+        assert torch.equal(y2, y) and torch.equal(args[place], h)
+    both = x.clone()
+    assert torch.equal(cuda.block_norm(both, w, r, pw, out=both)[0], y)
+    y2 = torch.full((rows, n + 4), 3.0, device="cuda")
+    m = cuda.Norm(residual=r.data_ptr(), weight=w.data_ptr(), post_weight=pw.data_ptr(), rows=rows, n=n, x_stride=n + 4, residual_stride=n + 4, y_stride=n + 4, post_norm=1, alpha=1.0,
+                  eps=1e-6)
+    assert cuda.lib.krk_cuda_block_norm(y2.data_ptr(), None, x.data_ptr(), C.byref(m), torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(y2[:, :n], y) and (y2[:, n:] == 3).all()
