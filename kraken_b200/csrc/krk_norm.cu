@@ -4,8 +4,8 @@
 //
 // Bound: reading x and the residual and writing h and y once. A block of threads has a row in registers from its loads to the last store: the two sums of
 // squares are a shuffle and a trip through shared memory each. Sums are f32, a thread's values first, then a tree. Weights and a shared gate come out of level 2.
-// Measured: one row of 4096 5.7 us (a launch; two trips to memory); 2048 rows, f16 out, two norms and a gate 25.4 us, 4.6 TB/s of 6.5. There two groups of four
-// values a thread are best: one (1024 threads a row) 29.5, four 27.6, eight 37.2.
+// Measured: one row of 4096 5.7 us (a launch; two trips to memory); 2048 rows, f16 out, two norms and a gate 25.4 us, 4.6 TB/s of a copy's 6.5. There two groups of four
+// values a thread are best of a block a row: one (1024 threads) 29.5, four 27.6, eight 37.2; blocks that stay, below, 21.1, 5.5 TB/s.
 #include "krk_common.cuh"
 
 #include <atomic>
@@ -301,8 +301,10 @@ int launch_block_norm(void *y, float *h_out, const float *x, const krk_cuda_norm
     const int groups = (int)(vec ? m.n / 4 : m.n);
     const int per = groups <= 512 ? 1 : groups <= 1024 ? 2 : groups <= 2048 ? 4 : groups <= 4096 ? 8 : 0;
     const int threads = per == 0 ? 1024 : ((groups + per - 1) / per + 31) / 32 * 32;
+    // Two norms, a gate, f16 out, us here and a block a row: rows of 4096 values, 300 6.7 and 6.5, 600 8.0 and 10.1, 2048 21.0 and 25.4, 8192 82.8 and 79.1; of 2048 values, 600 6.6
+    // and 6.6, 2048 13.9 and 14.4, 8192 46.5 and 49.4; of 1024, 2048 9.5 and 7.3.
     const int stay = 2 * sm_count();
-    if (vec && (per == 1 || per == 2) && groups >= 256 && m.gate_stride == 0 && m.rows >= 3 * (int64_t)stay) {
+    if (vec && (per == 1 || per == 2) && groups >= 512 && m.gate_stride == 0 && m.rows >= 2 * (int64_t)stay && m.rows * m.n <= 1 << 24) {
         const size_t shared = (size_t)3 * 2 * per * threads * 16;
         auto rows_kernel = per == 1 ? block_norm_rows_kernel<1> : block_norm_rows_kernel<2>;
         const int rc = raise_shared(per == 1 ? 0 : 1, rows_kernel, 3 * 2 * per * 512 * 16);

@@ -66,10 +66,17 @@ verify_stats_kernel(const __grid_constant__ VerifyParams p) {
     const float *x = (drafter ? p.q + row * p.q_stride : p.p + row * p.p_stride) + lo;
     if (tid == 0) s_seq = -1;
     __syncthreads();
-    for (int s = tid; s < p.n_seq; s += kStatThreads) {
-        const int a = p.row_start[s], b = p.row_start[s + 1];
-        if (row >= a && row < b && !(drafter && row == b - 1)) s_seq = s;   // (the drafter has nothing to say about a sequence's last row)
-    }
+    auto find = [&] {
+        for (int s = tid; s < p.n_seq; s += kStatThreads) {
+            const int a = p.row_start[s], b = p.row_start[s + 1];
+            if (row >= a && row < b && !(drafter && row == b - 1)) s_seq = s;   // (the drafter has nothing to say about a sequence's last row)
+        }
+        __syncthreads();
+        return s_seq;
+    };
+    // (a drafter's row may be one of those; the target's are read while their sequence is looked for)
+    int s = -1;
+    if (drafter && (s = find()) < 0) return;
     float v[kStatPer];
     auto at = [&](int i) { return VEC ? (i >> 2) * 4 * kStatThreads + 4 * tid + (i & 3) : i * kStatThreads + tid; };
 #pragma unroll
@@ -81,9 +88,7 @@ verify_stats_kernel(const __grid_constant__ VerifyParams p) {
             for (int c = i; c < i + 4; c++) v[c] = at(c) < n ? x[at(c)] : -INFINITY;
         }
     }
-    __syncthreads();
-    const int s = s_seq;
-    if (s < 0) return;
+    if (!drafter && (s = find()) < 0) return;
     const float inv = (float)fmin(per_temp(drafter && p.draft_temp ? p.draft_temp : p.temp, s), 1e37) * 1.44269504f;
     float m = -INFINITY;
     int best = INT32_MAX;
