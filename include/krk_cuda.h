@@ -356,7 +356,8 @@ int krk_cuda_attention_chunk(void *out, int out_dtype, const void *q, int q_dtyp
  *   positions [max_tok], slots int64 [max_tok]          of the tokens, as qk_norm_rope and kv_append want them; -1 slots where there is no page, and
  *                                                       0 and -1 behind the last token
  *   counts [4]                                          free pages left, pages that were missing, tokens, tokens beyond max_tok (they get nothing: the sequences end before them)
- * n_free itself stays as it is (counts has its successor), so that a call that is repeated gives the same. The struct is read before the call returns. */
+ * n_free itself stays as it is (counts has its successor), so that a call that is repeated gives the same. What is written overlaps nothing else (KRK_CUDA_EARG: the next
+ * step's kv_before may be this one's kv_len, but then in another place than its own kv_len). The struct is read before the call returns. */
 struct krk_cuda_step {
     const void *kv_before, *n_new;    /* int32 [n_seq] */
     void *page_table;                 /* int32 [n_seq][table_width]: read and written */
@@ -370,7 +371,7 @@ int krk_cuda_step_plan(const struct krk_cuda_step *host_step, void *stream);
 /* Between two blocks, for rows of n values:
  *   h = residual + alpha * gate * P(x),  P(x) = x / sqrt(mean(x^2) + eps) * (offset + post_weight)  (post_norm 0: x),   y = h / sqrt(mean(h^2) + eps) * (offset + weight)
  * h is f32, y f32 or, as the f16 X of krk_cuda_gemm, f16 (y_dtype). gate: a row for all (gate_stride 0) or one each. NULL: residual 0, gate and weights (with their offset) 1.
- * h_out may be x or the residual (with the same stride), else nothing overlaps; h_out NULL: h is not wanted. Strides in elements. The place of
+ * h_out and an f32 y may be x or the residual (with the same stride), not both the same, else nothing overlaps; h_out NULL: h is not wanted. Strides in elements. The place of
  * Backend::rmsnorm with add_inplace before it (include/krk/backend.hpp:855, 1340). */
 struct krk_cuda_norm {
     const void *residual, *gate, *post_weight, *weight;   /* f32 */
@@ -426,8 +427,8 @@ int krk_cuda_logits_adjust(void *out_f32, const void *logits_f32, const struct k
  * draft_logits NULL: the drafts are certain, q(t) = 1. temp[s] <= 0: greedy, a token is accepted where it is the lowest of the greatest logits, and that one stands in the place of
  * the first one that is not. temp NULL: 1; draft_temp NULL: temp (one of 0 or less counts as 1). Written: tokens int32 [rows], the accepted tokens, the drawn one, -1 behind it; n_accepted int32 [n_seq];
  * logprob f32 [rows] (may be NULL), the logarithm of p of what came out (greedy: under a temperature of 1), 0 beside a -1. Of a row with a NaN, an infinity or nothing
- * but -infinity nothing is accepted or drawn (-1); a greedy one passes over NaN. Weights and sums of a drawn row have 64 bits. Rows of no sequence stay as they were. The
- * workspace is scratch; calls that can overlap need one each. */
+ * but -infinity nothing is accepted or drawn (-1); a greedy one passes over NaN. Weights and sums of a drawn row have 64 bits. Rows of no sequence stay as they were. What is
+ * written overlaps nothing that is read (KRK_CUDA_EARG). The workspace is scratch; calls that can overlap need one each. */
 struct krk_cuda_verify {
     const void *row_start;            /* int32 [n_seq + 1] */
     const void *draft;                /* int32 [n_rows] */

@@ -1,5 +1,6 @@
 // The extern "C" surface declared in include/krk_cuda.h: argument checks, then a launch.
 // Nothing here computes on the host.
+#include <initializer_list>
 #include <cfloat>
 #include <atomic>
 #include <cstring>
@@ -552,6 +553,25 @@ int krk_cuda_attention_chunk(void *out, int out_dtype, const void *q, int q_dtyp
     return launch_attention_chunk(out, out_dtype, q, q_dtype, *cache, a, workspace, static_cast<cudaStream_t>(stream));
 }
 
+// Lists in memory, n of size bytes each: whether one that is written meets one that is read (other blocks of threads may read it later), or another one.
+struct List {
+    const void *at;
+    int64_t bytes;
+};
+static bool meet(const List &a, const List &b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+    return a.at && b.at && a.bytes > 0 && b.bytes > 0 && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+}
+static bool written_meets(std::initializer_list<List> written, std::initializer_list<List> read) {
+    for (const List &w : written) {
+        for (const List &r : read)
+            if (meet(w, r)) return true;
+        for (const List &other : written)
+            if (&other != &w && meet(w, other)) return true;
+    }
+    return false;
+}
+
 int krk_cuda_step_plan(const krk_cuda_step *s, void *stream) {
     if (!s) return KRK_CUDA_ENULL;
     if (s->n_seq < 0 || s->table_width < 0 || s->page_size < 1 || s->max_tok < 0 || s->max_tok > INT32_MAX || s->free_cap < 0 || s->free_cap > INT32_MAX) return KRK_CUDA_ESHAPE;
@@ -562,6 +582,11 @@ int krk_cuda_step_plan(const krk_cuda_step *s, void *stream) {
     for (const void *p : lists)
         if (!aligned(p, 4)) return KRK_CUDA_EALIGN;
     if (!aligned(s->slots, 8)) return KRK_CUDA_EALIGN;
+    const int64_t seqs = 4ll * s->n_seq;
+    const bool meets = written_meets({{s->q_start, seqs + 4}, {s->kv_len, seqs}, {s->last, seqs}, {s->positions, 4 * s->max_tok}, {s->slots, 8 * s->max_tok}, {s->counts, 16},
+                                      {s->page_table, seqs * s->table_width}},
+                                     {{s->kv_before, seqs}, {s->n_new, seqs}, {s->free_pages, 4 * s->free_cap}, {s->n_free, 4}});
+    if (meets) return KRK_CUDA_EARG;
     if (!device_state()) return KRK_CUDA_EDEVICE;
     return launch_step_plan(*s, static_cast<cudaStream_t>(stream));
 }
@@ -577,6 +602,9 @@ int krk_cuda_block_norm(void *y, void *h_out_f32, const void *x_f32, const krk_c
                         (m->gate && m->gate_stride > 0 && m->gate_stride < m->n)))
         return KRK_CUDA_ESHAPE;
     if (m->rows > 1 && h_out_f32 && ((h_out_f32 == x_f32 && m->h_stride != m->x_stride) || (h_out_f32 == m->residual && m->h_stride != m->residual_stride))) return KRK_CUDA_EARG;
+    if ((y == x_f32 && (m->y_dtype != KRK_CUDA_X_F32 || (m->rows > 1 && m->y_stride != m->x_stride))) || (y && y == m->residual && (m->y_dtype != KRK_CUDA_X_F32 || (m->rows > 1 && m->y_stride != m->residual_stride))) ||
+        y == h_out_f32)
+        return KRK_CUDA_EARG;
     const void *const floats[] = {h_out_f32, x_f32, m->residual, m->gate, m->post_weight, m->weight};
     for (const void *p : floats)
         if (!aligned(p, 4)) return KRK_CUDA_EALIGN;
@@ -604,6 +632,10 @@ int krk_cuda_verify_draft(void *tokens_i32, void *n_accepted_i32, void *logprob_
     const void *const lists[] = {tokens_i32, n_accepted_i32, logprob_f32, logits_f32, v->row_start, v->draft, v->accept_u, v->sample_u, v->temp, v->draft_temp, v->draft_logits};
     for (const void *p : lists)
         if (!aligned(p, 4)) return KRK_CUDA_EALIGN;
+    const int64_t rows = 4 * v->n_rows, seqs = 4ll * v->n_seq;
+    if (written_meets({{tokens_i32, rows}, {n_accepted_i32, seqs}, {logprob_f32, rows}},
+                      {{v->row_start, seqs + 4}, {v->draft, rows}, {v->accept_u, rows}, {v->sample_u, seqs}, {v->temp, seqs}, {v->draft_temp, seqs}}))
+        return KRK_CUDA_EARG;
     if (!device_state()) return KRK_CUDA_EDEVICE;
     const size_t need = v->n_rows == 0 ? 0 : verify_draft_workspace_bytes(*v);
     if (need > 0 && (!workspace || ws_bytes < need || !aligned(workspace, 16))) return KRK_CUDA_EWORKSPACE;

@@ -102,6 +102,28 @@ def test_verification_pointers():
     assert L.krk_cuda_verify_draft(None, None, None, None, C.byref(verify(n_seq=0)), None, 0, None) == 0
 
 
+def test_what_is_written_meets_nothing_else():
+    """Lists of a plan and of a verification in each other's place; y of a norm in the place of x as f16, under another stride, and in h's."""
+    at = {n: P + 0x10000 * i for i, n in enumerate(("kv_before", "n_new", "page_table", "free_pages", "n_free", "q_start", "kv_len", "last", "positions", "slots", "counts"))}
+
+    def plan(**k):
+        return L.krk_cuda_step_plan(C.byref(capi.Step(**{**at, **dict(max_tok=8, free_cap=9, n_seq=4, table_width=3, page_size=16), **k})), None)
+    for k in (dict(kv_len=at["kv_before"]), dict(kv_before=at["kv_len"] + 12), dict(counts=at["n_free"]), dict(n_free=at["counts"] + 8), dict(last=at["n_new"]),
+              dict(page_table=at["free_pages"] + 32), dict(kv_len=at["q_start"] + 16), dict(slots=at["positions"] + 24)):
+        assert plan(**k) == EARG
+    t, n, lp, x, W = (P + 0x10000 * i for i in range(5))
+    at = {n: P + 0x100000 + 0x10000 * i for i, n in enumerate(("row_start", "draft", "accept_u", "sample_u", "temp", "draft_temp"))}
+
+    def judge(tokens=t, accepted=n, logprob=lp, **k):
+        return L.krk_cuda_verify_draft(tokens, accepted, logprob, x, C.byref(capi.Verify(**{**at, **dict(n_rows=6, n_vocab=100, stride=100, n_seq=2), **k})), W, 1 << 20, None)
+    for k in (dict(tokens=at["draft"]), dict(logprob=at["accept_u"]), dict(tokens=at["draft"] + 20), dict(accepted=at["row_start"]), dict(logprob=t), dict(accepted=at["temp"])):
+        assert judge(**k) == EARG
+    X, Y = P + 0x10000, P + 0x20000
+    assert L.krk_cuda_block_norm(X, None, X, C.byref(norm(y_dtype=1)), None) == EARG
+    assert L.krk_cuda_block_norm(X, None, X, C.byref(norm(y_stride=104)), None) == EARG
+    assert L.krk_cuda_block_norm(Y, Y, X, C.byref(norm()), None) == EARG
+
+
 def test_the_binding_refuses():
     """On tensors that are not on a GPU, and what is no tensor."""
     import torch
