@@ -16,7 +16,7 @@
 // TFLOP/s; cuBLAS sustains 1372 on this card). There the exponential unit is as busy as the tensor pipe, so half of the exponentials are a polynomial's (604 -> 548 us for 8192 tokens).
 // f32 results take two terms of queries and weights, twice the products: 2048 tokens 121 us (2 x 283 TFLOP/s), 8192 tokens 980 to 1040. Over 8 and 4 bits what unpacks
 // the quants is the limit: 24 ragged sequences of up to 512 tokens behind up to 8000, 8 bits, 550 us; 4096 behind 8192 965; f32, three products, two chunks of up to 700
-// behind 5000, 420. Few tokens: a launch, pages, one item's latency: 33 tokens 23 us.
+// behind 5000, 406. Few tokens: a launch, pages, one item's latency: 33 tokens 21 us.
 #pragma once
 
 #include <cuda.h>
@@ -367,11 +367,11 @@ struct Chunk {
     static constexpr int kSlots = kRoom / kSlot > 6 ? 6 : kRoom / kSlot;
     static constexpr int kQ = kSlots * kSlot, kRawAt = kQ + kQSets * kQSet, kMeta = kRawAt + kRaws * kRaw, kBytes = kMeta + kMetaBytes + 1024;   // (begins on a 1024-byte boundary)
     // warps: softmax, copies, products, the one that finds items
-    static constexpr int kSoft = 4 * NQ, kCopies = KT == 2 ? 8 : QUANT ? 4 : 2, kProduct = kSoft + kCopies, kFinder = kProduct + 1, kWarps = KT == 2 ? kFinder + 1 : kSoft + (QUANT ? 8 : 4), kThreads = 32 * kWarps;
+    static constexpr int kSoft = 4 * NQ, kCopies = KT == 2 ? 8 : QUANT ? 4 : 2, kProduct = kSoft + kCopies, kFinder = kProduct + 1, kWarps = kSoft + (KT == 2 ? 12 : QUANT ? 8 : 4), kThreads = 32 * kWarps;
     // Registers of a thread, traded between groups of four warps (a spill goes to level 2: shared memory has what level 1 had). Launched with: 384 threads 168, 512 128.
-    static constexpr bool kTrade = NQ == 2;
-    static constexpr int kSoftRegs = QUANT ? 168 : 200, kCopyRegs = QUANT ? 88 : 104, kOtherRegs = QUANT ? 88 : 104;
-    static_assert(256 * kSoftRegs + 128 * (kCopyRegs + (QUANT ? kOtherRegs : 0)) <= (QUANT ? 512 * 128 : 384 * 168) , "registers of a launch");
+    static constexpr bool kTrade = NQ == 2 || KT == 2;
+    static constexpr int kSoftRegs = KT == 2 ? 184 : QUANT ? 168 : 200, kCopyRegs = KT == 2 ? 112 : QUANT ? 88 : 104, kOtherRegs = KT == 2 ? 104 : QUANT ? 88 : 104;
+    static_assert(!kTrade || 32 * (kSoft * kSoftRegs + (QUANT ? kCopies * kCopyRegs + 4 * kOtherRegs : 4 * kCopyRegs)) <= (QUANT ? 512 * 128 : 384 * 168), "registers of a launch");
     static constexpr uint32_t kO = 256;                              // column of the sums; of the second tile's: 128 more
     static constexpr uint32_t kS = NQ == 2 ? 128 : 64;               // from a place of scores to the next
     static_assert(kSlots >= 3, "a half tile of values and one of keys at work, one on its way");
