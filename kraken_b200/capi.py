@@ -517,7 +517,8 @@ class StepPlan(NamedTuple):
 def step_plan(kv_before, n_new, page_table, free_pages, n_free, page_size: int, max_tok: int, out=None, stream=None) -> StepPlan:
     """Pages, slots and positions of a step's new tokens from the requests' lengths (int32 [n_seq] each): sequence s has kv_before[s] positions and gets
     n_new[s] more; pages come off the stack free_pages[:n_free[0]] (int32; n_free int32 [1]) into page_table (int32 [n_seq, width], written in place), -1
-    where there are none. max_tok: places of positions and slots, whose rest is 0 and -1. out: a StepPlan to write into again."""
+    where there are none. max_tok: places of positions and slots, whose rest is 0 and -1. out: a StepPlan to write into again, none of whose lists is
+    read here (of two plans in turn, one's kv_len may be the next one's kv_before, and its counts[:1] the next one's n_free)."""
     return StepPlan(*_fc.step_plan(kv_before, n_new, page_table, free_pages, n_free, page_size, max_tok, tuple(out) if out is not None else None, stream))
 
 

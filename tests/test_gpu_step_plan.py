@@ -96,3 +96,23 @@ def test_capture(cuda):
     graph.replay()
     assert plan.positions.tolist() == [12, 13, 14, 15, 16, 16, 0, 0, 0, 0, 0, 0] and plan.slots.tolist() == [28, 29, 30, 31, 128, 112] + [-1] * 6
     assert table.tolist() == [[1, 8, -1, -1], [2, 7, -1, -1]] and plan.counts.tolist() == [2, 0, 6, 0]
+
+
+def test_two_plans_in_turn(cuda):
+    """A plan's lengths and counts are the next one's input where they lie; one plan in the place of its own is refused."""
+    import torch
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    table, free = torch.full((3, 40), -1, dtype=torch.int32, device="cuda"), torch.arange(100, dtype=torch.int32, device="cuda")
+    new = [i32(30, 1, 7), i32(5, 16, 0), i32(1, 1, 400)]
+    plans = [cuda.step_plan(i32(0, 0, 0), new[0], table, free, i32(100), 16, 50)]
+    plans.append(cuda.step_plan(plans[0].kv_len, new[1], table, free, plans[0].counts[:1], 16, 50))
+    cuda.step_plan(plans[1].kv_len, new[2], table, free, plans[1].counts[:1], 16, 500, out=None)
+    want = cuda.step_plan(plans[1].kv_len, i32(1, 1, 43), table.clone(), free, plans[1].counts[:1], 16, 50)
+    got = cuda.step_plan(plans[1].kv_len, i32(1, 1, 43), table, free, plans[1].counts[:1], 16, 50, out=plans[0]._replace(page_table=table))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert got.kv_len.tolist() == [36, 18, 50] and got.counts[0].item() == 100 - 3 - 2 - 4
+    for bad in (dict(kv_before=got.kv_len), dict(n_free=got.counts[:1]), dict(n_new=got.last)):
+        args = {**dict(kv_before=plans[1].kv_len, n_new=new[0], n_free=plans[1].counts[:1]), **bad}
+        with pytest.raises((ValueError, cuda.KrkCudaError)):
+            cuda.step_plan(args["kv_before"], args["n_new"], table, free, args["n_free"], 16, 50, out=got)
