@@ -514,15 +514,14 @@ __device__ __forceinline__ void products_p(uint32_t d, uint32_t a, uint32_t b_lo
                      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [x3], b1, %3, {%5, %5, %5, %5}, t;\n}\n"
                      ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(onto), "r"(0u), "r"(elected), "r"(kDescHi) : "memory");
 }
-// As capped, without a call: the hyperbolic tangent from one exponential (2^-22 off), f32: near zero from its series, whose next term is 2^-26 of it there.
-template <bool HALF>
+// As capped, without a call: the hyperbolic tangent from one exponential, 2^-22 of 1 off. Below 1/4, where that would be more and more of it (under a limit far above the scores
+// all of it), from its series, whose next term is 2^-26 of it there.
 __device__ __forceinline__ float capped_here(float x, float cap) {
-    const float y = x / cap, e = ex2(y * (2.0f * 1.44269504f));
-    float t = 1.0f - 2.0f * __frcp_rn(1.0f + e);
-    if constexpr (!HALF) {
-        const float z = y * y;
-        if (z < 0.0625f) t = fmaf(y * z, fmaf(z, fmaf(z, fmaf(z, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), y);
-    }
+    const float y = x / cap, z = y * y;
+    float r;   // (to its last place or the one beside)
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(y * (2.0f * 1.44269504f))));
+    float t = 1.0f - 2.0f * r;
+    if (z < 0.0625f) t = fmaf(y * z, fmaf(z, fmaf(z, fmaf(z, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), y);
     return cap * (1.44269504f * t);
 }
 // Two f32 at a time.
@@ -573,7 +572,7 @@ __device__ __forceinline__ float value_at(const uint8_t *pool, const __half *sca
 }
 
 // Log2 scores under a soft limit in place of products.
-template <bool HALF, int TP>
+template <int TP>
 __device__ __forceinline__ void soft_limit(uint32_t t_s, float sc, float cap) {
 #pragma unroll 1
     for (int c = 0; c < TP; c += 16) {
@@ -581,7 +580,7 @@ __device__ __forceinline__ void soft_limit(uint32_t t_s, float sc, float cap) {
         tmem_load16(t_s + c, v);
         tmem_loaded();
 #pragma unroll
-        for (int j = 0; j < 16; j++) v[j] = __float_as_uint(capped_here<HALF>(__uint_as_float(v[j]) * sc, cap));
+        for (int j = 0; j < 16; j++) v[j] = __float_as_uint(capped_here(__uint_as_float(v[j]) * sc, cap));
         tmem_store16(t_s + c, v);
     }
     tmem_stored();
@@ -841,7 +840,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 // What is rarely done has code of its own, and no more of it than has to be: code that is jumped over, or met for the first time, is fetched at
                 // the pace of thousands of clocks.
                 if (p.softcap > 0.0f) {   // log2 scores in place of the products
-                    soft_limit<HALF, TP>(t_s, sc, p.softcap);
+                    soft_limit<TP>(t_s, sc, p.softcap);
                     f = 1.0f;
                 }
                 uint32_t v[TP];

@@ -1,0 +1,78 @@
+"""Attention of chunks at the ends of its numbers: soft limits up to the largest f32, scales of zero and near it, windows up to the largest int, and values that are no numbers over
+8 and 4 bits in calls whose rows do not go to the kernel of trees. Against the definition in 64 bits; which rows go where is that of krk_attn_chunk.cu (max_q * group * head_dim above
+256 * 128)."""
+import numpy as np
+import pytest
+
+from test_gpu_attn_chunk import ACTS, KINDS, Batch
+
+pytestmark = pytest.mark.gpu
+
+
+def limited(b, s, rows, softcap, scale):
+    """(out, tolerance) of sequence s of a Batch, all of whose pages and numbers are there.
+
+    Per unit of a = sum(w |v|) / sum(w), as tests/chunk_plain.py derives them, but for the soft limit, whose error is counted against the score y = s / softcap that goes
+    in and not against the limit: below |y| = 1/4 an odd series of five terms (the next one, 1382 / 155925 y^11, is 1e-8 of y at 1/4) with its rounding, 2^-22; from there on 1 - 2 / (1 + e), e off by
+    2^-22 and its argument's rounding: 2^-22 of a tangent of 1, of one of 0.245 less than 2^-20. So 2^-20 of the greatest score."""
+    from chunk_plain import decoded, seen_of
+    torch = b.torch
+    n, c = b.lens[s], b.counts[s]
+    p = torch.arange(n, device="cuda")
+    at = b.table.cuda()[s, p // b.page].long(), slice(None), p % b.page
+    k, v = (decoded(a[at], None if x is None else x[at], b.kind) for a, x in ((b.cache.k, b.cache.k_scale), (b.cache.v, b.cache.v_scale)))
+    seen, q, quants, d = seen_of(c, n), b.q[rows].double(), b.kind != 0, b.d
+    out, tol = torch.zeros_like(q), torch.zeros_like(q)
+    for h in range(q.shape[1]):
+        kk, vv, qq = k[:, h // (q.shape[1] // b.kv)], v[:, h // (q.shape[1] // b.kv)], q[:, h]
+        x = torch.where(seen, qq @ kk.T, 0) * scale
+        size = (torch.where(seen, qq.abs() @ kk.abs().T, 0) * abs(scale)).amax(1, keepdim=True)
+        if softcap:
+            x = softcap * torch.tanh(x / softcap)
+        most = x.abs().amax(1, keepdim=True)
+        z = torch.where(seen, x, -torch.inf)
+        w = torch.exp(z - z.amax(1, keepdim=True))
+        total = w.sum(1, keepdim=True)
+        o, a = w @ vv / total, w @ vv.abs() / total
+        seen_n = seen.sum(1).double()[:, None]
+        off = (2.0 ** -11 * ((not b.q_half) + quants) if b.half else 2.0 ** -22 * (1 + quants)) * size + (d / 16 + 4) * (1 if b.half else 3 if quants else 2) * 2.0 ** -23 * size
+        if b.half and quants:
+            off = off + 2.0 ** -25 * qq.abs().sum(1, keepdim=True) * abs(scale)
+        off = off + 2.0 ** -22 * most + 2.0 ** -21 + (2.0 ** -20 * most if softcap else 0.0)
+        t = a * (2 * off + (2.0 ** -11 * (1 + quants) + 2.0 ** -12 if b.half else 2.0 ** -22 * (2 + quants)) + (seen_n / 16 + 300) * 2.0 ** -23) + seen_n * 2.0 ** -32 * vv.abs().amax() / total.clamp(min=1.0)
+        out[:, h], tol[:, h] = o, t + (2.0 ** -11 * o.abs() + 2.0 ** -25 * (2 + quants) if b.half else 0.0)
+    return out, tol
+
+
+def check(b, softcap=0.0, scale=None):
+    torch = b.torch
+    scale = b.d ** -0.5 if scale is None else scale
+    out = torch.full(b.q.shape, 7.0, device="cuda", dtype=torch.float16 if b.half else torch.float32)
+    b.cuda.attention_chunk(b.q, b.cache, scale=scale, softcap=softcap, out=out, **b.args())
+    row = 0
+    for s, c in enumerate(b.counts):
+        rows = slice(row, row + c)
+        want, tol = limited(b, s, rows, float(np.float32(softcap)), float(np.float32(scale)))
+        ratio = (out[rows].double() - want).abs() / tol
+        assert torch.isfinite(out[rows]).all() and float(ratio.max()) <= 1.0, f"softcap {softcap}, scale {scale}, sequence {s}: worst {float(ratio.max()):.3g} of the tolerance"
+        row += c
+    assert (out[row:] == 7.0).all()
+    return out[:row]
+
+
+# (rows * d above and below the border to the kernel of trees, which over 8 and 4 bits has the f32 results of the smaller one; a head that no two tiles of rows have room for)
+SHAPES = [(128, 2, 4, [140, 1], [900, 30]), (64, 1, 2, [40, 3], [300, 700]), (256, 1, 2, [130], [400])]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_soft_limits(cuda, kind, act, shape):
+    d, kv, group, counts, lens = shape
+    b = Batch(cuda, 31, KINDS[kind], d, kv, group, 16, counts, lens, act, q_size=4.0)
+    for limit in (1.0, 30.0, 300.0, 1e4, 1e6, 1e8, 1e30, 3e38, 3.4028234e38):
+        check(b, limit)
+    free = check(b).double()
+    huge = check(b, 1e30).double()
+    bound = sum((limited(b, 0, slice(0, counts[0]), c, d ** -0.5)[1] for c in (0.0, 1e30)))
+    assert ((free - huge).abs()[:counts[0]] <= bound).all()
