@@ -176,6 +176,9 @@ int launch_attention_chunk(void *out, int out_dtype, const void *q, int q_dtype,
     p.n_kv = cache.n_kv_heads, p.group = a.n_heads / cache.n_kv_heads, p.max_q = a.max_q, p.window = a.window, p.whole = f.whole, p.grid = f.grid;
     p.out_wide = (reinterpret_cast<uintptr_t>(out) | (uintptr_t)(a.out_stride * (out_dtype == KRK_CUDA_X_F16 ? 2 : 4))) % 32 == 0;
     p.q_half = q_dtype == KRK_CUDA_X_F16, p.out_half = out_dtype == KRK_CUDA_X_F16, p.scale = a.scale, p.softcap = a.softcap;
+    // Scores are masked before they are multiplied by the row's factor, which therefore must not be 0 (-infinity times 0). Under a soft limit they are multiplied first, and
+    // those of 0 stay 0, whatever the limit is.
+    if (p.scale == 0.0f && p.softcap == 0.0f) p.softcap = 1.0f;
     attn::divide_by(p.group, p.group_mul, p.group_shift);
     p.status = device_status_word();
     if (!p.status) return KRK_CUDA_EDEVICE;

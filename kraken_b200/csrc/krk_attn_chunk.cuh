@@ -810,7 +810,8 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
 #pragma unroll
                         for (int c = 0; c < NL; c++)
                             if (D % 128 == 0 || 32 * c + lane < kPer) put(r, 128 * c + 4 * lane, x[j][c], e);
-                        if (lane == j0 + j) sc = row_scale * __uint_as_float((uint32_t)(127 - e) << 23);
+                        // (never 0, which would make a NaN of a masked score's -infinity: products are below 2^35, those of the smallest normal factor as good as 0)
+                        if (lane == j0 + j) sc = fmaxf(row_scale * __uint_as_float((uint32_t)(127 - e) << 23), 1.17549435e-38f);
                     }
                 }
                 async_fence();

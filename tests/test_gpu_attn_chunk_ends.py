@@ -74,5 +74,33 @@ def test_soft_limits(cuda, kind, act, shape):
         check(b, limit)
     free = check(b).double()
     huge = check(b, 1e30).double()
-    bound = sum((limited(b, 0, slice(0, counts[0]), c, d ** -0.5)[1] for c in (0.0, 1e30)))
+    bound = sum(limited(b, 0, slice(0, counts[0]), c, d ** -0.5)[1] for c in (0.0, 1e30))
     assert ((free - huge).abs()[:counts[0]] <= bound).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_scales_of_nothing(cuda, kind, act, shape):
+    """A scale of zero is the mean of what a row sees; so is one that f32 does not hold beside the queries' powers of two, and one that holds but adds nothing to any score."""
+    d, kv, group, counts, lens = shape
+    b = Batch(cuda, 32, KINDS[kind], d, kv, group, 16, counts, lens, act)
+    rows = sum(counts)
+    for q_size, scale in ((1.0, 0.0), (1.0, -0.0), (1.0, 1e-30), (1e-6, 1e-37), (1e-6, 1e-42), (2.0 ** -20, -1e-40)):
+        was = b.q
+        b.q = (b.q * q_size).to(b.q.dtype)
+        for softcap in (0.0, 5.0):
+            check(b, softcap, scale)
+        b.q = was
+    mean = check(b, 0.0, 0.0)
+    b.q = b.q * 0
+    assert (check(b, 0.0, 1.0) == mean).all() and mean.shape[0] == rows
+    # windows, sinks, missing pages: the mean of what is left
+    b.table[0, 1] = -1
+    for more in (dict(window=20), dict(sinks=b.torch.randn(kv * group, device="cuda"))):
+        b.check(scale=0.0, **more)
+    # a key that is no number: 0 times it is none either, for the rows that see it
+    if KINDS[kind] == 0:
+        for odd in (np.inf, -np.inf, np.nan):
+            b.cache.k[b.table[0, 0].long(), 0, 3, 0] = odd
+            assert not b.torch.isfinite(b.cuda.attention_chunk(b.q, b.cache, scale=0.0, **b.args())[:counts[0], :group]).any()
