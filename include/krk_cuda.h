@@ -425,9 +425,10 @@ int krk_cuda_logits_adjust(void *out_f32, const void *logits_f32, const struct k
  *   in its place one is drawn from max(p - q, 0) (from p, where that leaves nothing), or, where all were accepted, from the last row's p:
  *   the lowest i with  sum_{k <= i} w_k > sample_u[s] * sum w
  * draft_logits NULL: the drafts are certain, q(t) = 1. temp[s] <= 0: greedy, a token is accepted where it is the lowest of the greatest logits, and that one stands in the place of
- * the first one that is not. temp NULL: 1; draft_temp NULL: temp (one of 0 or less counts as 1). Written: tokens int32 [rows], the accepted tokens, the drawn one, -1 behind it; n_accepted int32 [n_seq];
+ * the first one that is not. temp NULL: 1; draft_temp NULL: temp; draft_temp[s] <= 0: the drafter took its greatest logit, q is 1 at the lowest of its greatest. Written: tokens int32 [rows], the accepted tokens, the drawn one, -1 behind it; n_accepted int32 [n_seq];
  * logprob f32 [rows] (may be NULL), the logarithm of p of what came out (greedy: under a temperature of 1), 0 beside a -1. Of a row with a NaN, an infinity or nothing
- * but -infinity nothing is accepted or drawn (-1); a greedy one passes over NaN. Weights and sums of a drawn row have 64 bits. Rows of no sequence stay as they were. What is
+ * but -infinity nothing is accepted or drawn (-1); a greedy one passes over NaN. Such a row of the drafter's accepts nothing, and the token is drawn from p (a greedy drafter's: NaN
+ * is passed over, an infinity is the greatest). Weights and sums of a drawn row have 64 bits. Rows of no sequence stay as they were. What is
  * written overlaps nothing that is read (KRK_CUDA_EARG). The workspace is scratch; calls that can overlap need one each. */
 struct krk_cuda_verify {
     const void *row_start;            /* int32 [n_seq + 1] */

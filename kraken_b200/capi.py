@@ -536,7 +536,8 @@ def verify_draft(logits, row_start, draft, accept_u, sample_u, draft_logits=None
                  stream=None):
     """Drafted tokens against the target's probabilities: logits f32 [rows, vocab], sequence s has rows row_start[s] .. row_start[s + 1] (int32), one more than
     drafted tokens; draft int32 [rows] (a sequence's last one is not looked at); accept_u f32 [rows] and sample_u f32 [n_seq] in [0, 1); draft_logits
-    f32 [rows, vocab] of the drafter, None where its tokens are certain; temp, draft_temp f32 [n_seq] (0: greedy). Returns (tokens int32 [rows]: the
+    f32 [rows, vocab] of the drafter, None where its tokens are certain; temp, draft_temp f32 [n_seq] (0 or less: greedy, a
+    drafter's tokens were its greatest; draft_temp None: temp). Returns (tokens int32 [rows]: the
     accepted ones, the drawn one, -1; n_accepted int32 [n_seq]; logprob f32 [rows]); rows of no sequence are left as they were."""
     return _fc.verify_draft(logits, row_start, draft, accept_u, sample_u, draft_logits, temp, draft_temp, tokens, n_accepted, logprob, workspace, stream)
 

@@ -2,6 +2,7 @@
 //
 //   p = softmax(target row / T), q = softmax(drafter's row / T'):   token t of row r stays where  u_r q_r(t) < p_r(t)
 //   the first row that refuses: the lowest i with  sum_{k <= i} w_k > u sum w,  w = max(p - q, 0);   all stayed: the same with w = p of the last row
+// A drafter whose temperature is not above 0 took its greatest value: q is 1 there.
 //
 // Two kernels. The first reads every row once: maximum, where it is, and the sum of exponentials, by slices; bound by reading the rows. The second has a
 // cluster of blocks for each sequence: all its blocks judge the drafted tokens from the slices' sums, then the row that stopped is gone through again for
@@ -44,7 +45,7 @@ struct VerifyParams {
     int n_rows, n_vocab, n_seq, slices, vec;   // vec: rows begin on 16-byte boundaries
 };
 
-// The reciprocal of a temperature; greedy requests: 1.
+// The reciprocal of a temperature; greedy requests and drafters: 1.
 __device__ __forceinline__ double per_temp(const float *t, int s) {
     const float v = t ? t[s] : 1.0f;
     return v > 0.0f ? 1.0 / (double)v : 1.0;
@@ -195,7 +196,7 @@ verify_draw_kernel(const __grid_constant__ VerifyParams p) {
         return;   // (all blocks of the cluster)
     }
     const float t = p.temp ? p.temp[s] : 1.0f;
-    const bool greedy = !(t > 0.0f);
+    const bool greedy = !(t > 0.0f), sure = p.draft_temp && !(p.draft_temp[s] > 0.0f);   // sure: q is 1 at the lowest of the drafter's greatest values
     const double inv_p = fmin(per_temp(p.temp, s), 1e37), inv_q = fmin(per_temp(p.draft_temp ? p.draft_temp : p.temp, s), 1e37);
     if (tid == 0) s_stop = rows - 1, s_token = -1;
     cluster.sync();   // (all blocks are there to be written to)
@@ -213,9 +214,10 @@ verify_draw_kernel(const __grid_constant__ VerifyParams p) {
                 double qt = 1.0;
                 if (p.q) {
                     const Row qr = row_of(p, p.n_rows + row, inv_q, table);
-                    qt = exp_of(((double)p.q[row * p.q_stride + token] - (double)qr.m) * inv_q, table) / qr.sum;
+                    if (sure) qt = qr.at == token ? 1.0 : 0.0, ok = qr.at >= 0;
+                    else qt = exp_of(((double)p.q[row * p.q_stride + token] - (double)qr.m) * inv_q, table) / qr.sum;
                 }
-                ok = (double)p.accept_u[row] * qt < exp_of(a, table) / pr.sum;   // (no number: refused)
+                ok = ok && (double)p.accept_u[row] * qt < exp_of(a, table) / pr.sum;   // (no number: refused)
             }
             if (ok && rank == 0 && p.logprob && lane == 0) p.logprob[row] = (float)(a - log_of(pr.sum, table));
         }
@@ -225,15 +227,15 @@ verify_draw_kernel(const __grid_constant__ VerifyParams p) {
     const int stop = s_stop, row = r0 + stop;
     const bool last = stop == rows - 1;
     const float *x = p.p + row * p.p_stride, *y = p.q + row * p.q_stride;
-    const int certain = !p.q && !last ? p.draft[row] : -1;   // a token that has nothing left
-    const bool two = p.q && !last;
+    const bool two = p.q && !last && !sure;
     int token = -1;
     // (every warp for itself: they all find the same)
     const Row pr = row_of(p, row, inv_p, table);
     if (greedy) {
         token = pr.at;
     } else {
-        const Row qr = two ? row_of(p, p.n_rows + row, inv_q, table) : Row{0.0f, 0, 1.0};
+        const Row qr = p.q && !last ? row_of(p, p.n_rows + row, inv_q, table) : Row{0.0f, 0, 1.0};
+        const int certain = last || two ? -1 : p.q ? qr.at : p.draft[row];   // a token that has nothing left
         // ---- the sums of exponentials in 64 bits: each warp of the cluster has a part of the row, a lane eight values of 256 that follow each other
         const int per = ((p.n_vocab + kParts - 1) / kParts + 7) / 8 * 8, part = rank * kDrawWarps + warp;
         const int lo = min(p.n_vocab, part * per), hi = min(p.n_vocab, lo + per);
