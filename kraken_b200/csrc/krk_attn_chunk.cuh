@@ -913,8 +913,9 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                                 const bool b0 = take_out(x.x), b1 = take_out(x.y), b2 = take_out(x.z), b3 = take_out(x.w);
                                 if (b0 || b1 || b2 || b3) *w = x;
                             }
-                        async_fence();
                     }
+                    // (whoever took them out: a thread of the other tile of rows may have, and this one's products may be asked for before that thread's fence)
+                    async_fence();
                     __syncwarp();
                 }
                 // (one tile of rows: the products of two tiles may be in flight, which a parity does not tell apart behind the last one)

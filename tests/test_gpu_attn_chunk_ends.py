@@ -104,3 +104,25 @@ def test_scales_of_nothing(cuda, kind, act, shape):
         for odd in (np.inf, -np.inf, np.nan):
             b.cache.k[b.table[0, 0].long(), 0, 3, 0] = odd
             assert not b.torch.isfinite(b.cuda.attention_chunk(b.q, b.cache, scale=0.0, **b.args())[:counts[0], :group]).any()
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_two_tiles_of_rows_over_values_that_are_no_numbers(cuda, act, d):
+    """f16 caches: values that are no numbers at later tokens of a long chunk, in every tile that only some rows of a block see. Both tiles of rows look for them in the same memory;
+    rows that do not see them come out as from a clean cache, time after time."""
+    b = Batch(cuda, 33, 0, d, 2, 4, 16, [700, 90], [900, 90], act)
+    torch = b.torch
+    clean = torch.empty(b.q.shape, device="cuda", dtype=torch.float16 if b.half else torch.float32)
+    args = dict(scale=d ** -0.5, **b.args())
+    cuda.attention_chunk(b.q, b.cache, out=clean, **args)
+    odd = 200 + 64 * 5 + 3   # tokens before the 323rd of the first chunk do not see them
+    p = torch.arange(odd, 900, 2, device="cuda")
+    page = b.table[0].cuda()[p // 16].long()
+    values = torch.tensor([np.inf, -np.inf, np.nan], device="cuda", dtype=torch.float16)
+    b.cache.v[page, :, p % 16, 1::3] = values[torch.arange(len(p), device="cuda") % 3][:, None, None]
+    out = torch.empty_like(clean)
+    for _ in range(40):
+        cuda.attention_chunk(b.q, b.cache, out=out, **args)
+        assert (out[:odd - 200] == clean[:odd - 200]).all() and (out[700:790] == clean[700:790]).all()
+        assert not torch.isfinite(out[odd - 200:700, :, 1::3]).any() and (out[odd - 200:700, :, 0::3] == clean[odd - 200:700, :, 0::3]).all()
