@@ -572,6 +572,16 @@ static bool written_meets(std::initializer_list<List> written, std::initializer_
     return false;
 }
 
+// Likewise rows under a stride, which is not below their width where there are several: what lies between them may be anybody's.
+static bool meets_rows(const List &w, const void *base, int64_t rows, int64_t width, int64_t stride) {
+    if (!w.at || !base || w.bytes <= 0 || rows <= 0 || width <= 0) return false;
+    if (rows == 1) stride = width;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(w.at), y = reinterpret_cast<uintptr_t>(base);
+    if (x < y) return y - x < (uintptr_t)w.bytes;
+    const uintptr_t off = x - y, row = off / (uintptr_t)stride;
+    return row < (uintptr_t)rows && (off - row * (uintptr_t)stride < (uintptr_t)width || (row + 1 < (uintptr_t)rows && off + (uintptr_t)w.bytes > (row + 1) * (uintptr_t)stride));
+}
+
 int krk_cuda_step_plan(const krk_cuda_step *s, void *stream) {
     if (!s) return KRK_CUDA_ENULL;
     if (s->n_seq < 0 || s->table_width < 0 || s->page_size < 1 || s->max_tok < 0 || s->max_tok > INT32_MAX || s->free_cap < 0 || s->free_cap > INT32_MAX) return KRK_CUDA_ESHAPE;
@@ -633,11 +643,12 @@ int krk_cuda_verify_draft(void *tokens_i32, void *n_accepted_i32, void *logprob_
     for (const void *p : lists)
         if (!aligned(p, 4)) return KRK_CUDA_EALIGN;
     const int64_t rows = 4 * v->n_rows, seqs = 4ll * v->n_seq;
-    if (written_meets({{tokens_i32, rows}, {n_accepted_i32, seqs}, {logprob_f32, rows}},
-                      {{v->row_start, seqs + 4}, {v->draft, rows}, {v->accept_u, rows}, {v->sample_u, seqs}, {v->temp, seqs}, {v->draft_temp, seqs}}))
-        return KRK_CUDA_EARG;
-    if (!device_state()) return KRK_CUDA_EDEVICE;
     const size_t need = v->n_rows == 0 ? 0 : verify_draft_workspace_bytes(*v);
+    const std::initializer_list<List> written = {{tokens_i32, rows}, {n_accepted_i32, seqs}, {logprob_f32, rows}, {workspace, (int64_t)need}};
+    if (written_meets(written, {{v->row_start, seqs + 4}, {v->draft, rows}, {v->accept_u, rows}, {v->sample_u, seqs}, {v->temp, seqs}, {v->draft_temp, seqs}})) return KRK_CUDA_EARG;
+    for (const List &w : written)
+        if (meets_rows(w, logits_f32, v->n_rows, 4 * v->n_vocab, 4 * v->stride) || meets_rows(w, v->draft_logits, v->n_rows, 4 * v->n_vocab, 4 * v->draft_stride)) return KRK_CUDA_EARG;
+    if (!device_state()) return KRK_CUDA_EDEVICE;
     if (need > 0 && (!workspace || ws_bytes < need || !aligned(workspace, 16))) return KRK_CUDA_EWORKSPACE;
     return launch_verify_draft(static_cast<int32_t *>(tokens_i32), static_cast<int32_t *>(n_accepted_i32), static_cast<float *>(logprob_f32), static_cast<const float *>(logits_f32),
                                *v, workspace, static_cast<cudaStream_t>(stream));
