@@ -914,18 +914,16 @@ PyObject *block_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (!y) y = &(made_y = empty_like_device(*x, {rows, width}, half ? at::kHalf : at::kFloat));
     else if (!on_device(y, x, "out") || !tabled(y, x, y->scalar_type() == at::kHalf ? at::kHalf : at::kFloat, rows, "out")) return nullptr;
     if (h->size(1) != width || y->size(1) != width) return refuse("out, h_out: expected the shape of x"), nullptr;
-    if (rows == 0 || width == 0) {
-        PyObject *both = PyTuple_Pack(2, given_or_made(a[11], made_y), given_or_made(a[10], made_h));
-        return both;
-    }
     m.residual = Args::ptr(res), m.gate = Args::ptr(gate), m.post_weight = Args::ptr(post), m.weight = Args::ptr(w);
     m.rows = rows, m.n = width, m.x_stride = row_stride(x), m.h_stride = row_stride(h), m.y_stride = row_stride(y);
     if (res) m.residual_stride = row_stride(res);
     m.y_dtype = x_dtype(y);
-    int rc;
-    Py_BEGIN_ALLOW_THREADS rc = krk_cuda_block_norm(Args::ptr(y), Args::ptr(h), Args::ptr(x), &m, where.stream);
-    Py_END_ALLOW_THREADS
-    if (rc != 0) return fail(rc, "block_norm");
+    if (rows > 0 && width > 0) {
+        int rc;
+        Py_BEGIN_ALLOW_THREADS rc = krk_cuda_block_norm(Args::ptr(y), Args::ptr(h), Args::ptr(x), &m, where.stream);
+        Py_END_ALLOW_THREADS
+        if (rc != 0) return fail(rc, "block_norm");
+    }
     PyObject *oy = given_or_made(a[11], made_y), *oh = given_or_made(a[10], made_h);
     PyObject *both = oy && oh ? PyTuple_Pack(2, oy, oh) : nullptr;
     Py_XDECREF(oy);
