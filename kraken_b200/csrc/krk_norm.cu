@@ -175,12 +175,13 @@ block_norm_kernel(const __grid_constant__ NormParams p) {
     }
 }
 
-// Many rows: blocks that stay, two a multiprocessor, each with every gridDim.x-th row. A thread's values of the next two rows are on their way while it works on one
+// Many rows of 2564 values and more: blocks that stay, two a multiprocessor, each with every gridDim.x-th row. A thread's values of the next two rows are on their way while it works on one
 // (asynchronous copies into places of its own in shared memory, which nobody else reads), weights and a shared gate stay in its registers.
-template <int PER>
-__global__ void __launch_bounds__(512, 2)
+// A thread has two groups of four values of a row.
+constexpr int kRowsPer = 2, kRowsThreads = 512;
+__global__ void __launch_bounds__(kRowsThreads, 2)
 block_norm_rows_kernel(const __grid_constant__ NormParams p, int64_t rows) {
-    constexpr int kStages = 3;
+    constexpr int PER = kRowsPer;
     __shared__ float part[4][32];
     extern __shared__ float4 ahead[];   // [stage][x, residual][PER][thread]
     const int tid = threadIdx.x, threads = (int)blockDim.x, groups = p.n / 4;
@@ -269,14 +270,14 @@ block_norm_rows_kernel(const __grid_constant__ NormParams p, int64_t rows) {
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Once a device and form: the limit of shared memory.
-int raise_shared(int form, void (*kernel)(NormParams, int64_t), int bytes) {
-    static std::atomic<uint64_t> ready[2] = {};
+// Once a device: the limit of shared memory.
+int raise_shared() {
+    static std::atomic<uint64_t> ready = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess && !((ready[form].load(std::memory_order_acquire) >> dev) & 1)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e == cudaSuccess) ready[form].fetch_or(1ull << dev, std::memory_order_release);
+    if (e == cudaSuccess && !((ready.load(std::memory_order_acquire) >> dev) & 1)) {
+        e = cudaFuncSetAttribute(block_norm_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * 2 * kRowsPer * kRowsThreads * 16);
+        if (e == cudaSuccess) ready.fetch_or(1ull << dev, std::memory_order_release);
     }
     if (e == cudaSuccess) return KRK_CUDA_OK;
     note_cuda_error(e);
@@ -301,13 +302,13 @@ int launch_block_norm(void *y, float *h_out, const float *x, const krk_cuda_norm
     const int groups = (int)(vec ? m.n / 4 : m.n);
     const int per = groups <= 512 ? 1 : groups <= 1024 ? 2 : groups <= 2048 ? 4 : groups <= 4096 ? 8 : 0;
     const int threads = per == 0 ? 1024 : ((groups + per - 1) / per + 31) / 32 * 32;
-    // Two norms, a gate, f16 out, us here and a block a row: rows of 4096 values, 300 6.7 and 6.5, 600 8.0 and 10.1, 2048 21.0 and 25.4, 8192 82.8 and 79.1; of 2048 values, 600 6.6
-    // and 6.6, 2048 13.9 and 14.4, 8192 46.5 and 49.4; of 1024, 2048 9.5 and 7.3.
+    // Two norms, a gate, f16 out, us by blocks that stay and by a block a row: rows of 4096 values, 300 6.8 and 6.5, 600 9.9 and 10.7, 2048 21.1 and 23.3, 7000 71.1 and 66.4; 2048 rows of
+    // 3584 values 19.2 and 21.6, of 2640 16.5 and 17.2, of 2560 19.2 and 16.8, of 2304 17.9 and 14.9. One group of values a thread: 2048 rows of 2048 14.3 and 15.1, of 2044 15.3 both,
+    // of 1280 13.3 and 10.5, which does not pay for a form of its own.
     const int stay = 2 * sm_count();
-    if (vec && (per == 1 || per == 2) && groups >= 512 && m.gate_stride == 0 && m.rows >= 2 * (int64_t)stay && m.rows * m.n <= 1 << 24) {
-        const size_t shared = (size_t)3 * 2 * per * threads * 16;
-        auto rows_kernel = per == 1 ? block_norm_rows_kernel<1> : block_norm_rows_kernel<2>;
-        const int rc = raise_shared(per == 1 ? 0 : 1, rows_kernel, 3 * 2 * per * 512 * 16);
+    if (vec && per == kRowsPer && groups > 640 && m.gate_stride == 0 && m.rows >= 2 * (int64_t)stay && m.rows * m.n <= 1 << 24) {
+        const size_t shared = (size_t)3 * 2 * kRowsPer * threads * 16;
+        const int rc = raise_shared();
         if (rc != KRK_CUDA_OK) return rc;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)stay), cfg.blockDim = dim3((unsigned)threads), cfg.dynamicSmemBytes = shared, cfg.stream = st;
@@ -315,7 +316,7 @@ int launch_block_norm(void *y, float *h_out, const float *x, const krk_cuda_norm
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr, cfg.numAttrs = 1;
-        return launched(cudaLaunchKernelEx(&cfg, rows_kernel, p, (int64_t)m.rows));
+        return launched(cudaLaunchKernelEx(&cfg, block_norm_rows_kernel, p, (int64_t)m.rows));
     }
     auto kernel = vec ? (per == 1 ? block_norm_kernel<4, 1> : per == 2 ? block_norm_kernel<4, 2> : per == 4 ? block_norm_kernel<4, 4> : per == 8 ? block_norm_kernel<4, 8> : block_norm_kernel<4, 0>)
                       : (per == 1 ? block_norm_kernel<1, 1> : per == 2 ? block_norm_kernel<1, 2> : per == 4 ? block_norm_kernel<1, 4> : per == 8 ? block_norm_kernel<1, 8> : block_norm_kernel<1, 0>);

@@ -26,3 +26,11 @@ def test_empty_calls_keep_nothing(cuda, shape):
     del y, z
     gc.collect()
     assert gone[0]() is None and gone[1]() is None
+
+
+@pytest.mark.parametrize("n", [2044, 2048, 2560, 2564, 3000])
+@pytest.mark.parametrize("rows", [600, 1100])
+def test_many_rows_either_side_of_a_width(cuda, n, rows):
+    """Widths about those from which a thread has two groups of values, and from which blocks stay, as in test_gpu_block_norm.py."""
+    from test_gpu_block_norm import test_many_rows
+    test_many_rows(cuda, n, rows)
