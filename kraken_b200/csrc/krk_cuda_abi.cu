@@ -490,6 +490,7 @@ static int check_attention(const krk_cuda_kv_cache *cache, const krk_cuda_attent
     if (a.max_kv_len == 0) a.max_kv_len = room;
     if (a.max_kv_len > room || a.max_kv_len > (1ll << 30)) return KRK_CUDA_ESHAPE;
     if (a.window < 0 || (a.window > 0 && a.window < least_window) || !(a.softcap >= 0.0f && a.softcap <= FLT_MAX)) return KRK_CUDA_EARG;
+    if (a.window > (1 << 30)) a.window = 1 << 30;   // (positions are below that; a row's own, up to max_q below 0, less the window stays within 31 bits)
     return KRK_CUDA_OK;
 }
 

@@ -126,3 +126,18 @@ def test_two_tiles_of_rows_over_values_that_are_no_numbers(cuda, act, d):
         cuda.attention_chunk(b.q, b.cache, out=out, **args)
         assert (out[:odd - 200] == clean[:odd - 200]).all() and (out[700:790] == clean[700:790]).all()
         assert not torch.isfinite(out[odd - 200:700, :, 1::3]).any() and (out[odd - 200:700, :, 0::3] == clean[odd - 200:700, :, 0::3]).all()
+
+
+@pytest.mark.parametrize("kind,act,d", [("f16", "f32", 128), ("f16", "f16", 64), ("q8", "f16", 128), ("q8", "f32", 128), ("q4", "f32", 64)])
+def test_windows_wider_than_any_context(cuda, kind, act, d):
+    """Up to the largest int, also where a sequence has more rows than positions, whose first rows lie before position 0."""
+    for group in (1, 4):
+        b = Batch(cuda, 34, KINDS[kind], d, 1, group, 16, [250, 300, 40, 1], [240, 20, 700, 300], act)
+        free = b.check()
+        for window in (2 ** 31 - 1, 2 ** 31 - 100, 2 ** 30 + 1, 2 ** 30, 100000):
+            got = b.check(window=window)
+            assert ((got == 0) == (free == 0)).all()   # (the division of the work may be another one)
+    few = Batch(cuda, 35, KINDS[kind], d, 1, 4, 16, [60, 5], [50, 300], "f32")
+    tree = [cuda.attention_tree(few.q, few.cache, window=w, **few.args())[:65] for w in (0, 2 ** 31 - 1, 2 ** 30)]
+    want, tol, _ = few.want(d ** -0.5)
+    assert all(((t.double() - want[:65]).abs() <= tol[:65]).all() for t in tree)
