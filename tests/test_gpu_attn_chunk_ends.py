@@ -141,3 +141,82 @@ def test_windows_wider_than_any_context(cuda, kind, act, d):
     tree = [cuda.attention_tree(few.q, few.cache, window=w, **few.args())[:65] for w in (0, 2 ** 31 - 1, 2 ** 30)]
     want, tol, _ = few.want(d ** -0.5)
     assert all(((t.double() - want[:65]).abs() <= tol[:65]).all() for t in tree)
+
+
+@pytest.mark.parametrize("kind", ["q8", "q4"])
+@pytest.mark.parametrize("d,group", [(64, 7), (96, 4), (128, 4), (128, 1)])
+@pytest.mark.parametrize("window", [0, 200])
+def test_scales_that_are_no_numbers(cuda, kind, d, group, window):
+    """f32 results over 8 and 4 bits, more rows than go to the kernel of trees. Scales that are no numbers, and ones that take values beyond f16, where no row sees them (behind the last
+    position, in unused pages, before the window, at later tokens of the chunk): the same bits as without them. Values that are no numbers reach the rows that see them, in their block
+    of 32 alone."""
+    b = Batch(cuda, 41, KINDS[kind], d, 2, group, 16, [301, 7, 1], [805, 500, 1003], "f32")
+    torch = b.torch
+    clean = b.check(window=window)
+    first = 805 - 301
+    keep = torch.zeros((b.cache.n_pages, 16), dtype=torch.bool)
+    for s, (c, n) in enumerate(zip(b.counts, b.lens)):
+        p = torch.arange(max(0, n - c + 1 - window) if window else 0, n)
+        keep[b.table[s, p // 16].long(), p % 16] = True
+    keep = keep.cuda()[:, None, :, None]
+    odd = torch.tensor([np.nan, np.inf, -np.inf, 65504], dtype=torch.float16, device="cuda")
+    for a in (b.cache.k_scale, b.cache.v_scale):
+        a.copy_(torch.where(keep, a, odd[torch.randint(0, 4, a.shape, device="cuda")]))
+    assert (b.check(window=window) == clean).all()
+
+    def at(p):
+        return b.table[0, p // 16].long(), 1, p % 16
+    was_k, was_v = b.cache.k_scale.clone(), b.cache.v_scale.clone()
+    heads = slice(group, 2 * group)   # of key head 1
+    args = dict(scale=d ** -0.5, window=window, **b.args())
+    # one token of the chunk after the other: in a tile's middle, at its ends, in the last one
+    for i in (0, 1, 70, first % 64, 127, 200, 300):
+        b.cache.v_scale[at(first + i)][0] = (np.inf, np.nan)[i & 1]
+        out = cuda.attention_chunk(b.q, b.cache, **args)
+        sees = torch.arange(301, device="cuda") >= i
+        if window:
+            sees &= torch.arange(301, device="cuda") < i + window
+        assert (out[:301][~sees] == clean[:301][~sees]).all() and (out[301:309] == clean[301:309]).all() and (out[:301, :group] == clean[:301, :group]).all()
+        assert (out[:301, heads, 32:] == clean[:301, heads, 32:]).all() and (~torch.isfinite(out[:301][sees][:, heads, :32])).any(-1).all()
+        b.cache.v_scale.copy_(was_v)
+    b.cache.k_scale[at(first + 100)][d // 32 - 1] = np.nan
+    out = cuda.attention_chunk(b.q, b.cache, **args)
+    assert (out[:100] == clean[:100]).all() and not torch.isfinite(out[100:301 if not window else 300][:, heads]).any()
+    b.cache.k_scale.copy_(was_k)
+    # beside a scale that takes a value beyond f16, which has the call done anew: what is no number stays where it was seen
+    b.cache.v_scale[at(first + 150)][0], b.cache.v_scale[at(first + 20)][1] = np.inf, 60000.0
+    out = cuda.attention_chunk(b.q, b.cache, **args)
+    assert torch.isfinite(out[:150]).all() and (~torch.isfinite(out[150:301, heads, :32])).any(-1).all() and torch.isfinite(out[150:301, heads, 32:]).all()
+    b.cache.v_scale[at(first + 150)][0] = was_v[at(first + 150)][0]
+    b.check(window=window)
+    b.cache.v_scale.copy_(was_v)
+    assert (b.check(window=window) == clean).all() and cuda.device_status() == 0
+
+
+@pytest.mark.parametrize("kind", ["q8", "q4"])
+def test_more_rows_than_positions_and_missing_pages_in_two_terms(cuda, kind):
+    """As test_gpu_attn_chunk.py's test of rows that see nothing, with more rows than go to the kernel of trees."""
+    b = Batch(cuda, 42, KINDS[kind], 128, 1, 4, 16, [5, 3, 200, 140], [2, 0, 130, 40], "f32")
+    got = b.check()
+    assert (got[:3] == 0).all() and (got[5:78] == 0).all() and (got[208:308] == 0).all() and (got[308:] != 0).any(-1).all()
+    assert (b.check(sinks=b.torch.randn(4, device="cuda"))[:3] == 0).all()
+    b.lens[1] = -7
+    b.check()
+    b.check(window=40)
+    b = Batch(cuda, 43, KINDS[kind], 128, 1, 4, 16, [150, 20], [600, 20], "f32")
+    b.table[0, :5], b.table[0, 9], b.table[0, 20], b.table[1, 0] = -1, 1 << 30, b.cache.n_pages, -5
+    assert (b.check()[150:150 + 16] == 0).all()
+    b.check(window=40)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("d", [192, 256])
+def test_long_heads_with_sinks_and_soft_limits(cuda, kind, act, d):
+    b = Batch(cuda, 44, KINDS[kind], d, 2, 3, 32, [90, 1, 33], [700, 64, 33], act, q_size=4.0)
+    sinks = 3 * b.torch.randn(6, device="cuda", generator=b.torch.Generator("cuda").manual_seed(1))
+    sinks[1], sinks[2] = -np.inf, 60.0
+    b.check(sinks=sinks)
+    b.check(softcap=20.0, sinks=sinks, window=70)
+    b.check(window=1, sinks=sinks)
+    check(b, 1e8)
