@@ -184,7 +184,7 @@ __device__ __forceinline__ Row row_of(const VerifyParams &p, int item, double in
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads, 2)
 verify_draw_kernel(const __grid_constant__ VerifyParams p) {
     __shared__ double table[64], sums[3][kParts];   // [sum of p's exponentials, of q's, of weights][warps of the cluster]: this block writes its own to all of them
-    __shared__ int s_stop, s_token;
+    __shared__ int s_stop, s_token, s_certain;
     const cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cluster.block_rank(), s = blockIdx.x / kCluster;
     if (tid < 64) table[tid] = exp2((double)tid / 64.0);   // (published by the cluster's meeting)
@@ -226,6 +226,14 @@ verify_draw_kernel(const __grid_constant__ VerifyParams p) {
     __syncthreads();
     const int stop = s_stop, row = r0 + stop;
     const bool last = stop == rows - 1;
+    // a token that has nothing left (by way of shared memory: beside the sums, in every warp's registers, it cost spills, 64 sequences 189 us for 184)
+    if (warp == 0 && !last) {
+        const int at = !p.q ? p.draft[row] : sure ? row_of(p, p.n_rows + row, inv_q, table).at : -1;
+        if (lane == 0) s_certain = at;
+    }
+    if (tid == 0 && last) s_certain = -1;
+    __syncthreads();
+    const int certain = s_certain;
     const float *x = p.p + row * p.p_stride, *y = p.q + row * p.q_stride;
     const bool two = p.q && !last && !sure;
     int token = -1;
@@ -234,8 +242,7 @@ verify_draw_kernel(const __grid_constant__ VerifyParams p) {
     if (greedy) {
         token = pr.at;
     } else {
-        const Row qr = p.q && !last ? row_of(p, p.n_rows + row, inv_q, table) : Row{0.0f, 0, 1.0};
-        const int certain = last || two ? -1 : p.q ? qr.at : p.draft[row];   // a token that has nothing left
+        const Row qr = two ? row_of(p, p.n_rows + row, inv_q, table) : Row{0.0f, 0, 1.0};
         // ---- the sums of exponentials in 64 bits: each warp of the cluster has a part of the row, a lane eight values of 256 that follow each other
         const int per = ((p.n_vocab + kParts - 1) / kParts + 7) / 8 * 8, part = rank * kDrawWarps + warp;
         const int lo = min(p.n_vocab, part * per), hi = min(p.n_vocab, lo + per);
