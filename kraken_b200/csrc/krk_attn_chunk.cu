@@ -1,6 +1,9 @@
 // krk_cuda_attention_chunk: the choice of a launch's form, and the kernel that adds up the partial sums of divided items.
 #include "krk_attn_chunk.cuh"
 
+#include <algorithm>
+#include <cfloat>
+
 namespace krk_cuda {
 namespace attn {
 namespace {
@@ -179,6 +182,8 @@ int launch_attention_chunk(void *out, int out_dtype, const void *q, int q_dtype,
     // Scores are masked before they are multiplied by the row's factor, which therefore must not be 0 (-infinity times 0). Under a soft limit they are multiplied first, and
     // those of 0 stay 0, whatever the limit is.
     if (p.scale == 0.0f && p.softcap == 0.0f) p.softcap = 1.0f;
+    // (finite, so that a score of 0 stays 0 under the smallest limits)
+    p.per_cap = p.softcap > 0.0f ? std::min(1.0f / p.softcap, FLT_MAX) : 0.0f;
     attn::divide_by(p.group, p.group_mul, p.group_shift);
     p.status = device_status_word();
     if (!p.status) return KRK_CUDA_EDEVICE;

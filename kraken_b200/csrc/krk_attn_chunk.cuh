@@ -41,7 +41,7 @@ struct ChunkParams {
     int64_t n_pages;
     int table_width, page_size, max_len, n_seq, n_heads, n_kv, group, max_q, window, whole, grid, q_half, out_half, out_wide;   // out_wide: rows of out begin on 32-byte boundaries
     uint32_t group_mul, group_shift;      // row / group = row * group_mul >> group_shift, rows below 2^30
-    float scale, softcap;
+    float scale, softcap, per_cap;        // per_cap: 1 / softcap, finite
     int *status;
     // f16 caches: the pool's rows as boxes of 64 values of box_rows positions, a part of one page; behind the last row zeros come in
     int box_rows, pool_rows;
@@ -515,9 +515,9 @@ __device__ __forceinline__ void products_p(uint32_t d, uint32_t a, uint32_t b_lo
                      ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(onto), "r"(0u), "r"(elected), "r"(kDescHi) : "memory");
 }
 // As capped, without a call: the hyperbolic tangent from one exponential, 2^-22 of 1 off. Below 1/4, where that would be more and more of it (under a limit far above the scores
-// all of it), from its series, whose next term is 2^-26 of it there.
-__device__ __forceinline__ float capped_here(float x, float cap) {
-    const float y = x / cap, z = y * y;
+// all of it), from its series, whose next term is 2^-26 of it there. per_cap: a quotient's rounding and its own, 2^-22 at the largest limits, whose reciprocals have no leading bit.
+__device__ __forceinline__ float capped_here(float x, float cap, float per_cap) {
+    const float y = x * per_cap, z = y * y;
     float r;   // (to its last place or the one beside)
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(y * (2.0f * 1.44269504f))));
     float t = 1.0f - 2.0f * r;
@@ -573,14 +573,14 @@ __device__ __forceinline__ float value_at(const uint8_t *pool, const __half *sca
 
 // Log2 scores under a soft limit in place of products.
 template <int TP>
-__device__ __forceinline__ void soft_limit(uint32_t t_s, float sc, float cap) {
+__device__ __forceinline__ void soft_limit(uint32_t t_s, float sc, float cap, float per_cap) {
 #pragma unroll 1
     for (int c = 0; c < TP; c += 16) {
         uint32_t v[16];
         tmem_load16(t_s + c, v);
         tmem_loaded();
 #pragma unroll
-        for (int j = 0; j < 16; j++) v[j] = __float_as_uint(capped_here(__uint_as_float(v[j]) * sc, cap));
+        for (int j = 0; j < 16; j++) v[j] = __float_as_uint(capped_here(__uint_as_float(v[j]) * sc, cap, per_cap));
         tmem_store16(t_s + c, v);
     }
     tmem_stored();
@@ -841,7 +841,7 @@ attn_chunk_kernel(const __grid_constant__ ChunkParams p) {
                 // What is rarely done has code of its own, and no more of it than has to be: code that is jumped over, or met for the first time, is fetched at
                 // the pace of thousands of clocks.
                 if (p.softcap > 0.0f) {   // log2 scores in place of the products
-                    soft_limit<TP>(t_s, sc, p.softcap);
+                    soft_limit<TP>(t_s, sc, p.softcap, p.per_cap);
                     f = 1.0f;
                 }
                 uint32_t v[TP];

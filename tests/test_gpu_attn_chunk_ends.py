@@ -70,7 +70,7 @@ SHAPES = [(128, 2, 4, [140, 1], [900, 30]), (64, 1, 2, [40, 3], [300, 700]), (25
 def test_soft_limits(cuda, kind, act, shape):
     d, kv, group, counts, lens = shape
     b = Batch(cuda, 31, KINDS[kind], d, kv, group, 16, counts, lens, act, q_size=4.0)
-    for limit in (1.0, 30.0, 300.0, 1e4, 1e6, 1e8, 1e30, 3e38, 3.4028234e38):
+    for limit in (1e-40, 1e-3, 1.0, 30.0, 300.0, 1e4, 1e6, 1e8, 1e30, 3e38, 3.4028234e38):
         check(b, limit)
     free = check(b).double()
     huge = check(b, 1e30).double()
