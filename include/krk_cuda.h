@@ -342,7 +342,8 @@ int krk_cuda_attention_tree(void *out_f32, const void *q_f32, const struct krk_c
 
 /* The same over chunks of prompts, for max_q of any size: a row sees itself and the positions before it (host_attention->tree is NULL), with a window,
  * of one or more, only the nearest `window` of those. out and q are f32, or out f16 and q f32 or f16 (KRK_CUDA_X_F32, KRK_CUDA_X_F16; strides in
- * elements, multiples of 4 of f32 and 8 of f16). f32: queries and weights enter the products as above, what a weight adds ends at 2^-32 of the greatest value. f16: queries and weights enter with 11 bits, and 8- and
+ * elements, multiples of 4 of f32 and 8 of f16). f32: queries and weights enter the products as above, what a weight adds ends at 2^-32 of the greatest value; sums are cut off,
+ * not rounded, over runs of 2048 positions (3e-6 of a result and less; of values of one sign up to 2^-16). f16: queries and weights enter with 11 bits, and 8- and
  * 4-bit keys and values rounded to f16 (infinite beyond its range); maxima and sums are f32. Meant for sequences with tens of new tokens and more; single tokens among them
  * are taken too. A window that leaves a row nothing, and pages, lengths, infinities and rows of no sequence, are as above. */
 size_t krk_cuda_attention_chunk_workspace_bytes(const struct krk_cuda_kv_cache *host_cache, const struct krk_cuda_attention *host_attention, int out_dtype);

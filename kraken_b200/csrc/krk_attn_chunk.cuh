@@ -12,11 +12,17 @@
 // The reference that a softmax subtracts stands until a score passes it by 2^8: the sums in tensor memory are rescaled a few times a row, not each tile. The work
 // is divided by what blocks of rows cost (ChunkWalk), partial sums of divided items are added up by a second kernel in the order of the blocks.
 //
-// Bound: tensor pipe and power for f16 results of long chunks: 4096 tokens behind 8192, 32 heads of 128 over 8, 630 to 700 us by the card's temperature (980 to 1090
-// TFLOP/s; cuBLAS sustains 1372 on this card). There the exponential unit is as busy as the tensor pipe, so half of the exponentials are a polynomial's (604 -> 548 us for 8192 tokens).
-// f32 results take two terms of queries and weights, twice the products: 2048 tokens 121 us (2 x 283 TFLOP/s), 8192 tokens 980 to 1040. Over 8 and 4 bits what unpacks
-// the quants is the limit: 24 ragged sequences of up to 512 tokens behind up to 8000, 8 bits, 550 us; 4096 behind 8192 965; f32, three products, two chunks of up to 700
-// behind 5000, 406. Few tokens: a launch, pages, one item's latency: 33 tokens 21 us.
+// f16 results: queries (f32 ones) and weights have one f16 term, quants times scales are rounded to f16, half of the exponentials are 7.5e-5 off, all of them below the rounding of the
+// result or near it: against 64 bits 2.9e-4 over an f16 cache, 5.1e-4 to 6.4e-4 over 8 and 4 bits, where 2.1e-4 is the result's rounding alone. Second terms would be twice the products, as
+// f32 results have them: those are 2e-6 off over 2048 positions (additions in tensor memory cut off; see add_run).
+//
+// Bound, f16 results of long chunks: 4096 tokens behind 8192, 32 heads of 128 over 8, 633 us on a cool card, 655 with pauses (1965 MHz), 720 to 745 back to back, where the power
+// limit holds the clock at 1642 MHz (993 W): 920 to 1080 TFLOP/s; cuBLAS sustains 1372 on this card. The tensor pipe is busy 54 % of the cycles, the issue slots 47 %: products and the
+// softmax of the other tile of rows wait for each other. Half of the exponentials are a polynomial's since the exponential unit would be as busy as the pipe (604 -> 548 us for 8192 tokens).
+// f32 results take two terms of queries and weights, twice the products: 2048 tokens 121 to 124 us (2 x 280 TFLOP/s), 8192 tokens 980 to 1170. Over 8 and 4 bits what unpacks
+// the quants is the limit, each block of rows for itself: 24 ragged sequences of up to 512 tokens behind up to 8000, 8 bits, 557 us; 4096 behind 8192 950 to 990; f32, three products, two
+// chunks of up to 700 behind 5000, 405. A soft limit is a pass of its own over the scores: 2048 tokens 133 us for 74, f32 168 for 121. Few tokens: a launch, pages, one item's latency:
+// 33 tokens 21 us.
 #pragma once
 
 #include <cuda.h>

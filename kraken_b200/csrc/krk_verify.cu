@@ -12,7 +12,7 @@
 // 2e-8 off) one draw in 250 came out as a neighbour. So the drawn row's weights, their sums and the sums before them have 64 bits (weights to 4e-14). The
 // judgement compares two numbers once, for which sums of f32 exponentials do (their arguments' rounding: under 1e-6 of a sum), with the token's own in 64 bits.
 //
-// Measured, 128,256 tokens: one sequence of five rows 17 us (5 for the sums; the drawing waits for memory and for four meetings of its blocks), 64 sequences of up to
+// Measured, 128,256 tokens: one sequence of five rows 17.5 to 19 us (5 for the sums; the drawing waits for memory and for four meetings of its blocks), 64 sequences of up to
 // eight rows with a drafter's 130 us: 58 for the sums (265 MB, 4.6 TB/s), 72 for the drawing, bound by arithmetic in 64 bits (each weight twice: sums, then weights;
 // for p alone once). A block of 512 threads an SM, with exponentials of CUDA's own, took 182 there, and a scan of 32 weights after the other 51 for one sequence.
 #include "krk_common.cuh"
